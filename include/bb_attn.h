@@ -35,7 +35,8 @@ extern "C" {
  *        x_is_f32, and bb_int8_dequantize an output kind where it took out_is_f32 (the old values keep their
  *        meaning)
  *   203  bb_add_rms_norm, bb_silu_mul, bb_gemv and bb_gemv_norm added; later, with no parameter list changed and so
- *        under the same number, bb_gemv_norm_rope and bb_argmax_step (a library built before them lacks the symbols) */
+ *        under the same number, bb_gemv_norm_rope, bb_argmax_step and the bb_int4_* functions (a library built before
+ *        them lacks the symbols) */
 #define BB_ABI_VERSION 203
 int bb_version(void);
 
@@ -336,6 +337,56 @@ int bb_gemv_norm_rope(const void* w, int64_t sw, int N, int K, const void* x, co
  */
 int bb_rope_inplace(void* x, const int64_t* sx, int B, int Hh, int64_t T, int D, const void* cos, const void* sin,
                     const int64_t* sc, int is_f16, void* stream);
+
+/*
+ * KV cache in 4 bits (the reference has compressed caches of its own format, modal_rd/turbo_kv.py; this one is new).
+ *
+ * Format. A row of D elements (D = 32, 64, 128 or 256) is D / 32 groups of 32 consecutive elements. Per group, on values
+ * clamped to +-65504 and with NaN taken as 0, each operation in fp32:
+ *   z = fp16(min),  s = fp16(max((max - z) / 15, 0)),  code = rint((x - z) / s) clamped to 0 .. 15 (0 where s = 0);
+ * the value of an element is s * code + z in fp32. Byte b of a packed row holds element 2 b in its low and 2 b + 1 in its
+ * high four bits.
+ * A cache is codes [heads, cap, D / 2] bytes and params [heads, cap, D / 32, 2] fp16 (s, z), for K and for V: the rows of
+ * one head are contiguous, heads are sc[] apart. sc[4] = head strides of kq (bytes, a multiple of 16), kp (fp16 elements,
+ * even), vq and vp (alike). Codes are 16-byte aligned, params 4-byte aligned. A pointer into the middle of a cache (row a
+ * of every head) addresses its rows from a on.
+ *
+ * bb_int4_quantize writes `rows` rows of every head: xk [heads, rows, D] (strides sxk[2]: head, row, in elements; rows
+ * 16-byte aligned; x_kind 0 bf16, 1 fp32, 2 fp16) to (kq, kp) and, in the same launch, xv (strides sxv[2]) to (vq, vp).
+ * xv = NULL: one tensor (sc[0], sc[1]).
+ */
+int bb_int4_quantize(const void* xk, const int64_t* sxk, const void* xv, const int64_t* sxv, int x_kind, int heads,
+                     int64_t rows, int D, uint8_t* kq, void* kp, uint8_t* vq, void* vp, const int64_t* sc, void* stream);
+
+/* The values of `rows` rows of every head: outk (and, with vq, outv) [heads, rows, D] contiguous, 16-byte aligned
+ * (out_kind: 0 bf16, 1 fp32, 2 fp16; the fp32 value rounded to nearest even). vq = NULL: one tensor. */
+int bb_int4_dequantize(const uint8_t* kq, const void* kp, const uint8_t* vq, const void* vp, const int64_t* sc, int heads,
+                       int64_t rows, int D, void* outk, void* outv, int out_kind, void* stream);
+
+/*
+ * Exact attention of the last T tokens (1 .. 16) over the first n rows of a 4-bit cache: out [T, H, D] (strides so[2]:
+ * token, head) from q [T, H, D] (strides sq[2]), bf16 or fp16 (is_f16), scores and softmax in fp32 over the fp32 values of
+ * the cached rows. Token t attends every row, or with `causal` the first n - T + 1 + t. A token that attends no row
+ * gives zeros. D = 64 or 128; any number of query heads per KV head.
+ * n: T <= n <= cap. With n_dev (an int64 in device memory) the length is read there and clamped to 0 .. cap, and n is
+ * ignored; every launch shape then depends on cap alone, so a captured graph stays valid while the cache grows.
+ * Workspace: bb_int4_decode_workspace(n, ...), with n_dev bb_int4_decode_workspace(cap, ...).
+ */
+int bb_int4_decode(const void* q, const int64_t* sq, const uint8_t* kq, const void* kp, const uint8_t* vq, const void* vp,
+                   const int64_t* sc, int64_t n, const int64_t* n_dev, int64_t cap, int T, int H, int Hkv, int D,
+                   int is_f16, float scale, int causal, void* out, const int64_t* so, void* ws, size_t ws_bytes,
+                   void* stream);
+
+/* One step: the T tokens' K and V rows, knew / vnew [Hkv, T, D] of q's type (strides sknew[2], svnew[2]: head, token;
+ * 16-byte aligned rows), are quantised into rows n - T .. n - 1 of the cache, then bb_int4_decode. n counts the new rows;
+ * rows that a device-side length puts outside the cache are not written. */
+int bb_int4_decode_append(const void* q, const int64_t* sq, uint8_t* kq, void* kp, uint8_t* vq, void* vp,
+                          const int64_t* sc, const void* knew, const int64_t* sknew, const void* vnew,
+                          const int64_t* svnew, int64_t n, const int64_t* n_dev, int64_t cap, int T, int H, int Hkv,
+                          int D, int is_f16, float scale, int causal, void* out, const int64_t* so, void* ws,
+                          size_t ws_bytes, void* stream);
+
+size_t bb_int4_decode_workspace(int64_t n, int T, int H, int Hkv, int D);
 
 /*
  * Measurement helper (no reference counterpart): reads `bytes` (a multiple of 16, 16-byte aligned) of device memory

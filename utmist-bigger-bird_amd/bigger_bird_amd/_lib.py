@@ -66,6 +66,13 @@ SIGNATURES = {
     "bb_argmax_step": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "bb_stream_read": (_i32, [_vp, _sz, _vp, _i32, _vp]),
     "bb_int8_quantize_pair": (_i32, [_vp, _vp, _i32, _i64, _i64, _i32, _i64, _i32, _f32, _vp, _vp, _vp, _vp, _i32, _vp]),
+    "bb_int4_quantize": (_i32, [_vp, c_i64p, _vp, c_i64p, _i32, _i32, _i64, _i32, _vp, _vp, _vp, _vp, c_i64p, _vp]),
+    "bb_int4_dequantize": (_i32, [_vp, _vp, _vp, _vp, c_i64p, _i32, _i64, _i32, _vp, _vp, _i32, _vp]),
+    "bb_int4_decode": (_i32, [_vp, c_i64p, _vp, _vp, _vp, _vp, c_i64p, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _i32,
+                              _f32, _i32, _vp, c_i64p, _vp, _sz, _vp]),
+    "bb_int4_decode_append": (_i32, [_vp, c_i64p, _vp, _vp, _vp, _vp, c_i64p, _vp, c_i64p, _vp, c_i64p, _i64, _vp, _i64,
+                                     _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, c_i64p, _vp, _sz, _vp]),
+    "bb_int4_decode_workspace": (_sz, [_i64, _i32, _i32, _i32, _i32]),
 }
 
 

@@ -1,0 +1,366 @@
+"""KV cache in 4 bits on MI355X: writing rows, reading them back, and exact decode over the packed rows.
+
+The reference keeps compressed caches in formats of its own (modal_rd/turbo_kv.py); this one is new, and reaches the same
+places: an HF cache layer (`make_int4_cache`, next to `make_int8_cache`) whose handles RDAttention attends with `attend`.
+
+Format: asymmetric per token, KV head and group of 32 elements. On values clamped to +-65504, with NaN taken as 0, each
+operation in fp32: z = fp16(min), s = fp16(max((max - z) / 15, 0)), code = rint((x - z) / s) clamped to 0..15 (0 where
+s = 0); the value is s * code + z in fp32. Byte b of a packed row holds element 2 b (low four bits) and 2 b + 1. A cache
+is codes [Hkv, capacity, d / 2] uint8 and params [Hkv, capacity, d / 32, 2] fp16 (s, z), head-major, for K and for V:
+80 bytes a row at head_dim 128, against 130 in int8 and 256 in bf16.
+"""
+import contextlib
+
+import torch
+from transformers import DynamicCache
+
+from . import _lib
+from .kv_int8 import _KINDS, GROW, Int8KVLayer
+
+MAX_TOKENS = 16  # query tokens of one decode call
+_HEAD_DIMS = (32, 64, 128, 256)
+
+
+def _on(t):
+    """The device of t made current for a launch (nothing when it is already)."""
+    if t.get_device() == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _one_device(what, *tensors):
+    """Every tensor on one ROCm device (the kernels run on the stream of the first)."""
+    _lib.require_gpu(*tensors, what=what)
+    first = tensors[0].get_device()
+    if any(t is not None and t.get_device() != first for t in tensors):
+        raise ValueError(f"{what}: tensors on different devices")
+
+
+def _input_rows(x):
+    """x [..., t, d] as [heads, t, d] with 16-byte aligned rows (a copy where it is not)."""
+    x = x[None] if x.ndim == 2 else x.flatten(0, -3) if x.ndim > 3 else x
+    el = x.element_size()
+    if x.stride(-1) != 1 or x.data_ptr() % 16 or (x.stride(0) * el) % 16 or (x.stride(1) * el) % 16:
+        x = x.contiguous()
+    return x
+
+
+def _packed(what, q, p):
+    """(heads, rows, head_dim, head stride of q in bytes, head stride of p in elements) of packed rows: q [..., t, d / 2]
+    and p [..., t, d / 32, 2], the rows of a head back to back, one stride between heads."""
+    if q.dtype != torch.uint8 or p.dtype != torch.float16:
+        raise ValueError(f"{what}: codes must be uint8 and params float16")
+    if q.ndim < 2 or p.ndim != q.ndim + 1 or p.shape[:-2] != q.shape[:-1]:
+        raise ValueError(f"{what}: codes [..., t, d / 2] and params [..., t, d / 32, 2] must match")
+    if q.ndim != 3:
+        try:
+            q = q.view(-1, *q.shape[-2:]) if q.ndim > 3 else q[None]
+            p = p.view(-1, *p.shape[-3:]) if p.ndim > 4 else p[None]
+        except RuntimeError:
+            raise ValueError(f"{what}: packed rows need one stride between heads") from None
+    h, t, half = q.shape
+    if 2 * half not in _HEAD_DIMS or p.shape[2:] != (half // 16, 2):
+        raise ValueError(f"{what}: codes [..., t, d / 2] and params [..., t, d / 32, 2] must match (d 32, 64, 128 or 256)")
+    sq, sp = q.stride(), p.stride()
+    if (sq[2] != 1 or sp[3] != 1 or (sp[2] != 2 and half > 16) or t > 1 and (sq[1] != half or sp[1] != half // 8)
+            or h > 1 and (sq[0] < t * half or sp[0] < t * (half // 8))):
+        raise ValueError(f"{what}: the packed rows of a head must be contiguous and heads must not overlap")
+    return h, t, 2 * half, sq[0] if h > 1 else 0, sp[0] if h > 1 else 0
+
+
+def _new_packed(rows, d, device):
+    """Codes and params of `rows` (the leading dimensions) rows of d elements."""
+    return (torch.empty(*rows, d // 2, dtype=torch.uint8, device=device),
+            torch.empty(*rows, d // 32, 2, dtype=torch.float16, device=device))
+
+
+def _check_input(x):
+    if x.dtype not in _KINDS:
+        raise ValueError("quantize4: bf16, fp16 or fp32 input")
+    if x.ndim < 2 or x.shape[-1] not in _HEAD_DIMS:
+        raise ValueError("quantize4: rows [..., t, d] with d 32, 64, 128 or 256")
+
+
+def _check_out(x, out):
+    shape = _packed("quantize4", *out)[:3]
+    if out[0].shape[:-1] != x.shape[:-1] or shape[2] != x.shape[-1]:
+        raise ValueError("quantize4: out tensors must match x")
+
+
+def quantize4(x, out=None):
+    """[..., t, d] (bf16, fp16 or fp32, any strides) -> codes [..., t, d / 2] uint8, params [..., t, d / 32, 2] fp16.
+
+    `out` = (codes, params) to write into, e.g. the rows [a, b) of a cache: (k4[:, a:b], kp[:, a:b])."""
+    return quantize4_pair(x, None, out, None)[0]
+
+
+def quantize4_pair(xk, xv, out_k=None, out_v=None):
+    """quantize4(xk, out_k) and quantize4(xv, out_v) in one launch (a prompt's or a step's new K and V rows: one shape and
+    dtype). Returns ((codes, params) of K, (codes, params) of V)."""
+    _check_input(xk)
+    _one_device("quantize4", xk, xv, *(out_k or ()), *(out_v or ()))
+    if xv is not None and (xv.shape != xk.shape or xv.dtype != xk.dtype):
+        raise ValueError("quantize4: K and V rows must share a shape and dtype")
+    if out_k is None:
+        out_k = _new_packed(xk.shape[:-1], xk.shape[-1], xk.device)
+    else:
+        _check_out(xk, out_k)
+    if xv is not None:
+        if out_v is None:
+            out_v = _new_packed(xv.shape[:-1], xv.shape[-1], xv.device)
+        else:
+            _check_out(xv, out_v)
+    if xk.numel() == 0:
+        return out_k, out_v
+    a, b = _input_rows(xk), None if xv is None else _input_rows(xv)
+    _, _, d, skq, skp = _packed("quantize4", *out_k)
+    svq = svp = 0
+    if xv is not None:
+        _, _, _, svq, svp = _packed("quantize4", *out_v)
+    with _on(xk):
+        _lib.check(_lib.lib().bb_int4_quantize(
+            _lib.ptr(a), _lib.i64s(*a.stride()[:2]), _lib.ptr(b), None if b is None else _lib.i64s(*b.stride()[:2]),
+            _KINDS[a.dtype], a.shape[0], a.shape[1], d, _lib.ptr(out_k[0]), _lib.ptr(out_k[1]),
+            None if b is None else _lib.ptr(out_v[0]), None if b is None else _lib.ptr(out_v[1]),
+            _lib.i64s(skq, skp, svq, svp), _lib.stream_of(xk)))
+    return out_k, out_v
+
+
+def dequantize4(q, p, dtype):
+    """codes [..., t, d / 2], params [..., t, d / 32, 2] -> [..., t, d] in dtype (bf16, fp16 or fp32; the fp32 value
+    s * code + z rounded to nearest even). Rows [a, b) of a cache are read in place: (k4[:, a:b], kp[:, a:b])."""
+    return dequantize4_pair((q, p), None, dtype)[0]
+
+
+def dequantize4_pair(k, v, dtype):
+    """(dequantize4(*k, dtype), dequantize4(*v, dtype)) in one launch; k and v hold the same number of rows."""
+    if dtype not in _KINDS:
+        raise ValueError("dequantize4: bf16, fp16 or fp32 output")
+    _one_device("dequantize4", *k, *(v or ()))
+    h, t, d, skq, skp = _packed("dequantize4", *k)
+    svq = svp = 0
+    if v is not None:
+        hv, tv, dv, svq, svp = _packed("dequantize4", *v)
+        if (hv, tv, dv) != (h, t, d):
+            raise ValueError("dequantize4: K and V must hold the same rows")
+    outk = torch.empty(*k[0].shape[:-1], d, dtype=dtype, device=k[0].device)
+    outv = None if v is None else torch.empty(*v[0].shape[:-1], d, dtype=dtype, device=k[0].device)
+    if outk.numel() == 0:
+        return outk, outv
+    with _on(outk):
+        _lib.check(_lib.lib().bb_int4_dequantize(
+            _lib.ptr(k[0]), _lib.ptr(k[1]), None if v is None else _lib.ptr(v[0]), None if v is None else _lib.ptr(v[1]),
+            _lib.i64s(skq, skp, svq, svp), h, t, d, _lib.ptr(outk), _lib.ptr(outv), _KINDS[dtype],
+            _lib.stream_of(outk)))
+    return outk, outv
+
+
+def _rows16(x):
+    """x [a, b, d] with a contiguous head_dim and 16-byte aligned rows (a copy where it is not)."""
+    s = x.stride()
+    return x if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and x.data_ptr() % 16 == 0 else x.contiguous()
+
+
+def _decode(q, k4, kp, v4, vp, knew, vnew, n, scale, causal):
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("decode_int4: bf16 or fp16 query")
+    one = q.ndim == 2
+    if one:
+        q = q[None]
+    if q.ndim != 3 or k4.ndim != 3 or v4.ndim != 3:
+        raise ValueError("decode_int4: q [H, d] or [T, H, d] and caches [Hkv, capacity, ...]")
+    length = n if isinstance(n, torch.Tensor) else None
+    _one_device("decode_int4", q, k4, kp, v4, vp, knew, vnew, length)
+    hk, cap, d, skq, skp = _packed("decode_int4", k4, kp)
+    hv, capv, dv, svq, svp = _packed("decode_int4", v4, vp)
+    t, h, _ = q.shape
+    if (hv, capv, dv) != (hk, cap, d) or q.shape[2] != d or h % hk or not h:
+        raise ValueError("q [T,H,D] and the cache's Hkv heads must match")
+    if length is not None and (length.dtype != torch.int64 or length.numel() != 1):
+        raise ValueError("n must be an int64 tensor of one element (it is read in place by the kernels)")
+    q = _rows16(q)
+    new = (None,) * 4
+    if knew is not None:
+        if one and knew.ndim == 2:
+            knew, vnew = knew[:, None], vnew[:, None]
+        if knew.dtype != q.dtype or vnew.dtype != q.dtype or knew.shape != (hk, t, d) or vnew.shape != (hk, t, d):
+            raise ValueError("decode_int4_append: new rows must be [Hkv, T, d] (or [Hkv, d] for one token) of q's dtype")
+        knew, vnew = _rows16(knew), _rows16(vnew)
+        new = (_lib.ptr(knew), _lib.i64s(*knew.stride()[:2]), _lib.ptr(vnew), _lib.i64s(*vnew.stride()[:2]))
+    out = torch.empty(t, h, d, dtype=q.dtype, device=q.device)
+    L = _lib.lib()
+    rows = 0 if length is not None else int(n)
+    ws_bytes = L.bb_int4_decode_workspace(cap if length is not None else rows, t, h, hk, d)
+    ws = _lib.workspace(ws_bytes, q.device)
+    cache = (_lib.ptr(k4), _lib.ptr(kp), _lib.ptr(v4), _lib.ptr(vp), _lib.i64s(skq, skp, svq, svp))
+    rest = (rows, _lib.ptr(length), cap, t, h, hk, d, int(q.dtype == torch.float16), float(scale), int(bool(causal)),
+            _lib.ptr(out), _lib.i64s(h * d, d), _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
+    with _on(q):
+        if knew is None:
+            _lib.check(L.bb_int4_decode(_lib.ptr(q), _lib.i64s(*q.stride()[:2]), *cache, *rest))
+        else:
+            _lib.check(L.bb_int4_decode_append(_lib.ptr(q), _lib.i64s(*q.stride()[:2]), *cache, *new, *rest))
+    return out[0] if one else out
+
+
+def decode_int4(q, k4, kp, v4, vp, n, scale, causal=False):
+    """Exact attention of q [H, d] (one token) or [T, H, d] (the last T tokens, at most 16), bf16 or fp16, over the first
+    n rows of a 4-bit cache: codes k4 / v4 [Hkv, capacity, d / 2], params kp / vp [Hkv, capacity, d / 32, 2].
+
+    Every token attends all n rows (as RDAttention's cached steps do), or with `causal` token t the first n - T + 1 + t.
+    `n`: int, or an int64 GPU tensor of one element that the kernels read (clamped to 0 .. capacity), so that a captured
+    graph stays valid while the cache grows; a token that attends no row gives zeros. Returns q's shape and dtype."""
+    return _decode(q, k4, kp, v4, vp, None, None, n, scale, causal)
+
+
+def decode_int4_append(q, k4, kp, v4, vp, knew, vnew, n, scale, causal=False):
+    """One decode step: the new K / V rows knew / vnew [Hkv, T, d] ([Hkv, d] for one token; q's dtype, any strides) are
+    quantised into cache rows n - T .. n - 1 (as quantize4_pair would), and q attends as in decode_int4; n counts the
+    new rows. Rows that a device-side n puts outside the cache are not written."""
+    if knew is None or vnew is None:
+        raise ValueError("decode_int4_append: knew and vnew required")
+    return _decode(q, k4, kp, v4, vp, knew, vnew, n, scale, causal)
+
+
+class Int4Handle:
+    """Stands in for the K / V tensors of a decode step over an Int4KVLayer; RDAttention.exact_attention calls `attend`
+    (the protocol of the reference's compressed-cache handle, modal_rd/turbo_kv.py:129-141)."""
+
+    def __init__(self, layer, shape):
+        self.turbo, self.shape = layer, shape
+
+    def attend(self, q, scale):
+        """q [1, H, t, d] -> [1, H, t, d] attention of every query over the layer's whole cache. The step's new rows, when
+        the layer still holds them, are quantised by the same call (decode_int4_append)."""
+        layer = self.turbo
+        cache = (*layer.store_k.packed(), *layer.store_v.packed())
+        rows = q[0].transpose(0, 1)
+        pending = layer._pending
+        if pending is not None and pending[0].shape[1] == rows.shape[0] and pending[2] == layer.n - rows.shape[0]:
+            out = decode_int4_append(rows, *cache, pending[0], pending[1], layer.n, scale)
+            layer._pending = None
+        else:
+            layer._flush()
+            out = decode_int4(rows, *cache, layer.n, scale)
+        return out.transpose(0, 1)[None]
+
+
+class _Int4Rows:
+    """One cached tensor (K or V): codes [Hkv, capacity, d / 2] and params [Hkv, capacity, d / 32, 2]; rows [0, n) are
+    valid (n is kept by the owning layer). Capacity comes in GROW-row steps past what is needed."""
+
+    def __init__(self, hkv, d, rows, device):
+        if d not in _HEAD_DIMS:
+            raise ValueError("quantize4: rows [..., t, d] with d 32, 64, 128 or 256")
+        self.q, self.p = _new_packed((hkv, rows + GROW), d, device)
+
+    @property
+    def capacity(self):
+        return self.q.shape[1]
+
+    def packed(self):
+        return self.q, self.p
+
+    def ensure(self, n, need):
+        """Make room for rows [n, need), keeping rows [0, n)."""
+        if need <= self.capacity:
+            return
+        old_q, old_p = self.q, self.p
+        self.q = old_q.new_empty(old_q.shape[0], need + GROW, old_q.shape[2])
+        self.p = old_p.new_empty(old_p.shape[0], need + GROW, *old_p.shape[2:])
+        self.q[:, :n].copy_(old_q[:, :n])
+        self.p[:, :n].copy_(old_p[:, :n])
+
+    def rows(self, a, b):
+        return self.q[:, a:b], self.p[:, a:b]
+
+    def dequantized(self, n, dtype):
+        """[1, Hkv, n, d] in `dtype`."""
+        return dequantize4(*self.rows(0, n), dtype)[None]
+
+    def nbytes(self, n):
+        return n * self.q.shape[0] * (self.q.shape[2] + 2 * self.p[0, 0].numel())
+
+
+class Int4KVLayer(Int8KVLayer):
+    """HF cache layer with 4-bit K/V storage, batch size 1; the protocol of Int8KVLayer:
+
+    * prefill (the first update): the K/V are quantised into fresh row stores and the full-precision inputs are returned;
+    * later updates quantise the new rows (K and V in one launch) into spare capacity and return the dequantised cache,
+      or, for a step of at most `attend_tokens` tokens whose consumer opts in (cache kwargs {"bb_attend": True}) on a
+      bf16 or fp16 model with head_dim 64 or 128, Int4Handle stand-ins for decode_int4;
+    * assigning `keys` / `values` (kv_evict compacting the cache) re-quantises the given rows;
+    * `crop(-r)` drops the last r rows.
+    """
+
+    attend_tokens = MAX_TOKENS
+
+    def _flush(self):
+        """Quantise a step's rows still held for the fused decode (the handle was not attended)."""
+        if self._pending is not None:
+            kr, vr, row = self._pending
+            self._pending = None
+            self._write(kr, vr, row)
+
+    def _write(self, kr, vr, row):
+        end = row + kr.shape[1]
+        quantize4_pair(kr, vr, self.store_k.rows(row, end), self.store_v.rows(row, end))
+
+    @staticmethod
+    def _heads(x):
+        """[1, Hkv, t, d] -> [Hkv, t, d]."""
+        if x.ndim != 4 or x.shape[0] != 1:
+            raise NotImplementedError("Int4KVLayer is batch-size-1 only")
+        return x[0]
+
+    def _fill(self, x):
+        rows = self._heads(x)
+        h, t, d = rows.shape
+        store = _Int4Rows(h, d, t, x.device)
+        quantize4(rows, store.rows(0, t))
+        return store
+
+    def update(self, key_states, value_states, cache_kwargs=None, *args, **kwargs):
+        if not self.is_initialized:
+            self.lazy_initialization(key_states, value_states)
+        self._flush()
+        kr, vr = self._heads(key_states), self._heads(value_states)
+        h, t, d = kr.shape
+        if self.store_k is None:
+            sk, sv = _Int4Rows(h, d, t, kr.device), _Int4Rows(h, d, t, kr.device)
+            quantize4_pair(kr, vr, sk.rows(0, t), sv.rows(0, t))
+            self.store_k, self.store_v, self.n = sk, sv, t  # only now: rows that are refused leave the layer empty
+            return key_states, value_states
+        start, end = self.n, self.n + t
+        self.store_k.ensure(start, end)
+        self.store_v.ensure(start, end)
+        wants_handle = isinstance(cache_kwargs, dict) and cache_kwargs.get("bb_attend", False)
+        if (self.fused and wants_handle and 1 <= t <= self.attend_tokens and d in (64, 128)
+                and kr.dtype in (torch.bfloat16, torch.float16) and vr.dtype == kr.dtype and vr.shape == kr.shape):
+            # quantised when the handle is attended (or by _flush before any other use of the cache)
+            self._pending, self.n = (kr, vr, start), end
+            handle = Int4Handle(self, (1, h, end, d))
+            return handle, handle
+        self._write(kr, vr, start)
+        self.n = end
+        k, v = dequantize4_pair(self.store_k.rows(0, end), self.store_v.rows(0, end), self.dtype)
+        return k[None], v[None]
+
+    def batch_repeat_interleave(self, repeats):
+        raise NotImplementedError("Int4KVLayer is batch-size-1 only")
+
+    def batch_select_indices(self, indices):
+        raise NotImplementedError("Int4KVLayer is batch-size-1 only")
+
+
+def make_int4_cache(config, fused=True):
+    """A DynamicCache whose layers are Int4KVLayer. `fused=False` never hands out decode handles, even to consumers that
+    ask for them."""
+    cache = DynamicCache(config=config)
+    layers = []
+    for _ in range(config.get_text_config(decoder=True).num_hidden_layers):
+        layer = Int4KVLayer()
+        layer.fused = fused
+        layers.append(layer)
+    cache.layers = layers
+    return cache

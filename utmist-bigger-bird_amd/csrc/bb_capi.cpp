@@ -899,6 +899,147 @@ int bb_argmax(const void* x, int64_t n, int dtype, int64_t* out, void* stream) {
                                       static_cast<hipStream_t>(stream)), "bb_argmax");
 }
 
+// The checks that every entry point on a 4-bit cache shares; vq = null: one tensor.
+static int int4_cache_check(const char* what, const void* kq, const void* kp, const void* vq, const void* vp,
+                            const int64_t* sc) {
+  if (!kq || !kp || !sc || (vq != nullptr) != (vp != nullptr)) return fail("%s: null argument", what);
+  if (!aligned(kq, 16) || !aligned(kp, 4) || sc[0] % 16 || sc[1] % 2 ||
+      (vq && (!aligned(vq, 16) || !aligned(vp, 4) || sc[2] % 16 || sc[3] % 2)))
+    return fail("%s: codes must be 16-byte and params 4-byte aligned in every head", what);
+  return BB_OK;
+}
+
+static int int4_rows_check(const char* what, int heads, int64_t rows, int D, int kind) {
+  if (D != 32 && D != 64 && D != 128 && D != 256) return fail("%s: head_dim %d unsupported", what, D);
+  if (kind < 0 || kind > 2) return fail("%s: element kind %d unsupported (0 bf16, 1 fp32, 2 fp16)", what, kind);
+  if (heads < 0 || heads > 65535 || rows < 0 || rows > (int64_t)0xffffff00 / (D / 8))
+    return fail("%s: %d heads of %lld rows out of range", what, heads, (long long)rows);
+  return BB_OK;
+}
+
+int bb_int4_quantize(const void* xk, const int64_t* sxk, const void* xv, const int64_t* sxv, int x_kind, int heads,
+                     int64_t rows, int D, uint8_t* kq, void* kp, uint8_t* vq, void* vp, const int64_t* sc,
+                     void* stream) {
+  g_err[0] = 0;
+  if (!xk || !sxk || (xv && !sxv) || (xv != nullptr) != (vq != nullptr)) return fail("quantize4: null argument");
+  int rc = int4_cache_check("quantize4", kq, kp, vq, vp, sc);
+  if (rc == BB_OK) rc = int4_rows_check("quantize4", heads, rows, D, x_kind);
+  if (rc != BB_OK) return rc;
+  const int64_t el = x_kind == 1 ? 4 : 2;
+  if (!aligned(xk, 16) || (sxk[0] * el) % 16 || (sxk[1] * el) % 16 ||
+      (xv && (!aligned(xv, 16) || (sxv[0] * el) % 16 || (sxv[1] * el) % 16)))
+    return fail("quantize4: rows must be 16-byte aligned");
+  const bb::Int4Rows k{xk, kq, static_cast<uint32_t*>(kp), sxk[0], sxk[1], sc[0], sc[1] / 2};
+  bb::Int4Rows v = {};
+  if (xv) v = bb::Int4Rows{xv, vq, static_cast<uint32_t*>(vp), sxv[0], sxv[1], sc[2], sc[3] / 2};
+  return hip_status(bb::launch_int4_quantize(k, xv ? &v : nullptr, x_kind, heads, rows, D,
+                                             static_cast<hipStream_t>(stream)),
+                    "bb_int4_quantize");
+}
+
+int bb_int4_dequantize(const uint8_t* kq, const void* kp, const uint8_t* vq, const void* vp, const int64_t* sc, int heads,
+                       int64_t rows, int D, void* outk, void* outv, int out_kind, void* stream) {
+  g_err[0] = 0;
+  if (!outk || (outv != nullptr) != (vq != nullptr)) return fail("dequantize4: null argument");
+  int rc = int4_cache_check("dequantize4", kq, kp, vq, vp, sc);
+  if (rc == BB_OK) rc = int4_rows_check("dequantize4", heads, rows, D, out_kind);
+  if (rc != BB_OK) return rc;
+  if (!aligned(outk, 16) || !aligned(outv, 16)) return fail("dequantize4: outputs must be 16-byte aligned");
+  auto cache = [](const uint8_t* q, const void* pp, void* out, int64_t s0, int64_t s1) {
+    return bb::Int4Rows{out, const_cast<uint8_t*>(q), static_cast<uint32_t*>(const_cast<void*>(pp)), 0, 0, s0, s1 / 2};
+  };
+  const bb::Int4Rows k = cache(kq, kp, outk, sc[0], sc[1]);
+  bb::Int4Rows v = {};
+  if (vq) v = cache(vq, vp, outv, sc[2], sc[3]);
+  return hip_status(bb::launch_int4_dequantize(k, vq ? &v : nullptr, out_kind, heads, rows, D,
+                                               static_cast<hipStream_t>(stream)),
+                    "bb_int4_dequantize");
+}
+
+// Splits of the 4-bit decode: two workgroups per CU over all KV heads, of kInt4MinSplit keys at least (the kernels cut
+// the live length into this many equal parts, so that with a device-side length the splits follow it).
+static int int4_splits(int64_t n, int Hkv) {
+  const int64_t s = std::min(cdiv(n, bb::kInt4MinSplit), cdiv(2 * kCUs, Hkv));
+  return (int)std::max<int64_t>(1, s);
+}
+
+size_t bb_int4_decode_workspace(int64_t n, int T, int H, int Hkv, int D) {
+  if (n <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || D <= 0) return 0;
+  return (size_t)T * H * int4_splits(n, Hkv) * (D + 2) * sizeof(float);
+}
+
+// bb_int4_decode, and with new rows bb_int4_decode_append.
+static int int4_decode_impl(const void* q, const int64_t* sq, uint8_t* kq, void* kp, uint8_t* vq, void* vp,
+                            const int64_t* sc, const void* knew, const int64_t* sknew, const void* vnew,
+                            const int64_t* svnew, int64_t n, const int64_t* n_dev, int64_t cap, int T, int H, int Hkv,
+                            int D, int is_f16, float scale, int causal, void* out, const int64_t* so, void* ws,
+                            size_t ws_bytes, void* stream) {
+  if (!q || !sq || !out || !so || !vq) return fail("decode_int4: null argument");
+  const int rc = int4_cache_check("decode_int4", kq, kp, vq, vp, sc);
+  if (rc != BB_OK) return rc;
+  if (H <= 0 || Hkv <= 0 || H % Hkv || Hkv > 65535) return fail("q [T,H,D] and the cache's Hkv heads must match");
+  if (D != 64 && D != 128) return fail("decode_int4: head_dim %d unsupported (64 or 128)", D);
+  if (T < 1 || T > 16) return fail("decode_int4: %d query tokens unsupported (1 to 16)", T);
+  if (cap <= 0 || (!n_dev && n <= 0)) return fail("decode_int4: empty cache");
+  if (!n_dev && n > cap) return fail("decode_int4: %lld rows are past the cache capacity of %lld", (long long)n, (long long)cap);
+  if (!n_dev && n < T) return fail("Key sequence must be at least as long as query sequence");
+  if (!(scale > 0.0f)) return fail("scale must be positive");
+  if (!aligned(q, 16) || sq[0] % 8 || sq[1] % 8)
+    return fail("decode_int4: q needs a contiguous head_dim and 16-byte aligned rows");
+  if (!aligned(out, 16) || so[0] % 8 || so[1] % 8)
+    return fail("decode_int4: out needs a contiguous head_dim and 16-byte aligned rows");
+  if (knew && (!aligned(knew, 16) || !aligned(vnew, 16) || sknew[0] % 8 || sknew[1] % 8 || svnew[0] % 8 || svnew[1] % 8))
+    return fail("decode_int4: new rows need a contiguous head_dim and 16-byte aligned rows");
+  const int64_t most = n_dev ? cap : n;
+  const size_t need = bb_int4_decode_workspace(most, T, H, Hkv, D);
+  if (!ws || ws_bytes < need || !aligned(ws, 16)) return fail("workspace of %zu bytes required", need);
+  bb::Int4DecodeParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = static_cast<const uint16_t*>(q);
+  p.kq = kq; p.kp = static_cast<uint32_t*>(kp);
+  p.vq = vq; p.vp = static_cast<uint32_t*>(vp);
+  p.skq = sc[0]; p.skp = sc[1] / 2; p.svq = sc[2]; p.svp = sc[3] / 2;
+  p.sq0 = sq[0]; p.sq1 = sq[1];
+  p.so0 = so[0]; p.so1 = so[1];
+  if (knew) {
+    p.knew = static_cast<const uint16_t*>(knew);
+    p.vnew = static_cast<const uint16_t*>(vnew);
+    p.skn0 = sknew[0]; p.skn1 = sknew[1];
+    p.svn0 = svnew[0]; p.svn1 = svnew[1];
+  }
+  p.out = static_cast<uint16_t*>(out);
+  p.part = static_cast<float*>(ws);
+  p.n_dev = n_dev;
+  p.n = n; p.cap = cap;
+  p.T = T; p.H = H; p.Hkv = Hkv; p.D = D;
+  p.f16 = is_f16 ? 1 : 0;
+  p.causal = causal ? 1 : 0;
+  p.n_splits = int4_splits(most, Hkv);
+  p.c = (float)((double)scale * 1.4426950408889634);
+  return hip_status(bb::launch_int4_decode(p, static_cast<hipStream_t>(stream)), "bb_int4_decode");
+}
+
+int bb_int4_decode(const void* q, const int64_t* sq, const uint8_t* kq, const void* kp, const uint8_t* vq, const void* vp,
+                   const int64_t* sc, int64_t n, const int64_t* n_dev, int64_t cap, int T, int H, int Hkv, int D,
+                   int is_f16, float scale, int causal, void* out, const int64_t* so, void* ws, size_t ws_bytes,
+                   void* stream) {
+  g_err[0] = 0;
+  return int4_decode_impl(q, sq, const_cast<uint8_t*>(kq), const_cast<void*>(kp), const_cast<uint8_t*>(vq),
+                          const_cast<void*>(vp), sc, nullptr, nullptr, nullptr, nullptr, n, n_dev, cap, T, H, Hkv, D,
+                          is_f16, scale, causal, out, so, ws, ws_bytes, stream);
+}
+
+int bb_int4_decode_append(const void* q, const int64_t* sq, uint8_t* kq, void* kp, uint8_t* vq, void* vp,
+                          const int64_t* sc, const void* knew, const int64_t* sknew, const void* vnew,
+                          const int64_t* svnew, int64_t n, const int64_t* n_dev, int64_t cap, int T, int H, int Hkv,
+                          int D, int is_f16, float scale, int causal, void* out, const int64_t* so, void* ws,
+                          size_t ws_bytes, void* stream) {
+  g_err[0] = 0;
+  if (!knew || !vnew || !sknew || !svnew) return fail("decode_int4_append: null argument");
+  return int4_decode_impl(q, sq, kq, kp, vq, vp, sc, knew, sknew, vnew, svnew, n, n_dev, cap, T, H, Hkv, D, is_f16,
+                          scale, causal, out, so, ws, ws_bytes, stream);
+}
+
 int bb_stream_read(const void* buf, size_t bytes, uint32_t* sink, int workgroups, void* stream) {
   g_err[0] = 0;
   if (!buf || !sink) return fail("stream_read: null argument");

@@ -105,6 +105,36 @@ size_t decode_workspace_bytes(int H, int D, int n_splits);
 bool decode_fuses_append(const DecodeParams& p);
 hipError_t launch_decode(const DecodeParams& p, hipStream_t stream);
 
+// 4-bit KV cache (bb_int4.hip). One tensor's rows and its place in the cache; on the read back x is the output.
+struct Int4Rows {
+  const void* x;     // [heads, rows, D] (strides sx0 head, sx1 row, in elements); read back: contiguous
+  uint8_t* q;        // [heads, rows, D / 2] (head stride sq0 bytes)
+  uint32_t* p;       // [heads, rows, D / 32] of (s, z) fp16 pairs (head stride sp0)
+  int64_t sx0, sx1, sq0, sp0;
+};
+hipError_t launch_int4_quantize(const Int4Rows& k, const Int4Rows* v, int kind, int heads, int64_t rows, int D,
+                                hipStream_t stream);
+hipError_t launch_int4_dequantize(const Int4Rows& k, const Int4Rows* v, int kind, int heads, int64_t rows, int D,
+                                  hipStream_t stream);
+struct Int4DecodeParams {
+  const uint16_t* q;     // [T, H, D] (strides sq0 token, sq1 head)
+  uint8_t* kq;           // [Hkv, cap, D / 2] (head stride skq bytes)
+  uint32_t* kp;          // [Hkv, cap, D / 32] (head stride skp groups)
+  uint8_t* vq;
+  uint32_t* vp;
+  const uint16_t* knew;  // [Hkv, T, D] (strides skn0 head, skn1 token): the rows n - T .. n - 1 to append, or null
+  const uint16_t* vnew;
+  uint16_t* out;         // [T, H, D] (strides so0, so1)
+  float* part;           // [T, H][n_splits][D + 2]
+  const int64_t* n_dev;  // length in device memory, or null (then n)
+  int64_t n, cap;
+  int64_t sq0, sq1, skq, skp, svq, svp, skn0, skn1, svn0, svn1, so0, so1;
+  int T, H, Hkv, D, f16, causal, n_splits;
+  float c;               // scale * log2(e)
+};
+constexpr int64_t kInt4MinSplit = 256;  // keys of a split, at least
+hipError_t launch_int4_decode(const Int4DecodeParams& p, hipStream_t stream);
+
 // A decode step's new K / V row folded into the first kernel that reads the cache: the row at position n - 1 (n the
 // current length, which already counts it) is read from knew / vnew instead of the cache, and the lanes that read it
 // also write it to the cache rows (k, v), so that later kernels find it there. Only when 1 <= n <= cap; knew = null
