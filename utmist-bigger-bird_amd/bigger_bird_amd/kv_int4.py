@@ -9,7 +9,7 @@ s = 0); the value is s * code + z in fp32. Byte b of a packed row holds element 
 is codes [Hkv, capacity, d / 2] uint8 and params [Hkv, capacity, d / 32, 2] fp16 (s, z), head-major, for K and for V:
 80 bytes a row at head_dim 128, against 130 in int8 and 256 in bf16.
 """
-import contextlib
+import functools
 
 import torch
 from transformers import DynamicCache
@@ -19,21 +19,28 @@ from .kv_int8 import _KINDS, GROW, Int8KVLayer
 
 MAX_TOKENS = 16  # query tokens of one decode call
 _HEAD_DIMS = (32, 64, 128, 256)
+_HALVES = (16, 32, 64, 128)  # their packed rows' bytes
 
 
-def _on(t):
-    """The device of t made current for a launch (nothing when it is already)."""
-    if t.get_device() == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _launch_on(device, fn, *args):
+    """fn(*args) with `device` (an index) current, checked (a launch goes to the current device's context)."""
+    if device == torch.cuda.current_device():
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args)
+    if rc:
+        _lib.check(rc)
 
 
 def _one_device(what, *tensors):
-    """Every tensor on one ROCm device (the kernels run on the stream of the first)."""
-    _lib.require_gpu(*tensors, what=what)
-    first = tensors[0].get_device()
-    if any(t is not None and t.get_device() != first for t in tensors):
-        raise ValueError(f"{what}: tensors on different devices")
+    """The index of the one ROCm device that holds every tensor (the kernels run on the current stream there)."""
+    device = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != device or device < 0):
+            _lib.require_gpu(*tensors, what=what)
+            raise ValueError(f"{what}: tensors on different devices")
+    return device
 
 
 def _input_rows(x):
@@ -48,24 +55,34 @@ def _input_rows(x):
 def _packed(what, q, p):
     """(heads, rows, head_dim, head stride of q in bytes, head stride of p in elements) of packed rows: q [..., t, d / 2]
     and p [..., t, d / 32, 2], the rows of a head back to back, one stride between heads."""
-    if q.dtype != torch.uint8 or p.dtype != torch.float16:
+    if q.dtype is not torch.uint8 or p.dtype is not torch.float16:
         raise ValueError(f"{what}: codes must be uint8 and params float16")
-    if q.ndim < 2 or p.ndim != q.ndim + 1 or p.shape[:-2] != q.shape[:-1]:
-        raise ValueError(f"{what}: codes [..., t, d / 2] and params [..., t, d / 32, 2] must match")
     if q.ndim != 3:
+        if q.ndim < 2 or p.ndim != q.ndim + 1 or p.shape[:-2] != q.shape[:-1]:
+            raise ValueError(f"{what}: codes [..., t, d / 2] and params [..., t, d / 32, 2] must match")
         try:
             q = q.view(-1, *q.shape[-2:]) if q.ndim > 3 else q[None]
             p = p.view(-1, *p.shape[-3:]) if p.ndim > 4 else p[None]
         except RuntimeError:
             raise ValueError(f"{what}: packed rows need one stride between heads") from None
     h, t, half = q.shape
-    if 2 * half not in _HEAD_DIMS or p.shape[2:] != (half // 16, 2):
+    if half not in _HALVES or p.shape != (h, t, half // 16, 2):
         raise ValueError(f"{what}: codes [..., t, d / 2] and params [..., t, d / 32, 2] must match (d 32, 64, 128 or 256)")
-    sq, sp = q.stride(), p.stride()
-    if (sq[2] != 1 or sp[3] != 1 or (sp[2] != 2 and half > 16) or t > 1 and (sq[1] != half or sp[1] != half // 8)
-            or h > 1 and (sq[0] < t * half or sp[0] < t * (half // 8))):
+    q0, q1, q2 = q.stride()
+    p0, p1, p2, p3 = p.stride()
+    if (q2 != 1 or p3 != 1 or (p2 != 2 and half > 16) or (t > 1 and (q1 != half or p1 != half // 8))
+            or (h > 1 and (q0 < t * half or p0 < t * (half // 8)))):
         raise ValueError(f"{what}: the packed rows of a head must be contiguous and heads must not overlap")
-    return h, t, 2 * half, sq[0] if h > 1 else 0, sp[0] if h > 1 else 0
+    return (h, t, 2 * half, q0, p0) if h > 1 else (h, t, 2 * half, 0, 0)
+
+
+def _packed_pair(what, kq, kp, vq, vp):
+    """_packed of K, and of V (the same tuple where V is laid out as K is)."""
+    k = _packed(what, kq, kp)
+    if (vq.shape == kq.shape and vp.shape == kp.shape and vq.stride() == kq.stride() and vp.stride() == kp.stride()
+            and vq.dtype is torch.uint8 and vp.dtype is torch.float16):
+        return k, k
+    return k, _packed(what, vq, vp)
 
 
 def _new_packed(rows, d, device):
@@ -81,9 +98,8 @@ def _check_input(x):
         raise ValueError("quantize4: rows [..., t, d] with d 32, 64, 128 or 256")
 
 
-def _check_out(x, out):
-    shape = _packed("quantize4", *out)[:3]
-    if out[0].shape[:-1] != x.shape[:-1] or shape[2] != x.shape[-1]:
+def _check_out(x, out, layout):
+    if out[0].shape[:-1] != x.shape[:-1] or layout[2] != x.shape[-1]:
         raise ValueError("quantize4: out tensors must match x")
 
 
@@ -91,67 +107,77 @@ def quantize4(x, out=None):
     """[..., t, d] (bf16, fp16 or fp32, any strides) -> codes [..., t, d / 2] uint8, params [..., t, d / 32, 2] fp16.
 
     `out` = (codes, params) to write into, e.g. the rows [a, b) of a cache: (k4[:, a:b], kp[:, a:b])."""
-    return quantize4_pair(x, None, out, None)[0]
+    _check_input(x)
+    device = _one_device("quantize4", x, *(out or ()))
+    if out is None:
+        out = _new_packed(x.shape[:-1], x.shape[-1], x.device)
+    layout = _packed("quantize4", *out)
+    _check_out(x, out, layout)
+    if x.numel():
+        _write(device, x, None, out, (None, None), layout, (0,) * 5)
+    return out
 
 
 def quantize4_pair(xk, xv, out_k=None, out_v=None):
     """quantize4(xk, out_k) and quantize4(xv, out_v) in one launch (a prompt's or a step's new K and V rows: one shape and
     dtype). Returns ((codes, params) of K, (codes, params) of V)."""
     _check_input(xk)
-    _one_device("quantize4", xk, xv, *(out_k or ()), *(out_v or ()))
-    if xv is not None and (xv.shape != xk.shape or xv.dtype != xk.dtype):
+    device = _one_device("quantize4", xk, xv, *(out_k or ()), *(out_v or ()))
+    if xv.shape != xk.shape or xv.dtype != xk.dtype:
         raise ValueError("quantize4: K and V rows must share a shape and dtype")
     if out_k is None:
         out_k = _new_packed(xk.shape[:-1], xk.shape[-1], xk.device)
-    else:
-        _check_out(xk, out_k)
-    if xv is not None:
-        if out_v is None:
-            out_v = _new_packed(xv.shape[:-1], xv.shape[-1], xv.device)
-        else:
-            _check_out(xv, out_v)
-    if xk.numel() == 0:
-        return out_k, out_v
-    a, b = _input_rows(xk), None if xv is None else _input_rows(xv)
-    _, _, d, skq, skp = _packed("quantize4", *out_k)
-    svq = svp = 0
-    if xv is not None:
-        _, _, _, svq, svp = _packed("quantize4", *out_v)
-    with _on(xk):
-        _lib.check(_lib.lib().bb_int4_quantize(
-            _lib.ptr(a), _lib.i64s(*a.stride()[:2]), _lib.ptr(b), None if b is None else _lib.i64s(*b.stride()[:2]),
-            _KINDS[a.dtype], a.shape[0], a.shape[1], d, _lib.ptr(out_k[0]), _lib.ptr(out_k[1]),
-            None if b is None else _lib.ptr(out_v[0]), None if b is None else _lib.ptr(out_v[1]),
-            _lib.i64s(skq, skp, svq, svp), _lib.stream_of(xk)))
+    if out_v is None:
+        out_v = _new_packed(xk.shape[:-1], xk.shape[-1], xk.device)
+    k, v = _packed_pair("quantize4", *out_k, *out_v)
+    _check_out(xk, out_k, k)
+    if v is not k:
+        _check_out(xv, out_v, v)
+    if xk.numel():
+        _write(device, xk, xv, out_k, out_v, k, v)
     return out_k, out_v
+
+
+def _write(device, xk, xv, out_k, out_v, k, v):
+    """The launch of quantize4_pair (xv None: of one tensor); k and v are the layouts of the outputs."""
+    a = _input_rows(xk)
+    sa, pb, sb = a.stride(), None, None
+    if xv is not None:
+        b = _input_rows(xv)
+        pb, sb = b.data_ptr(), _lib.i64s(b.stride(0), b.stride(1))
+    _launch_on(device, _lib.lib().bb_int4_quantize, a.data_ptr(), _lib.i64s(sa[0], sa[1]), pb, sb, _KINDS[a.dtype],
+               a.shape[0], a.shape[1], k[2], out_k[0].data_ptr(), out_k[1].data_ptr(), _lib.ptr(out_v[0]),
+               _lib.ptr(out_v[1]), _lib.i64s(k[3], k[4], v[3], v[4]), _lib.stream_of(xk))
 
 
 def dequantize4(q, p, dtype):
     """codes [..., t, d / 2], params [..., t, d / 32, 2] -> [..., t, d] in dtype (bf16, fp16 or fp32; the fp32 value
     s * code + z rounded to nearest even). Rows [a, b) of a cache are read in place: (k4[:, a:b], kp[:, a:b])."""
-    return dequantize4_pair((q, p), None, dtype)[0]
+    if dtype not in _KINDS:
+        raise ValueError("dequantize4: bf16, fp16 or fp32 output")
+    device = _one_device("dequantize4", q, p)
+    k = _packed("dequantize4", q, p)
+    out = torch.empty(*q.shape[:-1], k[2], dtype=dtype, device=q.device)
+    if out.numel():
+        _launch_on(device, _lib.lib().bb_int4_dequantize, q.data_ptr(), p.data_ptr(), None, None, _lib.i64s(k[3], k[4], 0, 0),
+                   k[0], k[1], k[2], out.data_ptr(), None, _KINDS[dtype], _lib.stream_of(out))
+    return out
 
 
 def dequantize4_pair(k, v, dtype):
     """(dequantize4(*k, dtype), dequantize4(*v, dtype)) in one launch; k and v hold the same number of rows."""
     if dtype not in _KINDS:
         raise ValueError("dequantize4: bf16, fp16 or fp32 output")
-    _one_device("dequantize4", *k, *(v or ()))
-    h, t, d, skq, skp = _packed("dequantize4", *k)
-    svq = svp = 0
-    if v is not None:
-        hv, tv, dv, svq, svp = _packed("dequantize4", *v)
-        if (hv, tv, dv) != (h, t, d):
-            raise ValueError("dequantize4: K and V must hold the same rows")
-    outk = torch.empty(*k[0].shape[:-1], d, dtype=dtype, device=k[0].device)
-    outv = None if v is None else torch.empty(*v[0].shape[:-1], d, dtype=dtype, device=k[0].device)
-    if outk.numel() == 0:
-        return outk, outv
-    with _on(outk):
-        _lib.check(_lib.lib().bb_int4_dequantize(
-            _lib.ptr(k[0]), _lib.ptr(k[1]), None if v is None else _lib.ptr(v[0]), None if v is None else _lib.ptr(v[1]),
-            _lib.i64s(skq, skp, svq, svp), h, t, d, _lib.ptr(outk), _lib.ptr(outv), _KINDS[dtype],
-            _lib.stream_of(outk)))
+    device = _one_device("dequantize4", *k, *v)
+    lk, lv = _packed_pair("dequantize4", *k, *v)
+    if lv[:3] != lk[:3]:
+        raise ValueError("dequantize4: K and V must hold the same rows")
+    outk = torch.empty(*k[0].shape[:-1], lk[2], dtype=dtype, device=k[0].device)
+    outv = torch.empty(*v[0].shape[:-1], lk[2], dtype=dtype, device=k[0].device)
+    if outk.numel():
+        _launch_on(device, _lib.lib().bb_int4_dequantize, k[0].data_ptr(), k[1].data_ptr(), v[0].data_ptr(),
+                   v[1].data_ptr(), _lib.i64s(lk[3], lk[4], lv[3], lv[4]), lk[0], lk[1], lk[2], outk.data_ptr(),
+                   outv.data_ptr(), _KINDS[dtype], _lib.stream_of(outk))
     return outk, outv
 
 
@@ -161,8 +187,13 @@ def _rows16(x):
     return x if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and x.data_ptr() % 16 == 0 else x.contiguous()
 
 
+@functools.lru_cache(maxsize=64)
+def _workspace_bytes(rows, t, h, hk, d):
+    return _lib.lib().bb_int4_decode_workspace(rows, t, h, hk, d)
+
+
 def _decode(q, k4, kp, v4, vp, knew, vnew, n, scale, causal):
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
         raise ValueError("decode_int4: bf16 or fp16 query")
     one = q.ndim == 2
     if one:
@@ -170,36 +201,34 @@ def _decode(q, k4, kp, v4, vp, knew, vnew, n, scale, causal):
     if q.ndim != 3 or k4.ndim != 3 or v4.ndim != 3:
         raise ValueError("decode_int4: q [H, d] or [T, H, d] and caches [Hkv, capacity, ...]")
     length = n if isinstance(n, torch.Tensor) else None
-    _one_device("decode_int4", q, k4, kp, v4, vp, knew, vnew, length)
-    hk, cap, d, skq, skp = _packed("decode_int4", k4, kp)
-    hv, capv, dv, svq, svp = _packed("decode_int4", v4, vp)
-    t, h, _ = q.shape
-    if (hv, capv, dv) != (hk, cap, d) or q.shape[2] != d or h % hk or not h:
+    device = _one_device("decode_int4", q, k4, kp, v4, vp, knew, vnew, length)
+    k, v = _packed_pair("decode_int4", k4, kp, v4, vp)
+    hk, cap, d, skq, skp = k
+    t, h, dq = q.shape
+    if v[:3] != k[:3] or dq != d or not h or h % hk:
         raise ValueError("q [T,H,D] and the cache's Hkv heads must match")
-    if length is not None and (length.dtype != torch.int64 or length.numel() != 1):
+    if length is not None and (length.dtype is not torch.int64 or length.numel() != 1):
         raise ValueError("n must be an int64 tensor of one element (it is read in place by the kernels)")
     q = _rows16(q)
-    new = (None,) * 4
+    sq = q.stride()
+    L = _lib.lib()
+    fn, new = L.bb_int4_decode, ()
     if knew is not None:
-        if one and knew.ndim == 2:
+        if one and knew.ndim == 2 and vnew.ndim == 2:
             knew, vnew = knew[:, None], vnew[:, None]
         if knew.dtype != q.dtype or vnew.dtype != q.dtype or knew.shape != (hk, t, d) or vnew.shape != (hk, t, d):
             raise ValueError("decode_int4_append: new rows must be [Hkv, T, d] (or [Hkv, d] for one token) of q's dtype")
         knew, vnew = _rows16(knew), _rows16(vnew)
-        new = (_lib.ptr(knew), _lib.i64s(*knew.stride()[:2]), _lib.ptr(vnew), _lib.i64s(*vnew.stride()[:2]))
-    out = torch.empty(t, h, d, dtype=q.dtype, device=q.device)
-    L = _lib.lib()
-    rows = 0 if length is not None else int(n)
-    ws_bytes = L.bb_int4_decode_workspace(cap if length is not None else rows, t, h, hk, d)
-    ws = _lib.workspace(ws_bytes, q.device)
-    cache = (_lib.ptr(k4), _lib.ptr(kp), _lib.ptr(v4), _lib.ptr(vp), _lib.i64s(skq, skp, svq, svp))
-    rest = (rows, _lib.ptr(length), cap, t, h, hk, d, int(q.dtype == torch.float16), float(scale), int(bool(causal)),
-            _lib.ptr(out), _lib.i64s(h * d, d), _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
-    with _on(q):
-        if knew is None:
-            _lib.check(L.bb_int4_decode(_lib.ptr(q), _lib.i64s(*q.stride()[:2]), *cache, *rest))
-        else:
-            _lib.check(L.bb_int4_decode_append(_lib.ptr(q), _lib.i64s(*q.stride()[:2]), *cache, *new, *rest))
+        sk, sv = knew.stride(), vnew.stride()
+        fn = L.bb_int4_decode_append
+        new = (knew.data_ptr(), _lib.i64s(sk[0], sk[1]), vnew.data_ptr(), _lib.i64s(sv[0], sv[1]))
+    out = torch.empty((t, h, d), dtype=q.dtype, device=q.device)
+    ws_bytes = _workspace_bytes(cap, t, h, hk, d)  # for every length up to the capacity
+    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=q.device)
+    _launch_on(device, fn, q.data_ptr(), _lib.i64s(sq[0], sq[1]), k4.data_ptr(), kp.data_ptr(), v4.data_ptr(), vp.data_ptr(),
+               _lib.i64s(skq, skp, v[3], v[4]), *new, 0 if length is not None else int(n), _lib.ptr(length), cap, t, h, hk,
+               d, int(q.dtype is torch.float16), float(scale), int(bool(causal)), out.data_ptr(), _lib.i64s(h * d, d),
+               ws.data_ptr(), ws_bytes, _lib.stream_of(q))
     return out[0] if one else out
 
 

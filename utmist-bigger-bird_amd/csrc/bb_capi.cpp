@@ -977,7 +977,7 @@ static int int4_decode_impl(const void* q, const int64_t* sq, uint8_t* kq, void*
   if (!q || !sq || !out || !so || !vq) return fail("decode_int4: null argument");
   const int rc = int4_cache_check("decode_int4", kq, kp, vq, vp, sc);
   if (rc != BB_OK) return rc;
-  if (H <= 0 || Hkv <= 0 || H % Hkv || Hkv > 65535) return fail("q [T,H,D] and the cache's Hkv heads must match");
+  if (H <= 0 || Hkv <= 0 || H % Hkv || H > 65535) return fail("q [T,H,D] and the cache's Hkv heads must match");
   if (D != 64 && D != 128) return fail("decode_int4: head_dim %d unsupported (64 or 128)", D);
   if (T < 1 || T > 16) return fail("decode_int4: %d query tokens unsupported (1 to 16)", T);
   if (cap <= 0 || (!n_dev && n <= 0)) return fail("decode_int4: empty cache");
@@ -1015,6 +1015,10 @@ static int int4_decode_impl(const void* q, const int64_t* sq, uint8_t* kq, void*
   p.f16 = is_f16 ? 1 : 0;
   p.causal = causal ? 1 : 0;
   p.n_splits = int4_splits(most, Hkv);
+  p.G = H / Hkv;
+  p.inv_G = 1.0f / (float)p.G;
+  p.inv_splits = 1.0 / p.n_splits;
+  if (!n_dev) p.len = std::max(bb::kInt4MinSplit, cdiv(cdiv(n, p.n_splits), 16) * 16);
   p.c = (float)((double)scale * 1.4426950408889634);
   return hip_status(bb::launch_int4_decode(p, static_cast<hipStream_t>(stream)), "bb_int4_decode");
 }

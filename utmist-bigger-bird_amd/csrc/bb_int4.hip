@@ -128,27 +128,19 @@ __global__ __launch_bounds__(256) void int4_dequantize_kernel(Int4ReadSet s0, In
 
 // ---------------------------------------------------------------------------------------------------------------
 // Attention over the packed rows, split over the keys. Workgroup (split, KV head, pass): 4 waves against the split's keys,
-// wave w taking chunks w, w + 4, ... of 64 keys (128 at head_dim 64); a pass takes up to 16 query vectors (T tokens x G
-// heads of the KV head, token-major) in blocks of 4. The length may come from device memory; every launch shape depends on
-// host values alone.
+// wave w taking chunks w, w + 4, ... of 64 keys (128 at head_dim 64). The query vectors of a KV head are its T tokens x G
+// heads, token-major: up to 4 go to int4_decode_kernel, more to int4_decode_wide_kernel in passes of 16. The length may come
+// from device memory; every launch shape depends on host values alone.
 //
 // Mathematics. With k = s c + z per group of 32 (c the codes), q.k = sum_g s_g (q_g . c_g) + z_g sum(q_g), and
 // o = sum_j p_j s_j c_j + sum_j p_j z_j per column group: the codes go to the matrix cores as they are, exact in 16 bits, and
 // scales and minima are applied in fp32 to the sums (scores) or to the probabilities (values). A code becomes the 16-bit
 // float 16 + c by one shift and one and-or per two codes; the 16s are taken back from the sums.
 //
-//   scores  Lane (k, a) of 16 x 4 holds the 16 bytes of group a of key k (head_dim 64: group a & 1 of the key in half
-//           a >> 1). The query operand is block-diagonal: row 4 a + h holds group a of query h where the lane's quarter is
-//           a and zero elsewhere, so the four 16x16x32 products of a 1 KB piece leave in lane (k, a) the four queries' sums
-//           over its own group. One (s, z) word per lane turns them into scores; three lane swaps sum the groups and
-//           leave lane (k, a) with the whole score of query a alone, so that no lane's exponential is idle.
-//   values  V rows are transposed by ds_read_b64_tr_b4 (a lane gets 16 keys of one column). The probabilities times the
-//           scales of column group t go to column 4 t + h of the other operand, so one product serves all groups (the
-//           columns of a product whose rows are another group are not used). The 16s go with a row of ones.
-//
 // A chunk's 10 KB (codes and params of K and of V) stream straight into the wave's LDS with ten buffer loads that cover
-// whole lines, one chunk ahead. Pieces land so that the operand reads meet no bank twice: see the offsets at each.
-constexpr int kVecs = 16;            // query vectors of a pass
+// whole lines, two chunks ahead. Pieces land so that the operand reads meet no bank twice: see the offsets at each. V rows
+// are transposed on the way to the matrix cores by ds_read_b64_tr_b4 (a lane gets 16 keys of one column).
+constexpr int kVecs = 16;            // query vectors of a pass of the wide kernel
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kStage = 10240;        // K codes 4096 | K params 1024 | V codes 4096 | V params 1024
@@ -158,18 +150,18 @@ constexpr float kOver = 256.0f;      // a probability past this moves the runnin
 typedef int v2i_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void lds_void;
 
-BB_DEV int64_t live_length(const Int4DecodeParams& p) {
-  const int64_t n = p.n_dev ? *p.n_dev : p.n;
-  return n < 0 ? 0 : n > p.cap ? p.cap : n;
-}
+BB_DEV int64_t live_length(const Int4DecodeParams& p, int64_t raw) { return raw < 0 ? 0 : raw > p.cap ? p.cap : raw; }
 // Keys of a split: the live length in equal parts of whole 16 keys (the bytes per CU set the time, so the parts are not
-// rounded to chunks).
-BB_DEV int64_t split_keys(int64_t n, int n_splits) {
-  const int64_t len = ((n + n_splits - 1) / n_splits + 15) & ~(int64_t)15;
+// rounded to chunks); the host passes it as p.len unless the length is in device memory. ceil(n / n_splits) from the rounded reciprocal, put right by one where it is off: a 64-bit division
+// is hundreds of instructions ahead of the first load.
+BB_DEV int64_t split_keys(const Int4DecodeParams& p, int64_t n) {
+  int64_t len = (int64_t)((double)n * p.inv_splits);
+  if (len * p.n_splits < n) ++len;
+  len = (len + 15) & ~(int64_t)15;
   return len < kInt4MinSplit ? kInt4MinSplit : len;
 }
-// Keys that token t of T attends.
-BB_DEV int64_t seen_keys(const Int4DecodeParams& p, int64_t n, int t) { return p.causal ? n - p.T + 1 + t : n; }
+// The token of query vector v (v / G; v < 2^20, so the product with the rounded reciprocal is off by less than 1 / (2 G)).
+BB_DEV int token_of(const Int4DecodeParams& p, int v) { return (int)(((float)v + 0.5f) * p.inv_G); }
 
 BB_DEV f32x4_t mma16_bf16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -183,14 +175,21 @@ BB_DEV f32x4_t mma16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
 }
 
 // Eight codes as 16-bit floats 16 + c, in the order 0, 4, 1, 5, 2, 6, 3, 7 (the halves of the word side by side). 16.0 has
-// an ulp of 1/8 in bf16 and 1/64 in fp16, so a code is a shift away from its place in the mantissa.
+// an ulp of 1/8 in bf16 and 1/64 in fp16, so a code is a shift away from its place in the mantissa. The constants stay in
+// registers (`mask` scalar, `base` vector), where one v_and_or_b32 takes both; as literals they cost an instruction more.
 template <bool F16>
-BB_DEV bf16x8_t codes16(uint32_t w) {
-  constexpr uint32_t mask = F16 ? 0x03c003c0u : 0x00780078u, base = F16 ? 0x4c004c00u : 0x41804180u;
-  constexpr int sh = F16 ? 6 : 3;
-  return as_bf16x8(u32x4_t{((w << sh) & mask) | base, ((F16 ? w << 2 : w >> 1) & mask) | base,
-                           ((w >> (8 - sh)) & mask) | base, ((w >> (12 - sh)) & mask) | base});
-}
+struct Codes {
+  uint32_t mask, base;
+  BB_DEV Codes() : mask(F16 ? 0x03c003c0u : 0x00780078u), base(F16 ? 0x4c004c00u : 0x41804180u) {
+    asm("" : "+s"(mask));
+    asm("" : "+v"(base));
+  }
+  BB_DEV bf16x8_t operator()(uint32_t w) const {
+    constexpr int sh = F16 ? 6 : 3;
+    return as_bf16x8(u32x4_t{((w << sh) & mask) | base, ((F16 ? w << 2 : w >> 1) & mask) | base,
+                             ((w >> (8 - sh)) & mask) | base, ((w >> (12 - sh)) & mask) | base});
+  }
+};
 
 // The largest / sum over the 16 lanes of a DPP row, in every lane.
 BB_DEV float row_max(float v) {
@@ -226,124 +225,268 @@ BB_DEV void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// The step's new rows that lie in cache rows [begin, end): quantised there by the threads of a workgroup.
+// Eight bytes of LDS per lane, transposed in 4-bit units: lane l of 16 gets column l of the 16 lanes' rows, row r in four-bit
+// place r. `restrict` tells the compiler that no load into LDS in flight writes what is read here (the loop waits for the
+// chunk itself); without it the compiler waits for every load in flight, the next chunk's too.
+BB_DEV v2i_t read_tr4(const uint8_t* __restrict__ at) {
+  return __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) v2i_t*)at);
+}
+
+// Where a chunk's rows lie in its stage; key (0 .. CH - 1) is the row's place in the chunk. In a region of 16 rows K row
+// b3 b2 b1 b0 is at b2 b0 b3 b1, so that the 16 lanes of a score step, whose rows differ in b3, b1 and the region, read
+// 16-byte pieces in every bank once (the regions' pieces are shifted against each other as well).
+BB_DEV int k_place(int row) { return ((row >> 2) & 1) << 3 | (row & 1) << 2 | ((row >> 3) & 1) << 1 | ((row >> 1) & 1); }
+BB_DEV int k_unplace(int pos) { return ((pos >> 1) & 1) << 3 | (pos >> 3) << 2 | (pos & 1) << 1 | ((pos >> 2) & 1); }
 template <int D>
-BB_DEV void append_rows(const Int4DecodeParams& p, int64_t n, int64_t begin, int64_t end, int g, int tid) {
+BB_DEV int k_code_at(int key, int piece) {
+  const int region = (key >> 4) & 3, pos = k_place(key & 15);
+  if constexpr (D == 128) return 1024 * region + 64 * pos + 16 * (piece ^ (-region & 3));
+  else return 2048 * (key >> 6) + 512 * region + 32 * (pos ^ (4 * (region >> 1))) + 16 * piece;
+}
+// V row r's piece is shifted by the row, so that 16 rows' reads of one column block meet no bank twice.
+template <int D>
+BB_DEV int v_code_at(int key, int piece) {
+  const int region = (key >> 4) & 3, row = key & 15;
+  if constexpr (D == 128) return 1024 * region + 64 * row + 16 * (piece ^ (row >> 2));
+  else return 2048 * (key >> 6) + 512 * region + 32 * row + 16 * (piece ^ (row >> 3));
+}
+// Where lane (k, a) points for columns 16 db .. 16 db + 15 of the 64 keys of half hv: row 16 a + k, 8 bytes.
+template <int D>
+BB_DEV int v_block_at(int k, int a, int hv, int db) {
+  if constexpr (D == 128) return 1024 * a + 64 * k + 16 * ((db >> 1) ^ (k >> 2)) + 8 * (db & 1);
+  else return 2048 * hv + 512 * a + 32 * k + 16 * ((db >> 1) ^ (k >> 3)) + 8 * (db & 1);
+}
+// A key's params: 16 u + k of lane k and score step u; at head_dim 64 two neighbouring keys share a 16-byte piece.
+template <int D>
+BB_DEV int param_at(int key) {
+  const int k = 4 * ((key >> 4) & 3) + 2 * ((key >> 3) & 1) + ((key >> 1) & 1), u = (key >> 2) & 1, odd = key & 1;
+  if constexpr (D == 128) return 16 * (16 * (u + 2 * odd) + k);
+  else return 512 * u + 256 * (key >> 6) + 16 * k + 8 * odd;
+}
+
+// The step's new rows among the keys [first, first + CH) of the split (fewer than `count`): quantised into the chunk in
+// LDS, over what the cache held there, and by the first pass into the cache. No other chunk holds them, so nothing waits
+// for the stores.
+template <int D, int CH>
+BB_DEV void append_rows(const Int4DecodeParams& p, int64_t raw, int64_t begin, int first, int count, int g, int lane,
+                        uint8_t* s) {
   constexpr int LPR = D / 8;
-  const int c = tid % LPR;
-  for (int i = tid / LPR; i < 2 * p.T; i += kThreads / LPR) {  // the lanes of a row stay together
+  const int c = lane % LPR;
+  for (int i = lane / LPR; i < 2 * p.T; i += 64 / LPR) {  // the lanes of a row stay together
     const int t = i >> 1, vt = i & 1;
-    const int64_t row = n - p.T + t;
-    if (row < begin || row >= end) continue;
+    const int64_t row = raw - p.T + t, at = row - begin;
+    if (at < first || at >= first + CH || at >= count) continue;
     float v[8];
     load8(vt ? p.vnew : p.knew, vt ? g * p.svn0 + t * p.svn1 + 8 * c : g * p.skn0 + t * p.skn1 + 8 * c,
           p.f16 ? kKindF16 : kKindBf16, v);
     uint32_t param;
     const uint32_t w = quant8_4bit(v, param);
-    uint8_t* q = vt ? p.vq + g * p.svq : p.kq + g * p.skq;
-    uint32_t* pp = vt ? p.vp + g * p.svp : p.kp + g * p.skp;
-    *reinterpret_cast<uint32_t*>(q + row * (D / 2) + 4 * c) = w;
-    if (c % 4 == 0) pp[row * (D / kGroup) + c / 4] = param;
+    const int key = (int)at - first;
+    *reinterpret_cast<uint32_t*>(s + (vt ? kVq + v_code_at<D>(key, c / 4) : k_code_at<D>(key, c / 4)) + 4 * (c % 4)) = w;
+    if (c % 4 == 0) *reinterpret_cast<uint32_t*>(s + (vt ? kVp : kKp) + param_at<D>(key) + c) = param;
+    if (blockIdx.z == 0) {
+      *reinterpret_cast<uint32_t*>((vt ? p.vq + g * p.svq : p.kq + g * p.skq) + row * (D / 2) + 4 * c) = w;
+      if (c % 4 == 0) (vt ? p.vp + g * p.svp : p.kp + g * p.skp)[row * (D / kGroup) + c / 4] = param;
+    }
   }
 }
 
-// NB: blocks of 4 query vectors. TWO: a probability times a scale goes to the matrix cores as two bf16 terms (16
-// significant bits) instead of one.
-template <int D, bool F16, int NB, bool TWO>
-__global__ __launch_bounds__(kThreads, NB == 4 ? 1 : 2) void int4_decode_kernel(Int4DecodeParams p) {
-  __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][kStage];
-  constexpr int CH = D == 128 ? 64 : 128;      // keys of a chunk
-  constexpr int W = D == 128 ? 1 : 2;          // queries of a block whose scores a lane ends up with
-  constexpr int NG = D / kGroup, NDB = D / 16; // column groups, blocks of 16 columns
-  constexpr int HV = CH / 64;                  // 64-key halves of a chunk
-  constexpr int PROW = 2 * CH + 16;            // bytes of a probability row in LDS (16 more: rows on other banks)
-  const int split = blockIdx.x, g = blockIdx.y, v0 = blockIdx.z * kVecs;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int k = lane & 15, a = lane >> 4;
-  const int G = p.H / p.Hkv, R = p.T * G - v0 < kVecs ? p.T * G - v0 : kVecs;
-  const int64_t n = live_length(p), len = split_keys(n, p.n_splits), begin = split * len;
-  const int64_t end = begin + len < n ? begin + len : n;
-  const int count = end > begin ? (int)(end - begin) : 0;
-
-  if (p.knew != nullptr && gridDim.z == 1) {
-    // the length before clamping places the new rows; those outside the cache are left out
-    const int64_t raw = p.n_dev ? *p.n_dev : p.n;
-    const int64_t hi = begin + len < p.cap ? begin + len : p.cap;
-    if (raw > begin && raw - p.T < hi) {
-      append_rows<D>(p, raw, begin, hi, g, tid);
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the rows are in L2 before any wave of this workgroup reads them
-      __syncthreads();
+// One wave's stream of chunks: where lane l's 16 bytes of each load come from (load i lands at 1024 i + 16 l). Loads cover
+// whole contiguous kilobytes; inside, pieces are placed for the reads. Lane k of a score step u works on
+//   key(k, u) = 16 (k >> 2) + 8 ((k >> 1) & 1) + 4 (u & 1) + 2 (k & 1) + (u >> 1)     (+ 64 in the second half of 128)
+// so that a lane's four steps are four neighbouring elements of the value operand (the codes' order).
+BB_DEV int key_of_lane(int k) { return 16 * (k >> 2) + 8 * ((k >> 1) & 1) + 2 * (k & 1); }
+BB_DEV int key_of_step(int u) { return 4 * (u & 1) + (u >> 1); }
+template <int D>
+struct Stream {
+  uint32_t koff[2], voff, poff;
+  const uint8_t *kq, *vq;
+  const uint32_t *kp, *vp;
+  int count;
+  BB_DEV Stream(const Int4DecodeParams& p, int g, int64_t begin, int count_, int lane) : count(count_) {
+    const int k = lane & 15;
+    if constexpr (D == 128) {
+      koff[0] = koff[1] = 64 * k_unplace(lane >> 2) + 16 * (lane & 3);  // load i: pieces xor -i & 3
+      voff = 64 * (lane >> 2) + 16 * ((lane & 3) ^ (lane >> 4));
+      poff = 16 * (key_of_lane(k) + key_of_step(lane >> 4));
+    } else {
+      const int pos = (lane >> 1) & 15;
+      koff[0] = 512 * (lane >> 5) + 32 * k_unplace(pos) + 16 * (lane & 1);
+      koff[1] = 512 * (lane >> 5) + 32 * k_unplace(pos ^ 4) + 16 * (lane & 1);  // odd loads: regions 2 and 3
+      voff = 512 * (lane >> 5) + 32 * pos + 16 * ((lane & 1) ^ (pos >> 3));
+      poff = 8 * (64 * ((lane >> 4) & 1) + key_of_lane(k) + 4 * (lane >> 5));
     }
+    kq = p.kq + g * p.skq + begin * (D / 2);
+    vq = p.vq + g * p.svq + begin * (D / 2);
+    kp = p.kp + g * p.skp + begin * (D / kGroup);
+    vp = p.vp + g * p.svp + begin * (D / kGroup);
   }
-  if (count == 0 && p.n_splits > 1) return;  // no partial: the merge knows the live splits
-
-  // the query operand: fragment i of block b, element 2 m / 2 m + 1 = column 8 i + m / 8 i + m + 4 of the lane's group
-  bf16x8_t qa[NB][4];
-  f32x4_t qs[NB];  // sums of the queries' groups, where the scores are
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const int v = v0 + 4 * b + (k & 3);
-    const bool on = (k >> 2) == a && 4 * b + (k & 3) < R;
-    const uint16_t* qr = p.q + (on ? (v / G) * p.sq0 + (g * G + v % G) * p.sq1 + kGroup * (D == 128 ? a : a & 1) : 0);
-    qs[b] = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const u32x4_t w = on ? ld16(qr + 8 * i) : u32x4_t{0, 0, 0, 0};
-      qa[b][i] = as_bf16x8(u32x4_t{(w[0] & 0xffffu) | (w[2] << 16), (w[0] >> 16) | (w[2] & 0xffff0000u),
-                                   (w[1] & 0xffffu) | (w[3] << 16), (w[1] >> 16) | (w[3] & 0xffff0000u)});
-      constexpr uint32_t one = F16 ? 0x3c003c00u : 0x3f803f80u;
-      qs[b] = mma16<F16>(qa[b][i], as_bf16x8(u32x4_t{one, one, one, one}), qs[b]);
-    }
-  }
-
-  const int64_t row0 = begin;
-  auto rsrc = [&](const void* base, int64_t row_bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(static_cast<const uint8_t*>(base)) + row0 * row_bytes, 0,
-                                             (int)(count * row_bytes), 0x00020000);
-  };
-  const __amdgpu_buffer_rsrc_t kqr = rsrc(p.kq + g * p.skq, D / 2), kpr = rsrc(p.kp + g * p.skp, D / 8);
-  const __amdgpu_buffer_rsrc_t vqr = rsrc(p.vq + g * p.svq, D / 2), vpr = rsrc(p.vp + g * p.svp, D / 8);
-
-  // Where lane l's 16 bytes of load i come from (they land at 1024 i + 16 l). Loads cover whole contiguous kilobytes; inside,
-  // pieces are placed for the reads below. key(k, u) is the key of lane k in score step u, with
-  //   key(k, u) = 16 (k >> 2) + 8 ((k >> 1) & 1) + 4 (u & 1) + 2 (k & 1) + (u >> 1),
-  // so that a lane's four steps are four neighbouring elements of the value operand (codes16's order).
-  uint32_t koff[2], voff, poff;  // K codes: even and odd loads differ only by a constant xor
-  auto unplace = [](int pos) { return ((pos >> 1) & 1) << 3 | (pos >> 3) << 2 | (pos & 1) << 1 | ((pos >> 2) & 1); };
-  if constexpr (D == 128) {
-    koff[0] = 64 * unplace(lane >> 2) + 16 * (lane & 3);
-    koff[1] = 0;
-    voff = 64 * (lane >> 2) + 16 * ((lane & 3) ^ (lane >> 4));
-    const int kk = lane & 15, u = lane >> 4;  // params: slot 16 u + k holds key(k, u)
-    poff = 16 * (16 * (kk >> 2) + 8 * ((kk >> 1) & 1) + 4 * (u & 1) + 2 * (kk & 1) + (u >> 1));
-  } else {
-    const int pos = (lane >> 1) & 15;
-    koff[0] = 512 * (lane >> 5) + 32 * unplace(pos) + 16 * (lane & 1);
-    koff[1] = 512 * (lane >> 5) + 32 * unplace(pos ^ 4) + 16 * (lane & 1);
-    voff = 512 * (lane >> 5) + 32 * pos + 16 * ((lane & 1) ^ (pos >> 3));
-    const int kk = lane & 15, half = (lane >> 4) & 1, u = lane >> 5;  // slot 32 (u & 1) + 16 half + k: keys key(k, u), + 1
-    poff = 8 * (64 * half + 16 * (kk >> 2) + 8 * ((kk >> 1) & 1) + 4 * u + 2 * (kk & 1));
-  }
-  auto fetch = [&](int c, int st) {
-    uint8_t* base = sm[wave][st];
-    auto ld = [&](__amdgpu_buffer_rsrc_t r, int at, uint32_t off) {
+  // Chunk c into `stage`: always ten loads, so that the counts the waits go by are exact; past the split's last chunk they
+  // read nothing (the buffers' ranges end with it) and land zeros.
+  BB_DEV void fetch(uint8_t* stage, int c) const {
+    auto ld = [&](const void* base, int row_bytes, int at, uint32_t off) {
+      const __amdgpu_buffer_rsrc_t r =
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, count * row_bytes, 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          r, reinterpret_cast<lds_void*>(reinterpret_cast<uintptr_t>(base + at)), 16, off, 0, 0, 2 /* non-temporal */);
+          r, reinterpret_cast<lds_void*>(reinterpret_cast<uintptr_t>(stage + at)), 16, off, 0, 0, 2 /* non-temporal */);
     };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint32_t off;
-      if constexpr (D == 128) off = koff[0] ^ (16 * (-i & 3));  // the piece's bits are 4 and 5 of the offset
-      else off = koff[i & 1];
-      ld(kqr, 1024 * i, c * 4096 + 1024 * i + off);
+      const uint32_t off = D == 128 ? koff[0] ^ (16 * (-i & 3)) : koff[i & 1];  // head_dim 128: bits 4 and 5 are the piece
+      ld(kq, D / 2, 1024 * i, c * 4096 + 1024 * i + off);
     }
-    ld(kpr, kKp, c * 1024 + poff);
+    ld(kp, D / 8, kKp, c * 1024 + poff);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ld(vqr, kVq + 1024 * i, c * 4096 + 1024 * i + voff);
-    ld(vpr, kVp, c * 1024 + poff);
-  };
-  // where the reads of a stage start
-  uint32_t kread[2], kpread, vpread;
+    for (int i = 0; i < 4; ++i) ld(vq, D / 2, kVq + 1024 * i, c * 4096 + 1024 * i + voff);
+    ld(vp, D / 8, kVp, c * 1024 + poff);
+  }
+};
+
+// A split's part of a call.
+struct Part {
+  int64_t n, raw, begin;  // length, length before clamping, first key
+  int count, new_first;   // keys, and the first of them that may be a new row
+  BB_DEV Part(const Int4DecodeParams& p, int split) {
+    raw = n = p.n;
+    int64_t len = p.len;
+    if (p.n_dev) {
+      raw = *p.n_dev;
+      n = live_length(p, raw);
+      len = split_keys(p, n);
+    }
+    begin = split * len;
+    const int64_t left = n - begin;
+    count = (int)(left < 0 ? 0 : left < len ? left : len);
+    // the length before clamping places the new rows; those that it puts outside the cache are left out
+    const int64_t at = raw - p.T - begin;
+    new_first = p.knew != nullptr && at < count ? (int)(at < 0 ? 0 : at) : 0x7fffffff;
+  }
+  // How many of the split's keys query vector v attends.
+  BB_DEV int limit(const Int4DecodeParams& p, int v) const {
+    if (!p.causal) return count;
+    const int64_t seen = n - p.T + 1 + token_of(p, v) - begin;
+    return (int)(seen < 0 ? 0 : seen < count ? seen : count);
+  }
+};
+
+// A landed chunk made ready for the reads: the params that no load brought, and the new rows.
+template <int D, int CH>
+BB_DEV void complete(const Int4DecodeParams& p, const Part& part, const Stream<D>& in, int c, int g, int lane, uint8_t* s) {
+  wave_fence();
+  if constexpr (D == 64) {
+    // an odd last key's params share their 16-byte piece with a row past the range: read them apart
+    if ((part.count & 1) && (c + 1) * CH > part.count && lane < 4) {
+      const uint32_t* src = (lane & 2 ? in.vp : in.kp) + 2 * (part.count - 1) + (lane & 1);
+      *reinterpret_cast<uint32_t*>(s + (lane & 2 ? kVp : kKp) + param_at<D>(part.count - 1 - c * CH) + 4 * (lane & 1)) = *src;
+    }
+  }
+  if ((c + 1) * CH > part.new_first)
+    append_rows<D, CH>(p, part.raw, part.begin, c * CH, part.count, g, lane, s);
+  wave_fence();
+}
+
+// What a wave leaves in its own LDS when its chunks are done: NV vectors' maxima, sums, minima's parts per column group, and
+// the rest of their outputs (rows of D + 4 floats, so that the vectors lie on other banks).
+template <int D, int NV>
+struct WaveState {
+  float m[NV], l[NV], z[NV][D / kGroup], o[NV][D + 4];
+};
+
+// The four waves' states under one maximum: the split's partial, or with one split the output (a row without keys: zeros).
+template <int D, bool F16, int NV>
+BB_DEV void finish(const Int4DecodeParams& p, const uint8_t (*sm)[2][kStage], int R, int v0, int g, int split, int tid) {
+  __syncthreads();
+#pragma unroll 1
+  for (int i = tid; i < R * D; i += kThreads) {
+    const int r = i / D, d = i % D, v = v0 + r, t = token_of(p, v), hd = g * p.G + v - t * p.G;
+    float M = -1.0e30f, L = 0.0f, O = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, reinterpret_cast<const WaveState<D, NV>*>(sm[w])->m[r]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const WaveState<D, NV>* f = reinterpret_cast<const WaveState<D, NV>*>(sm[w]);
+      const float wt = fast_exp2(f->m[r] - M);
+      L += wt * f->l[r];
+      O += wt * (f->o[r][d] + f->z[r][d / kGroup]);
+    }
+    if (p.n_splits == 1) {
+      p.out[t * p.so0 + hd * p.so1 + d] = to16<F16>(L > 0.0f ? O / L : 0.0f);
+    } else {
+      float* dst = p.part + (((int64_t)t * p.H + hd) * p.n_splits + split) * (D + 2);
+      dst[d] = O;
+      if (d == 0) { dst[D] = M; dst[D + 1] = L; }
+    }
+  }
+}
+
+// A query's 8 columns w as an operand fragment in the codes' order: element 2 m / 2 m + 1 = column m / m + 4.
+BB_DEV bf16x8_t query_fragment(u32x4_t w, bool on) {
+  w = on ? w : u32x4_t{0, 0, 0, 0};
+  return as_bf16x8(u32x4_t{(w[0] & 0xffffu) | (w[2] << 16), (w[0] >> 16) | (w[2] & 0xffff0000u),
+                           (w[1] & 0xffffu) | (w[3] << 16), (w[1] >> 16) | (w[3] & 0xffff0000u)});
+}
+template <bool F16>
+BB_DEV bf16x8_t fragment_of_ones() {
+  constexpr uint32_t one = F16 ? 0x3c003c00u : 0x3f803f80u;
+  return as_bf16x8(u32x4_t{one, one, one, one});
+}
+
+// Probabilities times scales as operands of 16 bits: bf16, whatever the model's type (an fp16 product could fall below
+// its range). TWO puts each into two terms (16 significant bits): an fp16 output is finer than one bf16 term.
+template <bool TWO>
+BB_DEV void put_terms(const float (&q)[4], uint8_t* dst, int second) {
+  const uint32_t h0 = pack_bf16x2(q[0], q[1]), h1 = pack_bf16x2(q[2], q[3]);
+  *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{h0, h1};
+  if constexpr (TWO) {
+    const uint32_t l0 = pack_bf16x2(q[0] - __uint_as_float(h0 << 16), q[1] - __uint_as_float(h0 & 0xffff0000u));
+    const uint32_t l1 = pack_bf16x2(q[2] - __uint_as_float(h1 << 16), q[3] - __uint_as_float(h1 & 0xffff0000u));
+    *reinterpret_cast<u32x2_t*>(dst + second) = u32x2_t{l0, l1};
+  }
+}
+
+// Up to 4 query vectors.
+//   scores  Lane (k, a) of 16 x 4 holds the 16 bytes of group a of key k (head_dim 64: group a & 1 of the key in half
+//           a >> 1). The query operand is block-diagonal: row 4 a + h holds group a of query h where the lane's quarter is
+//           a and zero elsewhere, so the four 16x16x32 products of a 1 KB piece leave in lane (k, a) the four queries' sums
+//           over its own group. One (s, z) word per lane turns them into scores; three lane swaps sum the groups and
+//           leave lane (k, a) with the whole score of query a alone, so that no lane's exponential is idle.
+//   values  The probabilities times the scales of column group t go to column 4 t + h of the operand, so one product serves
+//           all groups (the columns of a product whose rows are another group are not used). The 16s go with a row of ones.
+template <int D, bool F16, bool TWO>
+__global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodeParams p) {
+  __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][kStage];
+  constexpr int CH = D == 128 ? 64 : 128;      // keys of a chunk
+  constexpr int W = D == 128 ? 1 : 2;          // queries whose scores a lane ends up with
+  constexpr int NG = D / kGroup, NDB = D / 16; // column groups, blocks of 16 columns
+  constexpr int HV = CH / 64;                  // 64-key halves of a chunk
+  constexpr int PROW = 2 * CH + 16;            // bytes of a probability row in LDS (16 more: rows on other banks)
+  const int split = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), k = lane & 15, a = lane >> 4, R = p.T * p.G;
+  const Part part(p, split);
+  if (part.count == 0 && p.n_splits > 1) return;  // no partial: the merge knows the live splits
+
+  // the queries' loads first, the first chunks' right behind them
+  u32x4_t qw[4];
+  const bool on = (k >> 2) == a && (k & 3) < R;
+  {
+    const int v = (k & 3) < R ? k & 3 : 0, t = token_of(p, v);
+    const uint16_t* qr = p.q + t * p.sq0 + (g * p.G + v - t * p.G) * p.sq1 + kGroup * (D == 128 ? a : a & 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) qw[j] = ld16(qr + 8 * j);
+  }
+  const Stream<D> in(p, g, part.begin, part.count, lane);
+  const int chunks = (part.count + CH - 1) / CH;
+  in.fetch(sm[wave][0], wave);
+  in.fetch(sm[wave][1], wave + kWaves);
+
+  bf16x8_t qa[4];  // fragment i: columns 8 i .. 8 i + 7 of the lane's group
+  f32x4_t qs = {0, 0, 0, 0};  // sums of the queries' groups, where the scores are
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    qa[i] = query_fragment(qw[i], on);
+    qs = mma16<F16>(qa[i], fragment_of_ones<F16>(), qs);
+  }
+  uint32_t kread[2], kpread, vpread;  // where the reads of a stage start
   if constexpr (D == 128) {
     kread[0] = kread[1] = 1024 * (k >> 2) + 64 * (k & 3) + 16 * (a ^ (-(k >> 2) & 3));
     kread[1] += 256;
@@ -356,273 +499,433 @@ __global__ __launch_bounds__(kThreads, NB == 4 ? 1 : 2) void int4_decode_kernel(
     kpread = kKp + 256 * (a >> 1) + 16 * k + 4 * (a & 1);
     vpread = kVp + 256 * (a >> 1) + 16 * k;
   }
-  const int key_k = (D == 128 ? 0 : 64 * (a >> 1)) + 16 * (k >> 2) + 8 * ((k >> 1) & 1) + 2 * (k & 1);
+  const int key_k = (D == 128 ? 0 : 64 * (a >> 1)) + key_of_lane(k);
+  int lim[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w) lim[w] = part.limit(p, D == 128 ? a : (a & 1) + 2 * w);
+  const int fewest = part.limit(p, 0);  // the first token's is the smallest
 
-  // how many of the split's keys each of the lane's queries attends, and the fewest over all
-  int lim[NB][W];
+  float m[W], l[W], zs[W][NG];
+  f32x4_t o[NDB], ones = {0, 0, 0, 0};
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+  for (int w = 0; w < W; ++w) {
+    m[w] = -1.0e30f;
+    l[w] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const int v = v0 + 4 * b + (D == 128 ? a : (a & 1) + 2 * w);
-      const int64_t seen = seen_keys(p, n, v / G) - begin;
-      lim[b][w] = (int)(seen < 0 ? 0 : seen < count ? seen : count);
-    }
-  int fewest;
-  {
-    const int64_t seen = seen_keys(p, n, v0 / G) - begin;
-    fewest = (int)(seen < 0 ? 0 : seen < count ? seen : count);
+    for (int t = 0; t < NG; ++t) zs[w][t] = 0.0f;
   }
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) o[db] = f32x4_t{0, 0, 0, 0};
 
-  float m[NB][W], l[NB][W], zs[NB][4];
-  f32x4_t o[NB][NDB], ones[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-#pragma unroll
-    for (int w = 0; w < W; ++w) { m[b][w] = -1.0e30f; l[b][w] = 0.0f; }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) zs[b][t] = 0.0f;
-    ones[b] = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-    for (int db = 0; db < NDB; ++db) o[b][db] = f32x4_t{0, 0, 0, 0};
-  }
-
-  const int chunks = (count + CH - 1) / CH;
+  const Codes<F16> k_codes;
+  const Codes<false> v_codes;
   int st = 0;
-  if (wave < chunks) fetch(wave, 0);
   for (int c = wave; c < chunks; c += kWaves, st ^= 1) {
-    if (c + kWaves < chunks) {
-      fetch(c + kWaves, st ^ 1);
-      __builtin_amdgcn_s_waitcnt(0x0F7A);  // vmcnt(10): this chunk's ten loads have landed
-    } else {
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-    }
-    wave_fence();
+    __builtin_amdgcn_s_waitcnt(0x0F7A);  // vmcnt(10): all but the next chunk's ten loads have landed
     uint8_t* s = sm[wave][st];
+    complete<D, CH>(p, part, in, c, g, lane, s);
     const bool whole = (c + 1) * CH <= fewest;
-    if constexpr (D == 64) {
-      // an odd last key's params share their 16-byte piece with a row past the range: read them apart
-      if ((count & 1) && (c + 1) * CH > count && lane < 4) {
-        const int key = count - 1 - c * CH, kk = 4 * ((key >> 4) & 3) + 2 * ((key >> 3) & 1) + ((key >> 1) & 1);
-        const uint32_t* src = (lane & 2 ? p.vp + g * p.svp : p.kp + g * p.skp) + 2 * (end - 1) + (lane & 1);
-        *reinterpret_cast<uint32_t*>(s + (lane & 2 ? kVp : kKp) + 512 * ((key >> 2) & 1) + 256 * (key >> 6) + 16 * kk +
-                                     8 * (key & 1) + 4 * (lane & 1)) = *src;
-      }
-    }
-    wave_fence();
 
-    float x[NB][W][4];
+    float x[W][4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const u32x4_t kw = *reinterpret_cast<const u32x4_t*>(s + kread[u >> 1] + (D == 128 ? 512 : 256) * (u & 1));
       uint32_t kp = *reinterpret_cast<const uint32_t*>(s + kpread + (D == 128 ? 256 * u : 512 * (u & 1) + 8 * (u >> 1)));
-      const int key = c * CH + key_k + 4 * (u & 1) + (u >> 1);
-      if (!whole) kp = key < count ? kp : 0u;
+      const int key = c * CH + key_k + key_of_step(u);
+      if (!whole) kp = key < part.count ? kp : 0u;
       const float sc = f16_lo(kp) * p.c, zc = fmaf(-16.0f, f16_lo(kp), f16_hi(kp)) * p.c;
-      f32x4_t acc[NB];
+      f32x4_t acc = {0, 0, 0, 0};
 #pragma unroll
-      for (int b = 0; b < NB; ++b) acc[b] = f32x4_t{0, 0, 0, 0};
+      for (int i = 0; i < 4; ++i) acc = mma16<F16>(qa[i], k_codes(kw[i]), acc);
+      float y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bf16x8_t kf = codes16<F16>(kw[i]);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) acc[b] = mma16<F16>(qa[b][i], kf, acc[b]);
+      for (int h = 0; h < 4; ++h) y[h] = fmaf(sc, acc[h], zc * qs[h]);
+      if constexpr (D == 128) {
+        x[0][u] = sum_rows16(sum_rows32(y[0], y[2]), sum_rows32(y[1], y[3]));
+      } else {
+        x[0][u] = sum_rows16(y[0], y[1]);
+        x[W - 1][u] = sum_rows16(y[2], y[3]);
       }
+      if (!whole) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        float y[4];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) y[h] = fmaf(sc, acc[b][h], zc * qs[b][h]);
-        if constexpr (D == 128) {
-          x[b][0][u] = sum_rows16(sum_rows32(y[0], y[2]), sum_rows32(y[1], y[3]));
-        } else {
-          x[b][0][u] = sum_rows16(y[0], y[1]);
-          x[b][1][u] = sum_rows16(y[2], y[3]);
-        }
-        if (!whole) {
-#pragma unroll
-          for (int w = 0; w < W; ++w)
-            if (key >= lim[b][w]) x[b][w][u] = -__builtin_huge_valf();
-        }
+        for (int w = 0; w < W; ++w)
+          if (key >= lim[w]) x[w][u] = -__builtin_huge_valf();
       }
     }
-    float pr[NB][W][4];
+    float pr[W][4];
     bool over = false;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int w = 0; w < W; ++w)
 #pragma unroll
-      for (int w = 0; w < W; ++w)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          pr[b][w][u] = fast_exp2(x[b][w][u] - m[b][w]);
-          over |= !(pr[b][w][u] <= kOver);
-        }
+      for (int u = 0; u < 4; ++u) {
+        pr[w][u] = fast_exp2(x[w][u] - m[w]);
+        over |= !(pr[w][u] <= kOver);
+      }
     if (__builtin_amdgcn_ballot_w64(over)) {
+      float alpha[W];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        float alpha[W];
+      for (int w = 0; w < W; ++w) {
+        float mx = row_max(fmaxf(fmaxf(x[w][0], x[w][1]), fmaxf(x[w][2], x[w][3])));
+        if constexpr (D == 64) mx = xhalf_max(mx);
+        const float mn = fmaxf(m[w], mx);
+        alpha[w] = fast_exp2(m[w] - mn);
+        m[w] = mn;
+        l[w] *= alpha[w];
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          float mx = row_max(fmaxf(fmaxf(x[b][w][0], x[b][w][1]), fmaxf(x[b][w][2], x[b][w][3])));
-          if constexpr (D == 64) mx = xhalf_max(mx);
-          const float mn = fmaxf(m[b][w], mx);
-          alpha[w] = fast_exp2(m[b][w] - mn);
-          m[b][w] = mn;
-          l[b][w] *= alpha[w];
+        for (int u = 0; u < 4; ++u) pr[w][u] = fast_exp2(x[w][u] - mn);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) pr[b][w][u] = fast_exp2(x[b][w][u] - mn);
+        for (int t = 0; t < NG; ++t) zs[w][t] *= alpha[w];
+      }
+      // column 4 t + h of the sums belongs to query h
+      float al[4];
 #pragma unroll
-          for (int t = 0; t < NG; ++t) zs[b][NG * w + t] *= alpha[w];
-        }
-        // column 4 t + h of the sums belongs to query h
-        float al[4];
+      for (int h = 0; h < 4; ++h)
+        al[h] = D == 128 ? lane_value(alpha[0], 16 * h) : lane_value(alpha[W - 1 ? h >> 1 : 0], 16 * (h & 1));
+      const float ac = k & 2 ? (k & 1 ? al[3] : al[2]) : (k & 1 ? al[1] : al[0]);
 #pragma unroll
-        for (int h = 0; h < 4; ++h) al[h] = D == 128 ? lane_value(alpha[0], 16 * h) : lane_value(alpha[W - 1 ? h >> 1 : 0], 16 * (h & 1));
-        const float ac = k & 2 ? (k & 1 ? al[3] : al[2]) : (k & 1 ? al[1] : al[0]);
+      for (int e = 0; e < 4; ++e) {
+        ones[e] *= ac;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          ones[b][e] *= ac;
-#pragma unroll
-          for (int db = 0; db < NDB; ++db) o[b][db][e] *= ac;
-        }
+        for (int db = 0; db < NDB; ++db) o[db][e] *= ac;
       }
     }
-    // probabilities times V scales, [4 t + h][key] in the space of the K rows, then the operand of every block
-    bf16x8_t pb[NB][2 * HV], pl[NB][2 * HV];
     uint32_t vp[4][NG];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int key = c * CH + key_k + 4 * (u & 1) + (u >> 1);
       if constexpr (D == 128) {
         const u32x4_t r = *reinterpret_cast<const u32x4_t*>(s + vpread + 256 * u);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) vp[u][t] = r[t];
+        for (int t = 0; t < NG; ++t) vp[u][t] = r[t];
       } else {
         const u32x2_t r = *reinterpret_cast<const u32x2_t*>(s + vpread + 512 * (u & 1) + 8 * (u >> 1));
         vp[u][0] = r[0];
         vp[u][1] = r[1];
       }
-      if (!whole) {
+    }
+    if (!whole) {
 #pragma unroll
-        for (int t = 0; t < NG; ++t) vp[u][t] = key < count ? vp[u][t] : 0u;
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int t = 0; t < NG; ++t) vp[u][t] = c * CH + key_k + key_of_step(u) < part.count ? vp[u][t] : 0u;
+    }
+    // probabilities times V scales, [4 t + h][key], in the space of the K rows
+    wave_fence();
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) l[w] += pr[w][u];
+#pragma unroll
+      for (int t = 0; t < NG; ++t) {
+        float q[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          q[u] = pr[w][u] * f16_lo(vp[u][t]);
+          // the sums take 24 off every code, so that a rounded probability meets -8..7: z + 8 s here
+          zs[w][t] = fmaf(pr[w][u], f16_hi(vp[u][t]), fmaf(8.0f, q[u], zs[w][t]));
+        }
+        const int col = D == 128 ? 4 * t + a : 4 * t + (a & 1) + 2 * w;
+        put_terms<TWO>(q, s + col * PROW + (D == 128 ? 0 : 128 * (a >> 1)) + 8 * k, 4 * NG * PROW);
       }
     }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      wave_fence();
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) l[b][w] += pr[b][w][u];
-#pragma unroll
-        for (int t = 0; t < NG; ++t) {
-          float q[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            q[u] = pr[b][w][u] * f16_lo(vp[u][t]);
-            // the sums take 24 off every code, so that a rounded probability meets -8..7: z + 8 s here
-            zs[b][NG * w + t] = fmaf(pr[b][w][u], f16_hi(vp[u][t]), fmaf(8.0f, q[u], zs[b][NG * w + t]));
-          }
-          const uint32_t h0 = pack_bf16x2(q[0], q[1]), h1 = pack_bf16x2(q[2], q[3]);
-          const int col = D == 128 ? 4 * t + a : 4 * t + (a & 1) + 2 * w;
-          uint8_t* dst = s + col * PROW + (D == 128 ? 0 : 128 * (a >> 1)) + 8 * k;
-          *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{h0, h1};
-          if constexpr (TWO) {
-            const uint32_t l0 = pack_bf16x2(q[0] - __uint_as_float(h0 << 16), q[1] - __uint_as_float(h0 & 0xffff0000u));
-            const uint32_t l1 = pack_bf16x2(q[2] - __uint_as_float(h1 << 16), q[3] - __uint_as_float(h1 & 0xffff0000u));
-            *reinterpret_cast<u32x2_t*>(dst + 4 * NG * PROW) = u32x2_t{l0, l1};
-          }
-        }
-      }
-      wave_fence();
+    wave_fence();
+    bf16x8_t pb[2 * HV], pl[2 * HV];
+    {
       const uint8_t* src = s + (D == 128 ? k : k & 7) * PROW + 32 * a;  // head_dim 64: columns 8..15 repeat and are not used
 #pragma unroll
       for (int j = 0; j < 2 * HV; ++j) {
-        pb[b][j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 128 * (j >> 1) + 16 * (j & 1)));
+        pb[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 128 * (j >> 1) + 16 * (j & 1)));
         if constexpr (TWO)
-          pl[b][j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 4 * NG * PROW + 128 * (j >> 1) + 16 * (j & 1)));
+          pl[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 4 * NG * PROW + 128 * (j >> 1) + 16 * (j & 1)));
       }
     }
-    const bf16x8_t one = as_bf16x8(u32x4_t{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int j = 0; j < 2 * HV; ++j) {
-        ones[b] = mma16_bf16(one, pb[b][j], ones[b]);
-        if constexpr (TWO) ones[b] = mma16_bf16(one, pl[b][j], ones[b]);
-      }
+    for (int j = 0; j < 2 * HV; ++j) {
+      ones = mma16_bf16(fragment_of_ones<false>(), pb[j], ones);
+      if constexpr (TWO) ones = mma16_bf16(fragment_of_ones<false>(), pl[j], ones);
+    }
 #pragma unroll
     for (int hv = 0; hv < HV; ++hv)
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
-        // lane k points at row 16 a + k, 8 bytes of column block db, and gets column k of the 16 rows
-        const uint32_t at = D == 128 ? 1024 * a + 64 * k + 16 * ((db >> 1) ^ (k >> 2)) + 8 * (db & 1)
-                                     : 2048 * hv + 512 * a + 32 * k + 16 * ((db >> 1) ^ (k >> 3)) + 8 * (db & 1);
-        const v2i_t t = __builtin_amdgcn_ds_read_tr4_b64_v2i32(reinterpret_cast<__attribute__((address_space(3))) v2i_t*>(
-            reinterpret_cast<uintptr_t>(s + kVq + at)));
+        const v2i_t t = read_tr4(s + kVq + v_block_at<D>(k, a, hv, db));
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const bf16x8_t vf = codes16<false>((uint32_t)(j ? t.y : t.x));
+          const bf16x8_t vf = v_codes((uint32_t)(j ? t.y : t.x));
+          o[db] = mma16_bf16(vf, pb[2 * hv + j], o[db]);
+          if constexpr (TWO) o[db] = mma16_bf16(vf, pl[2 * hv + j], o[db]);
+        }
+      }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this stage's reads are done before its next loads are issued
+    wave_fence();
+    in.fetch(s, c + 2 * kWaves);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): nothing lands in LDS any more
+
+  WaveState<D, 4>* mine = reinterpret_cast<WaveState<D, 4>*>(sm[wave]);
 #pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            o[b][db] = mma16_bf16(vf, pb[b][2 * hv + j], o[b][db]);
-            if constexpr (TWO) o[b][db] = mma16_bf16(vf, pl[b][2 * hv + j], o[b][db]);
+  for (int w = 0; w < W; ++w) {
+    const int v = D == 128 ? a : (a & 1) + 2 * w;
+    float sum = row_sum(l[w]);
+    if constexpr (D == 64) sum = xhalf_sum(sum);
+#pragma unroll
+    for (int t = 0; t < NG; ++t) {
+      float z = row_sum(zs[w][t]);
+      if constexpr (D == 64) z = xhalf_sum(z);
+      if (k == 0) mine->z[v][t] = z;
+    }
+    if (k == 0) {
+      mine->m[v] = m[w];
+      mine->l[v] = sum;
+    }
+  }
+  // lane (4 t + h, a) holds columns 16 db + 4 a .. + 3 of query h, those of group t valid: blocks 2 t and 2 t + 1
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    f32x4_t r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float lo = k & 4 ? o[2 + j][e] : o[j][e];
+      if constexpr (D == 128) lo = k & 8 ? (k & 4 ? o[6 + j][e] : o[4 + j][e]) : lo;
+      r[e] = fmaf(-24.0f, ones[e], lo);
+    }
+    if (D == 128 || k < 8) *reinterpret_cast<f32x4_t*>(&mine->o[k & 3][32 * (k >> 2) + 16 * j + 4 * a]) = r;
+  }
+  finish<D, F16, 4>(p, sm, R, 0, g, split, tid);
+}
+
+// 5 and more query vectors, 16 of them a pass: the rows of the query operand are the vectors, one product per key group of 32
+// columns (lane (k, a) reads word a of every group of its key), so that no row is zero by design and no lane swap is needed;
+// lane (k, a) gets the sums of vectors 4 a .. 4 a + 3 and applies the (s, z) of all groups of its key. The value operand is
+// built once per column group, in the space of the K rows, and serves that group's two blocks of columns. Against blocks of 4
+// vectors on the kernel above it takes a quarter of the products and of the accumulators.
+template <int D, bool F16, bool TWO>
+__global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4DecodeParams p) {
+  __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][kStage];
+  constexpr int CH = D == 128 ? 64 : 128;
+  constexpr int NG = D / kGroup, NDB = D / 16, HV = CH / 64;
+  constexpr int PROW = 144, PBLK = 16 * PROW;  // a probability row of 64 keys (16 bytes more: other banks), and 16 of them
+  constexpr int AT = TWO ? 1 : 2;              // (group, half) blocks of probabilities in LDS at a time
+  const int split = blockIdx.x, g = blockIdx.y, v0 = blockIdx.z * kVecs, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), k = lane & 15, a = lane >> 4;
+  const int R = p.T * p.G - v0 < kVecs ? p.T * p.G - v0 : kVecs;
+  const Part part(p, split);
+  if (part.count == 0 && p.n_splits > 1) return;
+
+  u32x4_t qw[NG];  // vector k, columns 8 a .. 8 a + 7 of every group
+  {
+    const int v = v0 + (k < R ? k : 0), t = token_of(p, v);
+    const uint16_t* qr = p.q + t * p.sq0 + (g * p.G + v - t * p.G) * p.sq1 + 8 * a;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) qw[j] = ld16(qr + kGroup * j);
+  }
+  const Stream<D> in(p, g, part.begin, part.count, lane);
+  const int chunks = (part.count + CH - 1) / CH;
+  in.fetch(sm[wave][0], wave);
+  in.fetch(sm[wave][1], wave + kWaves);
+
+  bf16x8_t qa[NG];
+  f32x4_t qs[NG];
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    qa[j] = query_fragment(qw[j], k < R);
+    qs[j] = mma16<F16>(qa[j], fragment_of_ones<F16>(), f32x4_t{0, 0, 0, 0});
+  }
+  uint32_t kread[4];  // head_dim 128: by group; 64: by u >> 1
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    kread[j] = D == 128 ? 1024 * (k >> 2) + 64 * (k & 3) + 16 * (j ^ (-(k >> 2) & 3)) + 4 * a
+                        : 512 * (k >> 2) + 32 * (k & 3) + 128 * ((k >> 3) ^ (j & 1)) + 4 * a;
+  int lim[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) lim[e] = part.limit(p, v0 + 4 * a + e);
+  const int fewest = part.limit(p, v0);
+
+  float m[4], l[4], zs[4][NG];
+  f32x4_t o[NDB], ones[NG];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    m[e] = -1.0e30f;
+    l[e] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < NG; ++t) zs[e][t] = 0.0f;
+  }
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) o[db] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+  for (int t = 0; t < NG; ++t) ones[t] = f32x4_t{0, 0, 0, 0};
+
+  const Codes<F16> k_codes;
+  const Codes<false> v_codes;
+  // the NG params words of a key, from the stage's K or V params
+  auto params = [&](const uint8_t* at, int hv, int u, bool whole, int key, uint32_t (&w)[NG]) {
+    if constexpr (D == 128) {
+      const u32x4_t r = *reinterpret_cast<const u32x4_t*>(at + 256 * u + 16 * k);
+#pragma unroll
+      for (int t = 0; t < NG; ++t) w[t] = r[t];
+    } else {
+      const u32x2_t r = *reinterpret_cast<const u32x2_t*>(at + 512 * (u & 1) + 256 * hv + 16 * k + 8 * (u >> 1));
+      w[0] = r[0];
+      w[1] = r[1];
+    }
+    if (!whole) {
+#pragma unroll
+      for (int t = 0; t < NG; ++t) w[t] = key < part.count ? w[t] : 0u;
+    }
+  };
+  int st = 0;
+  for (int c = wave; c < chunks; c += kWaves, st ^= 1) {
+    __builtin_amdgcn_s_waitcnt(0x0F7A);  // vmcnt(10)
+    uint8_t* s = sm[wave][st];
+    complete<D, CH>(p, part, in, c, g, lane, s);
+    const bool whole = (c + 1) * CH <= fewest;
+    const int key0 = c * CH + key_of_lane(k);
+
+    float x[HV][4][4];  // [half][step][vector]
+#pragma unroll
+    for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int key = key0 + 64 * hv + key_of_step(u);
+        uint32_t kp[NG];
+        params(s + kKp, hv, u, whole, key, kp);
+        f32x4_t y = {0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < NG; ++t) {
+          const uint32_t kw = *reinterpret_cast<const uint32_t*>(
+              s + (D == 128 ? kread[t] + 512 * (u & 1) + 256 * (u >> 1) : kread[u >> 1] + 2048 * hv + 256 * (u & 1) + 16 * t));
+          const f32x4_t acc = mma16<F16>(qa[t], k_codes(kw), f32x4_t{0, 0, 0, 0});
+          const float sc = f16_lo(kp[t]) * p.c, zc = fmaf(-16.0f, f16_lo(kp[t]), f16_hi(kp[t])) * p.c;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = fmaf(sc, acc[e], fmaf(zc, qs[t][e], y[e]));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[hv][u][e] = whole || key < lim[e] ? y[e] : -__builtin_huge_valf();
+      }
+    float pr[HV][4][4];
+    bool over = false;
+#pragma unroll
+    for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          pr[hv][u][e] = fast_exp2(x[hv][u][e] - m[e]);
+          over |= !(pr[hv][u][e] <= kOver);
+        }
+    if (__builtin_amdgcn_ballot_w64(over)) {
+      float alpha[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float mx = x[0][0][e];
+#pragma unroll
+        for (int i = 1; i < 4 * HV; ++i) mx = fmaxf(mx, x[i >> 2][i & 3][e]);
+        const float mn = fmaxf(m[e], row_max(mx));
+        alpha[e] = fast_exp2(m[e] - mn);
+        m[e] = mn;
+        l[e] *= alpha[e];
+#pragma unroll
+        for (int i = 0; i < 4 * HV; ++i) pr[i >> 2][i & 3][e] = fast_exp2(x[i >> 2][i & 3][e] - mn);
+#pragma unroll
+        for (int t = 0; t < NG; ++t) zs[e][t] *= alpha[e];
+      }
+      // column k of the sums is vector k, whose maximum quarter k >> 2 keeps as its element k & 3
+      float al[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) al[e] = __shfl(alpha[e], 16 * (k >> 2));
+      const float ac = k & 2 ? (k & 1 ? al[3] : al[2]) : (k & 1 ? al[1] : al[0]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+#pragma unroll
+        for (int t = 0; t < NG; ++t) ones[t][e] *= ac;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) o[db][e] *= ac;
+      }
+    }
+#pragma unroll
+    for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) l[e] += pr[hv][u][e];
+
+    // (column group, half) blocks: probabilities times scales into LDS, [vector][key], then that group's columns
+#pragma unroll
+    for (int i0 = 0; i0 < NG * HV; i0 += AT) {
+      wave_fence();
+#pragma unroll
+      for (int i = i0; i < i0 + AT; ++i) {
+        const int t = i / HV, hv = i % HV;
+        float q[4][4], zz[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uint32_t vp[NG];
+          params(s + kVp, hv, u, whole, key0 + 64 * hv + key_of_step(u), vp);
+          const float sc = f16_lo(vp[t]);
+          zz[u] = fmaf(8.0f, sc, f16_hi(vp[t]));  // the sums take 24 off every code
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            q[e][u] = pr[hv][u][e] * sc;
+            zs[e][t] = fmaf(pr[hv][u][e], zz[u], zs[e][t]);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) put_terms<TWO>(q[e], s + (i - i0) * PBLK + (4 * a + e) * PROW + 8 * k, PBLK);
+      }
+      wave_fence();
+#pragma unroll
+      for (int i = i0; i < i0 + AT; ++i) {
+        const int t = i / HV, hv = i % HV;
+        const uint8_t* src = s + (i - i0) * PBLK + k * PROW + 32 * a;
+        bf16x8_t pb[2], pl[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          pb[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 16 * j));
+          ones[t] = mma16_bf16(fragment_of_ones<false>(), pb[j], ones[t]);
+          if constexpr (TWO) {
+            pl[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + PBLK + 16 * j));
+            ones[t] = mma16_bf16(fragment_of_ones<false>(), pl[j], ones[t]);
+          }
+        }
+#pragma unroll
+        for (int db = 2 * t; db < 2 * t + 2; ++db) {
+          const v2i_t r = read_tr4(s + kVq + v_block_at<D>(k, a, hv, db));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const bf16x8_t vf = v_codes((uint32_t)(j ? r.y : r.x));
+            o[db] = mma16_bf16(vf, pb[j], o[db]);
+            if constexpr (TWO) o[db] = mma16_bf16(vf, pl[j], o[db]);
           }
         }
       }
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     wave_fence();
+    in.fetch(s, c + 2 * kWaves);
   }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
 
-  // the wave's state to its own LDS (all of its loads have landed): per vector m, l, the minima's part per group, o
-  constexpr int NV = 4 * NB;
-  float* mine = reinterpret_cast<float*>(sm[wave]);
-  float* const mm = mine, *const ll = mine + NV, *const zz = mine + 2 * NV, *const oo = mine + 2 * NV + NG * NV;
+  WaveState<D, kVecs>* mine = reinterpret_cast<WaveState<D, kVecs>*>(sm[wave]);
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
+  for (int e = 0; e < 4; ++e) {
+    const float sum = row_sum(l[e]);
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      float sum = row_sum(l[b][w]);
-      if constexpr (D == 64) sum = xhalf_sum(sum);
-      const int v = 4 * b + (D == 128 ? a : (a & 1) + 2 * w);
-      if (k == 0) {
-        mm[v] = m[b][w];
-        ll[v] = sum;
-      }
-#pragma unroll
-      for (int t = 0; t < NG; ++t) {
-        float z = row_sum(zs[b][NG * w + t]);
-        if constexpr (D == 64) z = xhalf_sum(z);
-        if (k == 0) zz[NG * v + t] = z;
-      }
+    for (int t = 0; t < NG; ++t) {
+      const float z = row_sum(zs[e][t]);
+      if (k == 0) mine->z[4 * a + e][t] = z;
     }
-#pragma unroll
-    for (int db = 0; db < NDB; ++db)
-      if ((k >> 2) == db / 2) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) oo[(4 * b + (k & 3)) * D + 16 * db + 4 * a + e] = fmaf(-24.0f, ones[b][e], o[b][db][e]);
-      }
-  }
-  __syncthreads();
-  for (int i = tid; i < R * D; i += kThreads) {
-    const int r = i / D, d = i % D, v = v0 + r, t = v / G, hd = g * G + v % G;
-    float M = -1.0e30f, L = 0.0f, O = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, reinterpret_cast<const float*>(sm[w])[r]);
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float* f = reinterpret_cast<const float*>(sm[w]);
-      const float wt = fast_exp2(f[r] - M);
-      L += wt * f[NV + r];
-      O += wt * (f[2 * NV + NG * NV + r * D + d] + f[2 * NV + NG * r + d / kGroup]);
-    }
-    if (p.n_splits == 1) {
-      p.out[t * p.so0 + hd * p.so1 + d] = to16<F16>(L > 0.0f ? O / L : 0.0f);
-    } else {
-      float* dst = p.part + (((int64_t)t * p.H + hd) * p.n_splits + split) * (D + 2);
-      dst[d] = O;
-      if (d == 0) { dst[D] = M; dst[D + 1] = L; }
+    if (k == 0) {
+      mine->m[4 * a + e] = m[e];
+      mine->l[4 * a + e] = sum;
     }
   }
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) {
+    f32x4_t r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = fmaf(-24.0f, ones[db / 2][e], o[db][e]);
+    *reinterpret_cast<f32x4_t*>(&mine->o[k][16 * db + 4 * a]) = r;
+  }
+  finish<D, F16, kVecs>(p, sm, R, v0, g, split, tid);
 }
 
 // The partials of the live splits under one maximum: a workgroup per (query vector, 16 columns), thread (column, lane group)
@@ -632,7 +935,11 @@ template <int D, bool F16>
 __global__ __launch_bounds__(kMergeCols * kMergeGroups) void int4_merge_kernel(Int4DecodeParams p) {
   __shared__ float sm_m[kMergeGroups], sm_l[kMergeGroups], sm_o[kMergeGroups][kMergeCols];
   const int v = blockIdx.x, dl = threadIdx.x % kMergeCols, grp = threadIdx.x / kMergeCols, d = kMergeCols * blockIdx.y + dl;
-  const int64_t n = live_length(p), len = split_keys(n, p.n_splits);
+  int64_t n = p.n, len = p.len;
+  if (p.n_dev) {
+    n = live_length(p, *p.n_dev);
+    len = split_keys(p, n);
+  }
   const int live = (int)((n + len - 1) / len);
   const float* base = p.part + (int64_t)v * p.n_splits * (D + 2);
   float M = -1.0e30f, L = 0.0f, O = 0.0f;
@@ -679,20 +986,14 @@ __global__ __launch_bounds__(kMergeCols * kMergeGroups) void int4_merge_kernel(I
   }
 }
 
-// The step's new rows in a launch of their own, where several passes read them.
-template <int D>
-__global__ __launch_bounds__(kThreads) void int4_append_kernel(Int4DecodeParams p) {
-  append_rows<D>(p, p.n_dev ? *p.n_dev : p.n, 0, p.cap, blockIdx.x, threadIdx.x);
-}
-
 template <int D, bool F16>
 hipError_t launch_decode_t(const Int4DecodeParams& p, hipStream_t stream) {
-  const int vecs = p.T * (p.H / p.Hkv), passes = (vecs + kVecs - 1) / kVecs;
-  if (p.knew && passes > 1) hipLaunchKernelGGL(int4_append_kernel<D>, dim3(p.Hkv), dim3(kThreads), 0, stream, p);
-  const dim3 grid(p.n_splits, p.Hkv, passes);
-  if (vecs <= 4) hipLaunchKernelGGL((int4_decode_kernel<D, F16, 1, F16>), grid, dim3(kThreads), 0, stream, p);
-  else if (vecs <= 8) hipLaunchKernelGGL((int4_decode_kernel<D, F16, 2, F16>), grid, dim3(kThreads), 0, stream, p);
-  else hipLaunchKernelGGL((int4_decode_kernel<D, F16, 4, F16>), grid, dim3(kThreads), 0, stream, p);
+  const int vecs = p.T * p.G;
+  if (vecs <= 4)
+    hipLaunchKernelGGL((int4_decode_kernel<D, F16, F16>), dim3(p.n_splits, p.Hkv), dim3(kThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL((int4_decode_wide_kernel<D, F16, F16>), dim3(p.n_splits, p.Hkv, (vecs + kVecs - 1) / kVecs),
+                       dim3(kThreads), 0, stream, p);
   if (p.n_splits > 1)
     hipLaunchKernelGGL((int4_merge_kernel<D, F16>), dim3(p.T * p.H, D / kMergeCols),
                        dim3(kMergeCols * kMergeGroups), 0, stream, p);

@@ -127,12 +127,15 @@ struct Int4DecodeParams {
   uint16_t* out;         // [T, H, D] (strides so0, so1)
   float* part;           // [T, H][n_splits][D + 2]
   const int64_t* n_dev;  // length in device memory, or null (then n)
-  int64_t n, cap;
+  int64_t n, cap, len;   // len: keys of a split (without n_dev)
   int64_t sq0, sq1, skq, skp, svq, svp, skn0, skn1, svn0, svn1, so0, so1;
   int T, H, Hkv, D, f16, causal, n_splits;
+  int G;                 // H / Hkv
+  float inv_G;
+  double inv_splits;     // 1 / n_splits
   float c;               // scale * log2(e)
 };
-constexpr int64_t kInt4MinSplit = 256;  // keys of a split, at least
+constexpr int64_t kInt4MinSplit = 256;  // keys of a split, at least (splits are whole 16 keys)
 hipError_t launch_int4_decode(const Int4DecodeParams& p, hipStream_t stream);
 
 // A decode step's new K / V row folded into the first kernel that reads the cache: the row at position n - 1 (n the
