@@ -341,10 +341,11 @@ int bb_rope_inplace(void* x, const int64_t* sx, int B, int Hh, int64_t T, int D,
 /*
  * KV cache in 4 bits (the reference has compressed caches of its own format, modal_rd/turbo_kv.py; this one is new).
  *
- * Format. A row of D elements (D = 32, 64, 128 or 256) is D / 32 groups of 32 consecutive elements. Per group, on values
- * clamped to +-65504 and with NaN taken as 0, each operation in fp32:
- *   z = fp16(min),  s = fp16(max((max - z) / 15, 0)),  code = rint((x - z) / s) clamped to 0 .. 15 (0 where s = 0);
- * the value of an element is s * code + z in fp32. Byte b of a packed row holds element 2 b in its low and 2 b + 1 in its
+ * Format. A row of D elements (D = 32, 64, 128 or 256) is D / 32 groups of 32 consecutive elements. Per group, with min and
+ * max clamped to +-65504 and NaN left out of them, each operation in fp32:
+ *   z = fp16(min),  s = fp16(max((max - z) / 15, 0)),  code = rint((x - z) / s) clamped to 0 .. 15 (0 where s = 0 or x is
+ *   NaN);
+ * the value of an element is s * code + z in fp32. A group of NaN alone has s = z = 0. Byte b of a packed row holds element 2 b in its low and 2 b + 1 in its
  * high four bits.
  * A cache is codes [heads, cap, D / 2] bytes and params [heads, cap, D / 32, 2] fp16 (s, z), for K and for V: the rows of
  * one head are contiguous, heads are sc[] apart. sc[4] = head strides of kq (bytes, a multiple of 16), kp (fp16 elements,

@@ -6,13 +6,17 @@ def quantize(x):
     """x [..., t, d] (any float type) -> codes [..., t, d] (0..15), s and z [..., t, d / 32], all float64: the format's fp32
     and fp16 roundings, every quantity in 64 bits between them."""
     r32 = lambda y: y.to(torch.float32).double()  # noqa: E731
-    w = x.double()
-    w = torch.where(torch.isnan(w), torch.zeros_like(w), w).clamp(-65504.0, 65504.0).unflatten(-1, (-1, 32))
-    z = w.amin(-1).to(torch.float16).double()
-    s = r32(r32(w.amax(-1) - z) / 15).clamp_min(0).to(torch.float16).double()
+    w = x.double().unflatten(-1, (-1, 32))
+    nan = torch.isnan(w)
+    lo = torch.where(nan, torch.inf, w).amin(-1)
+    hi = torch.where(nan, -torch.inf, w).amax(-1)
+    some = lo <= hi
+    lo, hi = (torch.where(some, y.clamp(-65504.0, 65504.0), 0.0) for y in (lo, hi))
+    z = lo.to(torch.float16).double()
+    s = r32(r32(hi - z) / 15).clamp_min(0).to(torch.float16).double()
     safe = torch.where(s > 0, s, torch.ones_like(s))
     code = torch.round(r32(r32(w - z[..., None]) / safe[..., None])).clamp(0, 15)
-    code = torch.where(s[..., None] > 0, code, torch.zeros_like(code))
+    code = torch.where((s[..., None] > 0) & ~nan, code, torch.zeros_like(code))
     return code.flatten(-2), s, z
 
 

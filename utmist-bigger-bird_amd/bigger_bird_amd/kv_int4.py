@@ -3,9 +3,9 @@
 The reference keeps compressed caches in formats of its own (modal_rd/turbo_kv.py); this one is new, and reaches the same
 places: an HF cache layer (`make_int4_cache`, next to `make_int8_cache`) whose handles RDAttention attends with `attend`.
 
-Format: asymmetric per token, KV head and group of 32 elements. On values clamped to +-65504, with NaN taken as 0, each
-operation in fp32: z = fp16(min), s = fp16(max((max - z) / 15, 0)), code = rint((x - z) / s) clamped to 0..15 (0 where
-s = 0); the value is s * code + z in fp32. Byte b of a packed row holds element 2 b (low four bits) and 2 b + 1. A cache
+Format: asymmetric per token, KV head and group of 32 elements. With min and max clamped to +-65504 and NaN left out of
+them, each operation in fp32: z = fp16(min), s = fp16(max((max - z) / 15, 0)), code = rint((x - z) / s) clamped to 0..15
+(0 where s = 0 or x is NaN; a group of NaN alone has s = z = 0); the value is s * code + z in fp32. Byte b of a packed row holds element 2 b (low four bits) and 2 b + 1. A cache
 is codes [Hkv, capacity, d / 2] uint8 and params [Hkv, capacity, d / 32, 2] fp16 (s, z), head-major, for K and for V:
 80 bytes a row at head_dim 128, against 130 in int8 and 256 in bf16.
 """

@@ -912,7 +912,8 @@ static int int4_cache_check(const char* what, const void* kq, const void* kp, co
 static int int4_rows_check(const char* what, int heads, int64_t rows, int D, int kind) {
   if (D != 32 && D != 64 && D != 128 && D != 256) return fail("%s: head_dim %d unsupported", what, D);
   if (kind < 0 || kind > 2) return fail("%s: element kind %d unsupported (0 bf16, 1 fp32, 2 fp16)", what, kind);
-  if (heads < 0 || heads > 65535 || rows < 0 || rows > (int64_t)0xffffff00 / (D / 8))
+  // a launch counts its threads in 32 bits: 16 elements each, in blocks of 256
+  if (heads < 0 || heads > 65535 || rows < 0 || rows > (int64_t)1 << 40 || cdiv(rows * D, 4096) * heads > 0xffffff)
     return fail("%s: %d heads of %lld rows out of range", what, heads, (long long)rows);
   return BB_OK;
 }

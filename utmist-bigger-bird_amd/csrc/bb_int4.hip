@@ -1,8 +1,8 @@
 // KV cache in 4 bits: the write, the read back, and the exact attention of a few query tokens over the packed rows.
 //
-// A row of D elements is D / 32 groups of 32. Per group, on values clamped to +-65504 (NaN counts as 0):
-//   z = fp16(min), s = fp16(max((max - z) / 15, 0)), code = rint((x - z) / s) clamped to 0..15 (0 where s = 0),
-// each operation in fp32; the value is s * code + z in fp32 (s * code is exact). s and z are rounded before the codes are
+// A row of D elements is D / 32 groups of 32. Per group, with min and max clamped to +-65504 and NaN left out of them:
+//   z = fp16(min), s = fp16(max((max - z) / 15, 0)), code = rint((x - z) / s) clamped to 0..15 (0 where s = 0 or x is NaN),
+// each operation in fp32; the value is s * code + z in fp32 (s * code is exact). A group of NaN alone has s = z = 0. s and z are rounded before the codes are
 // taken, so the codes make up for their rounding. Byte b of a packed row holds elements 2 b (low four bits) and 2 b + 1.
 //
 // The cache is head-major, codes [Hkv, cap, D / 2] and params [Hkv, cap, D / 32] of (s, z): the rows of one KV head are
@@ -23,49 +23,85 @@ BB_DEV float f16_lo(uint32_t w) { return (float)__builtin_bit_cast(_Float16, (ui
 BB_DEV float f16_hi(uint32_t w) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16)); }
 BB_DEV uint32_t f16_bits(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }  // round to nearest even
 
-// Eight elements of a row at x (16-byte aligned), in fp32.
-BB_DEV void load8(const void* x, int64_t off, int kind, float (&v)[8]) {
-  if (kind == kKindF32) {
-    const float* p = reinterpret_cast<const float*>(x) + off;
-    const f32x4_t a = *reinterpret_cast<const f32x4_t*>(p), b = *reinterpret_cast<const f32x4_t*>(p + 4);
+// N (a multiple of 8) elements of a row at x (16-byte aligned), in fp32.
+template <int KIND, int N>
+BB_DEV void load_row(const void* x, int64_t off, float (&v)[N]) {
+  if constexpr (KIND == kKindF32) {
+    const f32x4_t* p = reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(x) + off);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+    for (int j = 0; j < N / 4; ++j) {
+      const f32x4_t a = p[j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * j + i] = a[i];
+    }
   } else {
-    const u32x4_t a = ld16(reinterpret_cast<const uint16_t*>(x) + off);
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(x) + off;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = kind == kKindF16 ? f16_lo(a[i]) : bf16_to_f32((uint16_t)(a[i] & 0xffffu));
-      v[2 * i + 1] = kind == kKindF16 ? f16_hi(a[i]) : bf16_to_f32((uint16_t)(a[i] >> 16));
+    for (int j = 0; j < N / 8; ++j) {
+      const u32x4_t a = ld16(p + 8 * j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[8 * j + 2 * i] = KIND == kKindF16 ? f16_lo(a[i]) : __uint_as_float(a[i] << 16);
+        v[8 * j + 2 * i + 1] = KIND == kKindF16 ? f16_hi(a[i]) : __uint_as_float(a[i] & 0xffff0000u);
+      }
     }
   }
 }
 
-// Quantises the 8 elements v of a lane; the 4 lanes of an aligned quad hold one group and all take part. Returns the 8
-// codes, little-endian, and the group's (s, z) as packed fp16.
-BB_DEV uint32_t quant8_4bit(float (&v)[8], uint32_t& param) {
-  float lo = kF16Max, hi = -kF16Max;
+// Quantises the N elements v of a lane (8 or 16; the 32 / N lanes of a group are neighbours and all take part): their codes,
+// little-endian, and the group's (s, z) as packed fp16.
+//   * (max - z) / 15 is the correctly rounded quotient: one step of Newton's iteration on the residual, which an fma gives
+//     exactly, with the correctly rounded reciprocal of 15.
+//   * rint((x - z) / s) is taken from the product with the reciprocal, which is within 2^-18 of the quotient as long as that is
+//     below 16 (and past 15 either way where it is not): both round to the same integer unless the product lies within 2^-17
+//     of a half. A lane that holds such an element (one in 4000) takes the divisions.
+template <int N>
+BB_DEV void quant_4bit(const float (&v)[N], uint32_t (&w)[N / 8], uint32_t& param) {
+  float lo = __builtin_huge_valf(), hi = -__builtin_huge_valf();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[i] = v[i] == v[i] ? fminf(fmaxf(v[i], -kF16Max), kF16Max) : 0.0f;
+  for (int i = 0; i < N; ++i) {  // NaN operands are passed over
     lo = fminf(lo, v[i]);
     hi = fmaxf(hi, v[i]);
   }
   lo = fminf(lo, dpp_mov<0xB1>(lo));
   hi = fmaxf(hi, dpp_mov<0xB1>(hi));
-  lo = fminf(lo, dpp_mov<0x4E>(lo));
-  hi = fmaxf(hi, dpp_mov<0x4E>(hi));
+  if constexpr (N == 8) {
+    lo = fminf(lo, dpp_mov<0x4E>(lo));
+    hi = fmaxf(hi, dpp_mov<0x4E>(hi));
+  }
+  const bool some = lo <= hi;
+  lo = some ? fminf(fmaxf(lo, -kF16Max), kF16Max) : 0.0f;
+  hi = some ? fminf(fmaxf(hi, -kF16Max), kF16Max) : 0.0f;
   const uint32_t zb = f16_bits(lo);
   const float z = f16_lo(zb);
-  const uint32_t sb = f16_bits(fmaxf((hi - z) / 15.0f, 0.0f));
+  const float range = fmaxf(hi - z, 0.0f), q15 = range * (1.0f / 15.0f);
+  const uint32_t sb = f16_bits(fmaf(fmaf(-15.0f, q15, range), 1.0f / 15.0f, q15));
   const float s = f16_lo(sb);
   param = sb | (zb << 16);
-  uint32_t w = 0;
+  const float inv = s > 0.0f ? __builtin_amdgcn_rcpf(s) : 0.0f;
+  float half = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = s > 0.0f ? fminf(fmaxf(rintf((v[i] - z) / s), 0.0f), 15.0f) : 0.0f;
-    w |= (uint32_t)c << (4 * i);
+  for (int j = 0; j < N / 8; ++j) {
+    float part[2] = {0.0f, 0.0f};  // four codes each, exact in fp32
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float t = (v[8 * j + i] - z) * inv, c = rintf(t);
+      half = fmaxf(half, fabsf(t - c));
+      part[i / 4] = fmaf(__builtin_amdgcn_fmed3f(c, 0.0f, 15.0f), (float)(1 << (4 * (i % 4))), part[i / 4]);
+    }
+    w[j] = (uint32_t)part[0] | ((uint32_t)part[1] << 16);
   }
-  return w;
+  if (half > 0.5f - 0x1p-17f) {
+#pragma unroll
+    for (int j = 0; j < N / 8; ++j) {
+      w[j] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float c = s > 0.0f ? rintf((v[8 * j + i] - z) / s) : 0.0f;
+        w[j] |= (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * i);
+      }
+    }
+  }
 }
 
 struct Int4Set {  // one tensor's rows and their place in the cache
@@ -76,20 +112,22 @@ struct Int4Set {  // one tensor's rows and their place in the cache
   int64_t sq0, sp0;  // head strides of q (bytes) and p (groups)
 };
 
-// A lane takes 8 elements of a row; blockIdx.y is the head, blockIdx.z the tensor (K, V).
-template <int D>
-__global__ __launch_bounds__(256) void int4_quantize_kernel(Int4Set s0, Int4Set s1, int kind, int64_t rows) {
-  const Int4Set& s = blockIdx.z ? s1 : s0;
-  constexpr int LPR = D / 8;
-  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  const int c = threadIdx.x % LPR, h = blockIdx.y;
+// A lane takes half a group (16 elements) of a row; blockIdx.x counts heads within blocks of rows, so that the rows of a
+// token's heads, which neighbour each other where a projection left them, are read at about the same time; blockIdx.y is the
+// tensor (K, V).
+template <int D, int KIND>
+__global__ __launch_bounds__(256) void int4_quantize_kernel(Int4Set s0, Int4Set s1, int heads, int64_t rows) {
+  const Int4Set& s = blockIdx.y ? s1 : s0;
+  constexpr int LPR = D / 16;
+  const int h = blockIdx.x % (unsigned)heads, c = threadIdx.x % LPR;
+  const int64_t row = (int64_t)(blockIdx.x / (unsigned)heads) * (256 / LPR) + threadIdx.x / LPR;
   if (row >= rows) return;  // the lanes of a row leave together
-  float v[8];
-  load8(s.x, h * s.sx0 + row * s.sx1 + 8 * c, kind, v);
-  uint32_t param;
-  const uint32_t w = quant8_4bit(v, param);
-  *reinterpret_cast<uint32_t*>(s.q + h * s.sq0 + row * (D / 2) + 4 * c) = w;
-  if (c % 4 == 0) s.p[h * s.sp0 + row * (D / kGroup) + c / 4] = param;
+  float v[16];
+  load_row<KIND>(s.x, h * s.sx0 + row * s.sx1 + 16 * c, v);
+  uint32_t param, w[2];
+  quant_4bit(v, w, param);
+  *reinterpret_cast<u32x2_t*>(s.q + h * s.sq0 + row * (D / 2) + 8 * c) = u32x2_t{w[0], w[1]};
+  if (c % 2 == 0) s.p[h * s.sp0 + row * (D / kGroup) + c / 2] = param;
 }
 
 struct Int4ReadSet {
@@ -267,7 +305,7 @@ BB_DEV int param_at(int key) {
 // The step's new rows among the keys [first, first + CH) of the split (fewer than `count`): quantised into the chunk in
 // LDS, over what the cache held there, and by the first pass into the cache. No other chunk holds them, so nothing waits
 // for the stores.
-template <int D, int CH>
+template <int D, bool F16, int CH>
 BB_DEV void append_rows(const Int4DecodeParams& p, int64_t raw, int64_t begin, int first, int count, int g, int lane,
                         uint8_t* s) {
   constexpr int LPR = D / 8;
@@ -277,10 +315,11 @@ BB_DEV void append_rows(const Int4DecodeParams& p, int64_t raw, int64_t begin, i
     const int64_t row = raw - p.T + t, at = row - begin;
     if (at < first || at >= first + CH || at >= count) continue;
     float v[8];
-    load8(vt ? p.vnew : p.knew, vt ? g * p.svn0 + t * p.svn1 + 8 * c : g * p.skn0 + t * p.skn1 + 8 * c,
-          p.f16 ? kKindF16 : kKindBf16, v);
-    uint32_t param;
-    const uint32_t w = quant8_4bit(v, param);
+    load_row<F16 ? kKindF16 : kKindBf16>(vt ? p.vnew : p.knew,
+                                         vt ? g * p.svn0 + t * p.svn1 + 8 * c : g * p.skn0 + t * p.skn1 + 8 * c, v);
+    uint32_t param, codes[1];
+    quant_4bit(v, codes, param);
+    const uint32_t w = codes[0];
     const int key = (int)at - first;
     *reinterpret_cast<uint32_t*>(s + (vt ? kVq + v_code_at<D>(key, c / 4) : k_code_at<D>(key, c / 4)) + 4 * (c % 4)) = w;
     if (c % 4 == 0) *reinterpret_cast<uint32_t*>(s + (vt ? kVp : kKp) + param_at<D>(key) + c) = param;
@@ -370,7 +409,7 @@ struct Part {
 };
 
 // A landed chunk made ready for the reads: the params that no load brought, and the new rows.
-template <int D, int CH>
+template <int D, bool F16, int CH>
 BB_DEV void complete(const Int4DecodeParams& p, const Part& part, const Stream<D>& in, int c, int g, int lane, uint8_t* s) {
   wave_fence();
   if constexpr (D == 64) {
@@ -381,7 +420,7 @@ BB_DEV void complete(const Int4DecodeParams& p, const Part& part, const Stream<D
     }
   }
   if ((c + 1) * CH > part.new_first)
-    append_rows<D, CH>(p, part.raw, part.begin, c * CH, part.count, g, lane, s);
+    append_rows<D, F16, CH>(p, part.raw, part.begin, c * CH, part.count, g, lane, s);
   wave_fence();
 }
 
@@ -523,7 +562,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
   for (int c = wave; c < chunks; c += kWaves, st ^= 1) {
     __builtin_amdgcn_s_waitcnt(0x0F7A);  // vmcnt(10): all but the next chunk's ten loads have landed
     uint8_t* s = sm[wave][st];
-    complete<D, CH>(p, part, in, c, g, lane, s);
+    complete<D, F16, CH>(p, part, in, c, g, lane, s);
     const bool whole = (c + 1) * CH <= fewest;
 
     float x[W][4];
@@ -776,7 +815,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
   for (int c = wave; c < chunks; c += kWaves, st ^= 1) {
     __builtin_amdgcn_s_waitcnt(0x0F7A);  // vmcnt(10)
     uint8_t* s = sm[wave][st];
-    complete<D, CH>(p, part, in, c, g, lane, s);
+    complete<D, F16, CH>(p, part, in, c, g, lane, s);
     const bool whole = (c + 1) * CH <= fewest;
     const int key0 = c * CH + key_of_lane(k);
 
@@ -1006,20 +1045,28 @@ dim3 row_grid(int D, int heads, int64_t rows, bool two) {
 
 }  // namespace
 
+template <int D>
+static hipError_t launch_quantize_d(const Int4Set& s0, const Int4Set& s1, bool two, int kind, int heads, int64_t rows,
+                                    hipStream_t stream) {
+  const dim3 grid((unsigned)((rows + 4096 / D - 1) / (4096 / D) * heads), two ? 2u : 1u);
+  if (kind == kKindF32) hipLaunchKernelGGL((int4_quantize_kernel<D, kKindF32>), grid, dim3(256), 0, stream, s0, s1, heads, rows);
+  else if (kind == kKindF16) hipLaunchKernelGGL((int4_quantize_kernel<D, kKindF16>), grid, dim3(256), 0, stream, s0, s1, heads, rows);
+  else hipLaunchKernelGGL((int4_quantize_kernel<D, kKindBf16>), grid, dim3(256), 0, stream, s0, s1, heads, rows);
+  return hipGetLastError();
+}
+
 hipError_t launch_int4_quantize(const Int4Rows& k, const Int4Rows* v, int kind, int heads, int64_t rows, int D,
                                 hipStream_t stream) {
   if (rows <= 0 || heads <= 0) return hipSuccess;
   const Int4Set s0{k.x, k.q, k.p, k.sx0, k.sx1, k.sq0, k.sp0};
   const Int4Set s1 = v ? Int4Set{v->x, v->q, v->p, v->sx0, v->sx1, v->sq0, v->sp0} : s0;
-  const dim3 grid = row_grid(D, heads, rows, v != nullptr);
   switch (D) {
-    case 32: hipLaunchKernelGGL(int4_quantize_kernel<32>, grid, dim3(256), 0, stream, s0, s1, kind, rows); break;
-    case 64: hipLaunchKernelGGL(int4_quantize_kernel<64>, grid, dim3(256), 0, stream, s0, s1, kind, rows); break;
-    case 128: hipLaunchKernelGGL(int4_quantize_kernel<128>, grid, dim3(256), 0, stream, s0, s1, kind, rows); break;
-    case 256: hipLaunchKernelGGL(int4_quantize_kernel<256>, grid, dim3(256), 0, stream, s0, s1, kind, rows); break;
+    case 32: return launch_quantize_d<32>(s0, s1, v != nullptr, kind, heads, rows, stream);
+    case 64: return launch_quantize_d<64>(s0, s1, v != nullptr, kind, heads, rows, stream);
+    case 128: return launch_quantize_d<128>(s0, s1, v != nullptr, kind, heads, rows, stream);
+    case 256: return launch_quantize_d<256>(s0, s1, v != nullptr, kind, heads, rows, stream);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 hipError_t launch_int4_dequantize(const Int4Rows& k, const Int4Rows* v, int kind, int heads, int64_t rows, int D,
