@@ -52,11 +52,11 @@ BB_DEV void load_row(const void* x, int64_t off, float (&v)[N]) {
 // little-endian, and the group's (s, z) as packed fp16.
 //   * (max - z) / 15 is the correctly rounded quotient: one step of Newton's iteration on the residual, which an fma gives
 //     exactly, with the correctly rounded reciprocal of 15.
-//   * rint((x - z) / s) is taken from the product with the reciprocal, which is within 2^-18 of the quotient as long as that is
-//     below 16 (and past 15 either way where it is not): both round to the same integer unless the product lies within 2^-17
-//     of a half. A lane that holds such an element (one in 4000) takes the divisions.
+//   * (x - z) / s likewise, with the hardware's reciprocal: off the correctly rounded quotient at most where that is far from
+//     a half (tried for every fp16 s, reciprocals off by up to 2 ulps and 40 floats to each side of every half).
+// v holds infinities and values past fp16's range until the rare branch puts them in it (the residual of an infinity is NaN).
 template <int N>
-BB_DEV void quant_4bit(const float (&v)[N], uint32_t (&w)[N / 8], uint32_t& param) {
+BB_DEV void quant_4bit(float (&v)[N], uint32_t (&w)[N / 8], uint32_t& param) {
   float lo = __builtin_huge_valf(), hi = -__builtin_huge_valf();
 #pragma unroll
   for (int i = 0; i < N; ++i) {  // NaN operands are passed over
@@ -70,6 +70,10 @@ BB_DEV void quant_4bit(const float (&v)[N], uint32_t (&w)[N / 8], uint32_t& para
     hi = fmaxf(hi, dpp_mov<0x4E>(hi));
   }
   const bool some = lo <= hi;
+  if (hi > kF16Max) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = v[i] > kF16Max ? kF16Max : v[i];
+  }
   lo = some ? fminf(fmaxf(lo, -kF16Max), kF16Max) : 0.0f;
   hi = some ? fminf(fmaxf(hi, -kF16Max), kF16Max) : 0.0f;
   const uint32_t zb = f16_bits(lo);
@@ -79,28 +83,16 @@ BB_DEV void quant_4bit(const float (&v)[N], uint32_t (&w)[N / 8], uint32_t& para
   const float s = f16_lo(sb);
   param = sb | (zb << 16);
   const float inv = s > 0.0f ? __builtin_amdgcn_rcpf(s) : 0.0f;
-  float half = 0.0f;
 #pragma unroll
   for (int j = 0; j < N / 8; ++j) {
     float part[2] = {0.0f, 0.0f};  // four codes each, exact in fp32
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float t = (v[8 * j + i] - z) * inv, c = rintf(t);
-      half = fmaxf(half, fabsf(t - c));
+      const float d = v[8 * j + i] - z, t = d * inv, c = rintf(fmaf(fmaf(-t, s, d), inv, t));
+      // (NaN comes out of the median as 0)
       part[i / 4] = fmaf(__builtin_amdgcn_fmed3f(c, 0.0f, 15.0f), (float)(1 << (4 * (i % 4))), part[i / 4]);
     }
     w[j] = (uint32_t)part[0] | ((uint32_t)part[1] << 16);
-  }
-  if (half > 0.5f - 0x1p-17f) {
-#pragma unroll
-    for (int j = 0; j < N / 8; ++j) {
-      w[j] = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float c = s > 0.0f ? rintf((v[8 * j + i] - z) / s) : 0.0f;
-        w[j] |= (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * i);
-      }
-    }
   }
 }
 
@@ -137,6 +129,9 @@ struct Int4ReadSet {
   int64_t sq0, sp0;
 };
 
+// The values are stored past the caches (the stores are as fast, and packed rows that lie in the 256 MB cache stay there: K and V
+// of 65536 rows x 8 heads x 128 read back 74 -> 48 us, of 131072 rows 145 -> 140; reading the values next is no slower: at
+// 16 MB of them 10.8 -> 10.6 us for both, at 64 MB 28.6 -> 26.1).
 template <int D>
 __global__ __launch_bounds__(256) void int4_dequantize_kernel(Int4ReadSet s0, Int4ReadSet s1, int kind, int64_t rows) {
   const Int4ReadSet& s = blockIdx.z ? s1 : s0;
@@ -152,15 +147,15 @@ __global__ __launch_bounds__(256) void int4_dequantize_kernel(Int4ReadSet s0, In
   for (int i = 0; i < 8; ++i) v[i] = fmaf(sc, (float)((w >> (4 * i)) & 15u), z);
   const int64_t off = (h * rows + row) * D + 8 * c;
   if (kind == kKindF32) {
-    float* o = reinterpret_cast<float*>(s.out) + off;
-    *reinterpret_cast<f32x4_t*>(o) = f32x4_t{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<f32x4_t*>(o + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+    f32x4_t* o = reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(s.out) + off);
+    __builtin_nontemporal_store(f32x4_t{v[0], v[1], v[2], v[3]}, o);
+    __builtin_nontemporal_store(f32x4_t{v[4], v[5], v[6], v[7]}, o + 1);
   } else {
     u32x4_t o;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       o[i] = kind == kKindF16 ? pack2<true>(v[2 * i], v[2 * i + 1]) : pack2<false>(v[2 * i], v[2 * i + 1]);
-    st16(reinterpret_cast<uint16_t*>(s.out) + off, o);
+    __builtin_nontemporal_store(o, reinterpret_cast<u32x4_t*>(reinterpret_cast<uint16_t*>(s.out) + off));
   }
 }
 
@@ -1039,10 +1034,6 @@ hipError_t launch_decode_t(const Int4DecodeParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-dim3 row_grid(int D, int heads, int64_t rows, bool two) {
-  return dim3((unsigned)((rows + 2048 / D - 1) / (2048 / D)), (unsigned)heads, two ? 2u : 1u);
-}
-
 }  // namespace
 
 template <int D>
@@ -1069,20 +1060,26 @@ hipError_t launch_int4_quantize(const Int4Rows& k, const Int4Rows* v, int kind, 
   }
 }
 
+template <int D>
+static hipError_t launch_dequantize_d(const Int4ReadSet& s0, const Int4ReadSet& s1, bool two, int kind, int heads,
+                                      int64_t rows, hipStream_t stream) {
+  const dim3 grid((unsigned)((rows + 2048 / D - 1) / (2048 / D)), (unsigned)heads, two ? 2u : 1u);
+  hipLaunchKernelGGL(int4_dequantize_kernel<D>, grid, dim3(256), 0, stream, s0, s1, kind, rows);
+  return hipGetLastError();
+}
+
 hipError_t launch_int4_dequantize(const Int4Rows& k, const Int4Rows* v, int kind, int heads, int64_t rows, int D,
                                   hipStream_t stream) {
   if (rows <= 0 || heads <= 0) return hipSuccess;
   const Int4ReadSet s0{k.q, k.p, const_cast<void*>(k.x), k.sq0, k.sp0};
   const Int4ReadSet s1 = v ? Int4ReadSet{v->q, v->p, const_cast<void*>(v->x), v->sq0, v->sp0} : s0;
-  const dim3 grid = row_grid(D, heads, rows, v != nullptr);
   switch (D) {
-    case 32: hipLaunchKernelGGL(int4_dequantize_kernel<32>, grid, dim3(256), 0, stream, s0, s1, kind, rows); break;
-    case 64: hipLaunchKernelGGL(int4_dequantize_kernel<64>, grid, dim3(256), 0, stream, s0, s1, kind, rows); break;
-    case 128: hipLaunchKernelGGL(int4_dequantize_kernel<128>, grid, dim3(256), 0, stream, s0, s1, kind, rows); break;
-    case 256: hipLaunchKernelGGL(int4_dequantize_kernel<256>, grid, dim3(256), 0, stream, s0, s1, kind, rows); break;
+    case 32: return launch_dequantize_d<32>(s0, s1, v != nullptr, kind, heads, rows, stream);
+    case 64: return launch_dequantize_d<64>(s0, s1, v != nullptr, kind, heads, rows, stream);
+    case 128: return launch_dequantize_d<128>(s0, s1, v != nullptr, kind, heads, rows, stream);
+    case 256: return launch_dequantize_d<256>(s0, s1, v != nullptr, kind, heads, rows, stream);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 hipError_t launch_int4_decode(const Int4DecodeParams& p, hipStream_t stream) {
