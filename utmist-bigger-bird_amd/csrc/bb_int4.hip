@@ -167,8 +167,8 @@ __global__ __launch_bounds__(256) void int4_dequantize_kernel(Int4ReadSet s0, In
 //
 // Mathematics. With k = s c + z per group of 32 (c the codes), q.k = sum_g s_g (q_g . c_g) + z_g sum(q_g), and
 // o = sum_j p_j s_j c_j + sum_j p_j z_j per column group: the codes go to the matrix cores as they are, exact in 16 bits, and
-// scales and minima are applied in fp32 to the sums (scores) or to the probabilities (values). A code becomes the 16-bit
-// float 16 + c by one shift and one and-or per two codes; the 16s are taken back from the sums.
+// scales and minima are applied in fp32 to the sums (scores) or to the probabilities (values). A code becomes a 16-bit float
+// base + c by an and-or per two codes (see Codes); the bases are taken back from the sums.
 //
 // A chunk's 10 KB (codes and params of K and of V) stream straight into the wave's LDS with ten buffer loads that cover
 // whole lines, two chunks ahead. Pieces land so that the operand reads meet no bank twice: see the offsets at each. V rows
@@ -207,22 +207,48 @@ BB_DEV f32x4_t mma16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
   else return mma16_bf16(a, b, c);
 }
 
-// Eight codes as 16-bit floats 16 + c, in the order 0, 4, 1, 5, 2, 6, 3, 7 (the halves of the word side by side). 16.0 has
-// an ulp of 1/8 in bf16 and 1/64 in fp16, so a code is a shift away from its place in the mantissa. The constants stay in
-// registers (`mask` scalar, `base` vector), where one v_and_or_b32 takes both; as literals they cost an instruction more.
+// Eight codes as 16-bit floats base + c, in the order 0, 4, 1, 5, 2, 6, 3, 7 (the halves of the word side by side). In fp16
+// 64.0 has an ulp of 1/16: bits 4..7 of a half are a code in its place. In bf16 128.0 has an ulp of 1 (bits 0..3) and 16.0 one
+// of 1/8 (bits 3..6); no place serves two pairs. So of the four pairs three take a shift. The constants stay in registers
+// (masks scalar, bases vector), where one v_and_or_b32 takes both; as literals they cost an instruction more.
 template <bool F16>
 struct Codes {
-  uint32_t mask, base;
-  BB_DEV Codes() : mask(F16 ? 0x03c003c0u : 0x00780078u), base(F16 ? 0x4c004c00u : 0x41804180u) {
+  uint32_t mask0, mask, base0, base;
+  BB_DEV Codes()
+      : mask0(0x000f000fu), mask(F16 ? 0x00f000f0u : 0x00780078u), base0(0x43004300u), base(F16 ? 0x54005400u : 0x41804180u) {
     asm("" : "+s"(mask));
     asm("" : "+v"(base));
+    if constexpr (!F16) {
+      asm("" : "+s"(mask0));
+      asm("" : "+v"(base0));
+    }
   }
   BB_DEV bf16x8_t operator()(uint32_t w) const {
-    constexpr int sh = F16 ? 6 : 3;
-    return as_bf16x8(u32x4_t{((w << sh) & mask) | base, ((F16 ? w << 2 : w >> 1) & mask) | base,
-                             ((w >> (8 - sh)) & mask) | base, ((w >> (12 - sh)) & mask) | base});
+    if constexpr (F16)
+      return as_bf16x8(u32x4_t{((w << 4) & mask) | base, (w & mask) | base, ((w >> 4) & mask) | base, ((w >> 8) & mask) | base});
+    else
+      return as_bf16x8(u32x4_t{(w & mask0) | base0, ((w >> 1) & mask) | base, ((w >> 5) & mask) | base, ((w >> 9) & mask) | base});
+  }
+  // A fragment of the bases themselves, 8 added to each with CENTRE.
+  template <bool CENTRE>
+  BB_DEV static bf16x8_t bases() {
+    if constexpr (F16) return as_bf16x8(u32x4_t{0x54005400u, 0x54005400u, 0x54005400u, 0x54005400u});
+    else if constexpr (CENTRE) return as_bf16x8(u32x4_t{0x43084308u, 0x41c041c0u, 0x41c041c0u, 0x41c041c0u});
+    else return as_bf16x8(u32x4_t{0x43004300u, 0x41804180u, 0x41804180u, 0x41804180u});
   }
 };
+
+// a times the low / high fp16 half of w, in one instruction (fp32 product, rounded once).
+BB_DEV float mul_lo(float a, uint32_t w) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(a), "v"(w));
+  return r;
+}
+BB_DEV float mul_hi(float a, uint32_t w) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "=v"(r) : "v"(a), "v"(w));
+  return r;
+}
 
 // The largest / sum over the 16 lanes of a DPP row, in every lane.
 BB_DEV float row_max(float v) {
@@ -355,24 +381,26 @@ struct Stream {
     kp = p.kp + g * p.skp + begin * (D / kGroup);
     vp = p.vp + g * p.svp + begin * (D / kGroup);
   }
-  // Chunk c into `stage`: always ten loads, so that the counts the waits go by are exact; past the split's last chunk they
-  // read nothing (the buffers' ranges end with it) and land zeros.
-  BB_DEV void fetch(uint8_t* stage, int c) const {
-    auto ld = [&](const void* base, int row_bytes, int at, uint32_t off) {
-      const __amdgpu_buffer_rsrc_t r =
-          __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, count * row_bytes, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          r, reinterpret_cast<lds_void*>(reinterpret_cast<uintptr_t>(stage + at)), 16, off, 0, 0, 2 /* non-temporal */);
-    };
+  // Chunk c's K or V into `stage`: always five loads, so that the counts the waits go by are exact; past the split's last chunk
+  // they read nothing (the buffers' ranges end with it) and land zeros.
+  BB_DEV void fetch_k(uint8_t* stage, int c) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t off = D == 128 ? koff[0] ^ (16 * (-i & 3)) : koff[i & 1];  // head_dim 128: bits 4 and 5 are the piece
-      ld(kq, D / 2, 1024 * i, c * 4096 + 1024 * i + off);
+      load(kq, D / 2, stage + 1024 * i, c * 4096 + 1024 * i + off);
     }
-    ld(kp, D / 8, kKp, c * 1024 + poff);
+    load(kp, D / 8, stage + kKp, c * 1024 + poff);
+  }
+  BB_DEV void fetch_v(uint8_t* stage, int c) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ld(vq, D / 2, kVq + 1024 * i, c * 4096 + 1024 * i + voff);
-    ld(vp, D / 8, kVp, c * 1024 + poff);
+    for (int i = 0; i < 4; ++i) load(vq, D / 2, stage + kVq + 1024 * i, c * 4096 + 1024 * i + voff);
+    load(vp, D / 8, stage + kVp, c * 1024 + poff);
+  }
+  BB_DEV void load(const void* base, int row_bytes, uint8_t* to, uint32_t off) const {
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, count * row_bytes, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, reinterpret_cast<lds_void*>(reinterpret_cast<uintptr_t>(to)), 16, off, 0, 0,
+                                             2 /* non-temporal */);
   }
 };
 
@@ -403,9 +431,11 @@ struct Part {
   }
 };
 
-// A landed chunk made ready for the reads: the params that no load brought, and the new rows.
+// The rest of a split's last chunks, once they have landed: the params that no load brought, and the new rows.
 template <int D, bool F16, int CH>
 BB_DEV void complete(const Int4DecodeParams& p, const Part& part, const Stream<D>& in, int c, int g, int lane, uint8_t* s) {
+  if ((c + 1) * CH <= part.count && (c + 1) * CH <= part.new_first) return;
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): V too
   wave_fence();
   if constexpr (D == 64) {
     // an odd last key's params share their 16-byte piece with a row past the range: read them apart
@@ -485,7 +515,8 @@ BB_DEV void put_terms(const float (&q)[4], uint8_t* dst, int second) {
 //           over its own group. One (s, z) word per lane turns them into scores; three lane swaps sum the groups and
 //           leave lane (k, a) with the whole score of query a alone, so that no lane's exponential is idle.
 //   values  The probabilities times the scales of column group t go to column 4 t + h of the operand, so one product serves
-//           all groups (the columns of a product whose rows are another group are not used). The 16s go with a row of ones.
+//           all groups (the columns of a product whose rows are another group are not used). A row of the bases plus 8 gives
+//           what those add (the products meet codes shifted to -8..7, which halves what a rounded probability costs).
 template <int D, bool F16, bool TWO>
 __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodeParams p) {
   __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][kStage];
@@ -499,7 +530,9 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
   const Part part(p, split);
   if (part.count == 0 && p.n_splits > 1) return;  // no partial: the merge knows the live splits
 
-  // the queries' loads first, the first chunks' right behind them
+  const Stream<D> in(p, g, part.begin, part.count, lane);
+  in.fetch_k(sm[wave][0], wave);
+  in.fetch_v(sm[wave][0], wave);
   u32x4_t qw[4];
   const bool on = (k >> 2) == a && (k & 3) < R;
   {
@@ -508,17 +541,22 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
 #pragma unroll
     for (int j = 0; j < 4; ++j) qw[j] = ld16(qr + 8 * j);
   }
-  const Stream<D> in(p, g, part.begin, part.count, lane);
+  in.fetch_k(sm[wave][1], wave + kWaves);
+  in.fetch_v(sm[wave][1], wave + kWaves);
   const int chunks = (part.count + CH - 1) / CH;
-  in.fetch(sm[wave][0], wave);
-  in.fetch(sm[wave][1], wave + kWaves);
 
   bf16x8_t qa[4];  // fragment i: columns 8 i .. 8 i + 7 of the lane's group
-  f32x4_t qs = {0, 0, 0, 0};  // sums of the queries' groups, where the scores are
+  f32x4_t qs = {0, 0, 0, 0}, qb = {0, 0, 0, 0};  // sums of the queries' groups times p.c, and what the bases add to the products
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     qa[i] = query_fragment(qw[i], on);
     qs = mma16<F16>(qa[i], fragment_of_ones<F16>(), qs);
+    qb = mma16<F16>(qa[i], Codes<F16>::template bases<false>(), qb);
+  }
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    qs[h] *= p.c;
+    qb[h] = -qb[h];
   }
   uint32_t kread[2], kpread, vpread;  // where the reads of a stage start
   if constexpr (D == 128) {
@@ -540,7 +578,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
   const int fewest = part.limit(p, 0);  // the first token's is the smallest
 
   float m[W], l[W], zs[W][NG];
-  f32x4_t o[NDB], ones = {0, 0, 0, 0};
+  f32x4_t o[NDB], base = {0, 0, 0, 0};  // base: what the bases and the 8s add to the sums
 #pragma unroll
   for (int w = 0; w < W; ++w) {
     m[w] = -1.0e30f;
@@ -555,7 +593,8 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
   const Codes<false> v_codes;
   int st = 0;
   for (int c = wave; c < chunks; c += kWaves, st ^= 1) {
-    __builtin_amdgcn_s_waitcnt(0x0F7A);  // vmcnt(10): all but the next chunk's ten loads have landed
+    __builtin_amdgcn_s_waitcnt(0x0F7F);  // vmcnt(15): this chunk's K has landed; its V and the next chunk may be in flight
+    wave_fence();
     uint8_t* s = sm[wave][st];
     complete<D, F16, CH>(p, part, in, c, g, lane, s);
     const bool whole = (c + 1) * CH <= fewest;
@@ -567,13 +606,13 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
       uint32_t kp = *reinterpret_cast<const uint32_t*>(s + kpread + (D == 128 ? 256 * u : 512 * (u & 1) + 8 * (u >> 1)));
       const int key = c * CH + key_k + key_of_step(u);
       if (!whole) kp = key < part.count ? kp : 0u;
-      const float sc = f16_lo(kp) * p.c, zc = fmaf(-16.0f, f16_lo(kp), f16_hi(kp)) * p.c;
-      f32x4_t acc = {0, 0, 0, 0};
+      const float sc = mul_lo(p.c, kp);
+      f32x4_t acc = qb;
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc = mma16<F16>(qa[i], k_codes(kw[i]), acc);
       float y[4];
 #pragma unroll
-      for (int h = 0; h < 4; ++h) y[h] = fmaf(sc, acc[h], zc * qs[h]);
+      for (int h = 0; h < 4; ++h) y[h] = fmaf(sc, acc[h], mul_hi(qs[h], kp));
       if constexpr (D == 128) {
         x[0][u] = sum_rows16(sum_rows32(y[0], y[2]), sum_rows32(y[1], y[3]));
       } else {
@@ -618,11 +657,13 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
       const float ac = k & 2 ? (k & 1 ? al[3] : al[2]) : (k & 1 ? al[1] : al[0]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        ones[e] *= ac;
+        base[e] *= ac;
 #pragma unroll
         for (int db = 0; db < NDB; ++db) o[db][e] *= ac;
       }
     }
+    __builtin_amdgcn_s_waitcnt(0x0F7A);  // vmcnt(10): this chunk's V too
+    wave_fence();
     uint32_t vp[4][NG];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -653,8 +694,8 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
         float q[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          q[u] = pr[w][u] * f16_lo(vp[u][t]);
-          // the sums take 24 off every code, so that a rounded probability meets -8..7: z + 8 s here
+          q[u] = mul_lo(pr[w][u], vp[u][t]);
+          // the sums take 8 off every code, so that a rounded probability meets -8..7: z + 8 s here
           zs[w][t] = fmaf(pr[w][u], f16_hi(vp[u][t]), fmaf(8.0f, q[u], zs[w][t]));
         }
         const int col = D == 128 ? 4 * t + a : 4 * t + (a & 1) + 2 * w;
@@ -672,10 +713,13 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
           pl[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 4 * NG * PROW + 128 * (j >> 1) + 16 * (j & 1)));
       }
     }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the probabilities are read, the K rows' space is free
+    wave_fence();
+    in.fetch_k(s, c + 2 * kWaves);
 #pragma unroll
     for (int j = 0; j < 2 * HV; ++j) {
-      ones = mma16_bf16(fragment_of_ones<false>(), pb[j], ones);
-      if constexpr (TWO) ones = mma16_bf16(fragment_of_ones<false>(), pl[j], ones);
+      base = mma16_bf16(Codes<false>::bases<true>(), pb[j], base);
+      if constexpr (TWO) base = mma16_bf16(Codes<false>::bases<true>(), pl[j], base);
     }
 #pragma unroll
     for (int hv = 0; hv < HV; ++hv)
@@ -689,9 +733,9 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
           if constexpr (TWO) o[db] = mma16_bf16(vf, pl[2 * hv + j], o[db]);
         }
       }
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this stage's reads are done before its next loads are issued
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the V rows are read
     wave_fence();
-    in.fetch(s, c + 2 * kWaves);
+    in.fetch_v(s, c + 2 * kWaves);
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): nothing lands in LDS any more
 
@@ -720,7 +764,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
     for (int e = 0; e < 4; ++e) {
       float lo = k & 4 ? o[2 + j][e] : o[j][e];
       if constexpr (D == 128) lo = k & 8 ? (k & 4 ? o[6 + j][e] : o[4 + j][e]) : lo;
-      r[e] = fmaf(-24.0f, ones[e], lo);
+      r[e] = lo - base[e];
     }
     if (D == 128 || k < 8) *reinterpret_cast<f32x4_t*>(&mine->o[k & 3][32 * (k >> 2) + 16 * j + 4 * a]) = r;
   }
@@ -745,6 +789,9 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
   const Part part(p, split);
   if (part.count == 0 && p.n_splits > 1) return;
 
+  const Stream<D> in(p, g, part.begin, part.count, lane);
+  in.fetch_k(sm[wave][0], wave);
+  in.fetch_v(sm[wave][0], wave);
   u32x4_t qw[NG];  // vector k, columns 8 a .. 8 a + 7 of every group
   {
     const int v = v0 + (k < R ? k : 0), t = token_of(p, v);
@@ -752,17 +799,22 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
 #pragma unroll
     for (int j = 0; j < NG; ++j) qw[j] = ld16(qr + kGroup * j);
   }
-  const Stream<D> in(p, g, part.begin, part.count, lane);
+  in.fetch_k(sm[wave][1], wave + kWaves);
+  in.fetch_v(sm[wave][1], wave + kWaves);
   const int chunks = (part.count + CH - 1) / CH;
-  in.fetch(sm[wave][0], wave);
-  in.fetch(sm[wave][1], wave + kWaves);
 
   bf16x8_t qa[NG];
-  f32x4_t qs[NG];
+  f32x4_t qs[NG], qb[NG];
 #pragma unroll
   for (int j = 0; j < NG; ++j) {
     qa[j] = query_fragment(qw[j], k < R);
     qs[j] = mma16<F16>(qa[j], fragment_of_ones<F16>(), f32x4_t{0, 0, 0, 0});
+    qb[j] = mma16<F16>(qa[j], Codes<F16>::template bases<false>(), f32x4_t{0, 0, 0, 0});
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      qs[j][e] *= p.c;
+      qb[j][e] = -qb[j][e];
+    }
   }
   uint32_t kread[4];  // head_dim 128: by group; 64: by u >> 1
 #pragma unroll
@@ -775,7 +827,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
   const int fewest = part.limit(p, v0);
 
   float m[4], l[4], zs[4][NG];
-  f32x4_t o[NDB], ones[NG];
+  f32x4_t o[NDB], base[NG];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     m[e] = -1.0e30f;
@@ -786,7 +838,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
 #pragma unroll
   for (int db = 0; db < NDB; ++db) o[db] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-  for (int t = 0; t < NG; ++t) ones[t] = f32x4_t{0, 0, 0, 0};
+  for (int t = 0; t < NG; ++t) base[t] = f32x4_t{0, 0, 0, 0};
 
   const Codes<F16> k_codes;
   const Codes<false> v_codes;
@@ -808,7 +860,8 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
   };
   int st = 0;
   for (int c = wave; c < chunks; c += kWaves, st ^= 1) {
-    __builtin_amdgcn_s_waitcnt(0x0F7A);  // vmcnt(10)
+    __builtin_amdgcn_s_waitcnt(0x0F7F);  // vmcnt(15): K
+    wave_fence();
     uint8_t* s = sm[wave][st];
     complete<D, F16, CH>(p, part, in, c, g, lane, s);
     const bool whole = (c + 1) * CH <= fewest;
@@ -827,10 +880,10 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
         for (int t = 0; t < NG; ++t) {
           const uint32_t kw = *reinterpret_cast<const uint32_t*>(
               s + (D == 128 ? kread[t] + 512 * (u & 1) + 256 * (u >> 1) : kread[u >> 1] + 2048 * hv + 256 * (u & 1) + 16 * t));
-          const f32x4_t acc = mma16<F16>(qa[t], k_codes(kw), f32x4_t{0, 0, 0, 0});
-          const float sc = f16_lo(kp[t]) * p.c, zc = fmaf(-16.0f, f16_lo(kp[t]), f16_hi(kp[t])) * p.c;
+          const f32x4_t acc = mma16<F16>(qa[t], k_codes(kw), qb[t]);
+          const float sc = mul_lo(p.c, kp[t]), z = f16_hi(kp[t]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = fmaf(sc, acc[e], fmaf(zc, qs[t][e], y[e]));
+          for (int e = 0; e < 4; ++e) y[e] = fmaf(sc, acc[e], fmaf(z, qs[t][e], y[e]));
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[hv][u][e] = whole || key < lim[e] ? y[e] : -__builtin_huge_valf();
@@ -870,7 +923,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
 #pragma unroll
-        for (int t = 0; t < NG; ++t) ones[t][e] *= ac;
+        for (int t = 0; t < NG; ++t) base[t][e] *= ac;
 #pragma unroll
         for (int db = 0; db < NDB; ++db) o[db][e] *= ac;
       }
@@ -882,6 +935,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
 #pragma unroll
         for (int e = 0; e < 4; ++e) l[e] += pr[hv][u][e];
 
+    __builtin_amdgcn_s_waitcnt(0x0F7A);  // vmcnt(10): this chunk's V too
     // (column group, half) blocks: probabilities times scales into LDS, [vector][key], then that group's columns
 #pragma unroll
     for (int i0 = 0; i0 < NG * HV; i0 += AT) {
@@ -895,7 +949,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
           uint32_t vp[NG];
           params(s + kVp, hv, u, whole, key0 + 64 * hv + key_of_step(u), vp);
           const float sc = f16_lo(vp[t]);
-          zz[u] = fmaf(8.0f, sc, f16_hi(vp[t]));  // the sums take 24 off every code
+          zz[u] = fmaf(8.0f, sc, f16_hi(vp[t]));  // the sums take 8 off every code
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             q[e][u] = pr[hv][u][e] * sc;
@@ -914,10 +968,10 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           pb[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 16 * j));
-          ones[t] = mma16_bf16(fragment_of_ones<false>(), pb[j], ones[t]);
+          base[t] = mma16_bf16(Codes<false>::bases<true>(), pb[j], base[t]);
           if constexpr (TWO) {
             pl[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + PBLK + 16 * j));
-            ones[t] = mma16_bf16(fragment_of_ones<false>(), pl[j], ones[t]);
+            base[t] = mma16_bf16(Codes<false>::bases<true>(), pl[j], base[t]);
           }
         }
 #pragma unroll
@@ -932,9 +986,10 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
         }
       }
     }
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this stage's reads are done before its next loads are issued
     wave_fence();
-    in.fetch(s, c + 2 * kWaves);
+    in.fetch_k(s, c + 2 * kWaves);
+    in.fetch_v(s, c + 2 * kWaves);
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
 
@@ -956,7 +1011,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
   for (int db = 0; db < NDB; ++db) {
     f32x4_t r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = fmaf(-24.0f, ones[db / 2][e], o[db][e]);
+    for (int e = 0; e < 4; ++e) r[e] = o[db][e] - base[db / 2][e];
     *reinterpret_cast<f32x4_t*>(&mine->o[k][16 * db + 4 * a]) = r;
   }
   finish<D, F16, kVecs>(p, sm, R, v0, g, split, tid);
