@@ -389,6 +389,10 @@ int bb_int4_decode_append(const void* q, const int64_t* sq, uint8_t* kq, void* k
 
 size_t bb_int4_decode_workspace(int64_t n, int T, int H, int Hkv, int D);
 
+/* The longest cache (n, or with n_dev the capacity) that a call with this many query vectors per KV head (T H / Hkv) attends
+ * in one split: one launch, and a workspace of 0 bytes (NULL). */
+int64_t bb_int4_decode_one_split(int vectors, int D);
+
 /*
  * Measurement helper (no reference counterpart): reads `bytes` (a multiple of 16, 16-byte aligned) of device memory
  * with non-temporal 16-byte loads, one contiguous range per each of `workgroups` workgroups of 256 threads, and

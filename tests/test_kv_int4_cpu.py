@@ -48,8 +48,8 @@ def _refused(rc, text):
 
 
 def _decode(**kw):
-    a = dict(q=FAKE, sq=(1024, 128), kq=FAKE, kp=FAKE, vq=FAKE, vp=FAKE, sc=(6400, 800, 6400, 800), n=100, n_dev=None,
-             cap=100, T=1, H=8, Hkv=2, D=128, f16=0, scale=0.1, causal=0, out=FAKE, so=(1024, 128), ws=FAKE,
+    a = dict(q=FAKE, sq=(1024, 128), kq=FAKE, kp=FAKE, vq=FAKE, vp=FAKE, sc=(64000, 8000, 64000, 8000), n=1000, n_dev=None,
+             cap=1000, T=1, H=8, Hkv=2, D=128, f16=0, scale=0.1, causal=0, out=FAKE, so=(1024, 128), ws=FAKE,
              ws_bytes=1 << 30)
     a.update(kw)
     for key in ("sq", "sc", "so"):
@@ -59,10 +59,10 @@ def _decode(**kw):
 
 @pytest.mark.parametrize("kw,text", [
     (dict(q=None), "null"), (dict(vq=None), "null"), (dict(kp=None), "null"), (dict(sc=None), "null"),
-    (dict(kq=FAKE + 8), "aligned"), (dict(vp=FAKE + 2), "aligned"), (dict(sc=(6400, 801, 6400, 800)), "aligned"),
-    (dict(sc=(6408, 800, 6400, 800)), "aligned"), (dict(H=7), "must match"), (dict(Hkv=0), "must match"),
+    (dict(kq=FAKE + 8), "aligned"), (dict(vp=FAKE + 2), "aligned"), (dict(sc=(64000, 8001, 64000, 8000)), "aligned"),
+    (dict(sc=(64008, 8000, 64000, 8000)), "aligned"), (dict(H=7), "must match"), (dict(Hkv=0), "must match"),
     (dict(D=32), "head_dim 32"), (dict(D=256), "head_dim 256"), (dict(T=0), "1 to 16"), (dict(T=17), "1 to 16"),
-    (dict(n=0), "empty"), (dict(n=-1), "empty"), (dict(cap=0), "empty"), (dict(n=101), "capacity"),
+    (dict(n=0), "empty"), (dict(n=-1), "empty"), (dict(cap=0), "empty"), (dict(n=1001), "capacity"),
     (dict(n=3, T=4), "at least as long"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(q=FAKE + 8), "aligned"), (dict(sq=(1024, 132)), "aligned"), (dict(out=FAKE + 4), "aligned"),
     (dict(ws=None), "workspace"), (dict(ws_bytes=100), "workspace"), (dict(n_dev=FAKE, ws_bytes=100), "workspace")])
@@ -108,8 +108,14 @@ def test_empty_writes_launch_nothing():
 def test_workspace_grows_with_the_call():
     L = _lib.lib()
     assert L.bb_int4_decode_workspace(0, 1, 8, 2, 128) == 0 and L.bb_int4_decode_workspace(10, 1, 0, 2, 128) == 0
-    small, large = (L.bb_int4_decode_workspace(n, 1, 32, 8, 128) for n in (100, 131072))
+    small, large = (L.bb_int4_decode_workspace(n, 1, 32, 8, 128) for n in (1000, 131072))
     assert 0 < small < large <= 256 * 1024 * 1024
+    for t, d in ((1, 128), (1, 64), (4, 128), (16, 64)):  # one split: nothing to merge
+        one = L.bb_int4_decode_one_split(t * 4, d)
+        assert one >= 256 and L.bb_int4_decode_workspace(one, t, 32, 8, d) == 0
+        assert L.bb_int4_decode_workspace(one + 1, t, 32, 8, d) > 0
+    sizes = [L.bb_int4_decode_workspace(n, 2, 12, 4, 64) for n in range(1, 40000, 37)]
+    assert sizes == sorted(sizes), "a workspace for the capacity serves every length"
     assert L.bb_int4_decode_workspace(131072, 4, 32, 8, 128) >= 4 * large // 2
 
 

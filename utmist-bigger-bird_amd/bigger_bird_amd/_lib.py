@@ -73,6 +73,7 @@ SIGNATURES = {
     "bb_int4_decode_append": (_i32, [_vp, c_i64p, _vp, _vp, _vp, _vp, c_i64p, _vp, c_i64p, _vp, c_i64p, _i64, _vp, _i64,
                                      _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, c_i64p, _vp, _sz, _vp]),
     "bb_int4_decode_workspace": (_sz, [_i64, _i32, _i32, _i32, _i32]),
+    "bb_int4_decode_one_split": (_i64, [_i32, _i32]),
 }
 
 

@@ -17,6 +17,8 @@ from transformers import DynamicCache
 from . import _lib
 from .kv_int8 import _KINDS, GROW, Int8KVLayer
 
+# Stride arrays by their values (read-only to the library): made once per layout instead of three times a call.
+_strides = functools.lru_cache(maxsize=1024)(_lib.i64s)
 MAX_TOKENS = 16  # query tokens of one decode call
 _HEAD_DIMS = (32, 64, 128, 256)
 _HALVES = (16, 32, 64, 128)  # their packed rows' bytes
@@ -144,10 +146,10 @@ def _write(device, xk, xv, out_k, out_v, k, v):
     sa, pb, sb = a.stride(), None, None
     if xv is not None:
         b = _input_rows(xv)
-        pb, sb = b.data_ptr(), _lib.i64s(b.stride(0), b.stride(1))
-    _launch_on(device, _lib.lib().bb_int4_quantize, a.data_ptr(), _lib.i64s(sa[0], sa[1]), pb, sb, _KINDS[a.dtype],
+        pb, sb = b.data_ptr(), _strides(b.stride(0), b.stride(1))
+    _launch_on(device, _lib.lib().bb_int4_quantize, a.data_ptr(), _strides(sa[0], sa[1]), pb, sb, _KINDS[a.dtype],
                a.shape[0], a.shape[1], k[2], out_k[0].data_ptr(), out_k[1].data_ptr(), _lib.ptr(out_v[0]),
-               _lib.ptr(out_v[1]), _lib.i64s(k[3], k[4], v[3], v[4]), _lib.stream_of(xk))
+               _lib.ptr(out_v[1]), _strides(k[3], k[4], v[3], v[4]), _lib.stream_of(xk))
 
 
 def dequantize4(q, p, dtype):
@@ -159,7 +161,7 @@ def dequantize4(q, p, dtype):
     k = _packed("dequantize4", q, p)
     out = torch.empty(*q.shape[:-1], k[2], dtype=dtype, device=q.device)
     if out.numel():
-        _launch_on(device, _lib.lib().bb_int4_dequantize, q.data_ptr(), p.data_ptr(), None, None, _lib.i64s(k[3], k[4], 0, 0),
+        _launch_on(device, _lib.lib().bb_int4_dequantize, q.data_ptr(), p.data_ptr(), None, None, _strides(k[3], k[4], 0, 0),
                    k[0], k[1], k[2], out.data_ptr(), None, _KINDS[dtype], _lib.stream_of(out))
     return out
 
@@ -172,11 +174,11 @@ def dequantize4_pair(k, v, dtype):
     lk, lv = _packed_pair("dequantize4", *k, *v)
     if lv[:3] != lk[:3]:
         raise ValueError("dequantize4: K and V must hold the same rows")
-    outk = torch.empty(*k[0].shape[:-1], lk[2], dtype=dtype, device=k[0].device)
-    outv = torch.empty(*v[0].shape[:-1], lk[2], dtype=dtype, device=k[0].device)
+    outk = k[0].new_empty((*k[0].shape[:-1], lk[2]), dtype=dtype)
+    outv = torch.empty_like(outk) if v[0].shape == k[0].shape else k[0].new_empty((*v[0].shape[:-1], lk[2]), dtype=dtype)
     if outk.numel():
         _launch_on(device, _lib.lib().bb_int4_dequantize, k[0].data_ptr(), k[1].data_ptr(), v[0].data_ptr(),
-                   v[1].data_ptr(), _lib.i64s(lk[3], lk[4], lv[3], lv[4]), lk[0], lk[1], lk[2], outk.data_ptr(),
+                   v[1].data_ptr(), _strides(lk[3], lk[4], lv[3], lv[4]), lk[0], lk[1], lk[2], outk.data_ptr(),
                    outv.data_ptr(), _KINDS[dtype], _lib.stream_of(outk))
     return outk, outv
 
@@ -190,6 +192,12 @@ def _rows16(x):
 @functools.lru_cache(maxsize=64)
 def _workspace_bytes(rows, t, h, hk, d):
     return _lib.lib().bb_int4_decode_workspace(rows, t, h, hk, d)
+
+
+@functools.lru_cache(maxsize=64)
+def _one_split(vectors, d):
+    """The longest cache that the library attends in one split, which needs no workspace."""
+    return _lib.lib().bb_int4_decode_one_split(vectors, d)
 
 
 def _decode(q, k4, kp, v4, vp, knew, vnew, n, scale, causal):
@@ -221,14 +229,18 @@ def _decode(q, k4, kp, v4, vp, knew, vnew, n, scale, causal):
         knew, vnew = _rows16(knew), _rows16(vnew)
         sk, sv = knew.stride(), vnew.stride()
         fn = L.bb_int4_decode_append
-        new = (knew.data_ptr(), _lib.i64s(sk[0], sk[1]), vnew.data_ptr(), _lib.i64s(sv[0], sv[1]))
-    out = torch.empty((t, h, d), dtype=q.dtype, device=q.device)
-    ws_bytes = _workspace_bytes(cap, t, h, hk, d)  # for every length up to the capacity
-    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=q.device)
-    _launch_on(device, fn, q.data_ptr(), _lib.i64s(sq[0], sq[1]), k4.data_ptr(), kp.data_ptr(), v4.data_ptr(), vp.data_ptr(),
-               _lib.i64s(skq, skp, v[3], v[4]), *new, 0 if length is not None else int(n), _lib.ptr(length), cap, t, h, hk,
-               d, int(q.dtype is torch.float16), float(scale), int(bool(causal)), out.data_ptr(), _lib.i64s(h * d, d),
-               ws.data_ptr(), ws_bytes, _lib.stream_of(q))
+        new = (knew.data_ptr(), _strides(sk[0], sk[1]), vnew.data_ptr(), _strides(sv[0], sv[1]))
+    out = torch.empty_like(q) if sq == (h * d, d, 1) else q.new_empty((t, h, d))
+    rows = cap if length is not None else int(n)
+    if rows <= _one_split(t * (h // hk), d):  # no partials
+        ws, ws_bytes = None, 0
+    else:
+        ws_bytes = _workspace_bytes(cap, t, h, hk, d)  # for every length up to the capacity
+        ws = k4.new_empty(ws_bytes)
+    _launch_on(device, fn, q.data_ptr(), _strides(sq[0], sq[1]), k4.data_ptr(), kp.data_ptr(), v4.data_ptr(), vp.data_ptr(),
+               _strides(skq, skp, v[3], v[4]), *new, rows, _lib.ptr(length), cap, t, h, hk,
+               d, int(q.dtype is torch.float16), float(scale), int(bool(causal)), out.data_ptr(), _strides(h * d, d),
+               _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
     return out[0] if one else out
 
 

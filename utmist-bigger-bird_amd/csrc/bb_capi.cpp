@@ -957,16 +957,23 @@ int bb_int4_dequantize(const uint8_t* kq, const void* kp, const uint8_t* vq, con
                     "bb_int4_dequantize");
 }
 
+// Short caches go to one split per KV head: one launch, no merge. Up to 3 chunks of 64 keys (128 at head_dim 64) for each of a
+// workgroup's 4 waves, 2 for the wide kernel (GPU time of one split against splits of 256 keys: 8 KV heads x 4 heads of 128,
+// 512 keys 7.0 and 8.8 us, 768 8.3 and 8.9, 1024 9.6 and 8.9; head_dim 64, 1536 keys 8.6 and 8.8, 2048 10.1 and 8.8; 16
+// vectors, 512 keys 12.4 and 12.7, 768 14.2 and 12.5). The host's 3.4 us for the second launch come on top.
+int64_t bb_int4_decode_one_split(int vectors, int D) { return (vectors <= 4 ? 768 : 512) * (D == 64 ? 2 : 1); }
+
 // Splits of the 4-bit decode: two workgroups per CU over all KV heads, of kInt4MinSplit keys at least (the kernels cut
 // the live length into this many equal parts, so that with a device-side length the splits follow it).
-static int int4_splits(int64_t n, int Hkv) {
-  const int64_t s = std::min(cdiv(n, bb::kInt4MinSplit), cdiv(2 * kCUs, Hkv));
-  return (int)std::max<int64_t>(1, s);
+static int int4_splits(int64_t n, int T, int H, int Hkv, int D) {
+  if (n <= bb_int4_decode_one_split(T * (H / Hkv), D)) return 1;
+  return (int)std::min(cdiv(n, bb::kInt4MinSplit), cdiv(2 * kCUs, Hkv));
 }
 
 size_t bb_int4_decode_workspace(int64_t n, int T, int H, int Hkv, int D) {
-  if (n <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || D <= 0) return 0;
-  return (size_t)T * H * int4_splits(n, Hkv) * (D + 2) * sizeof(float);
+  if (n <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0) return 0;
+  const int splits = int4_splits(n, T, H, Hkv, D);
+  return splits == 1 ? 0 : (size_t)T * H * splits * (D + 2) * sizeof(float);
 }
 
 // bb_int4_decode, and with new rows bb_int4_decode_append.
@@ -993,7 +1000,7 @@ static int int4_decode_impl(const void* q, const int64_t* sq, uint8_t* kq, void*
     return fail("decode_int4: new rows need a contiguous head_dim and 16-byte aligned rows");
   const int64_t most = n_dev ? cap : n;
   const size_t need = bb_int4_decode_workspace(most, T, H, Hkv, D);
-  if (!ws || ws_bytes < need || !aligned(ws, 16)) return fail("workspace of %zu bytes required", need);
+  if (need && (!ws || ws_bytes < need || !aligned(ws, 16))) return fail("workspace of %zu bytes required", need);
   bb::Int4DecodeParams p;
   memset(&p, 0, sizeof(p));
   p.q = static_cast<const uint16_t*>(q);
@@ -1015,7 +1022,7 @@ static int int4_decode_impl(const void* q, const int64_t* sq, uint8_t* kq, void*
   p.T = T; p.H = H; p.Hkv = Hkv; p.D = D;
   p.f16 = is_f16 ? 1 : 0;
   p.causal = causal ? 1 : 0;
-  p.n_splits = int4_splits(most, Hkv);
+  p.n_splits = int4_splits(most, T, H, Hkv, D);
   p.G = H / Hkv;
   p.inv_G = 1.0f / (float)p.G;
   p.inv_splits = 1.0 / p.n_splits;
