@@ -973,7 +973,7 @@ static int int4_splits(int64_t n, int T, int H, int Hkv, int D) {
 size_t bb_int4_decode_workspace(int64_t n, int T, int H, int Hkv, int D) {
   if (n <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0) return 0;
   const int splits = int4_splits(n, T, H, Hkv, D);
-  return splits == 1 ? 0 : (size_t)T * H * splits * (D + 2) * sizeof(float);
+  return splits == 1 ? 0 : (size_t)T * H * splits * bb::int4_part_row(D) * sizeof(float);
 }
 
 // bb_int4_decode, and with new rows bb_int4_decode_append.

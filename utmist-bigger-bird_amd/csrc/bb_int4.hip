@@ -461,23 +461,28 @@ template <int D, bool F16, int NV>
 BB_DEV void finish(const Int4DecodeParams& p, const uint8_t (*sm)[2][kStage], int R, int v0, int g, int split, int tid) {
   __syncthreads();
 #pragma unroll 1
-  for (int i = tid; i < R * D; i += kThreads) {
-    const int r = i / D, d = i % D, v = v0 + r, t = token_of(p, v), hd = g * p.G + v - t * p.G;
-    float M = -1.0e30f, L = 0.0f, O = 0.0f;
+  for (int i = tid; i < R * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4)), v = v0 + r, t = token_of(p, v), hd = g * p.G + v - t * p.G;
+    float M = -1.0e30f, L = 0.0f;
+    f32x4_t O = {0, 0, 0, 0};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) M = fmaxf(M, reinterpret_cast<const WaveState<D, NV>*>(sm[w])->m[r]);
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const WaveState<D, NV>* f = reinterpret_cast<const WaveState<D, NV>*>(sm[w]);
-      const float wt = fast_exp2(f->m[r] - M);
+      const float wt = fast_exp2(f->m[r] - M), z = f->z[r][d / kGroup];
+      const f32x4_t o = *reinterpret_cast<const f32x4_t*>(&f->o[r][d]);
       L += wt * f->l[r];
-      O += wt * (f->o[r][d] + f->z[r][d / kGroup]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] = fmaf(wt, o[e] + z, O[e]);
     }
     if (p.n_splits == 1) {
-      p.out[t * p.so0 + hd * p.so1 + d] = to16<F16>(L > 0.0f ? O / L : 0.0f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] = L > 0.0f ? O[e] / L : 0.0f;
+      *reinterpret_cast<u32x2_t*>(p.out + t * p.so0 + hd * p.so1 + d) = u32x2_t{pack2<F16>(O[0], O[1]), pack2<F16>(O[2], O[3])};
     } else {
-      float* dst = p.part + (((int64_t)t * p.H + hd) * p.n_splits + split) * (D + 2);
-      dst[d] = O;
+      float* dst = p.part + (((int64_t)t * p.H + hd) * p.n_splits + split) * int4_part_row(D);
+      *reinterpret_cast<f32x4_t*>(dst + d) = O;
       if (d == 0) { dst[D] = M; dst[D + 1] = L; }
     }
   }
@@ -1030,7 +1035,7 @@ __global__ __launch_bounds__(kMergeCols * kMergeGroups) void int4_merge_kernel(I
     len = split_keys(p, n);
   }
   const int live = (int)((n + len - 1) / len);
-  const float* base = p.part + (int64_t)v * p.n_splits * (D + 2);
+  const float* base = p.part + (int64_t)v * p.n_splits * int4_part_row(D);
   float M = -1.0e30f, L = 0.0f, O = 0.0f;
   for (int i0 = grp; i0 < live; i0 += kMergeGroups * kMergePer) {
     float mv[kMergePer], lv[kMergePer], ov[kMergePer];
@@ -1038,7 +1043,7 @@ __global__ __launch_bounds__(kMergeCols * kMergeGroups) void int4_merge_kernel(I
     for (int i = 0; i < kMergePer; ++i) {
       const int s = i0 + kMergeGroups * i;
       const bool ok = s < live;
-      const float* r = base + (int64_t)(ok ? s : 0) * (D + 2);
+      const float* r = base + (int64_t)(ok ? s : 0) * int4_part_row(D);
       mv[i] = ok ? r[D] : -1.0e30f;
       lv[i] = ok ? r[D + 1] : 0.0f;
       ov[i] = ok ? r[d] : 0.0f;

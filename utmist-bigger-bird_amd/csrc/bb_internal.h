@@ -125,7 +125,7 @@ struct Int4DecodeParams {
   const uint16_t* knew;  // [Hkv, T, D] (strides skn0 head, skn1 token): the rows n - T .. n - 1 to append, or null
   const uint16_t* vnew;
   uint16_t* out;         // [T, H, D] (strides so0, so1)
-  float* part;           // [T, H][n_splits][D + 2]
+  float* part;           // [T, H][n_splits] rows of int4_part_row(D) floats: the output's D, maximum, sum
   const int64_t* n_dev;  // length in device memory, or null (then n)
   int64_t n, cap, len;   // len: keys of a split (without n_dev)
   int64_t sq0, sq1, skq, skp, svq, svp, skn0, skn1, svn0, svn1, so0, so1;
@@ -136,6 +136,7 @@ struct Int4DecodeParams {
   float c;               // scale * log2(e)
 };
 constexpr int64_t kInt4MinSplit = 256;  // keys of a split, at least (splits are whole 16 keys)
+constexpr int int4_part_row(int D) { return D + 4; }  // whole 16-byte pieces
 hipError_t launch_int4_decode(const Int4DecodeParams& p, hipStream_t stream);
 
 // A decode step's new K / V row folded into the first kernel that reads the cache: the row at position n - 1 (n the
