@@ -431,18 +431,28 @@ struct Part {
   }
 };
 
-// The rest of a split's last chunks, once they have landed: the params that no load brought, and the new rows.
+// The rest of a split's last chunks, once they have landed: the params that no load brought or that no key has, and the new
+// rows.
 template <int D, bool F16, int CH>
 BB_DEV void complete(const Int4DecodeParams& p, const Part& part, const Stream<D>& in, int c, int g, int lane, uint8_t* s) {
   if ((c + 1) * CH <= part.count && (c + 1) * CH <= part.new_first) return;
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): V too
   wave_fence();
-  if constexpr (D == 64) {
-    // an odd last key's params share their 16-byte piece with a row past the range: read them apart
-    if ((part.count & 1) && (c + 1) * CH > part.count && lane < 4) {
-      const uint32_t* src = (lane & 2 ? in.vp : in.kp) + 2 * (part.count - 1) + (lane & 1);
-      *reinterpret_cast<uint32_t*>(s + (lane & 2 ? kVp : kKp) + param_at<D>(part.count - 1 - c * CH) + 4 * (lane & 1)) = *src;
+  if ((c + 1) * CH > part.count) {
+    if constexpr (D == 64) {
+      // an odd last key's params share their 16-byte piece with a row past the range: read them apart
+      if ((part.count & 1) && lane < 4) {
+        const uint32_t* src = (lane & 2 ? in.vp : in.kp) + 2 * (part.count - 1) + (lane & 1);
+        *reinterpret_cast<uint32_t*>(s + (lane & 2 ? kVp : kKp) + param_at<D>(part.count - 1 - c * CH) + 4 * (lane & 1)) = *src;
+      }
     }
+    // scale and minimum 0 for the V rows past the end, whatever lies there (a probability of 0 times NaN is NaN)
+#pragma unroll
+    for (int key = lane; key < CH; key += 64)
+      if (c * CH + key >= part.count) {
+#pragma unroll
+        for (int t = 0; t < D / kGroup; ++t) *reinterpret_cast<uint32_t*>(s + kVp + param_at<D>(key) + 4 * t) = 0u;
+      }
   }
   if ((c + 1) * CH > part.new_first)
     append_rows<D, F16, CH>(p, part.raw, part.begin, c * CH, part.count, g, lane, s);
@@ -602,15 +612,12 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
     wave_fence();
     uint8_t* s = sm[wave][st];
     complete<D, F16, CH>(p, part, in, c, g, lane, s);
-    const bool whole = (c + 1) * CH <= fewest;
 
     float x[W][4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const u32x4_t kw = *reinterpret_cast<const u32x4_t*>(s + kread[u >> 1] + (D == 128 ? 512 : 256) * (u & 1));
-      uint32_t kp = *reinterpret_cast<const uint32_t*>(s + kpread + (D == 128 ? 256 * u : 512 * (u & 1) + 8 * (u >> 1)));
-      const int key = c * CH + key_k + key_of_step(u);
-      if (!whole) kp = key < part.count ? kp : 0u;
+      const uint32_t kp = *reinterpret_cast<const uint32_t*>(s + kpread + (D == 128 ? 256 * u : 512 * (u & 1) + 8 * (u >> 1)));
       const float sc = mul_lo(p.c, kp);
       f32x4_t acc = qb;
 #pragma unroll
@@ -624,22 +631,25 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
         x[0][u] = sum_rows16(y[0], y[1]);
         x[W - 1][u] = sum_rows16(y[2], y[3]);
       }
-      if (!whole) {
+    }
+    if (c * CH + CH > fewest) {
+      asm volatile("; a branch: most chunks are whole");
 #pragma unroll
-        for (int w = 0; w < W; ++w)
-          if (key >= lim[w]) x[w][u] = -__builtin_huge_valf();
-      }
+      for (int w = 0; w < W; ++w)
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (c * CH + key_k + key_of_step(u) >= lim[w]) x[w][u] = -__builtin_huge_valf();
     }
     float pr[W][4];
-    bool over = false;
+    float most = 0.0f;
 #pragma unroll
     for (int w = 0; w < W; ++w)
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         pr[w][u] = fast_exp2(x[w][u] - m[w]);
-        over |= !(pr[w][u] <= kOver);
+        most = fmaxf(most, pr[w][u]);
       }
-    if (__builtin_amdgcn_ballot_w64(over)) {
+    if (__builtin_amdgcn_ballot_w64(most > kOver)) {
       float alpha[W];
 #pragma unroll
       for (int w = 0; w < W; ++w) {
@@ -681,12 +691,6 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
         vp[u][0] = r[0];
         vp[u][1] = r[1];
       }
-    }
-    if (!whole) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int t = 0; t < NG; ++t) vp[u][t] = c * CH + key_k + key_of_step(u) < part.count ? vp[u][t] : 0u;
     }
     // probabilities times V scales, [4 t + h][key], in the space of the K rows
     wave_fence();
@@ -808,18 +812,30 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
   in.fetch_v(sm[wave][1], wave + kWaves);
   const int chunks = (part.count + CH - 1) / CH;
 
-  bf16x8_t qa[NG];
-  f32x4_t qs[NG], qb[NG];
+  // qz: the group sums as three bf16 terms each (24 bits), so that one product per step adds up z times them over the groups,
+  // z in two terms (its 11 bits); lane (k, a) holds vector k's group a (head_dim 64: a < 2)
+  bf16x8_t qa[NG], qz;
+  f32x4_t qb[NG];
+  {
+    float sum = 0.0f;
 #pragma unroll
-  for (int j = 0; j < NG; ++j) {
-    qa[j] = query_fragment(qw[j], k < R);
-    qs[j] = mma16<F16>(qa[j], fragment_of_ones<F16>(), f32x4_t{0, 0, 0, 0});
-    qb[j] = mma16<F16>(qa[j], Codes<F16>::template bases<false>(), f32x4_t{0, 0, 0, 0});
+    for (int j = 0; j < NG; ++j) {
+      qa[j] = query_fragment(qw[j], k < R);
+      const f32x4_t c = mma16<F16>(fragment_of_ones<F16>(), qa[j], f32x4_t{0, 0, 0, 0});  // every row: vector k's sum
+      sum = a == j ? c[0] : sum;
+      qb[j] = mma16<F16>(qa[j], Codes<F16>::template bases<false>(), f32x4_t{0, 0, 0, 0});
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      qs[j][e] *= p.c;
-      qb[j][e] = -qb[j][e];
+      for (int e = 0; e < 4; ++e) qb[j][e] = -qb[j][e];
     }
+    u32x4_t w = {0, 0, 0, 0};
+    sum *= p.c;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      const uint32_t top = __float_as_uint(sum) & 0xffff0000u;
+      w[j] = top | (top >> 16);
+      sum -= __uint_as_float(top);
+    }
+    qz = as_bf16x8(w);
   }
   uint32_t kread[4];  // head_dim 128: by group; 64: by u >> 1
 #pragma unroll
@@ -848,7 +864,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
   const Codes<F16> k_codes;
   const Codes<false> v_codes;
   // the NG params words of a key, from the stage's K or V params
-  auto params = [&](const uint8_t* at, int hv, int u, bool whole, int key, uint32_t (&w)[NG]) {
+  auto params = [&](const uint8_t* at, int hv, int u, uint32_t (&w)[NG]) {
     if constexpr (D == 128) {
       const u32x4_t r = *reinterpret_cast<const u32x4_t*>(at + 256 * u + 16 * k);
 #pragma unroll
@@ -858,10 +874,6 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
       w[0] = r[0];
       w[1] = r[1];
     }
-    if (!whole) {
-#pragma unroll
-      for (int t = 0; t < NG; ++t) w[t] = key < part.count ? w[t] : 0u;
-    }
   };
   int st = 0;
   for (int c = wave; c < chunks; c += kWaves, st ^= 1) {
@@ -869,32 +881,43 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
     wave_fence();
     uint8_t* s = sm[wave][st];
     complete<D, F16, CH>(p, part, in, c, g, lane, s);
-    const bool whole = (c + 1) * CH <= fewest;
-    const int key0 = c * CH + key_of_lane(k);
 
     float x[HV][4][4];  // [half][step][vector]
 #pragma unroll
     for (int hv = 0; hv < HV; ++hv)
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int key = key0 + 64 * hv + key_of_step(u);
         uint32_t kp[NG];
-        params(s + kKp, hv, u, whole, key, kp);
-        f32x4_t y = {0, 0, 0, 0};
+        params(s + kKp, hv, u, kp);
+        const float z = f16_hi(*reinterpret_cast<const uint32_t*>(
+            s + kKp + 16 * k + (D == 128 ? 256 * u + 4 * a : 512 * (u & 1) + 256 * hv + 8 * (u >> 1) + 4 * (a & 1))));
+        const uint32_t top = __float_as_uint(z) & 0xffff0000u;
+        const uint32_t zw = (top >> 16) | (__float_as_uint(z - __uint_as_float(top)) & 0xffff0000u);
+        f32x4_t y = mma16_bf16(qz, as_bf16x8(u32x4_t{zw, zw, zw, 0u}), f32x4_t{0, 0, 0, 0});
 #pragma unroll
         for (int t = 0; t < NG; ++t) {
           const uint32_t kw = *reinterpret_cast<const uint32_t*>(
               s + (D == 128 ? kread[t] + 512 * (u & 1) + 256 * (u >> 1) : kread[u >> 1] + 2048 * hv + 256 * (u & 1) + 16 * t));
           const f32x4_t acc = mma16<F16>(qa[t], k_codes(kw), qb[t]);
-          const float sc = mul_lo(p.c, kp[t]), z = f16_hi(kp[t]);
+          const float sc = mul_lo(p.c, kp[t]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = fmaf(sc, acc[e], fmaf(z, qs[t][e], y[e]));
+          for (int e = 0; e < 4; ++e) y[e] = fmaf(sc, acc[e], y[e]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[hv][u][e] = whole || key < lim[e] ? y[e] : -__builtin_huge_valf();
+        for (int e = 0; e < 4; ++e) x[hv][u][e] = y[e];
       }
+    if (c * CH + CH > fewest) {
+      asm volatile("; a branch: most chunks are whole");
+#pragma unroll
+      for (int hv = 0; hv < HV; ++hv)
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c * CH + key_of_lane(k) + 64 * hv + key_of_step(u) >= lim[e]) x[hv][u][e] = -__builtin_huge_valf();
+    }
     float pr[HV][4][4];
-    bool over = false;
+    float most = 0.0f;
 #pragma unroll
     for (int hv = 0; hv < HV; ++hv)
 #pragma unroll
@@ -902,9 +925,9 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           pr[hv][u][e] = fast_exp2(x[hv][u][e] - m[e]);
-          over |= !(pr[hv][u][e] <= kOver);
+          most = fmaxf(most, pr[hv][u][e]);
         }
-    if (__builtin_amdgcn_ballot_w64(over)) {
+    if (__builtin_amdgcn_ballot_w64(most > kOver)) {
       float alpha[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -952,7 +975,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           uint32_t vp[NG];
-          params(s + kVp, hv, u, whole, key0 + 64 * hv + key_of_step(u), vp);
+          params(s + kVp, hv, u, vp);
           const float sc = f16_lo(vp[t]);
           zz[u] = fmaf(8.0f, sc, f16_hi(vp[t]));  // the sums take 8 off every code
 #pragma unroll
