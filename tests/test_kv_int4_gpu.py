@@ -144,7 +144,8 @@ DECODE = [
     (511, 7, 3, 1, 128, BF16, True), (1000, 1, 24, 8, 128, FP16, False), (1025, 4, 32, 8, 64, FP16, True),
     (4099, 1, 32, 8, 64, FP16, False), (8111, 1, 32, 16, 128, BF16, False), (20011, 1, 32, 32, 128, FP16, False),
     (20011, 8, 8, 2, 128, BF16, True), (33000, 4, 32, 8, 128, BF16, True), (131072, 1, 32, 8, 128, BF16, False),
-    (131071, 3, 8, 4, 128, FP16, True),
+    (131071, 3, 8, 4, 128, FP16, True), (700, 1, 32, 1, 128, BF16, False), (301, 2, 600, 600, 64, BF16, True),
+    (769, 1, 8, 2, 128, BF16, False), (1537, 1, 4, 1, 64, FP16, False), (5003, 16, 24, 1, 64, BF16, True),
 ]
 
 
@@ -221,6 +222,44 @@ def test_decode_small_and_large_scales(dev):
         for dtype in (BF16, FP16):
             q = torch.randn(1, H, d, generator=gen, device=dev).to(dtype)
             _check_decode(decode_int4(q, *cache, n, d ** -0.5), q, cache, n, d ** -0.5, False)
+
+
+@pytest.mark.parametrize("T,H,Hkv,d", [(1, 8, 2, 128), (4, 8, 2, 64), (3, 16, 2, 128)])
+def test_decode_nonfinite_query_stays_with_its_row(T, H, Hkv, d, dev):
+    _say("nonfinite query", T, H, Hkv, d)
+    gen = torch.Generator(device=dev).manual_seed(6)
+    n = 500
+    cache = (*_cache(gen, Hkv, n, n + 3, d, dev), *_cache(gen, Hkv, n, n + 3, d, dev))
+    q = torch.randn(T, H, d, generator=gen, device=dev).to(BF16)
+    want = decode_int4(q, *cache, n, 0.1)
+    for bad in (float("nan"), float("inf")):
+        q2 = q.clone()
+        q2[T - 1, 3, 5] = bad
+        got = decode_int4(q2, *cache, n, 0.1)
+        got[T - 1, 3] = want[T - 1, 3]
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("d,lengths", [(64, (1, 2, 3, 31, 33, 127, 128, 129, 255, 513, 1535)),
+                                       (128, (1, 2, 3, 31, 33, 63, 65, 129, 191, 255, 767))])
+@pytest.mark.parametrize("heads", [(4, 2), (16, 2)])
+def test_decode_every_tail(d, lengths, heads, dev):
+    """Lengths that end inside a step, a chunk and a piece of params, in one split: narrow and wide kernel, host and device
+    length, with a new last row."""
+    _say("tails", d, heads)
+    gen = torch.Generator(device=dev).manual_seed(d)
+    H, Hkv = heads
+    cache = (*_cache(gen, Hkv, 1600, 1601, d, dev), *_cache(gen, Hkv, 1600, 1601, d, dev))
+    q = torch.randn(1, H, d, generator=gen, device=dev).to(FP16)
+    k, v = _rows(gen, Hkv, 1, d, FP16, dev), _rows(gen, Hkv, 1, d, FP16, dev)
+    for n in lengths:
+        _check_decode(decode_int4(q, *cache, n, d ** -0.5), q, cache, n, d ** -0.5, False)
+        mine = [x.clone() for x in cache]
+        got = decode_int4_append(q, *mine, k, v, torch.tensor([n], device=dev), d ** -0.5)
+        _check_decode(got, q, mine, n, d ** -0.5, False)
+        want = plain.pack(*plain.quantize(v))
+        assert torch.equal(mine[2][:, n - 1:n], want[0]) and torch.equal(mine[3][:, n - 1:n], want[1])
+        assert torch.equal(mine[2][:, n:], cache[2][:, n:]) and torch.equal(mine[0][:, :n - 1], cache[0][:, :n - 1])
 
 
 def test_decode_device_length_clamped_and_empty(dev):
@@ -443,6 +482,27 @@ def test_layer_pending_rows_on_every_path(dev):
     with pytest.raises(ValueError):
         layer.update(k[..., :1, :], v[..., :1, :], {"bb_attend": True})[0].attend(q.float(), 0.1)
     assert torch.equal(layer.keys[..., 310:, :], want_k[..., :1, :]), "a refused attend loses no row"
+
+
+def test_handle_with_many_vectors_reads_the_cache_back(dev):
+    """16 tokens of 16 query heads over one KV head: more vectors than the handle gives to the decode kernel."""
+    _say("many vectors")
+    g = torch.Generator(device=dev).manual_seed(9)
+    H, d, n = 16, 128, 400
+    layer = Int4KVLayer()
+    k, v = (torch.randn(1, 1, n, d, generator=g, device=dev).to(BF16) for _ in range(2))
+    layer.update(k[..., :n - 16, :], v[..., :n - 16, :])
+    handle, _ = layer.update(k[..., n - 16:, :], v[..., n - 16:, :], {"bb_attend": True})
+    assert isinstance(handle, Int4Handle)
+    q = torch.randn(1, H, 16, d, generator=g, device=dev).to(BF16)
+    more = torch.randn(1, H, 20, d, generator=g, device=dev).to(BF16)  # more tokens than a call of the kernel takes
+    for qq in (q, more):
+        t = qq.shape[2]
+        out = _attn(H, 1, d).exact_attention(qq, handle, handle, t, n)
+        assert layer._pending is None and out.shape == (1, H, t, d)
+        cache = (*layer.store_k.rows(0, n), *layer.store_v.rows(0, n))
+        want, _ = plain.attend(qq[0].transpose(0, 1), *cache, n, d ** -0.5)
+        assert (out[0].transpose(0, 1).double() - want).abs().max() < 2e-2  # the flash kernel's bar over 16-bit values
 
 
 KW = dict(sink=8, window=96, vertical=24, n_route=16, exact_tail=24, block_m=16, block_n=16)

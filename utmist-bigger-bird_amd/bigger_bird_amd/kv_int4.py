@@ -15,11 +15,16 @@ import torch
 from transformers import DynamicCache
 
 from . import _lib
+from .flash import exact_attention
 from .kv_int8 import _KINDS, GROW, Int8KVLayer
 
 # Stride arrays by their values (read-only to the library): made once per layout instead of three times a call.
 _strides = functools.lru_cache(maxsize=1024)(_lib.i64s)
 MAX_TOKENS = 16  # query tokens of one decode call
+# Query vectors per KV head (tokens x heads) up to which a handle attends the packed rows; the kernel takes 16 a pass over the
+# cache. Against reading the cache back and flash attention over it, whole calls (us), 8 KV heads x 4 of 128 over 131072 rows:
+# 4 tokens 41 and 367, 16 tokens (64 vectors) 150 and 369; 4 x 8, 16 tokens (128 vectors) 163 and 224; over 16384 rows 42 and 47.
+_HANDLE_VECTORS = 128
 _HEAD_DIMS = (32, 64, 128, 256)
 _HALVES = (16, 32, 64, 128)  # their packed rows' bytes
 
@@ -272,8 +277,13 @@ class Int4Handle:
 
     def attend(self, q, scale):
         """q [1, H, t, d] -> [1, H, t, d] attention of every query over the layer's whole cache. The step's new rows, when
-        the layer still holds them, are quantised by the same call (decode_int4_append)."""
+        the layer still holds them, are quantised by the same call (decode_int4_append). More queries than a few passes
+        take attend the cache read back."""
         layer = self.turbo
+        groups = q.shape[1] // layer.store_k.q.shape[0]
+        if q.shape[2] > MAX_TOKENS or q.shape[2] * groups > _HANDLE_VECTORS:
+            k, v = layer.read_back(q.dtype)
+            return exact_attention(q[0], k, v, num_heads=q.shape[1], kv_groups=groups, scale=scale)[None]
         cache = (*layer.store_k.packed(), *layer.store_v.packed())
         rows = q[0].transpose(0, 1)
         pending = layer._pending
@@ -384,8 +394,13 @@ class Int4KVLayer(Int8KVLayer):
             return handle, handle
         self._write(kr, vr, start)
         self.n = end
-        k, v = dequantize4_pair(self.store_k.rows(0, end), self.store_v.rows(0, end), self.dtype)
+        k, v = self.read_back(self.dtype)
         return k[None], v[None]
+
+    def read_back(self, dtype):
+        """The cached K and V [Hkv, n, d] in `dtype`, one launch."""
+        self._flush()
+        return dequantize4_pair(self.store_k.rows(0, self.n), self.store_v.rows(0, self.n), dtype)
 
     def batch_repeat_interleave(self, repeats):
         raise NotImplementedError("Int4KVLayer is batch-size-1 only")
