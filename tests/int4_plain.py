@@ -42,8 +42,8 @@ def attend(q, k4, kp, v4, vp, n, scale, causal=False):
     """q [T, H, d] over the first n rows of a packed cache, in 64 bits: (out [T, H, d], bound [T, H, d]).
 
     The bound is what a kernel that works in fp32 with 16-bit matrix operands may be off before its output is rounded:
-      * a probability times a V scale as one 16-bit operand of 8 significant bits is off by 2^-8 of itself at most, and
-        meets codes shifted to -8..7: 2^-8 * 8 sum_j p_j s_j;
+      * a probability times a V scale as two operands of 8 significant bits each is off by 2^-16 of itself at most, and
+        meets codes shifted to -8..7: 2^-16 * 8 sum_j p_j s_j;
       * a score is a sum over d of products q (16 + code) s and q z in fp32: at most 64 roundings of 2^-24 of their absolute
         sum (31 s + |z|) |q| scale, the probabilities then are off by as much (exp), and the fp32 exponential and the sums
         over keys (chains of at most 4096) by 4096 * 2^-24 relative;
@@ -66,5 +66,5 @@ def attend(q, k4, kp, v4, vp, n, scale, causal=False):
             p = torch.softmax(x, -1)
             dx = 64 * 2.0 ** -24 * scale * (qq.abs() @ kabs[:m].T).amax(-1, keepdim=True) + 4096 * 2.0 ** -24
             out[t, g * G:(g + 1) * G] = p @ v[:m]
-            tol[t, g * G:(g + 1) * G] = 2.0 ** -8 * 8 * (p @ vs[:m]) + 2 * dx * (p @ v[:m].abs())
+            tol[t, g * G:(g + 1) * G] = 2.0 ** -16 * 8 * (p @ vs[:m]) + 2 * dx * (p @ v[:m].abs())
     return out, tol

@@ -21,7 +21,12 @@ constexpr float kF16Max = 65504.0f;
 
 BB_DEV float f16_lo(uint32_t w) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(w & 0xffffu)); }
 BB_DEV float f16_hi(uint32_t w) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16)); }
-BB_DEV uint32_t f16_bits(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }  // round to nearest even
+// f rounded to nearest even. f passes through an empty asm: the compiler would otherwise shrink an fp32 operation before it to one
+// that rounds to fp16 directly, where the format rounds to fp32 first.
+BB_DEV uint32_t f16_bits(float f) {
+  asm("" : "+v"(f));
+  return __builtin_bit_cast(uint16_t, (_Float16)f);
+}
 
 // N (a multiple of 8) elements of a row at x (16-byte aligned), in fp32.
 template <int KIND, int N>
@@ -154,7 +159,7 @@ __global__ __launch_bounds__(256) void int4_dequantize_kernel(Int4ReadSet s0, In
     u32x4_t o;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      o[i] = kind == kKindF16 ? pack2<true>(v[2 * i], v[2 * i + 1]) : pack2<false>(v[2 * i], v[2 * i + 1]);
+      o[i] = kind == kKindF16 ? f16_bits(v[2 * i]) | (f16_bits(v[2 * i + 1]) << 16) : pack2<false>(v[2 * i], v[2 * i + 1]);
     __builtin_nontemporal_store(o, reinterpret_cast<u32x4_t*>(reinterpret_cast<uint16_t*>(s.out) + off));
   }
 }
@@ -510,17 +515,16 @@ BB_DEV bf16x8_t fragment_of_ones() {
   return as_bf16x8(u32x4_t{one, one, one, one});
 }
 
-// Probabilities times scales as operands of 16 bits: bf16, whatever the model's type (an fp16 product could fall below
-// its range). TWO puts each into two terms (16 significant bits): an fp16 output is finer than one bf16 term.
-template <bool TWO>
-BB_DEV void put_terms(const float (&q)[4], uint8_t* dst, int second) {
+// Probabilities times scales as operands of 16 bits: two bf16 terms each (16 significant bits), the second PLANE bytes behind the
+// first. bf16 whatever the model's type (an fp16 product could fall below its range); one term alone would double the error
+// of a bf16 output (2.7e-3 of its norm instead of 1.6e-3, measured) and is coarser than an fp16 one.
+template <int PLANE>
+BB_DEV void put_terms(const float (&q)[4], uint8_t* dst) {
   const uint32_t h0 = pack_bf16x2(q[0], q[1]), h1 = pack_bf16x2(q[2], q[3]);
+  const uint32_t l0 = pack_bf16x2(q[0] - __uint_as_float(h0 << 16), q[1] - __uint_as_float(h0 & 0xffff0000u));
+  const uint32_t l1 = pack_bf16x2(q[2] - __uint_as_float(h1 << 16), q[3] - __uint_as_float(h1 & 0xffff0000u));
   *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{h0, h1};
-  if constexpr (TWO) {
-    const uint32_t l0 = pack_bf16x2(q[0] - __uint_as_float(h0 << 16), q[1] - __uint_as_float(h0 & 0xffff0000u));
-    const uint32_t l1 = pack_bf16x2(q[2] - __uint_as_float(h1 << 16), q[3] - __uint_as_float(h1 & 0xffff0000u));
-    *reinterpret_cast<u32x2_t*>(dst + second) = u32x2_t{l0, l1};
-  }
+  *reinterpret_cast<u32x2_t*>(dst + PLANE) = u32x2_t{l0, l1};
 }
 
 // Up to 4 query vectors.
@@ -532,7 +536,7 @@ BB_DEV void put_terms(const float (&q)[4], uint8_t* dst, int second) {
 //   values  The probabilities times the scales of column group t go to column 4 t + h of the operand, so one product serves
 //           all groups (the columns of a product whose rows are another group are not used). A row of the bases plus 8 gives
 //           what those add (the products meet codes shifted to -8..7, which halves what a rounded probability costs).
-template <int D, bool F16, bool TWO>
+template <int D, bool F16>
 __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodeParams p) {
   __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][kStage];
   constexpr int CH = D == 128 ? 64 : 128;      // keys of a chunk
@@ -708,7 +712,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
           zs[w][t] = fmaf(pr[w][u], f16_hi(vp[u][t]), fmaf(8.0f, q[u], zs[w][t]));
         }
         const int col = D == 128 ? 4 * t + a : 4 * t + (a & 1) + 2 * w;
-        put_terms<TWO>(q, s + col * PROW + (D == 128 ? 0 : 128 * (a >> 1)) + 8 * k, 4 * NG * PROW);
+        put_terms<4 * NG * PROW>(q, s + col * PROW + (D == 128 ? 0 : 128 * (a >> 1)) + 8 * k);
       }
     }
     wave_fence();
@@ -718,8 +722,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
 #pragma unroll
       for (int j = 0; j < 2 * HV; ++j) {
         pb[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 128 * (j >> 1) + 16 * (j & 1)));
-        if constexpr (TWO)
-          pl[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 4 * NG * PROW + 128 * (j >> 1) + 16 * (j & 1)));
+        pl[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 4 * NG * PROW + 128 * (j >> 1) + 16 * (j & 1)));
       }
     }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the probabilities are read, the K rows' space is free
@@ -728,7 +731,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
 #pragma unroll
     for (int j = 0; j < 2 * HV; ++j) {
       base = mma16_bf16(Codes<false>::bases<true>(), pb[j], base);
-      if constexpr (TWO) base = mma16_bf16(Codes<false>::bases<true>(), pl[j], base);
+      base = mma16_bf16(Codes<false>::bases<true>(), pl[j], base);
     }
 #pragma unroll
     for (int hv = 0; hv < HV; ++hv)
@@ -739,7 +742,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
         for (int j = 0; j < 2; ++j) {
           const bf16x8_t vf = v_codes((uint32_t)(j ? t.y : t.x));
           o[db] = mma16_bf16(vf, pb[2 * hv + j], o[db]);
-          if constexpr (TWO) o[db] = mma16_bf16(vf, pl[2 * hv + j], o[db]);
+          o[db] = mma16_bf16(vf, pl[2 * hv + j], o[db]);
         }
       }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the V rows are read
@@ -785,13 +788,12 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
 // lane (k, a) gets the sums of vectors 4 a .. 4 a + 3 and applies the (s, z) of all groups of its key. The value operand is
 // built once per column group, in the space of the K rows, and serves that group's two blocks of columns. Against blocks of 4
 // vectors on the kernel above it takes a quarter of the products and of the accumulators.
-template <int D, bool F16, bool TWO>
+template <int D, bool F16>
 __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4DecodeParams p) {
   __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][kStage];
   constexpr int CH = D == 128 ? 64 : 128;
   constexpr int NG = D / kGroup, NDB = D / 16, HV = CH / 64;
   constexpr int PROW = 144, PBLK = 16 * PROW;  // a probability row of 64 keys (16 bytes more: other banks), and 16 of them
-  constexpr int AT = TWO ? 1 : 2;              // (group, half) blocks of probabilities in LDS at a time
   const int split = blockIdx.x, g = blockIdx.y, v0 = blockIdx.z * kVecs, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), k = lane & 15, a = lane >> 4;
   const int R = p.T * p.G - v0 < kVecs ? p.T * p.G - v0 : kVecs;
@@ -966,51 +968,41 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
     __builtin_amdgcn_s_waitcnt(0x0F7A);  // vmcnt(10): this chunk's V too
     // (column group, half) blocks: probabilities times scales into LDS, [vector][key], then that group's columns
 #pragma unroll
-    for (int i0 = 0; i0 < NG * HV; i0 += AT) {
+    for (int i = 0; i < NG * HV; ++i) {
+      const int t = i / HV, hv = i % HV;
       wave_fence();
+      float q[4][4];
 #pragma unroll
-      for (int i = i0; i < i0 + AT; ++i) {
-        const int t = i / HV, hv = i % HV;
-        float q[4][4], zz[4];
+      for (int u = 0; u < 4; ++u) {
+        uint32_t vp[NG];
+        params(s + kVp, hv, u, vp);
+        const float sc = f16_lo(vp[t]), zz = fmaf(8.0f, sc, f16_hi(vp[t]));  // the sums take 8 off every code
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          uint32_t vp[NG];
-          params(s + kVp, hv, u, vp);
-          const float sc = f16_lo(vp[t]);
-          zz[u] = fmaf(8.0f, sc, f16_hi(vp[t]));  // the sums take 8 off every code
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            q[e][u] = pr[hv][u][e] * sc;
-            zs[e][t] = fmaf(pr[hv][u][e], zz[u], zs[e][t]);
-          }
+        for (int e = 0; e < 4; ++e) {
+          q[e][u] = pr[hv][u][e] * sc;
+          zs[e][t] = fmaf(pr[hv][u][e], zz, zs[e][t]);
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) put_terms<TWO>(q[e], s + (i - i0) * PBLK + (4 * a + e) * PROW + 8 * k, PBLK);
       }
-      wave_fence();
 #pragma unroll
-      for (int i = i0; i < i0 + AT; ++i) {
-        const int t = i / HV, hv = i % HV;
-        const uint8_t* src = s + (i - i0) * PBLK + k * PROW + 32 * a;
-        bf16x8_t pb[2], pl[2];
+      for (int e = 0; e < 4; ++e) put_terms<PBLK>(q[e], s + (4 * a + e) * PROW + 8 * k);
+      wave_fence();
+      const uint8_t* src = s + k * PROW + 32 * a;
+      bf16x8_t pb[2], pl[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        pb[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 16 * j));
+        pl[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + PBLK + 16 * j));
+        base[t] = mma16_bf16(Codes<false>::bases<true>(), pb[j], base[t]);
+        base[t] = mma16_bf16(Codes<false>::bases<true>(), pl[j], base[t]);
+      }
+#pragma unroll
+      for (int db = 2 * t; db < 2 * t + 2; ++db) {
+        const v2i_t r = read_tr4(s + kVq + v_block_at<D>(k, a, hv, db));
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          pb[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 16 * j));
-          base[t] = mma16_bf16(Codes<false>::bases<true>(), pb[j], base[t]);
-          if constexpr (TWO) {
-            pl[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + PBLK + 16 * j));
-            base[t] = mma16_bf16(Codes<false>::bases<true>(), pl[j], base[t]);
-          }
-        }
-#pragma unroll
-        for (int db = 2 * t; db < 2 * t + 2; ++db) {
-          const v2i_t r = read_tr4(s + kVq + v_block_at<D>(k, a, hv, db));
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const bf16x8_t vf = v_codes((uint32_t)(j ? r.y : r.x));
-            o[db] = mma16_bf16(vf, pb[j], o[db]);
-            if constexpr (TWO) o[db] = mma16_bf16(vf, pl[j], o[db]);
-          }
+          const bf16x8_t vf = v_codes((uint32_t)(j ? r.y : r.x));
+          o[db] = mma16_bf16(vf, pb[j], o[db]);
+          o[db] = mma16_bf16(vf, pl[j], o[db]);
         }
       }
     }
@@ -1115,9 +1107,9 @@ template <int D, bool F16>
 hipError_t launch_decode_t(const Int4DecodeParams& p, hipStream_t stream) {
   const int vecs = p.T * p.G;
   if (vecs <= 4)
-    hipLaunchKernelGGL((int4_decode_kernel<D, F16, F16>), dim3(p.n_splits, p.Hkv), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((int4_decode_kernel<D, F16>), dim3(p.n_splits, p.Hkv), dim3(kThreads), 0, stream, p);
   else
-    hipLaunchKernelGGL((int4_decode_wide_kernel<D, F16, F16>), dim3(p.n_splits, p.Hkv, (vecs + kVecs - 1) / kVecs),
+    hipLaunchKernelGGL((int4_decode_wide_kernel<D, F16>), dim3(p.n_splits, p.Hkv, (vecs + kVecs - 1) / kVecs),
                        dim3(kThreads), 0, stream, p);
   if (p.n_splits > 1)
     hipLaunchKernelGGL((int4_merge_kernel<D, F16>), dim3(p.T * p.H, D / kMergeCols),
