@@ -65,7 +65,9 @@ def _decode(**kw):
     (dict(n=0), "empty"), (dict(n=-1), "empty"), (dict(cap=0), "empty"), (dict(n=1001), "capacity"),
     (dict(n=3, T=4), "at least as long"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(q=FAKE + 8), "aligned"), (dict(sq=(1024, 132)), "aligned"), (dict(out=FAKE + 4), "aligned"),
-    (dict(ws=None), "workspace"), (dict(ws_bytes=100), "workspace"), (dict(n_dev=FAKE, ws_bytes=100), "workspace")])
+    (dict(ws=None), "workspace"), (dict(ws_bytes=100), "workspace"),
+    (dict(n=1 << 34, cap=1 << 34, sc=(0, 0, 0, 0)), "out of range"), (dict(n_dev=FAKE, cap=2 ** 63 - 1), "out of range"),
+    (dict(n_dev=FAKE, ws_bytes=100), "workspace")])
 def test_decode_refusals(kw, text):
     _refused(_lib.lib().bb_int4_decode(*_decode(**kw), None), text)
 
@@ -83,7 +85,7 @@ def test_append_refusals(new, text):
 @pytest.mark.parametrize("kw,text", [
     (dict(x=None), "null"), (dict(D=48), "head_dim 48"), (dict(kind=3), "element kind"), (dict(x=FAKE + 4), "aligned"),
     (dict(sx=(132, 128)), "aligned"), (dict(rows=1 << 40), "out of range"), (dict(rows=-1), "out of range"),
-    (dict(heads=70000), "out of range"), (dict(vq=None), "null"), (dict(sc=(8, 8, 16, 8)), "aligned")])
+    (dict(heads=1, rows=(0xffffff + 1) * 16), "out of range"), (dict(heads=70000), "out of range"), (dict(vq=None), "null"), (dict(sc=(8, 8, 16, 8)), "aligned")])
 def test_write_and_read_refusals(kw, text):
     a = dict(x=FAKE, sx=(1280, 128), kind=0, heads=2, rows=10, D=128, q=FAKE, p=FAKE, vq=FAKE, vp=FAKE,
              sc=(640, 80, 640, 80))

@@ -5,9 +5,10 @@ places: an HF cache layer (`make_int4_cache`, next to `make_int8_cache`) whose h
 
 Format: asymmetric per token, KV head and group of 32 elements. With min and max clamped to +-65504 and NaN left out of
 them, each operation in fp32: z = fp16(min), s = fp16(max((max - z) / 15, 0)), code = rint((x - z) / s) clamped to 0..15
-(0 where s = 0 or x is NaN; a group of NaN alone has s = z = 0); the value is s * code + z in fp32. Byte b of a packed row holds element 2 b (low four bits) and 2 b + 1. A cache
-is codes [Hkv, capacity, d / 2] uint8 and params [Hkv, capacity, d / 32, 2] fp16 (s, z), head-major, for K and for V:
-80 bytes a row at head_dim 128, against 130 in int8 and 256 in bf16.
+(0 where s = 0 or x is NaN; a group of NaN alone has s = z = 0); the value is s * code + z in fp32. Byte b of a packed row
+holds elements 2 b (low four bits) and 2 b + 1. A cache is codes [Hkv, capacity, d / 2] uint8 and params
+[Hkv, capacity, d / 32, 2] fp16 (s, z), head-major, for K and for V: 80 bytes a row at head_dim 128, against 130 in int8
+and 256 in bf16.
 """
 import functools
 
@@ -23,7 +24,7 @@ _strides = functools.lru_cache(maxsize=1024)(_lib.i64s)
 MAX_TOKENS = 16  # query tokens of one decode call
 # Query vectors per KV head (tokens x heads) up to which a handle attends the packed rows; the kernel takes 16 a pass over the
 # cache. Against reading the cache back and flash attention over it, whole calls (us), 8 KV heads x 4 of 128 over 131072 rows:
-# 4 tokens 41 and 367, 16 tokens (64 vectors) 150 and 369; 4 x 8, 16 tokens (128 vectors) 163 and 224; over 16384 rows 42 and 47.
+# 4 tokens 49 and 366, 16 tokens (64 vectors) 175 and 368; 4 x 8, 16 tokens (128 vectors) 192 and 224; over 16384 rows 46 and 48.
 _HANDLE_VECTORS = 128
 _HEAD_DIMS = (32, 64, 128, 256)
 _HALVES = (16, 32, 64, 128)  # their packed rows' bytes
@@ -159,7 +160,8 @@ def _write(device, xk, xv, out_k, out_v, k, v):
 
 def dequantize4(q, p, dtype):
     """codes [..., t, d / 2], params [..., t, d / 32, 2] -> [..., t, d] in dtype (bf16, fp16 or fp32; the fp32 value
-    s * code + z rounded to nearest even). Rows [a, b) of a cache are read in place: (k4[:, a:b], kp[:, a:b])."""
+    s * code + z rounded to nearest even, in fp16 infinite past 65504, which the top code of a group that spans nearly all of
+    fp16's range can be). Rows [a, b) of a cache are read in place: (k4[:, a:b], kp[:, a:b])."""
     if dtype not in _KINDS:
         raise ValueError("dequantize4: bf16, fp16 or fp32 output")
     device = _one_device("dequantize4", q, p)

@@ -912,8 +912,10 @@ static int int4_cache_check(const char* what, const void* kq, const void* kp, co
 static int int4_rows_check(const char* what, int heads, int64_t rows, int D, int kind) {
   if (D != 32 && D != 64 && D != 128 && D != 256) return fail("%s: head_dim %d unsupported", what, D);
   if (kind < 0 || kind > 2) return fail("%s: element kind %d unsupported (0 bf16, 1 fp32, 2 fp16)", what, kind);
-  // a launch counts its threads in 32 bits: 16 elements each, in blocks of 256
-  if (heads < 0 || heads > 65535 || rows < 0 || rows > (int64_t)1 << 40 || cdiv(rows * D, 4096) * heads > 0xffffff)
+  // a launch counts its threads in 32 bits per dimension, in blocks of 256: the write's take 16 elements each over all heads,
+  // the read back's 8 each of one head
+  if (heads < 0 || heads > 65535 || rows < 0 || rows > (int64_t)1 << 40 || cdiv(rows * D, 4096) * heads > 0xffffff ||
+      cdiv(rows * D, 2048) > 0xffffff)
     return fail("%s: %d heads of %lld rows out of range", what, heads, (long long)rows);
   return BB_OK;
 }
@@ -959,15 +961,15 @@ int bb_int4_dequantize(const uint8_t* kq, const void* kp, const uint8_t* vq, con
 
 // Short caches go to one split per KV head: one launch, no merge. Up to 3 chunks of 64 keys (128 at head_dim 64) for each of a
 // workgroup's 4 waves, 2 for the wide kernel (GPU time of one split against splits of 256 keys: 8 KV heads x 4 heads of 128,
-// 512 keys 7.0 and 8.8 us, 768 8.3 and 8.9, 1024 9.6 and 8.9; head_dim 64, 1536 keys 8.6 and 8.8, 2048 10.1 and 8.8; 16
-// vectors, 512 keys 12.4 and 12.7, 768 14.2 and 12.5). The host's 3.4 us for the second launch come on top.
+// 512 keys 7.1 and 8.6 us, 768 8.5 and 8.6, 1024 9.9 and 8.6; head_dim 64, 1536 keys 8.6 and 8.6, 2048 10.0 and 8.6; 16
+// vectors, 512 keys 10.7 and 10.9, 768 13.2 and 11.2). The host's 3.4 us for the second launch come on top.
 int64_t bb_int4_decode_one_split(int vectors, int D) { return (vectors <= 4 ? 768 : 512) * (D == 64 ? 2 : 1); }
 
 // Splits of the 4-bit decode: two workgroups per CU over all KV heads, of kInt4MinSplit keys at least (the kernels cut
 // the live length into this many equal parts, so that with a device-side length the splits follow it).
 static int int4_splits(int64_t n, int T, int H, int Hkv, int D) {
   if (n <= bb_int4_decode_one_split(T * (H / Hkv), D)) return 1;
-  return (int)std::min(cdiv(n, bb::kInt4MinSplit), cdiv(2 * kCUs, Hkv));
+  return (int)std::min((n - 1) / bb::kInt4MinSplit + 1, cdiv(2 * kCUs, Hkv));
 }
 
 size_t bb_int4_decode_workspace(int64_t n, int T, int H, int Hkv, int D) {
@@ -999,6 +1001,9 @@ static int int4_decode_impl(const void* q, const int64_t* sq, uint8_t* kq, void*
   if (knew && (!aligned(knew, 16) || !aligned(vnew, 16) || sknew[0] % 8 || sknew[1] % 8 || svnew[0] % 8 || svnew[1] % 8))
     return fail("decode_int4: new rows need a contiguous head_dim and 16-byte aligned rows");
   const int64_t most = n_dev ? cap : n;
+  const int splits = int4_splits(most, T, H, Hkv, D);
+  if ((most - 1) / splits >= 1 << 24)  // byte offsets within a split are 32 bits
+    return fail("decode_int4: %lld rows of %d heads out of range", (long long)most, Hkv);
   const size_t need = bb_int4_decode_workspace(most, T, H, Hkv, D);
   if (need && (!ws || ws_bytes < need || !aligned(ws, 16))) return fail("workspace of %zu bytes required", need);
   bb::Int4DecodeParams p;
@@ -1022,7 +1027,7 @@ static int int4_decode_impl(const void* q, const int64_t* sq, uint8_t* kq, void*
   p.T = T; p.H = H; p.Hkv = Hkv; p.D = D;
   p.f16 = is_f16 ? 1 : 0;
   p.causal = causal ? 1 : 0;
-  p.n_splits = int4_splits(most, T, H, Hkv, D);
+  p.n_splits = splits;
   p.G = H / Hkv;
   p.inv_G = 1.0f / (float)p.G;
   p.inv_splits = 1.0 / p.n_splits;
