@@ -85,7 +85,8 @@ def test_append_refusals(new, text):
 @pytest.mark.parametrize("kw,text", [
     (dict(x=None), "null"), (dict(D=48), "head_dim 48"), (dict(kind=3), "element kind"), (dict(x=FAKE + 4), "aligned"),
     (dict(sx=(132, 128)), "aligned"), (dict(rows=1 << 40), "out of range"), (dict(rows=-1), "out of range"),
-    (dict(heads=1, rows=(0xffffff + 1) * 16), "out of range"), (dict(heads=70000), "out of range"), (dict(vq=None), "null"), (dict(sc=(8, 8, 16, 8)), "aligned")])
+    (dict(heads=1, rows=(0xffffff + 1) * 16), "out of range"), (dict(heads=70000), "out of range"),
+    (dict(vq=None), "null"), (dict(sc=(8, 8, 16, 8)), "aligned")])
 def test_write_and_read_refusals(kw, text):
     a = dict(x=FAKE, sx=(1280, 128), kind=0, heads=2, rows=10, D=128, q=FAKE, p=FAKE, vq=FAKE, vp=FAKE,
              sc=(640, 80, 640, 80))

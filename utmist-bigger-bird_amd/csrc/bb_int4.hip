@@ -2,8 +2,9 @@
 //
 // A row of D elements is D / 32 groups of 32. Per group, with min and max clamped to +-65504 and NaN left out of them:
 //   z = fp16(min), s = fp16(max((max - z) / 15, 0)), code = rint((x - z) / s) clamped to 0..15 (0 where s = 0 or x is NaN),
-// each operation in fp32; the value is s * code + z in fp32 (s * code is exact). A group of NaN alone has s = z = 0. s and z are rounded before the codes are
-// taken, so the codes make up for their rounding. Byte b of a packed row holds elements 2 b (low four bits) and 2 b + 1.
+// each operation in fp32; the value is s * code + z in fp32 (s * code is exact). A group of NaN alone has s = z = 0. s and z
+// are rounded before the codes are taken, so the codes make up for their rounding. Byte b of a packed row holds elements 2 b
+// (low four bits) and 2 b + 1.
 //
 // The cache is head-major, codes [Hkv, cap, D / 2] and params [Hkv, cap, D / 32] of (s, z): the rows of one KV head are
 // one contiguous range, so that a workgroup that streams them reads whole 128-byte lines (64-byte rows of one head between
@@ -111,7 +112,8 @@ struct Int4Set {  // one tensor's rows and their place in the cache
 
 // A lane takes half a group (16 elements) of a row; blockIdx.x counts heads within blocks of rows, so that the rows of a
 // token's heads, which neighbour each other where a projection left them, are read at about the same time; blockIdx.y is the
-// tensor (K, V).
+// tensor (K, V). Bound by memory: K and V of 131072 rows x 8 heads x 128 in bf16 (0.54 GB read, 0.17 GB written) take 123 us,
+// 5.7 TB/s; with true divisions, 8 elements a lane, the arithmetic set the time (208 us).
 template <int D, int KIND>
 __global__ __launch_bounds__(256) void int4_quantize_kernel(Int4Set s0, Int4Set s1, int heads, int64_t rows) {
   const Int4Set& s = blockIdx.y ? s1 : s0;
@@ -134,6 +136,7 @@ struct Int4ReadSet {
   int64_t sq0, sp0;
 };
 
+// A lane takes 8 elements; memory alone bounds it (131072 rows as above: 0.70 GB in 138 us, 5.1 TB/s, where a copy reaches 4.9).
 // The values are stored past the caches (the stores are as fast, and packed rows that lie in the 256 MB cache stay there: K and V
 // of 65536 rows x 8 heads x 128 read back 74 -> 48 us, of 131072 rows 145 -> 140; reading the values next is no slower: at
 // 16 MB of them 10.8 -> 10.6 us for both, at 64 MB 28.6 -> 26.1).
@@ -190,8 +193,8 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 BB_DEV int64_t live_length(const Int4DecodeParams& p, int64_t raw) { return raw < 0 ? 0 : raw > p.cap ? p.cap : raw; }
 // Keys of a split: the live length in equal parts of whole 16 keys (the bytes per CU set the time, so the parts are not
-// rounded to chunks); the host passes it as p.len unless the length is in device memory. ceil(n / n_splits) from the rounded reciprocal, put right by one where it is off: a 64-bit division
-// is hundreds of instructions ahead of the first load.
+// rounded to chunks); the host passes it as p.len unless the length is in device memory. ceil(n / n_splits) from the rounded
+// reciprocal, put right by one where it is off: a 64-bit division is hundreds of instructions ahead of the first load.
 BB_DEV int64_t split_keys(const Int4DecodeParams& p, int64_t n) {
   int64_t len = (int64_t)((double)n * p.inv_splits);
   if (len * p.n_splits < n) ++len;
@@ -515,8 +518,8 @@ BB_DEV bf16x8_t fragment_of_ones() {
   return as_bf16x8(u32x4_t{one, one, one, one});
 }
 
-// Probabilities times scales as operands of 16 bits: two bf16 terms each (16 significant bits), the second PLANE bytes behind the
-// first. bf16 whatever the model's type (an fp16 product could fall below its range); one term alone would double the error
+// Probabilities times scales as operands of 16 bits: two bf16 terms each (16 significant bits), the second PLANE bytes behind
+// the first. bf16 whatever the model's type (an fp16 product could fall below its range); one term alone would double the error
 // of a bf16 output (2.7e-3 of its norm instead of 1.6e-3, measured) and is coarser than an fp16 one.
 template <int PLANE>
 BB_DEV void put_terms(const float (&q)[4], uint8_t* dst) {
@@ -536,6 +539,11 @@ BB_DEV void put_terms(const float (&q)[4], uint8_t* dst) {
 //   values  The probabilities times the scales of column group t go to column 4 t + h of the operand, so one product serves
 //           all groups (the columns of a product whose rows are another group are not used). A row of the bases plus 8 gives
 //           what those add (the products meet codes shifted to -8..7, which halves what a rounded probability costs).
+// What bounds it, measured: 131072 rows x 8 KV heads x 4 heads of 128 (168 MB) take 31.5 us, 5.3 TB/s, and the merge 4; with the
+// arithmetic taken out the loads alone and the merge take 30.3 together. The rest is the first chunks' way from memory and the
+// last chunks' arithmetic, which nothing overlaps: of two stages a wave, 160 KB a CU are in flight from the start, and a split
+// is 8 chunks a wave here. 64 splits a head, two workgroups per CU, 34.9 us with the merge; 48 splits 39.4, 96 splits 37.2;
+// plain instead of non-temporal loads 39.1 against 37.3 when that was tried.
 template <int D, bool F16>
 __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodeParams p) {
   __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][kStage];
@@ -788,6 +796,9 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
 // lane (k, a) gets the sums of vectors 4 a .. 4 a + 3 and applies the (s, z) of all groups of its key. The value operand is
 // built once per column group, in the space of the K rows, and serves that group's two blocks of columns. Against blocks of 4
 // vectors on the kernel above it takes a quarter of the products and of the accumulators.
+// The VALU bounds it: about 820 instructions a chunk (codes to floats 220, probabilities times scales into two terms 350), 4000
+// cycles on a SIMD. 16 vectors x 8 KV heads x 128 over 32768 rows (42 MB) take 19.4 us: 6 us until the data is there, and the
+// two chunks of a wave behind it.
 template <int D, bool F16>
 __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4DecodeParams p) {
   __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][kStage];
@@ -1038,9 +1049,9 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
 }
 
 // The partials of the live splits under one maximum: a workgroup per (query vector, 32 columns), thread (4 columns, group)
-// folding every 16th split, 4 loaded at a time; the groups then combine through LDS. A row without keys is zero. (GPU time of
-// decode and merge over 8111 rows, 32 splits: 11.3 us with 16 groups, 11.7 with 32, 12.3 with 64; 11.6 with one column a
-// thread, 16 columns a workgroup.)
+// folding every 16th split, 4 loaded at a time; the groups then combine through LDS. A row without keys is zero. Latency
+// bounds it (2.2 to 4 us for 0.5 to 4 MB). GPU time of decode and merge over 8111 rows, 32 splits: 11.4 us with 8 groups, 11.6
+// with 16, 12.1 with 32, 12.6 with 64; over 131072 rows, 64 splits, 8 and 16 are even and 64 takes 1 us more.
 constexpr int kMergeCols = 32, kMergeLanes = kMergeCols / 4, kMergeGroups = 16, kMergePer = 4;
 template <int D, bool F16>
 __global__ __launch_bounds__(kMergeLanes * kMergeGroups) void int4_merge_kernel(Int4DecodeParams p) {
