@@ -237,11 +237,9 @@ struct Codes {
     else
       return as_bf16x8(u32x4_t{(w & mask0) | base0, ((w >> 1) & mask) | base, ((w >> 5) & mask) | base, ((w >> 9) & mask) | base});
   }
-  // A fragment of the bases themselves, 8 added to each with CENTRE.
-  template <bool CENTRE>
+  // A fragment of the bases themselves.
   BB_DEV static bf16x8_t bases() {
     if constexpr (F16) return as_bf16x8(u32x4_t{0x54005400u, 0x54005400u, 0x54005400u, 0x54005400u});
-    else if constexpr (CENTRE) return as_bf16x8(u32x4_t{0x43084308u, 0x41c041c0u, 0x41c041c0u, 0x41c041c0u});
     else return as_bf16x8(u32x4_t{0x43004300u, 0x41804180u, 0x41804180u, 0x41804180u});
   }
 };
@@ -280,6 +278,12 @@ BB_DEV float sum_rows16(float a, float b) {
 BB_DEV float sum_rows32(float a, float b) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// The sum / largest over the four quarters of the wave, in every lane.
+BB_DEV float quarters_sum(float v) { return xhalf_sum(sum_rows16(v, v)); }
+BB_DEV float quarters_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return xhalf_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
 BB_DEV float lane_value(float v, int lane) {
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
@@ -518,16 +522,11 @@ BB_DEV bf16x8_t fragment_of_ones() {
   return as_bf16x8(u32x4_t{one, one, one, one});
 }
 
-// Probabilities times scales as operands of 16 bits: two bf16 terms each (16 significant bits), the second PLANE bytes behind
-// the first. bf16 whatever the model's type (an fp16 product could fall below its range); one term alone would double the error
+// Probabilities times scales as operands of 16 bits: two bf16 terms each (off by 2^-17 at most). bf16 whatever the model's type (an fp16 product could fall below its range); one term alone would double the error
 // of a bf16 output (2.7e-3 of its norm instead of 1.6e-3, measured) and is coarser than an fp16 one.
-template <int PLANE>
-BB_DEV void put_terms(const float (&q)[4], uint8_t* dst) {
-  const uint32_t h0 = pack_bf16x2(q[0], q[1]), h1 = pack_bf16x2(q[2], q[3]);
-  const uint32_t l0 = pack_bf16x2(q[0] - __uint_as_float(h0 << 16), q[1] - __uint_as_float(h0 & 0xffff0000u));
-  const uint32_t l1 = pack_bf16x2(q[2] - __uint_as_float(h1 << 16), q[3] - __uint_as_float(h1 & 0xffff0000u));
-  *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{h0, h1};
-  *reinterpret_cast<u32x2_t*>(dst + PLANE) = u32x2_t{l0, l1};
+BB_DEV u32x2_t two_terms(float q0, float q1) {
+  const uint32_t hi = pack_bf16x2(q0, q1);
+  return u32x2_t{hi, pack_bf16x2(q0 - __uint_as_float(hi << 16), q1 - __uint_as_float(hi & 0xffff0000u))};
 }
 
 // Up to 4 query vectors.
@@ -537,8 +536,8 @@ BB_DEV void put_terms(const float (&q)[4], uint8_t* dst) {
 //           over its own group. One (s, z) word per lane turns them into scores; three lane swaps sum the groups and
 //           leave lane (k, a) with the whole score of query a alone, so that no lane's exponential is idle.
 //   values  The probabilities times the scales of column group t go to column 4 t + h of the operand, so one product serves
-//           all groups (the columns of a product whose rows are another group are not used). A row of the bases plus 8 gives
-//           what those add (the products meet codes shifted to -8..7, which halves what a rounded probability costs).
+//           all groups (the columns of a product whose rows are another group are not used). A row of the bases gives what
+//           those add.
 // What bounds it, measured: 131072 rows x 8 KV heads x 4 heads of 128 (168 MB) take 31.5 us, 5.3 TB/s, and the merge 4; with the
 // arithmetic taken out the loads alone and the merge take 30.3 together. The rest is the first chunks' way from memory and the
 // last chunks' arithmetic, which nothing overlaps: of two stages a wave, 160 KB a CU are in flight from the start, and a split
@@ -578,7 +577,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
   for (int i = 0; i < 4; ++i) {
     qa[i] = query_fragment(qw[i], on);
     qs = mma16<F16>(qa[i], fragment_of_ones<F16>(), qs);
-    qb = mma16<F16>(qa[i], Codes<F16>::template bases<false>(), qb);
+    qb = mma16<F16>(qa[i], Codes<F16>::bases(), qb);
   }
 #pragma unroll
   for (int h = 0; h < 4; ++h) {
@@ -605,7 +604,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
   const int fewest = part.limit(p, 0);  // the first token's is the smallest
 
   float m[W], l[W], zs[W][NG];
-  f32x4_t o[NDB], base = {0, 0, 0, 0};  // base: what the bases and the 8s add to the sums
+  f32x4_t o[NDB], base = {0, 0, 0, 0};  // base: what the bases add to the sums
 #pragma unroll
   for (int w = 0; w < W; ++w) {
     m[w] = -1.0e30f;
@@ -716,11 +715,13 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           q[u] = mul_lo(pr[w][u], vp[u][t]);
-          // the sums take 8 off every code, so that a rounded probability meets -8..7: z + 8 s here
-          zs[w][t] = fmaf(pr[w][u], f16_hi(vp[u][t]), fmaf(8.0f, q[u], zs[w][t]));
+          zs[w][t] = fmaf(pr[w][u], f16_hi(vp[u][t]), zs[w][t]);
         }
         const int col = D == 128 ? 4 * t + a : 4 * t + (a & 1) + 2 * w;
-        put_terms<4 * NG * PROW>(q, s + col * PROW + (D == 128 ? 0 : 128 * (a >> 1)) + 8 * k);
+        const u32x2_t q01 = two_terms(q[0], q[1]), q23 = two_terms(q[2], q[3]);
+        uint8_t* dst = s + col * PROW + (D == 128 ? 0 : 128 * (a >> 1)) + 8 * k;
+        *reinterpret_cast<u32x2_t*>(dst) = u32x2_t{q01[0], q23[0]};
+        *reinterpret_cast<u32x2_t*>(dst + 4 * NG * PROW) = u32x2_t{q01[1], q23[1]};
       }
     }
     wave_fence();
@@ -738,8 +739,8 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
     in.fetch_k(s, c + 2 * kWaves);
 #pragma unroll
     for (int j = 0; j < 2 * HV; ++j) {
-      base = mma16_bf16(Codes<false>::bases<true>(), pb[j], base);
-      base = mma16_bf16(Codes<false>::bases<true>(), pl[j], base);
+      base = mma16_bf16(Codes<false>::bases(), pb[j], base);
+      base = mma16_bf16(Codes<false>::bases(), pl[j], base);
     }
 #pragma unroll
     for (int hv = 0; hv < HV; ++hv)
@@ -791,20 +792,17 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
   finish<D, F16, 4>(p, sm, R, 0, g, split, tid);
 }
 
-// 5 and more query vectors, 16 of them a pass: the rows of the query operand are the vectors, one product per key group of 32
-// columns (lane (k, a) reads word a of every group of its key), so that no row is zero by design and no lane swap is needed;
-// lane (k, a) gets the sums of vectors 4 a .. 4 a + 3 and applies the (s, z) of all groups of its key. The value operand is
-// built once per column group, in the space of the K rows, and serves that group's two blocks of columns. Against blocks of 4
-// vectors on the kernel above it takes a quarter of the products and of the accumulators.
-// The VALU bounds it: about 820 instructions a chunk (codes to floats 220, probabilities times scales into two terms 350), 4000
-// cycles on a SIMD. 16 vectors x 8 KV heads x 128 over 32768 rows (42 MB) take 19.4 us: 6 us until the data is there, and the
-// two chunks of a wave behind it.
+// 5 and more query vectors, 16 of them a pass: column k of every product is vector k.
+//   scores  Rows are keys: lane (k, a) reads word a of every group of key k as the codes' operand, one product per group, and is
+//           left with vector k's sums over keys 4 a .. 4 a + 3 of the step, to which it applies those keys' (s, z).
+//   values  The lane's probabilities are the operand of the values' products as they are: with keys in the order of key_of_lane
+//           and key_of_step, a lane's 16 keys of 64 are those whose V codes the transposing read hands to its quarter. So no
+//           probability passes through LDS, and the maxima, sums and minima's parts stay with one vector per lane.
 template <int D, bool F16>
 __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4DecodeParams p) {
   __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][kStage];
   constexpr int CH = D == 128 ? 64 : 128;
   constexpr int NG = D / kGroup, NDB = D / 16, HV = CH / 64;
-  constexpr int PROW = 144, PBLK = 16 * PROW;  // a probability row of 64 keys (16 bytes more: other banks), and 16 of them
   const int split = blockIdx.x, g = blockIdx.y, v0 = blockIdx.z * kVecs, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), k = lane & 15, a = lane >> 4;
   const int R = p.T * p.G - v0 < kVecs ? p.T * p.G - v0 : kVecs;
@@ -828,7 +826,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
   // qz: the group sums as three bf16 terms each (24 bits), so that one product per step adds up z times them over the groups,
   // z in two terms (its 11 bits); lane (k, a) holds vector k's group a (head_dim 64: a < 2)
   bf16x8_t qa[NG], qz;
-  f32x4_t qb[NG];
+  f32x4_t qb[NG];  // what the bases add to the sums, negative
   {
     float sum = 0.0f;
 #pragma unroll
@@ -836,12 +834,11 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
       qa[j] = query_fragment(qw[j], k < R);
       const f32x4_t c = mma16<F16>(fragment_of_ones<F16>(), qa[j], f32x4_t{0, 0, 0, 0});  // every row: vector k's sum
       sum = a == j ? c[0] : sum;
-      qb[j] = mma16<F16>(qa[j], Codes<F16>::template bases<false>(), f32x4_t{0, 0, 0, 0});
+      qb[j] = mma16<F16>(Codes<F16>::bases(), qa[j], f32x4_t{0, 0, 0, 0});
 #pragma unroll
       for (int e = 0; e < 4; ++e) qb[j][e] = -qb[j][e];
     }
     u32x4_t w = {0, 0, 0, 0};
-    sum *= p.c;
 #pragma unroll
     for (int j = 0; j < 3; ++j) {
       const uint32_t top = __float_as_uint(sum) & 0xffff0000u;
@@ -855,70 +852,69 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
   for (int j = 0; j < 4; ++j)
     kread[j] = D == 128 ? 1024 * (k >> 2) + 64 * (k & 3) + 16 * (j ^ (-(k >> 2) & 3)) + 4 * a
                         : 512 * (k >> 2) + 32 * (k & 3) + 128 * ((k >> 3) ^ (j & 1)) + 4 * a;
-  int lim[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) lim[e] = part.limit(p, v0 + 4 * a + e);
-  const int fewest = part.limit(p, v0);
+  const int lim = part.limit(p, v0 + k), fewest = part.limit(p, v0);
 
-  float m[4], l[4], zs[4][NG];
+  float m = -1.0e30f, l = 0.0f, zs[NG];
   f32x4_t o[NDB], base[NG];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    m[e] = -1.0e30f;
-    l[e] = 0.0f;
-#pragma unroll
-    for (int t = 0; t < NG; ++t) zs[e][t] = 0.0f;
-  }
 #pragma unroll
   for (int db = 0; db < NDB; ++db) o[db] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-  for (int t = 0; t < NG; ++t) base[t] = f32x4_t{0, 0, 0, 0};
+  for (int t = 0; t < NG; ++t) {
+    zs[t] = 0.0f;
+    base[t] = f32x4_t{0, 0, 0, 0};
+  }
 
   const Codes<F16> k_codes;
   const Codes<false> v_codes;
-  // the NG params words of a key, from the stage's K or V params
-  auto params = [&](const uint8_t* at, int hv, int u, uint32_t (&w)[NG]) {
+  // the NG params words of key 16 a + 8 (e >> 1) + 2 (e & 1) + key_of_step(u) of half hv, from the stage's K or V params
+  auto params = [&](const uint8_t* at, int hv, int u, int e, uint32_t (&w)[NG]) {
     if constexpr (D == 128) {
-      const u32x4_t r = *reinterpret_cast<const u32x4_t*>(at + 256 * u + 16 * k);
+      const u32x4_t r = *reinterpret_cast<const u32x4_t*>(at + 256 * u + 64 * a + 16 * e);
 #pragma unroll
       for (int t = 0; t < NG; ++t) w[t] = r[t];
     } else {
-      const u32x2_t r = *reinterpret_cast<const u32x2_t*>(at + 512 * (u & 1) + 256 * hv + 16 * k + 8 * (u >> 1));
+      const u32x2_t r = *reinterpret_cast<const u32x2_t*>(at + 512 * (u & 1) + 256 * hv + 64 * a + 16 * e + 8 * (u >> 1));
       w[0] = r[0];
       w[1] = r[1];
     }
   };
   int st = 0;
   for (int c = wave; c < chunks; c += kWaves, st ^= 1) {
-    __builtin_amdgcn_s_waitcnt(0x0F7F);  // vmcnt(15): K
+    __builtin_amdgcn_s_waitcnt(0x0F7F);  // vmcnt(15): this chunk's K has landed; its V and the next chunk may be in flight
     wave_fence();
     uint8_t* s = sm[wave][st];
     complete<D, F16, CH>(p, part, in, c, g, lane, s);
 
-    float x[HV][4][4];  // [half][step][vector]
+    float x[HV][4][4];  // [half][step][key of the lane's four], not yet times p.c
 #pragma unroll
     for (int hv = 0; hv < HV; ++hv)
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        uint32_t kp[NG];
-        params(s + kKp, hv, u, kp);
         const float z = f16_hi(*reinterpret_cast<const uint32_t*>(
             s + kKp + 16 * k + (D == 128 ? 256 * u + 4 * a : 512 * (u & 1) + 256 * hv + 8 * (u >> 1) + 4 * (a & 1))));
         const uint32_t top = __float_as_uint(z) & 0xffff0000u;
         const uint32_t zw = (top >> 16) | (__float_as_uint(z - __uint_as_float(top)) & 0xffff0000u);
-        f32x4_t y = mma16_bf16(qz, as_bf16x8(u32x4_t{zw, zw, zw, 0u}), f32x4_t{0, 0, 0, 0});
+        const f32x4_t y = mma16_bf16(as_bf16x8(u32x4_t{zw, zw, zw, 0u}), qz, f32x4_t{0, 0, 0, 0});
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[hv][u][e] = y[e];
+        f32x4_t acc[NG];
 #pragma unroll
         for (int t = 0; t < NG; ++t) {
           const uint32_t kw = *reinterpret_cast<const uint32_t*>(
               s + (D == 128 ? kread[t] + 512 * (u & 1) + 256 * (u >> 1) : kread[u >> 1] + 2048 * hv + 256 * (u & 1) + 16 * t));
-          const f32x4_t acc = mma16<F16>(qa[t], k_codes(kw), qb[t]);
-          const float sc = mul_lo(p.c, kp[t]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = fmaf(sc, acc[e], y[e]);
+          acc[t] = mma16<F16>(k_codes(kw), qa[t], qb[t]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[hv][u][e] = y[e];
+        for (int e = 0; e < 4; ++e) {
+          uint32_t kp[NG];
+          params(s + kKp, hv, u, e, kp);
+#pragma unroll
+          for (int t = 0; t < NG; ++t) x[hv][u][e] = fmaf(f16_lo(kp[t]), acc[t][e], x[hv][u][e]);
+        }
       }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the K rows are read, their space is free
+    wave_fence();
+    in.fetch_k(s, c + 2 * kWaves);
     if (c * CH + CH > fewest) {
       asm volatile("; a branch: most chunks are whole");
 #pragma unroll
@@ -927,7 +923,8 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
         for (int u = 0; u < 4; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (c * CH + key_of_lane(k) + 64 * hv + key_of_step(u) >= lim[e]) x[hv][u][e] = -__builtin_huge_valf();
+            if (c * CH + 64 * hv + 16 * a + 8 * (e >> 1) + 2 * (e & 1) + key_of_step(u) >= lim)
+              x[hv][u][e] = -__builtin_huge_valf();
     }
     float pr[HV][4][4];
     float most = 0.0f;
@@ -937,106 +934,89 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          pr[hv][u][e] = fast_exp2(x[hv][u][e] - m[e]);
+          pr[hv][u][e] = fast_exp2(fmaf(x[hv][u][e], p.c, -m));
           most = fmaxf(most, pr[hv][u][e]);
         }
     if (__builtin_amdgcn_ballot_w64(most > kOver)) {
-      float alpha[4];
+      float mx = x[0][0][0];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float mx = x[0][0][e];
+      for (int i = 1; i < 16 * HV; ++i) mx = fmaxf(mx, x[i >> 4][(i >> 2) & 3][i & 3]);
+      const float mn = fmaxf(m, quarters_max(mx) * p.c), alpha = fast_exp2(m - mn);
+      m = mn;
+      l *= alpha;
 #pragma unroll
-        for (int i = 1; i < 4 * HV; ++i) mx = fmaxf(mx, x[i >> 2][i & 3][e]);
-        const float mn = fmaxf(m[e], row_max(mx));
-        alpha[e] = fast_exp2(m[e] - mn);
-        m[e] = mn;
-        l[e] *= alpha[e];
+      for (int i = 0; i < 16 * HV; ++i)
+        pr[i >> 4][(i >> 2) & 3][i & 3] = fast_exp2(fmaf(x[i >> 4][(i >> 2) & 3][i & 3], p.c, -mn));
 #pragma unroll
-        for (int i = 0; i < 4 * HV; ++i) pr[i >> 2][i & 3][e] = fast_exp2(x[i >> 2][i & 3][e] - mn);
+      for (int t = 0; t < NG; ++t) {
+        zs[t] *= alpha;
 #pragma unroll
-        for (int t = 0; t < NG; ++t) zs[e][t] *= alpha[e];
+        for (int e = 0; e < 4; ++e) base[t][e] *= alpha;
       }
-      // column k of the sums is vector k, whose maximum quarter k >> 2 keeps as its element k & 3
-      float al[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) al[e] = __shfl(alpha[e], 16 * (k >> 2));
-      const float ac = k & 2 ? (k & 1 ? al[3] : al[2]) : (k & 1 ? al[1] : al[0]);
+      for (int db = 0; db < NDB; ++db)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-#pragma unroll
-        for (int t = 0; t < NG; ++t) base[t][e] *= ac;
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) o[db][e] *= ac;
-      }
+        for (int e = 0; e < 4; ++e) o[db][e] *= alpha;
     }
 #pragma unroll
-    for (int hv = 0; hv < HV; ++hv)
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) l[e] += pr[hv][u][e];
+    for (int i = 0; i < 16 * HV; ++i) l += pr[i >> 4][(i >> 2) & 3][i & 3];
 
-    __builtin_amdgcn_s_waitcnt(0x0F7A);  // vmcnt(10): this chunk's V too
-    // (column group, half) blocks: probabilities times scales into LDS, [vector][key], then that group's columns
+    __builtin_amdgcn_s_waitcnt(0x0F7F);  // vmcnt(15): this chunk's V; the next chunk and the K behind it may be in flight
+    wave_fence();
 #pragma unroll
-    for (int i = 0; i < NG * HV; ++i) {
-      const int t = i / HV, hv = i % HV;
-      wave_fence();
-      float q[4][4];
+    for (int hv = 0; hv < HV; ++hv) {
+      v2i_t vw[NDB];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        uint32_t vp[NG];
-        params(s + kVp, hv, u, vp);
-        const float sc = f16_lo(vp[t]), zz = fmaf(8.0f, sc, f16_hi(vp[t]));  // the sums take 8 off every code
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          q[e][u] = pr[hv][u][e] * sc;
-          zs[e][t] = fmaf(pr[hv][u][e], zz, zs[e][t]);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) put_terms<PBLK>(q[e], s + (4 * a + e) * PROW + 8 * k);
-      wave_fence();
-      const uint8_t* src = s + k * PROW + 32 * a;
-      bf16x8_t pb[2], pl[2];
+      for (int db = 0; db < NDB; ++db) vw[db] = read_tr4(s + kVq + v_block_at<D>(k, a, hv, db));
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        pb[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + 16 * j));
-        pl[j] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(src + PBLK + 16 * j));
-        base[t] = mma16_bf16(Codes<false>::bases<true>(), pb[j], base[t]);
-        base[t] = mma16_bf16(Codes<false>::bases<true>(), pl[j], base[t]);
-      }
+        // element 2 (2 (e & 1) + (u >> 1)) + (u & 1) of operand j is key (u, e) with e >> 1 = j
+        uint32_t vp[4][2][NG];
 #pragma unroll
-      for (int db = 2 * t; db < 2 * t + 2; ++db) {
-        const v2i_t r = read_tr4(s + kVq + v_block_at<D>(k, a, hv, db));
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const bf16x8_t vf = v_codes((uint32_t)(j ? r.y : r.x));
-          o[db] = mma16_bf16(vf, pb[j], o[db]);
-          o[db] = mma16_bf16(vf, pl[j], o[db]);
+          for (int e = 0; e < 2; ++e) params(s + kVp, hv, u, 2 * j + e, vp[u][e]);
+#pragma unroll
+        for (int t = 0; t < NG; ++t) {
+          u32x4_t hi, lo;
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float p0 = pr[hv][2 * i][2 * j + e], p1 = pr[hv][2 * i + 1][2 * j + e];
+              const uint32_t w0 = vp[2 * i][e][t], w1 = vp[2 * i + 1][e][t];
+              const u32x2_t q = two_terms(mul_lo(p0, w0), mul_lo(p1, w1));
+              hi[2 * e + i] = q[0];
+              lo[2 * e + i] = q[1];
+              zs[t] = fmaf(p0, f16_hi(w0), fmaf(p1, f16_hi(w1), zs[t]));
+            }
+          base[t] = mma16_bf16(Codes<false>::bases(), as_bf16x8(hi), base[t]);
+          base[t] = mma16_bf16(Codes<false>::bases(), as_bf16x8(lo), base[t]);
+#pragma unroll
+          for (int db = 2 * t; db < 2 * t + 2; ++db) {
+            const bf16x8_t vf = v_codes((uint32_t)(j ? vw[db].y : vw[db].x));
+            o[db] = mma16_bf16(vf, as_bf16x8(hi), o[db]);
+            o[db] = mma16_bf16(vf, as_bf16x8(lo), o[db]);
+          }
         }
       }
     }
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this stage's reads are done before its next loads are issued
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the V rows are read
     wave_fence();
-    in.fetch_k(s, c + 2 * kWaves);
     in.fetch_v(s, c + 2 * kWaves);
   }
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): nothing lands in LDS any more
 
   WaveState<D, kVecs>* mine = reinterpret_cast<WaveState<D, kVecs>*>(sm[wave]);
+  l = quarters_sum(l);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float sum = row_sum(l[e]);
-#pragma unroll
-    for (int t = 0; t < NG; ++t) {
-      const float z = row_sum(zs[e][t]);
-      if (k == 0) mine->z[4 * a + e][t] = z;
-    }
-    if (k == 0) {
-      mine->m[4 * a + e] = m[e];
-      mine->l[4 * a + e] = sum;
-    }
+  for (int t = 0; t < NG; ++t) {
+    zs[t] = quarters_sum(zs[t]);
+    if (a == 0) mine->z[k][t] = zs[t];
+  }
+  if (a == 0) {
+    mine->m[k] = m;
+    mine->l[k] = l;
   }
 #pragma unroll
   for (int db = 0; db < NDB; ++db) {
