@@ -524,9 +524,14 @@ BB_DEV bf16x8_t fragment_of_ones() {
 
 // Probabilities times scales as operands of 16 bits: two bf16 terms each (off by 2^-17 at most). bf16 whatever the model's type (an fp16 product could fall below its range); one term alone would double the error
 // of a bf16 output (2.7e-3 of its norm instead of 1.6e-3, measured) and is coarser than an fp16 one.
+// The rests are dot products of the first terms with (-1, 0) and (0, -1) added to the numbers, one instruction each. (The asm
+// keeps the compiler from rounding a number a second time to have its first term alone, and (-1, 0) in a register: as an inline
+// constant the instruction reads it as (0, -1).)
 BB_DEV u32x2_t two_terms(float q0, float q1) {
-  const uint32_t hi = pack_bf16x2(q0, q1);
-  return u32x2_t{hi, pack_bf16x2(q0 - __uint_as_float(hi << 16), q1 - __uint_as_float(hi & 0xffff0000u))};
+  uint32_t hi = pack_bf16x2(q0, q1), first = 0x0000bf80u;
+  asm("" : "+v"(hi));
+  asm("" : "+s"(first));
+  return u32x2_t{hi, pack_bf16x2(dot2<false>(hi, first, q0), dot2<false>(hi, 0xbf800000u, q1))};
 }
 
 // Up to 4 query vectors.
