@@ -42,8 +42,9 @@ def attend(q, k4, kp, v4, vp, n, scale, causal=False):
     """q [T, H, d] over the first n rows of a packed cache, in 64 bits: (out [T, H, d], bound [T, H, d]).
 
     The bound is what a kernel that works in fp32 with 16-bit matrix operands may be off before its output is rounded:
-      * a probability times a V scale as two operands of 8 significant bits each is off by 2^-16 of itself at most, and
-        meets codes shifted to -8..7: 2^-16 * 8 sum_j p_j s_j;
+      * a probability times a V scale as two operands of 8 significant bits each is off by 2^-17 of itself at most (the first
+        operand's rest is at most 2^-8 of the power of two below the number, and rounding a rest of that size is off by 2^-9 of
+        it), and meets codes of 0..15: 2^-17 * 15 < 2^-16 * 8, times sum_j p_j s_j;
       * a score is a sum over d of products q (16 + code) s and q z in fp32: at most 64 roundings of 2^-24 of their absolute
         sum (31 s + |z|) |q| scale, the probabilities then are off by as much (exp), and the fp32 exponential and the sums
         over keys (chains of at most 4096) by 4096 * 2^-24 relative;

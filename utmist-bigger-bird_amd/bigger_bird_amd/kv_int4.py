@@ -24,7 +24,7 @@ _strides = functools.lru_cache(maxsize=1024)(_lib.i64s)
 MAX_TOKENS = 16  # query tokens of one decode call
 # Query vectors per KV head (tokens x heads) up to which a handle attends the packed rows; the kernel takes 16 a pass over the
 # cache. Against reading the cache back and flash attention over it, whole calls (us), 8 KV heads x 4 of 128 over 131072 rows:
-# 4 tokens 49 and 366, 16 tokens (64 vectors) 175 and 368; 4 x 8, 16 tokens (128 vectors) 192 and 224; over 16384 rows 46 and 48.
+# 4 tokens 43 and 365, 16 tokens (64 vectors) 158 and 367; 4 x 8, 16 tokens (128 vectors) 169 and 225; over 16384 rows 40 and 47.
 _HANDLE_VECTORS = 128
 _HEAD_DIMS = (32, 64, 128, 256)
 _HALVES = (16, 32, 64, 128)  # their packed rows' bytes
