@@ -351,6 +351,48 @@ def test_captured_step_follows_the_length(T, d, dtype, dev):
             assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), f"cache after replay {i}"
 
 
+@pytest.mark.parametrize("T,H,Hkv,d,dtype", [(1, 8, 2, 128, BF16), (4, 8, 2, 128, FP16), (3, 20, 2, 64, BF16)])
+def test_two_captured_steps_with_partials(T, H, Hkv, d, dtype, dev):
+    """Two steps captured over caches of several splits, in one memory pool, replayed in turn while both lengths grow, the live
+    splits with them: every replay equals the eager step bit for bit, cache bytes included."""
+    _say("two graphs", T, H, Hkv, d, dtype)
+    gen = torch.Generator(device=dev).manual_seed(53)
+    steps, graphs = 4, []
+    for n0, cap, filled in ((900, 5000, 4900), (2550, 2700, 2550)):
+        cache = (*_cache(gen, Hkv, filled, cap, d, dev), *_cache(gen, Hkv, filled, cap, d, dev))
+        q = torch.randn(T, H, d, generator=gen, device=dev).to(dtype)
+        k, v = (_rows(gen, Hkv, T, d, dtype, dev).contiguous() for _ in range(2))
+        scratch = [x.clone() for x in cache]
+        eager = [x.clone() for x in cache]
+        length = torch.tensor([n0], device=dev)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):  # warm-up on copies
+            decode_int4_append(q, *scratch, k, v, length + T, d ** -0.5)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0][0].pool() if graphs else None):
+            length.add_(T)
+            out = decode_int4_append(q, *cache, k, v, length, d ** -0.5)
+        graphs.append((graph, cache, eager, q, k, v, length, out, n0))
+    for i in range(steps):
+        for graph, cache, eager, q, k, v, length, out, n0 in graphs:
+            for x in (q, k, v):
+                x.copy_(torch.randn(x.shape, generator=gen, device=dev))
+            jump = 400 if n0 == 900 else 0  # rows that the cache holds already
+            length.add_(jump)
+            graph.replay()
+            torch.cuda.synchronize()
+            n = n0 + (i + 1) * (T + jump)
+            assert length.item() == n
+            want = decode_int4_append(q, *eager, k, v, torch.tensor([n], device=dev), d ** -0.5)
+            _check_decode(out, q, eager, n, d ** -0.5, False)
+            assert torch.equal(out, want), f"replay {i}"
+            for x, y in zip(cache, eager):
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), f"cache after replay {i}"
+
+
 def test_two_streams_at_once(dev):
     """Calls on two streams, each with its own cache, interleaved: every result as alone, and the same on every call."""
     _say("streams")
