@@ -345,8 +345,8 @@ int bb_rope_inplace(void* x, const int64_t* sx, int B, int Hh, int64_t T, int D,
  * max clamped to +-65504 and NaN left out of them, each operation in fp32:
  *   z = fp16(min),  s = fp16(max((max - z) / 15, 0)),  code = rint((x - z) / s) clamped to 0 .. 15 (0 where s = 0 or x is
  *   NaN);
- * the value of an element is s * code + z in fp32. A group of NaN alone has s = z = 0. Byte b of a packed row holds element 2 b in its low and 2 b + 1 in its
- * high four bits.
+ * the value of an element is s * code + z in fp32. A group of NaN alone has s = z = 0. Byte b of a packed row holds element
+ * 2 b in its low and 2 b + 1 in its high four bits.
  * A cache is codes [heads, cap, D / 2] bytes and params [heads, cap, D / 32, 2] fp16 (s, z), for K and for V: the rows of
  * one head are contiguous, heads are sc[] apart. sc[4] = head strides of kq (bytes, a multiple of 16), kp (fp16 elements,
  * even), vq and vp (alike). Codes are 16-byte aligned, params 4-byte aligned. A pointer into the middle of a cache (row a
@@ -371,7 +371,8 @@ int bb_int4_dequantize(const uint8_t* kq, const void* kp, const uint8_t* vq, con
  * gives zeros. D = 64 or 128; any number of query heads per KV head.
  * n: T <= n <= cap. With n_dev (an int64 in device memory) the length is read there and clamped to 0 .. cap, and n is
  * ignored; every launch shape then depends on cap alone, so a captured graph stays valid while the cache grows.
- * Workspace: bb_int4_decode_workspace(n, ...), with n_dev bb_int4_decode_workspace(cap, ...).
+ * Workspace: bb_int4_decode_workspace(n, ...), with n_dev bb_int4_decode_workspace(cap, ...). Splits of 2^24 keys and more
+ * (2^33 / Hkv rows) are refused, as are writes and reads back of 2^35 elements a head and more.
  */
 int bb_int4_decode(const void* q, const int64_t* sq, const uint8_t* kq, const void* kp, const uint8_t* vq, const void* vp,
                    const int64_t* sc, int64_t n, const int64_t* n_dev, int64_t cap, int T, int H, int Hkv, int D,
