@@ -175,8 +175,9 @@ __global__ __launch_bounds__(256) void int4_dequantize_kernel(Int4ReadSet s0, In
 //
 // Mathematics. With k = s c + z per group of 32 (c the codes), q.k = sum_g s_g (q_g . c_g) + z_g sum(q_g), and
 // o = sum_j p_j s_j c_j + sum_j p_j z_j per column group: the codes go to the matrix cores as they are, exact in 16 bits, and
-// scales and minima are applied in fp32 to the sums (scores) or to the probabilities (values). A code becomes a 16-bit float
-// base + c by an and-or per two codes (see Codes); the bases are taken back from the sums.
+// scales and minima are applied in fp32 to the sums (scores) or to the probabilities (values). In the scores a code becomes a
+// 16-bit float base + c by an and-or per two codes (see Codes), and the bases are taken back from the sums; in the values it is
+// a subnormal number (see ValueCodes).
 //
 // A chunk's 10 KB (codes and params of K and of V) stream straight into the wave's LDS with ten buffer loads that cover
 // whole lines, two chunks ahead. Pieces land so that the operand reads meet no bank twice: see the offsets at each. V rows
@@ -215,7 +216,7 @@ BB_DEV f32x4_t mma16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
   else return mma16_bf16(a, b, c);
 }
 
-// Eight codes as 16-bit floats base + c, in the order 0, 4, 1, 5, 2, 6, 3, 7 (the halves of the word side by side). In fp16
+// Eight K codes as 16-bit floats base + c, in the order 0, 4, 1, 5, 2, 6, 3, 7 (the halves of the word side by side). In fp16
 // 64.0 has an ulp of 1/16: bits 4..7 of a half are a code in its place. In bf16 128.0 has an ulp of 1 (bits 0..3) and 16.0 one
 // of 1/8 (bits 3..6); no place serves two pairs. So of the four pairs three take a shift. The constants stay in registers
 // (masks scalar, bases vector), where one v_and_or_b32 takes both; as literals they cost an instruction more.
@@ -243,6 +244,21 @@ struct Codes {
     else return as_bf16x8(u32x4_t{0x43004300u, 0x41804180u, 0x41804180u, 0x41804180u});
   }
 };
+
+// Eight V codes as subnormal bf16 numbers, in the same order: the matrix cores take them exactly, and no base has to come off
+// again. (With bases the sums are 17 times what is wanted, and so is their rounding: over 131072 rows 3.6e-5 of an output's norm
+// instead of 6e-6, over 1000000 in 64 splits 2.7e-4 instead of 4e-5, at the same time.) Bits 0..3 of a half are c * 2^-133, bits
+// 3..6 c * 2^-130; the first pair's probabilities carry the factor of 8 between them (prob_up). 2^64 on all of them keeps the
+// products in fp32's normal range.
+struct ValueCodes {
+  uint32_t mask0, mask;
+  BB_DEV ValueCodes() : mask0(0x000f000fu), mask(0x00780078u) {}
+  BB_DEV bf16x8_t operator()(uint32_t w) const {
+    return as_bf16x8(u32x4_t{w & mask0, (w >> 1) & mask, (w >> 5) & mask, (w >> 9) & mask});
+  }
+};
+BB_DEV float prob_up(bool first_pair) { return first_pair ? 0x1p67f : 0x1p64f; }
+constexpr float kSumDown = 0x1p66f;  // what brings the sums back: 2^130 / 2^64
 
 // a times the low / high fp16 half of w, in one instruction (fp32 product, rounded once).
 BB_DEV float mul_lo(float a, uint32_t w) {
@@ -522,8 +538,10 @@ BB_DEV bf16x8_t fragment_of_ones() {
   return as_bf16x8(u32x4_t{one, one, one, one});
 }
 
-// Probabilities times scales as operands of 16 bits: two bf16 terms each (off by 2^-17 at most). bf16 whatever the model's type (an fp16 product could fall below its range); one term alone would double the error
-// of a bf16 output (2.7e-3 of its norm instead of 1.6e-3, measured) and is coarser than an fp16 one.
+// Probabilities times scales as operands of 16 bits: two bf16 terms each (off by 2^-17 at most). bf16 whatever the model's type
+// (an fp16 product could fall below its range); one term alone would double the error of a bf16 output (2.7e-3 of its norm
+// instead of 1.6e-3, measured) and is coarser than an fp16 one. With two the sums are off by 5e-6 of the output's norm, a
+// fortieth of an fp16 output's own rounding; a third would bring that to 1e-6 (8111 rows) and costs 3 to 7 % of the kernel.
 // The rests are dot products of the first terms with (-1, 0) and (0, -1) added to the numbers, one instruction each. (The asm
 // keeps the compiler from rounding a number a second time to have its first term alone, and (-1, 0) in a register: as an inline
 // constant the instruction reads it as (0, -1).)
@@ -541,8 +559,7 @@ BB_DEV u32x2_t two_terms(float q0, float q1) {
 //           over its own group. One (s, z) word per lane turns them into scores; three lane swaps sum the groups and
 //           leave lane (k, a) with the whole score of query a alone, so that no lane's exponential is idle.
 //   values  The probabilities times the scales of column group t go to column 4 t + h of the operand, so one product serves
-//           all groups (the columns of a product whose rows are another group are not used). A row of the bases gives what
-//           those add.
+//           all groups (the columns of a product whose rows are another group are not used).
 // What bounds it, measured: 131072 rows x 8 KV heads x 4 heads of 128 (168 MB) take 31.8 us, 5.3 TB/s, and the merge 4; with the
 // arithmetic taken out the loads alone and the merge take 30.3 together. The rest is the first chunks' way from memory and the
 // last chunks' arithmetic, which nothing overlaps: with two stages a wave 160 KB a CU are in flight from the start, and a split
@@ -607,9 +624,10 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
 #pragma unroll
   for (int w = 0; w < W; ++w) lim[w] = part.limit(p, D == 128 ? a : (a & 1) + 2 * w);
   const int fewest = part.limit(p, 0);  // the first token's is the smallest
+  const float up01 = prob_up(k % 2 == 0);  // a lane's steps 0 and 1: the first pair of its operand's eight keys where k is even
 
   float m[W], l[W], zs[W][NG];
-  f32x4_t o[NDB], base = {0, 0, 0, 0};  // base: what the bases add to the sums
+  f32x4_t o[NDB];
 #pragma unroll
   for (int w = 0; w < W; ++w) {
     m[w] = -1.0e30f;
@@ -621,7 +639,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
   for (int db = 0; db < NDB; ++db) o[db] = f32x4_t{0, 0, 0, 0};
 
   const Codes<F16> k_codes;
-  const Codes<false> v_codes;
+  const ValueCodes v_codes;
   int st = 0;
   for (int c = wave; c < chunks; c += kWaves, st ^= 1) {
     __builtin_amdgcn_s_waitcnt(0x0F7F);  // vmcnt(15): this chunk's K has landed; its V and the next chunk may be in flight
@@ -688,7 +706,6 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
       const float ac = k & 2 ? (k & 1 ? al[3] : al[2]) : (k & 1 ? al[1] : al[0]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        base[e] *= ac;
 #pragma unroll
         for (int db = 0; db < NDB; ++db) o[db][e] *= ac;
       }
@@ -713,15 +730,17 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
 #pragma unroll
     for (int w = 0; w < W; ++w) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) l[w] += pr[w][u];
+      for (int u = 0; u < 4; ++u) {
+        l[w] += pr[w][u];
+#pragma unroll
+        for (int t = 0; t < NG; ++t) zs[w][t] = fmaf(pr[w][u], f16_hi(vp[u][t]), zs[w][t]);
+        pr[w][u] *= u < 2 ? up01 : prob_up(false);
+      }
 #pragma unroll
       for (int t = 0; t < NG; ++t) {
         float q[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          q[u] = mul_lo(pr[w][u], vp[u][t]);
-          zs[w][t] = fmaf(pr[w][u], f16_hi(vp[u][t]), zs[w][t]);
-        }
+        for (int u = 0; u < 4; ++u) q[u] = mul_lo(pr[w][u], vp[u][t]);
         const int col = D == 128 ? 4 * t + a : 4 * t + (a & 1) + 2 * w;
         const u32x2_t q01 = two_terms(q[0], q[1]), q23 = two_terms(q[2], q[3]);
         uint8_t* dst = s + col * PROW + (D == 128 ? 0 : 128 * (a >> 1)) + 8 * k;
@@ -742,11 +761,6 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the probabilities are read, the K rows' space is free
     wave_fence();
     in.fetch_k(s, c + 2 * kWaves);
-#pragma unroll
-    for (int j = 0; j < 2 * HV; ++j) {
-      base = mma16_bf16(Codes<false>::bases(), pb[j], base);
-      base = mma16_bf16(Codes<false>::bases(), pl[j], base);
-    }
 #pragma unroll
     for (int hv = 0; hv < HV; ++hv)
 #pragma unroll
@@ -790,7 +804,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
     for (int e = 0; e < 4; ++e) {
       float lo = k & 4 ? o[2 + j][e] : o[j][e];
       if constexpr (D == 128) lo = k & 8 ? (k & 4 ? o[6 + j][e] : o[4 + j][e]) : lo;
-      r[e] = lo - base[e];
+      r[e] = lo * kSumDown;
     }
     if (D == 128 || k < 8) *reinterpret_cast<f32x4_t*>(&mine->o[k & 3][32 * (k >> 2) + 16 * j + 4 * a]) = r;
   }
@@ -864,17 +878,14 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
   const int lim = part.limit(p, v0 + k), fewest = part.limit(p, v0);
 
   float m = -1.0e30f, l = 0.0f, zs[NG];
-  f32x4_t o[NDB], base[NG];
+  f32x4_t o[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) o[db] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-  for (int t = 0; t < NG; ++t) {
-    zs[t] = 0.0f;
-    base[t] = f32x4_t{0, 0, 0, 0};
-  }
+  for (int t = 0; t < NG; ++t) zs[t] = 0.0f;
 
   const Codes<F16> k_codes;
-  const Codes<false> v_codes;
+  const ValueCodes v_codes;
   // the NG params words of key 16 a + 8 (e >> 1) + 2 (e & 1) + key_of_step(u) of half hv, from the stage's K or V params
   auto params = [&](const uint8_t* at, int hv, int u, int e, uint32_t (&w)[NG]) {
     if constexpr (D == 128) {
@@ -957,11 +968,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
       for (int i = 0; i < 16 * HV; ++i)
         pr[i >> 4][(i >> 2) & 3][i & 3] = fast_exp2(fmaf(x[i >> 4][(i >> 2) & 3][i & 3], p.c, -mn));
 #pragma unroll
-      for (int t = 0; t < NG; ++t) {
-        zs[t] *= alpha;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) base[t][e] *= alpha;
-      }
+      for (int t = 0; t < NG; ++t) zs[t] *= alpha;
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -994,13 +1001,12 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
             for (int i = 0; i < 2; ++i) {
               const float p0 = pr[hv][2 * i][2 * j + e], p1 = pr[hv][2 * i + 1][2 * j + e];
               const uint32_t w0 = vp[2 * i][e][t], w1 = vp[2 * i + 1][e][t];
-              const u32x2_t q = two_terms(mul_lo(p0, w0), mul_lo(p1, w1));
+              const float up = prob_up(e == 0 && i == 0);
+              const u32x2_t q = two_terms(mul_lo(p0 * up, w0), mul_lo(p1 * up, w1));
               hi[2 * e + i] = q[0];
               lo[2 * e + i] = q[1];
               zs[t] = fmaf(p0, f16_hi(w0), fmaf(p1, f16_hi(w1), zs[t]));
             }
-          base[t] = mma16_bf16(Codes<false>::bases(), as_bf16x8(hi), base[t]);
-          base[t] = mma16_bf16(Codes<false>::bases(), as_bf16x8(lo), base[t]);
 #pragma unroll
           for (int db = 2 * t; db < 2 * t + 2; ++db) {
             const bf16x8_t vf = v_codes((uint32_t)(j ? vw[db].y : vw[db].x));
@@ -1031,7 +1037,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
   for (int db = 0; db < NDB; ++db) {
     f32x4_t r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = o[db][e] - base[db / 2][e];
+    for (int e = 0; e < 4; ++e) r[e] = o[db][e] * kSumDown;
     *reinterpret_cast<f32x4_t*>(&mine->o[k][16 * db + 4 * a]) = r;
   }
   finish<D, F16, kVecs>(p, sm, R, v0, g, split, tid);
