@@ -46,3 +46,63 @@ def test_sums_keep_their_bits(dev):
         print(f"head {h}: off {off / want.norm():.2e}, rounding {rounding.norm() / want.norm():.2e}, "
               f"limit {limit / want.norm():.2e}", flush=True)
         assert off <= 1.02 * limit
+
+
+def _cache(gen, hk, n, cap, d, dev):
+    """Packed K and V of n rows, the spare rows behind them of NaN params."""
+    out = []
+    for _ in range(2):
+        q4 = torch.randint(0, 256, (hk, cap, d // 2), generator=gen, device=dev, dtype=torch.uint8)
+        p4 = torch.full((hk, cap, d // 32, 2), float("nan"), device=dev, dtype=FP16)
+        x = torch.randn(hk, n, d, generator=gen, device=dev) * torch.exp(0.7 * torch.randn(hk, 1, d, generator=gen, device=dev))
+        q4[:, :n], p4[:, :n] = plain.pack(*plain.quantize(x))
+        out += [q4, p4]
+    return out
+
+
+# one split and several; up to 4 vectors of a KV head, and more
+SHAPES = [(500, 1, 8, 2, 128), (500, 4, 8, 2, 64), (4000, 1, 8, 2, 64), (4000, 1, 8, 2, 128), (4000, 3, 16, 2, 128),
+          (5000, 2, 20, 2, 64)]
+
+
+@pytest.mark.parametrize("n,T,H,Hkv,d", SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_nonfinite_query_gives_nan(n, T, H, Hkv, d, dtype, dev):
+    """A NaN or an infinity of either sign in one query is a NaN row, as in the formula, with a host and a device length, and no
+    other row changes; a token that attends no row stays zeros whatever its query holds."""
+    _say("nonfinite", n, T, H, Hkv, d, dtype)
+    gen = torch.Generator(device=dev).manual_seed(n + T)
+    cache = _cache(gen, Hkv, n, n + 3, d, dev)
+    q = torch.randn(T, H, d, generator=gen, device=dev).to(dtype)
+    want = decode_int4(q, *cache, n, 0.1, causal=True)
+    assert torch.isfinite(want.float()).all()
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        q2 = q.clone()
+        q2[T - 1, 3, 5] = bad
+        for length in (n, torch.tensor([n], device=dev)):
+            got = decode_int4(q2, *cache, length, 0.1, causal=True)
+            assert got[T - 1, 3].isnan().all(), bad
+            if length is n:
+                got[T - 1, 3] = want[T - 1, 3]
+                assert torch.equal(got, want)
+        if T > 1:
+            q2[0, 1, 7] = bad
+            got = decode_int4(q2, *cache, torch.tensor([T - 1], device=dev), 0.1, causal=True)
+            assert (got[0] == 0).all() and got[T - 1, 3].isnan().all()
+        assert (decode_int4(q2, *cache, torch.tensor([0], device=dev), 0.1) == 0).all()
+
+
+@pytest.mark.parametrize("n,T,H,Hkv,d", SHAPES)
+def test_infinite_scores(n, T, H, Hkv, d, dev):
+    """Keys at which every product is positive: an infinite element makes every score +inf or -inf, which is NaN either way."""
+    _say("infinite scores", n, T, H, Hkv, d)
+    gen = torch.Generator(device=dev).manual_seed(n)
+    k, v = (torch.rand(Hkv, n, d, generator=gen, device=dev) + 0.5 for _ in range(2))
+    cache = (*plain.pack(*plain.quantize(k)), *plain.pack(*plain.quantize(v)))
+    q = torch.ones(T, H, d, device=dev, dtype=BF16)
+    q[T - 1, 0] *= float("inf")
+    q[T - 1, 1] *= -float("inf")
+    got = decode_int4(q, *cache, n, 0.1)
+    assert got[T - 1, :2].isnan().all()
+    got[T - 1, :2] = 0
+    assert torch.isfinite(got.float()).all()

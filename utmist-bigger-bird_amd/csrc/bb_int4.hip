@@ -205,6 +205,10 @@ BB_DEV int64_t split_keys(const Int4DecodeParams& p, int64_t n) {
 // The token of query vector v (v / G; v < 2^20, so the product with the rounded reciprocal is off by less than 1 / (2 G)).
 BB_DEV int token_of(const Int4DecodeParams& p, int v) { return (int)(((float)v + 0.5f) * p.inv_G); }
 
+// The first keys that token t attends of a cache of n rows; none or less: the token's output is zeros. Every other one is the
+// quotient of its sums, so that a query that is not finite, and scores that are all -inf, give NaN as the formula does.
+BB_DEV int64_t attended(const Int4DecodeParams& p, int64_t n, int t) { return p.causal ? n - p.T + 1 + t : n; }
+
 BB_DEV f32x4_t mma16_bf16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -454,7 +458,7 @@ struct Part {
   // How many of the split's keys query vector v attends.
   BB_DEV int limit(const Int4DecodeParams& p, int v) const {
     if (!p.causal) return count;
-    const int64_t seen = n - p.T + 1 + token_of(p, v) - begin;
+    const int64_t seen = attended(p, n, token_of(p, v)) - begin;
     return (int)(seen < 0 ? 0 : seen < count ? seen : count);
   }
 };
@@ -494,9 +498,10 @@ struct WaveState {
   float m[NV], l[NV], z[NV][D / kGroup], o[NV][D + 4];
 };
 
-// The four waves' states under one maximum: the split's partial, or with one split the output (a row without keys: zeros).
+// The four waves' states under one maximum: the split's partial, or with one split the output.
 template <int D, bool F16, int NV>
-BB_DEV void finish(const Int4DecodeParams& p, const uint8_t (*sm)[2][kStage], int R, int v0, int g, int split, int tid) {
+BB_DEV void finish(const Int4DecodeParams& p, const Part& part, const uint8_t (*sm)[2][kStage], int R, int v0, int g,
+                   int split, int tid) {
   __syncthreads();
 #pragma unroll 1
   for (int i = tid; i < R * (D / 4); i += kThreads) {
@@ -516,7 +521,7 @@ BB_DEV void finish(const Int4DecodeParams& p, const uint8_t (*sm)[2][kStage], in
     }
     if (p.n_splits == 1) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) O[e] = L > 0.0f ? O[e] / L : 0.0f;
+      for (int e = 0; e < 4; ++e) O[e] = attended(p, part.n, t) > 0 ? O[e] / L : 0.0f;
       *reinterpret_cast<u32x2_t*>(p.out + t * p.so0 + hd * p.so1 + d) = u32x2_t{pack2<F16>(O[0], O[1]), pack2<F16>(O[2], O[3])};
     } else {
       float* dst = p.part + (((int64_t)t * p.H + hd) * p.n_splits + split) * int4_part_row(D);
@@ -808,7 +813,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
     }
     if (D == 128 || k < 8) *reinterpret_cast<f32x4_t*>(&mine->o[k & 3][32 * (k >> 2) + 16 * j + 4 * a]) = r;
   }
-  finish<D, F16, 4>(p, sm, R, 0, g, split, tid);
+  finish<D, F16, 4>(p, part, sm, R, 0, g, split, tid);
 }
 
 // 5 and more query vectors, 16 of them a pass: column k of every product is vector k.
@@ -1040,13 +1045,13 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
     for (int e = 0; e < 4; ++e) r[e] = o[db][e] * kSumDown;
     *reinterpret_cast<f32x4_t*>(&mine->o[k][16 * db + 4 * a]) = r;
   }
-  finish<D, F16, kVecs>(p, sm, R, v0, g, split, tid);
+  finish<D, F16, kVecs>(p, part, sm, R, v0, g, split, tid);
 }
 
 // The partials of the live splits under one maximum: a workgroup per (query vector, 32 columns), thread (4 columns, group)
-// folding every 16th split, 4 loaded at a time; the groups then combine through LDS. A row without keys is zero. Latency
-// bounds it (2.2 to 4 us for 0.5 to 4 MB). GPU time of decode and merge over 8111 rows, 32 splits: 11.4 us with 8 groups, 11.6
-// with 16, 12.1 with 32, 12.6 with 64; over 131072 rows, 64 splits, 8 and 16 are even and 64 takes 1 us more.
+// folding every 16th split, 4 loaded at a time; the groups then combine through LDS. Latency bounds it (2.2 to 4 us for
+// 0.5 to 4 MB). GPU time of decode and merge over 8111 rows, 32 splits: 11.4 us with 8 groups, 11.6 with 16, 12.1 with 32, 12.6
+// with 64; over 131072 rows, 64 splits, 8 and 16 are even and 64 takes 1 us more.
 constexpr int kMergeCols = 32, kMergeLanes = kMergeCols / 4, kMergeGroups = 16, kMergePer = 4;
 template <int D, bool F16>
 __global__ __launch_bounds__(kMergeLanes * kMergeGroups) void int4_merge_kernel(Int4DecodeParams p) {
@@ -1105,7 +1110,8 @@ __global__ __launch_bounds__(kMergeLanes * kMergeGroups) void int4_merge_kernel(
       lt += w * sm_l[i];
       ot += w * sm_o[i][d];
     }
-    p.out[(v / p.H) * p.so0 + (v % p.H) * p.so1 + d0 + d] = to16<F16>(lt > 0.0f ? ot / lt : 0.0f);
+    const int t = v / p.H;
+    p.out[t * p.so0 + (v % p.H) * p.so1 + d0 + d] = to16<F16>(attended(p, n, t) > 0 ? ot / lt : 0.0f);
   }
 }
 
