@@ -106,3 +106,39 @@ def test_infinite_scores(n, T, H, Hkv, d, dev):
     assert got[T - 1, :2].isnan().all()
     got[T - 1, :2] = 0
     assert torch.isfinite(got.float()).all()
+
+
+@pytest.mark.parametrize("n,T,H,Hkv,d", SHAPES)
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_scores_far_from_zero(n, T, H, Hkv, d, sign, dev):
+    """Scores of about -1e32 and 1e32, finite in fp32. Keys that are all alike score the same, so the output is V's mean; with one
+    key that scores higher by more than any rounding it is that key's V row. Both hold to the output's rounding and to the sums'
+    of probabilities that are exactly 1: 2^-17 of a V scale times 15 for the two terms, and 2^-20 of the largest sum (s c + |z|) for
+    the fp32 sums and scales. Rows next to them with ordinary queries stay within int4_plain's bound (not bit for bit: a wave moves
+    all its vectors' running maxima when one of them rises, and then their roundings are others)."""
+    _say("far", n, T, H, Hkv, d, sign)
+    gen = torch.Generator(device=dev).manual_seed(n + 1)
+    k = (torch.rand(Hkv, 1, d, generator=gen, device=dev) + 0.5).expand(Hkv, n, d).clone()
+    v = torch.randn(Hkv, n, d, generator=gen, device=dev)
+    q = torch.randn(T, H, d, generator=gen, device=dev).to(BF16)
+    far = torch.zeros(T, H, dtype=torch.bool, device=dev)
+    far[:, 1::2] = True
+    q2 = torch.where(far[..., None], torch.full_like(q, sign * 1e30), q)
+    vq = plain.pack(*plain.quantize(v))
+    vv, vs = plain.values(*vq)
+    top = (vs * 15 + vq[1][..., 1].double().abs().repeat_interleave(32, -1)).amax((0, 1))
+    for planted in (None, 0, n // 2, n - 1):
+        if planted is not None:
+            k[:, planted] *= 1.5 if sign > 0 else 0.5
+        cache = (*plain.pack(*plain.quantize(k)), *vq)
+        near, near_tol = plain.attend(q, *cache, n, 0.1)
+        for length in (n, torch.tensor([n], device=dev)):
+            got = decode_int4(q2, *cache, length, 0.1)
+            near_err = (got.double() - near).abs()
+            assert (near_err <= near_tol + 2.0 ** -8 * (near.abs() + near_tol))[~far].all()
+            want = (vv.mean(1) if planted is None else vv[:, planted]).repeat_interleave(H // Hkv, 0)
+            tol = 2.0 ** -8 * want.abs() + 2.0 ** -17 * 15 * vs.amax() + 2.0 ** -20 * top
+            err = (got.double() - want).abs()
+            assert (err <= tol)[far].all(), (planted, err[far].max().item())
+        if planted is not None:
+            k[:, planted] /= 1.5 if sign > 0 else 0.5

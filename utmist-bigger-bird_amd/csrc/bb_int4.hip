@@ -188,6 +188,7 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kStage = 10240;        // K codes 4096 | K params 1024 | V codes 4096 | V params 1024
 constexpr int kKp = 4096, kVq = 5120, kVp = 9216;
 constexpr float kOver = 256.0f;      // a probability past this moves the running maximum
+constexpr float kLowest = -3.402823466e38f;  // -FLT_MAX, what a running maximum starts from: no finite score lies below it
 
 typedef int v2i_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void lds_void;
@@ -506,7 +507,7 @@ BB_DEV void finish(const Int4DecodeParams& p, const Part& part, const uint8_t (*
 #pragma unroll 1
   for (int i = tid; i < R * (D / 4); i += kThreads) {
     const int r = i / (D / 4), d = 4 * (i % (D / 4)), v = v0 + r, t = token_of(p, v), hd = g * p.G + v - t * p.G;
-    float M = -1.0e30f, L = 0.0f;
+    float M = kLowest, L = 0.0f;
     f32x4_t O = {0, 0, 0, 0};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) M = fmaxf(M, reinterpret_cast<const WaveState<D, NV>*>(sm[w])->m[r]);
@@ -635,7 +636,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
   f32x4_t o[NDB];
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    m[w] = -1.0e30f;
+    m[w] = kLowest;
     l[w] = 0.0f;
 #pragma unroll
     for (int t = 0; t < NG; ++t) zs[w][t] = 0.0f;
@@ -882,7 +883,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
                         : 512 * (k >> 2) + 32 * (k & 3) + 128 * ((k >> 3) ^ (j & 1)) + 4 * a;
   const int lim = part.limit(p, v0 + k), fewest = part.limit(p, v0);
 
-  float m = -1.0e30f, l = 0.0f, zs[NG];
+  float m = kLowest, l = 0.0f, zs[NG];
   f32x4_t o[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) o[db] = f32x4_t{0, 0, 0, 0};
@@ -910,7 +911,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
     uint8_t* s = sm[wave][st];
     complete<D, F16, CH>(p, part, in, c, g, lane, s);
 
-    float x[HV][4][4];  // [half][step][key of the lane's four], not yet times p.c
+    float x[HV][4][4];  // [half][step][key of the lane's four]
 #pragma unroll
     for (int hv = 0; hv < HV; ++hv)
 #pragma unroll
@@ -935,6 +936,7 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
           params(s + kKp, hv, u, e, kp);
 #pragma unroll
           for (int t = 0; t < NG; ++t) x[hv][u][e] = fmaf(f16_lo(kp[t]), acc[t][e], x[hv][u][e]);
+          x[hv][u][e] *= p.c;  // rounded: as one fma with the maximum, keys that tie at a score past 2^30 would differ
         }
       }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the K rows are read, their space is free
@@ -959,19 +961,19 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4Decod
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          pr[hv][u][e] = fast_exp2(fmaf(x[hv][u][e], p.c, -m));
+          pr[hv][u][e] = fast_exp2(x[hv][u][e] - m);
           most = fmaxf(most, pr[hv][u][e]);
         }
     if (__builtin_amdgcn_ballot_w64(most > kOver)) {
       float mx = x[0][0][0];
 #pragma unroll
       for (int i = 1; i < 16 * HV; ++i) mx = fmaxf(mx, x[i >> 4][(i >> 2) & 3][i & 3]);
-      const float mn = fmaxf(m, quarters_max(mx) * p.c), alpha = fast_exp2(m - mn);
+      const float mn = fmaxf(m, quarters_max(mx)), alpha = fast_exp2(m - mn);
       m = mn;
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < 16 * HV; ++i)
-        pr[i >> 4][(i >> 2) & 3][i & 3] = fast_exp2(fmaf(x[i >> 4][(i >> 2) & 3][i & 3], p.c, -mn));
+        pr[i >> 4][(i >> 2) & 3][i & 3] = fast_exp2(x[i >> 4][(i >> 2) & 3][i & 3] - mn);
 #pragma unroll
       for (int t = 0; t < NG; ++t) zs[t] *= alpha;
 #pragma unroll
@@ -1065,7 +1067,7 @@ __global__ __launch_bounds__(kMergeLanes * kMergeGroups) void int4_merge_kernel(
   }
   const int live = (int)((n + len - 1) / len);
   const float* base = p.part + (int64_t)v * p.n_splits * int4_part_row(D);
-  float M = -1.0e30f, L = 0.0f;
+  float M = kLowest, L = 0.0f;
   f32x4_t O = {0, 0, 0, 0};
   for (int i0 = grp; i0 < live; i0 += kMergeGroups * kMergePer) {
     float mv[kMergePer], lv[kMergePer];
@@ -1075,7 +1077,7 @@ __global__ __launch_bounds__(kMergeLanes * kMergeGroups) void int4_merge_kernel(
       const int s = i0 + kMergeGroups * i;
       const bool ok = s < live;
       const float* r = base + (int64_t)(ok ? s : i0) * int4_part_row(D);
-      mv[i] = ok ? r[D] : -1.0e30f;
+      mv[i] = ok ? r[D] : kLowest;
       lv[i] = ok ? r[D + 1] : 0.0f;
       ov[i] = *reinterpret_cast<const f32x4_t*>(r + d0 + c);
     }
