@@ -1,0 +1,32 @@
+"""4-bit KV cache without a GPU: the host's layouts, limits and the cache layer's bookkeeping at their edges."""
+import pytest
+import torch
+
+from bigger_bird_amd import kv_int4
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _at(x, elements):
+    """x's values, contiguous, `elements` elements past an aligned address."""
+    buf = torch.empty(x.numel() + elements, dtype=x.dtype, device=x.device)
+    return buf[elements:].view(x.shape).copy_(x)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_rows_are_copied_to_an_aligned_place(dtype):
+    """Contiguous tensors at any address, and odd strides of dimensions of length 1, which torch counts as contiguous too."""
+    gen = torch.Generator().manual_seed(3)
+    cases = [_at(torch.randn(shape, generator=gen).to(dtype), o) for o in (1, 2, 3) for shape in
+             ((5, 128), (2, 5, 64), (3, 2, 5, 32), (1, 1, 128))]
+    cases += [torch.randn(1, 1, 131, generator=gen).to(dtype)[..., :128], torch.randn(1, 7, 132, generator=gen).to(dtype)[:, :1, :128]]
+    for x in cases:
+        y = kv_int4._input_rows(x)
+        el = y.element_size()
+        assert y.ndim == 3 and torch.equal(y, x.reshape(-1, *x.shape[-2:]))
+        assert y.data_ptr() % 16 == 0 and y.stride(-1) == 1 and not any(s * el % 16 for s in y.stride()[:2])
+        if dtype is not FP32 and x.ndim == 3:
+            y = kv_int4._rows16(x)
+            assert torch.equal(y, x) and y.data_ptr() % 16 == 0 and y.stride(-1) == 1 and not any(s % 8 for s in y.stride()[:2])
+    x = torch.zeros(2, 5, 128, dtype=dtype)
+    assert kv_int4._input_rows(x).data_ptr() == x.data_ptr(), "aligned rows are taken where they are"

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import int4_plain as plain
-from bigger_bird_amd.kv_int4 import decode_int4
+from bigger_bird_amd.kv_int4 import decode_int4, decode_int4_append, quantize4, quantize4_pair
 
 pytestmark = pytest.mark.gpu
 
@@ -142,3 +142,37 @@ def test_scores_far_from_zero(n, T, H, Hkv, d, sign, dev):
             assert (err <= tol)[far].all(), (planted, err[far].max().item())
         if planted is not None:
             k[:, planted] /= 1.5 if sign > 0 else 0.5
+
+
+def _at(x, elements):
+    """x's values, contiguous, `elements` elements past an aligned address."""
+    buf = torch.empty(x.numel() + elements, dtype=x.dtype, device=x.device)
+    return buf[elements:].view(x.shape).copy_(x)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_contiguous_rows_at_any_address(dtype, dev):
+    """Rows, queries and new rows that are contiguous but start between 16-byte addresses give what aligned ones give."""
+    _say("addresses", dtype)
+    gen = torch.Generator(device=dev).manual_seed(4)
+    for shape in ((9, 128), (3, 9, 64), (2, 3, 9, 32), (1, 1, 256)):
+        x, y = (torch.randn(shape, generator=gen, device=dev).to(dtype) for _ in range(2))
+        want = [*quantize4(x), *quantize4(y)]
+        for o in (1, 3):
+            assert all(map(torch.equal, quantize4(_at(x, o)), want[:2]))
+            (kq, kp), (vq, vp) = quantize4_pair(_at(x, o), _at(y, 2), None, None)
+            assert all(map(torch.equal, (kq, kp, vq, vp), want))
+    if dtype is FP32:
+        return
+    for T, H, Hkv, d in ((1, 8, 2, 128), (3, 8, 2, 64)):
+        n = 700
+        cache = _cache(gen, Hkv, n, n + 3, d, dev)
+        q = torch.randn(T, H, d, generator=gen, device=dev).to(dtype)
+        k, v = (torch.randn(Hkv, T, d, generator=gen, device=dev).to(dtype) for _ in range(2))
+        want = decode_int4(q, *cache, n, 0.1)
+        for o in (1, 3):
+            assert torch.equal(decode_int4(_at(q, o), *cache, n, 0.1), want)
+        a, b = ([x.clone() for x in cache] for _ in range(2))
+        assert torch.equal(decode_int4_append(_at(q, 1), *a, _at(k, 3), _at(v, 1), n + T, 0.1),
+                           decode_int4_append(q, *b, k, v, n + T, 0.1))
+        assert all(torch.equal(x[:, :n + T], y[:, :n + T]) for x, y in zip(a, b))

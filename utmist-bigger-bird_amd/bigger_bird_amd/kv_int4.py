@@ -51,12 +51,18 @@ def _one_device(what, *tensors):
     return device
 
 
+def _copy(x):
+    """x in fresh memory, row after row (x.contiguous() is x itself where only its address, or the stride of a dimension of
+    length 1, keeps its rows from being aligned)."""
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
+
+
 def _input_rows(x):
     """x [..., t, d] as [heads, t, d] with 16-byte aligned rows (a copy where it is not)."""
     x = x[None] if x.ndim == 2 else x.flatten(0, -3) if x.ndim > 3 else x
     el = x.element_size()
     if x.stride(-1) != 1 or x.data_ptr() % 16 or (x.stride(0) * el) % 16 or (x.stride(1) * el) % 16:
-        x = x.contiguous()
+        x = _copy(x)
     return x
 
 
@@ -193,7 +199,7 @@ def dequantize4_pair(k, v, dtype):
 def _rows16(x):
     """x [a, b, d] with a contiguous head_dim and 16-byte aligned rows (a copy where it is not)."""
     s = x.stride()
-    return x if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and x.data_ptr() % 16 == 0 else x.contiguous()
+    return x if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and x.data_ptr() % 16 == 0 else _copy(x)
 
 
 @functools.lru_cache(maxsize=64)
