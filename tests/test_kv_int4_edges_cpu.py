@@ -30,3 +30,32 @@ def test_rows_are_copied_to_an_aligned_place(dtype):
             assert torch.equal(y, x) and y.data_ptr() % 16 == 0 and y.stride(-1) == 1 and not any(s % 8 for s in y.stride()[:2])
     x = torch.zeros(2, 5, 128, dtype=dtype)
     assert kv_int4._input_rows(x).data_ptr() == x.data_ptr(), "aligned rows are taken where they are"
+
+
+def _layer(hk=2, n=5, d=64, dtype=BF16, monkeypatch=None):
+    """A layer that holds n rows, on the CPU (its stores are never launched on)."""
+    layer = kv_int4.Int4KVLayer()
+    layer.lazy_initialization(torch.zeros(1, hk, n, d, dtype=dtype), None)
+    layer.store_k, layer.store_v, layer.n = kv_int4._Int4Rows(hk, d, n, "cpu"), kv_int4._Int4Rows(hk, d, n, "cpu"), n
+    return layer
+
+
+def test_refused_write_keeps_the_pending_rows(monkeypatch):
+    """Rows behind a handle stay with the layer until a write of them has succeeded."""
+    layer = _layer()
+    x = torch.randn(1, 2, 1, 64).to(BF16)
+    layer.update(x, x, {"bb_attend": True})
+    pending, calls = layer._pending, []
+    assert pending is not None and layer.n == 6
+
+    def refuse(*a):
+        raise RuntimeError("out of memory")
+
+    monkeypatch.setattr(kv_int4, "quantize4_pair", refuse)
+    with pytest.raises(RuntimeError):
+        layer.nbytes()
+    assert layer._pending is pending and layer.n == 6
+    monkeypatch.setattr(kv_int4, "quantize4_pair", lambda *a: calls.append(a))
+    layer.nbytes()
+    assert layer._pending is None and len(calls) == 1
+    assert torch.equal(calls[0][0], x[0]) and calls[0][2][0].data_ptr() == layer.store_k.q[:, 5:].data_ptr()

@@ -357,9 +357,8 @@ class Int4KVLayer(Int8KVLayer):
     def _flush(self):
         """Quantise a step's rows still held for the fused decode (the handle was not attended)."""
         if self._pending is not None:
-            kr, vr, row = self._pending
-            self._pending = None
-            self._write(kr, vr, row)
+            self._write(*self._pending)
+            self._pending = None  # only now: a write that fails keeps the rows
 
     def _write(self, kr, vr, row):
         end = row + kr.shape[1]
