@@ -59,3 +59,14 @@ def test_refused_write_keeps_the_pending_rows(monkeypatch):
     layer.nbytes()
     assert layer._pending is None and len(calls) == 1
     assert torch.equal(calls[0][0], x[0]) and calls[0][2][0].data_ptr() == layer.store_k.q[:, 5:].data_ptr()
+
+
+@pytest.mark.parametrize("k,v", [((1, 3, 1, 64), (1, 3, 1, 64)), ((1, 2, 1, 128), (1, 2, 1, 128)), ((1, 2, 1, 64), (1, 2, 1, 128)),
+                                 ((1, 2, 1, 64), (1, 1, 1, 64)), ((1, 2, 1, 64), (1, 2, 2, 64))])
+@pytest.mark.parametrize("attend", [True, False])
+def test_rows_of_another_shape_are_refused_at_once(k, v, attend):
+    """A step whose rows do not fit the cache is refused by the update, before the layer counts them."""
+    layer = _layer()
+    with pytest.raises(ValueError, match="rows"):
+        layer.update(torch.zeros(k, dtype=BF16), torch.zeros(v, dtype=BF16), {"bb_attend": attend})
+    assert layer.n == 5 and layer._pending is None and layer.store_k.capacity == 5 + kv_int4.GROW

@@ -320,6 +320,10 @@ class _Int4Rows:
     def packed(self):
         return self.q, self.p
 
+    def takes(self, x):
+        """Whether rows x [Hkv, t, d] fit this store."""
+        return x.shape[0] == self.q.shape[0] and x.shape[2] == 2 * self.q.shape[2] and x.get_device() == self.q.get_device()
+
     def ensure(self, n, need):
         """Make room for rows [n, need), keeping rows [0, n)."""
         if need <= self.capacity:
@@ -389,12 +393,14 @@ class Int4KVLayer(Int8KVLayer):
             quantize4_pair(kr, vr, sk.rows(0, t), sv.rows(0, t))
             self.store_k, self.store_v, self.n = sk, sv, t  # only now: rows that are refused leave the layer empty
             return key_states, value_states
+        if vr.shape != kr.shape or not (self.store_k.takes(kr) and self.store_v.takes(vr)):
+            raise ValueError("Int4KVLayer: K and V rows must have the cache's heads, head_dim and device, and be as many")
         start, end = self.n, self.n + t
         self.store_k.ensure(start, end)
         self.store_v.ensure(start, end)
         wants_handle = isinstance(cache_kwargs, dict) and cache_kwargs.get("bb_attend", False)
         if (self.fused and wants_handle and 1 <= t <= self.attend_tokens and d in (64, 128)
-                and kr.dtype in (torch.bfloat16, torch.float16) and vr.dtype == kr.dtype and vr.shape == kr.shape):
+                and kr.dtype in (torch.bfloat16, torch.float16) and vr.dtype == kr.dtype):
             # quantised when the handle is attended (or by _flush before any other use of the cache)
             self._pending, self.n = (kr, vr, start), end
             handle = Int4Handle(self, (1, h, end, d))
