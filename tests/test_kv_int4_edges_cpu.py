@@ -70,3 +70,19 @@ def test_rows_of_another_shape_are_refused_at_once(k, v, attend):
     with pytest.raises(ValueError, match="rows"):
         layer.update(torch.zeros(k, dtype=BF16), torch.zeros(v, dtype=BF16), {"bb_attend": attend})
     assert layer.n == 5 and layer._pending is None and layer.store_k.capacity == 5 + kv_int4.GROW
+
+
+def test_handles_need_rows_before_the_step(monkeypatch):
+    """A handle's queries attend every row. That is a cached step; several tokens that are the whole cache are a prompt, which
+    RDAttention attends causally from K and V themselves."""
+    layer = _layer()
+    monkeypatch.setattr(kv_int4, "quantize4_pair", lambda *a: None)
+    monkeypatch.setattr(kv_int4, "dequantize4_pair", lambda k, v, dtype: (torch.zeros(*k[0].shape[:2], 64),) * 2)
+    for held, t, handle in ((5, 3, True), (5, 1, True), (0, 3, False), (0, 1, True)):
+        layer.crop(-100)
+        layer.n = held
+        x = torch.zeros(1, 2, t, 64, dtype=BF16)
+        k, v = layer.update(x, x, {"bb_attend": True})
+        assert isinstance(k, kv_int4.Int4Handle) == handle and layer.n == held + t, (held, t)
+        if not handle:
+            assert k.shape == v.shape == (1, 2, held + t, 64) and layer._pending is None

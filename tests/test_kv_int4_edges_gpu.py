@@ -176,3 +176,32 @@ def test_contiguous_rows_at_any_address(dtype, dev):
         assert torch.equal(decode_int4_append(_at(q, 1), *a, _at(k, 3), _at(v, 1), n + T, 0.1),
                            decode_int4_append(q, *b, k, v, n + T, 0.1))
         assert all(torch.equal(x[:, :n + T], y[:, :n + T]) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("t", [1, 2, 16, 40])
+def test_prompt_after_a_crop_to_nothing_is_causal(t, dev):
+    """A layer cropped to no rows takes a new prompt: RDAttention attends it causally, as it does any t == n, however short."""
+    _say("crop to nothing", t)
+    from types import SimpleNamespace
+
+    from bigger_bird_amd import RDAttention
+    from bigger_bird_amd.kv_int4 import Int4KVLayer
+
+    H, Hkv, d = 8, 2, 64
+    base = SimpleNamespace(config=SimpleNamespace(num_attention_heads=H, num_key_value_heads=Hkv), layer_idx=0, head_dim=d,
+                           scaling=d ** -0.5, q_proj=None, k_proj=None, v_proj=None, o_proj=None)
+    attn, layer = RDAttention(base, sink=64, window=16384, vertical=512, exact_tail=256), Int4KVLayer()
+    gen = torch.Generator(device=dev).manual_seed(t)
+    q, k, v = (torch.randn(1, h, t, d, generator=gen, device=dev).to(BF16) for h in (H, Hkv, Hkv))
+    layer.update(torch.randn_like(k).repeat(1, 1, 30, 1), torch.randn_like(v).repeat(1, 1, 30, 1))
+    layer.crop(-30 * t)
+    assert layer.get_seq_length() == 0
+    kk, vv = layer.update(k, v, {"bb_attend": True})
+    out = attn.exact_attention(q, kk, vv, t, t)
+    cache = (*plain.pack(*plain.quantize(k[0])), *plain.pack(*plain.quantize(v[0])))
+    want, _ = plain.attend(q[0].transpose(0, 1), *cache, t, d ** -0.5, True)
+    # K and V rounded to bf16 (2^-8 each: a score of |q| |k| d^-0.5 sums, a value), probabilities and output in bf16
+    kd, vd = (plain.values(*cache[i:i + 2])[0].abs() for i in (0, 2))
+    dx = 2.0 ** -8 * d ** -0.5 * torch.matmul(q[0].double().abs().view(Hkv, -1, d), kd.transpose(1, 2)).max()
+    assert (out[0].transpose(0, 1).double() - want).abs().max() <= (2 * dx + 3 * 2.0 ** -8) * vd.max()
+    assert layer.get_seq_length() == t

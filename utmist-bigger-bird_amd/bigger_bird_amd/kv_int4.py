@@ -350,8 +350,8 @@ class Int4KVLayer(Int8KVLayer):
 
     * prefill (the first update): the K/V are quantised into fresh row stores and the full-precision inputs are returned;
     * later updates quantise the new rows (K and V in one launch) into spare capacity and return the dequantised cache,
-      or, for a step of at most `attend_tokens` tokens whose consumer opts in (cache kwargs {"bb_attend": True}) on a
-      bf16 or fp16 model with head_dim 64 or 128, Int4Handle stand-ins for decode_int4;
+      or, for a step of at most `attend_tokens` tokens behind cached ones (or of one token) whose consumer opts in (cache
+      kwargs {"bb_attend": True}) on a bf16 or fp16 model with head_dim 64 or 128, Int4Handle stand-ins for decode_int4;
     * assigning `keys` / `values` (kv_evict compacting the cache) re-quantises the given rows;
     * `crop(-r)` drops the last r rows.
     """
@@ -399,7 +399,8 @@ class Int4KVLayer(Int8KVLayer):
         self.store_k.ensure(start, end)
         self.store_v.ensure(start, end)
         wants_handle = isinstance(cache_kwargs, dict) and cache_kwargs.get("bb_attend", False)
-        if (self.fused and wants_handle and 1 <= t <= self.attend_tokens and d in (64, 128)
+        # a handle's queries attend every row; several tokens that are the whole cache are a prompt, attended causally
+        if (self.fused and wants_handle and 1 <= t <= self.attend_tokens and (start or t == 1) and d in (64, 128)
                 and kr.dtype in (torch.bfloat16, torch.float16) and vr.dtype == kr.dtype):
             # quantised when the handle is attended (or by _flush before any other use of the cache)
             self._pending, self.n = (kr, vr, start), end
