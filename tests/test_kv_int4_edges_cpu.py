@@ -1,4 +1,6 @@
 """4-bit KV cache without a GPU: the host's layouts, limits and the cache layer's bookkeeping at their edges."""
+import math
+
 import pytest
 import torch
 
@@ -86,3 +88,11 @@ def test_handles_need_rows_before_the_step(monkeypatch):
         assert isinstance(k, kv_int4.Int4Handle) == handle and layer.n == held + t, (held, t)
         if not handle:
             assert k.shape == v.shape == (1, 2, held + t, 64) and layer._pending is None
+
+
+@pytest.mark.parametrize("lead", [(0,), (2, 0), (1, 8, 0), (2, 0, 5), (0, 2, 5), (3, 2, 2, 0)])
+def test_layouts_without_rows(lead):
+    """No rows, or no heads, in any number of dimensions."""
+    q, p = kv_int4._new_packed(lead, 128, "cpu")
+    h, t, d, _, _ = kv_int4._packed("quantize4", q, p)
+    assert (h, t, d) == (math.prod(lead[:-1]), lead[-1], 128)

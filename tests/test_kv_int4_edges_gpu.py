@@ -4,7 +4,8 @@ import pytest
 import torch
 
 import int4_plain as plain
-from bigger_bird_amd.kv_int4 import decode_int4, decode_int4_append, quantize4, quantize4_pair
+from bigger_bird_amd.kv_int4 import (decode_int4, decode_int4_append, dequantize4, dequantize4_pair, quantize4,
+                                     quantize4_pair)
 
 pytestmark = pytest.mark.gpu
 
@@ -205,3 +206,13 @@ def test_prompt_after_a_crop_to_nothing_is_causal(t, dev):
     dx = 2.0 ** -8 * d ** -0.5 * torch.matmul(q[0].double().abs().view(Hkv, -1, d), kd.transpose(1, 2)).max()
     assert (out[0].transpose(0, 1).double() - want).abs().max() <= (2 * dx + 3 * 2.0 ** -8) * vd.max()
     assert layer.get_seq_length() == t
+
+
+@pytest.mark.parametrize("shape", [(0, 128), (1, 8, 0, 64), (2, 0, 5, 128), (3, 2, 2, 0, 32)])
+def test_no_rows_in_any_number_of_dimensions(shape, dev):
+    _say("no rows", shape)
+    x = torch.zeros(shape, device=dev)
+    k, v = quantize4_pair(x, x)
+    one = quantize4(x, k)
+    assert one[0].shape == (*shape[:-1], shape[-1] // 2) and one[1].shape == (*shape[:-1], shape[-1] // 32, 2)
+    assert dequantize4(*one, BF16).shape == shape and all(y.shape == shape for y in dequantize4_pair(k, v, FP32))

@@ -75,8 +75,9 @@ def _packed(what, q, p):
         if q.ndim < 2 or p.ndim != q.ndim + 1 or p.shape[:-2] != q.shape[:-1]:
             raise ValueError(f"{what}: codes [..., t, d / 2] and params [..., t, d / 32, 2] must match")
         try:
-            q = q.view(-1, *q.shape[-2:]) if q.ndim > 3 else q[None]
-            p = p.view(-1, *p.shape[-3:]) if p.ndim > 4 else p[None]
+            heads = q.shape[:-2].numel()  # (spelled out: -1 is ambiguous where there are no rows)
+            q = q.view(heads, *q.shape[-2:]) if q.ndim > 3 else q[None]
+            p = p.view(heads, *p.shape[-3:]) if p.ndim > 4 else p[None]
         except RuntimeError:
             raise ValueError(f"{what}: packed rows need one stride between heads") from None
     h, t, half = q.shape
