@@ -216,3 +216,13 @@ def test_no_rows_in_any_number_of_dimensions(shape, dev):
     one = quantize4(x, k)
     assert one[0].shape == (*shape[:-1], shape[-1] // 2) and one[1].shape == (*shape[:-1], shape[-1] // 32, 2)
     assert dequantize4(*one, BF16).shape == shape and all(y.shape == shape for y in dequantize4_pair(k, v, FP32))
+
+
+def test_cache_without_heads_is_refused(dev):
+    _say("no heads")
+    q = torch.zeros(1, 8, 128, device=dev, dtype=BF16)
+    none = quantize4(torch.zeros(0, 5, 128, device=dev))
+    with pytest.raises(ValueError, match="must match"):
+        decode_int4(q, *none, *none, 5, 0.1)
+    with pytest.raises(ValueError, match="must match"):
+        decode_int4(q[:, :0], *none, *none, 5, 0.1)

@@ -227,7 +227,7 @@ def _decode(q, k4, kp, v4, vp, knew, vnew, n, scale, causal):
     k, v = _packed_pair("decode_int4", k4, kp, v4, vp)
     hk, cap, d, skq, skp = k
     t, h, dq = q.shape
-    if v[:3] != k[:3] or dq != d or not h or h % hk:
+    if v[:3] != k[:3] or dq != d or not h or not hk or h % hk:
         raise ValueError("q [T,H,D] and the cache's Hkv heads must match")
     if length is not None and (length.dtype is not torch.int64 or length.numel() != 1):
         raise ValueError("n must be an int64 tensor of one element (it is read in place by the kernels)")
