@@ -354,13 +354,15 @@ int bb_rope_inplace(void* x, const int64_t* sx, int B, int Hh, int64_t T, int D,
  *
  * bb_int4_quantize writes `rows` rows of every head: xk [heads, rows, D] (strides sxk[2]: head, row, in elements; rows
  * 16-byte aligned; x_kind 0 bf16, 1 fp32, 2 fp16) to (kq, kp) and, in the same launch, xv (strides sxv[2]) to (vq, vp).
- * xv = NULL: one tensor (sc[0], sc[1]).
+ * xv = NULL: one tensor (sc[0], sc[1]). Writes of 2^35 elements a head and more, or of about 2^36 over all heads
+ * (ceil(rows * D / 4096) * heads >= 2^24), are refused.
  */
 int bb_int4_quantize(const void* xk, const int64_t* sxk, const void* xv, const int64_t* sxv, int x_kind, int heads,
                      int64_t rows, int D, uint8_t* kq, void* kp, uint8_t* vq, void* vp, const int64_t* sc, void* stream);
 
 /* The values of `rows` rows of every head: outk (and, with vq, outv) [heads, rows, D] contiguous, 16-byte aligned
- * (out_kind: 0 bf16, 1 fp32, 2 fp16; the fp32 value rounded to nearest even). vq = NULL: one tensor. */
+ * (out_kind: 0 bf16, 1 fp32, 2 fp16; the fp32 value rounded to nearest even). vq = NULL: one tensor. 2^35 elements a head and
+ * more are refused, whatever the number of heads. */
 int bb_int4_dequantize(const uint8_t* kq, const void* kp, const uint8_t* vq, const void* vp, const int64_t* sc, int heads,
                        int64_t rows, int D, void* outk, void* outv, int out_kind, void* stream);
 
@@ -372,7 +374,7 @@ int bb_int4_dequantize(const uint8_t* kq, const void* kp, const uint8_t* vq, con
  * n: T <= n <= cap. With n_dev (an int64 in device memory) the length is read there and clamped to 0 .. cap, and n is
  * ignored; every launch shape then depends on cap alone, so a captured graph stays valid while the cache grows.
  * Workspace: bb_int4_decode_workspace(n, ...), with n_dev bb_int4_decode_workspace(cap, ...). Splits of 2^24 keys and more
- * (2^33 / Hkv rows) are refused, as are writes and reads back of 2^35 elements a head and more.
+ * (2^33 / Hkv rows) are refused.
  */
 int bb_int4_decode(const void* q, const int64_t* sq, const uint8_t* kq, const void* kp, const uint8_t* vq, const void* vp,
                    const int64_t* sc, int64_t n, const int64_t* n_dev, int64_t cap, int T, int H, int Hkv, int D,

@@ -96,3 +96,19 @@ def test_layouts_without_rows(lead):
     q, p = kv_int4._new_packed(lead, 128, "cpu")
     h, t, d, _, _ = kv_int4._packed("quantize4", q, p)
     assert (h, t, d) == (math.prod(lead[:-1]), lead[-1], 128)
+
+
+@pytest.mark.parametrize("heads,rows,write,read", [
+    (8, 2 ** 26, False, True), (64, 2 ** 23, False, True), (8, 2 ** 26 - 32, True, True), (1, 2 ** 28 - 16, True, True),
+    (1, 2 ** 28, False, False), (2, 2 ** 28, False, False)])
+def test_limits_over_several_heads(heads, rows, write, read):
+    """A write takes less than 2^36 elements over all heads and less than 2^35 a head, a read back less than 2^35 a head, whatever
+    the heads. (A size that is taken meets the refusal of a misaligned pointer behind that check: nothing is launched.)"""
+    from bigger_bird_amd import _lib
+
+    L, at = _lib.lib(), 1 << 20
+    sx, sc = _lib.i64s(rows * 128, 128), _lib.i64s(rows * 64, rows * 8, rows * 64, rows * 8)
+    for taken, call in ((write, lambda: L.bb_int4_quantize(at + 8, sx, None, None, 0, heads, rows, 128, at, at, None, None, sc, None)),
+                        (read, lambda: L.bb_int4_dequantize(at, at, None, None, sc, heads, rows, 128, at + 8, None, 0, None))):
+        with pytest.raises(ValueError, match="aligned" if taken else "out of range"):
+            _lib.check(call())

@@ -909,13 +909,13 @@ static int int4_cache_check(const char* what, const void* kq, const void* kp, co
   return BB_OK;
 }
 
-static int int4_rows_check(const char* what, int heads, int64_t rows, int D, int kind) {
+static int int4_rows_check(const char* what, int heads, int64_t rows, int D, int kind, bool folded) {
   if (D != 32 && D != 64 && D != 128 && D != 256) return fail("%s: head_dim %d unsupported", what, D);
   if (kind < 0 || kind > 2) return fail("%s: element kind %d unsupported (0 bf16, 1 fp32, 2 fp16)", what, kind);
-  // a launch counts its threads in 32 bits per dimension, in blocks of 256: the write's take 16 elements each over all heads,
-  // the read back's 8 each of one head
-  if (heads < 0 || heads > 65535 || rows < 0 || rows > (int64_t)1 << 40 || cdiv(rows * D, 4096) * heads > 0xffffff ||
-      cdiv(rows * D, 2048) > 0xffffff)
+  // a launch counts its threads in 32 bits per dimension, in blocks of 256: the read back's take 8 elements each of one head,
+  // the write's 16 each over all heads (folded)
+  if (heads < 0 || heads > 65535 || rows < 0 || rows > (int64_t)1 << 40 || cdiv(rows * D, 2048) > 0xffffff ||
+      (folded && cdiv(rows * D, 4096) * heads > 0xffffff))
     return fail("%s: %d heads of %lld rows out of range", what, heads, (long long)rows);
   return BB_OK;
 }
@@ -926,7 +926,7 @@ int bb_int4_quantize(const void* xk, const int64_t* sxk, const void* xv, const i
   g_err[0] = 0;
   if (!xk || !sxk || (xv && !sxv) || (xv != nullptr) != (vq != nullptr)) return fail("quantize4: null argument");
   int rc = int4_cache_check("quantize4", kq, kp, vq, vp, sc);
-  if (rc == BB_OK) rc = int4_rows_check("quantize4", heads, rows, D, x_kind);
+  if (rc == BB_OK) rc = int4_rows_check("quantize4", heads, rows, D, x_kind, true);
   if (rc != BB_OK) return rc;
   const int64_t el = x_kind == 1 ? 4 : 2;
   if (!aligned(xk, 16) || (sxk[0] * el) % 16 || (sxk[1] * el) % 16 ||
@@ -945,7 +945,7 @@ int bb_int4_dequantize(const uint8_t* kq, const void* kp, const uint8_t* vq, con
   g_err[0] = 0;
   if (!outk || (outv != nullptr) != (vq != nullptr)) return fail("dequantize4: null argument");
   int rc = int4_cache_check("dequantize4", kq, kp, vq, vp, sc);
-  if (rc == BB_OK) rc = int4_rows_check("dequantize4", heads, rows, D, out_kind);
+  if (rc == BB_OK) rc = int4_rows_check("dequantize4", heads, rows, D, out_kind, false);
   if (rc != BB_OK) return rc;
   if (!aligned(outk, 16) || !aligned(outv, 16)) return fail("dequantize4: outputs must be 16-byte aligned");
   auto cache = [](const uint8_t* q, const void* pp, void* out, int64_t s0, int64_t s1) {
