@@ -112,3 +112,20 @@ def test_limits_over_several_heads(heads, rows, write, read):
                         (read, lambda: L.bb_int4_dequantize(at, at, None, None, sc, heads, rows, 128, at + 8, None, 0, None))):
         with pytest.raises(ValueError, match="aligned" if taken else "out of range"):
             _lib.check(call())
+
+
+def test_reset_zeroes_the_rows_in_place(monkeypatch):
+    """DynamicLayer.reset: every cached value is zero, the length and the buffers stay; rows behind a handle are rows like any."""
+    layer = _layer()
+    for store in (layer.store_k, layer.store_v):
+        store.q.fill_(0x5A)
+        store.p.fill_(2.0)
+    x = torch.ones(1, 2, 2, 64, dtype=BF16)
+    layer.update(x, x, {"bb_attend": True})
+    buffers = [y.data_ptr() for s in (layer.store_k, layer.store_v) for y in s.packed()]
+    layer.reset()
+    assert layer.n == 7 and layer._pending is None
+    assert buffers == [y.data_ptr() for s in (layer.store_k, layer.store_v) for y in s.packed()]
+    for store in (layer.store_k, layer.store_v):
+        assert not store.q[:, :7].any() and not store.p[:, :7].any()
+    kv_int4.Int4KVLayer().reset()  # a layer that holds nothing

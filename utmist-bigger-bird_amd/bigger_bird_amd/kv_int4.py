@@ -417,6 +417,13 @@ class Int4KVLayer(Int8KVLayer):
         self._flush()
         return dequantize4_pair(self.store_k.rows(0, self.n), self.store_v.rows(0, self.n), dtype)
 
+    def reset(self):
+        """Every row zero, in place, as DynamicLayer's (whose own form would zero the dequantised copies)."""
+        self._pending = None
+        if self.store_k is not None:
+            for part in (*self.store_k.rows(0, self.n), *self.store_v.rows(0, self.n)):
+                part.zero_()
+
     def batch_repeat_interleave(self, repeats):
         raise NotImplementedError("Int4KVLayer is batch-size-1 only")
 
