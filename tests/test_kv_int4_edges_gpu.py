@@ -226,3 +226,52 @@ def test_cache_without_heads_is_refused(dev):
         decode_int4(q, *none, *none, 5, 0.1)
     with pytest.raises(ValueError, match="must match"):
         decode_int4(q[:, :0], *none, *none, 5, 0.1)
+
+
+@pytest.mark.parametrize("T,G,d,dtype", [(1, 1, 128, BF16), (2, 4, 64, FP16), (5, 1, 128, BF16)])
+def test_512_and_more_kv_heads_are_one_split(T, G, d, dtype, dev):
+    """More KV heads than workgroups at once: one split and no workspace past the lengths where short caches end."""
+    _say("heads", T, G, d, dtype)
+    from bigger_bird_amd import _lib
+
+    gen = torch.Generator(device=dev).manual_seed(T)
+    hk, n = 520, 2003
+    assert n > _lib.lib().bb_int4_decode_one_split(T * G, d) and _lib.lib().bb_int4_decode_workspace(n, T, hk * G, hk, d) == 0
+    cache = _cache(gen, hk, n, n + 1, d, dev)
+    q = torch.randn(T, hk * G, d, generator=gen, device=dev).to(dtype)
+    for length in (n, torch.tensor([n], device=dev)):
+        got = decode_int4(q, *cache, length, d ** -0.5, causal=True).double()
+        for h in (0, 7, 259, 519):
+            heads = slice(h * G, h * G + G)
+            want, tol = plain.attend(q[:, heads], *(x[h:h + 1] for x in cache), n, d ** -0.5, True)
+            tol = tol + (2.0 ** -8 if dtype is BF16 else 2.0 ** -11) * (want.abs() + tol) + (2.0 ** -25 if dtype is FP16 else 0)
+            assert ((got[:, heads] - want).abs() <= tol).all(), h
+
+
+def test_rows_past_32_bit_offsets_to_the_rounding(dev):
+    """One KV head with 70 million rows (4.5 GB of codes) that are zero but for planted ones, whose constant K rows score 17 and
+    whose V rows are read past 2^32 bytes. The other rows add exactly 1 each to the sums and nothing to the outputs, so what
+    is off is the output's half step; 2^-17 of a V scale times 15 and the fp32 sums' 2^-20 of s c + |z|, times the probability; and
+    the probability itself by 17 log2(e) roundings of 2^-23 relative in the score and a few in the exponentials: 2^-17."""
+    _say("70M rows")
+    n, H, d = 70_000_003, 4, 128
+    k4, v4 = (torch.zeros(1, n, d // 2, dtype=torch.uint8, device=dev) for _ in range(2))
+    kp, vp = (torch.zeros(1, n, d // 32, 2, dtype=FP16, device=dev) for _ in range(2))
+    q = torch.ones(1, H, d, device=dev, dtype=BF16)
+    x = torch.full((1, 1, d), 16.0, device=dev, dtype=BF16)
+    y = torch.arange(d, device=dev, dtype=FP32).to(BF16)[None, None]
+    yq = plain.pack(*plain.quantize(y))
+    yv, ys = (t[0, 0] for t in plain.values(*yq))
+    size = 15 * ys + yq[1][0, 0, :, 1].double().abs().repeat_interleave(32)
+    weight = torch.tensor(17.0, dtype=torch.float64).exp().item()
+    for planted, at in enumerate((n - 4, n - 1, 5), 1):
+        out = None
+        if at == n - 1:
+            out = decode_int4_append(q, k4, kp, v4, vp, x, y, n, 17.0 / 2048)
+        else:
+            quantize4_pair(x, y, (k4[:, at:at + 1], kp[:, at:at + 1]), (v4[:, at:at + 1], vp[:, at:at + 1]))
+            out = decode_int4(q, k4, kp, v4, vp, n, 17.0 / 2048)
+        p = planted * weight / (planted * weight + n - planted)
+        want = p * yv
+        tol = 2.0 ** -8 * want + p * (2.0 ** -17 * 15 * ys + 2.0 ** -20 * size) + 2.0 ** -17 * want
+        assert ((out[0].double() - want).abs() <= tol).all(), planted

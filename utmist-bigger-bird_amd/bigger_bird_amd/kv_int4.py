@@ -420,9 +420,10 @@ class Int4KVLayer(Int8KVLayer):
     def reset(self):
         """Every row zero, in place, as DynamicLayer's (whose own form would zero the dequantised copies)."""
         self._pending = None
-        if self.store_k is not None:
-            for part in (*self.store_k.rows(0, self.n), *self.store_v.rows(0, self.n)):
-                part.zero_()
+        for store in (self.store_k, self.store_v):
+            if store is not None:
+                for part in store.rows(0, self.n):
+                    part.zero_()
 
     def batch_repeat_interleave(self, repeats):
         raise NotImplementedError("Int4KVLayer is batch-size-1 only")
