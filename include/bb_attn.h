@@ -370,7 +370,8 @@ int bb_int4_dequantize(const uint8_t* kq, const void* kp, const uint8_t* vq, con
  * Exact attention of the last T tokens (1 .. 16) over the first n rows of a 4-bit cache: out [T, H, D] (strides so[2]:
  * token, head) from q [T, H, D] (strides sq[2]), bf16 or fp16 (is_f16), scores and softmax in fp32 over the fp32 values of
  * the cached rows. Token t attends every row, or with `causal` the first n - T + 1 + t. A token that attends no row
- * gives zeros. D = 64 or 128; any number of query heads per KV head.
+ * gives zeros; a query that is not finite, or whose scores are not, gives NaN (bf16 elements past 2^115 overflow fp32 on the
+ * way). D = 64 or 128; any number of query heads per KV head.
  * n: T <= n <= cap. With n_dev (an int64 in device memory) the length is read there and clamped to 0 .. cap, and n is
  * ignored; every launch shape then depends on cap alone, so a captured graph stays valid while the cache grows.
  * Workspace: bb_int4_decode_workspace(n, ...), with n_dev bb_int4_decode_workspace(cap, ...). Splits of 2^24 keys and more

@@ -159,7 +159,7 @@ class RDAttention(nn.Module):
             return self._forward_autograd(q, k, v, position_embeddings, past_key_values)
         q, k = rope_inplace(q, *position_embeddings), rope_inplace(k, *position_embeddings)
         if past_key_values is not None:
-            # the cache kwargs tell an Int8KVLayer that this module takes fused decode handles (exact_attention)
+            # the cache kwargs tell an Int8KVLayer or Int4KVLayer that this module takes decode handles (exact_attention)
             k, v = past_key_values.update(k, v, self.layer_idx, {"bb_attend": True})
         n = k.shape[-2]
         if b != 1:
@@ -204,7 +204,7 @@ class RDAttention(nn.Module):
 
     def exact_attention(self, q, k, v, t, n):
         """Exact attention: t == n causal prefill, or t < n over all n cached keys (modal_rd/attention.py:137-141)."""
-        if getattr(k, "turbo", None) is not None:      # compressed KV cache handle, one decode token
+        if getattr(k, "turbo", None) is not None:      # compressed KV cache handle: one token, in 4 bits up to 16
             return k.attend(q, self.scaling)
         if t == n:
             none = torch.empty((self.num_heads, 1, 0), dtype=torch.int32, device=q.device)  # no route slots

@@ -23,8 +23,10 @@ from .kv_int8 import _KINDS, GROW, Int8KVLayer
 _strides = functools.lru_cache(maxsize=1024)(_lib.i64s)
 MAX_TOKENS = 16  # query tokens of one decode call
 # Query vectors per KV head (tokens x heads) up to which a handle attends the packed rows; the kernel takes 16 a pass over the
-# cache. Against reading the cache back and flash attention over it, whole calls (us), 8 KV heads x 4 of 128 over 131072 rows:
-# 4 tokens 43 and 365, 16 tokens (64 vectors) 158 and 367; 4 x 8, 16 tokens (128 vectors) 169 and 225; over 16384 rows 40 and 47.
+# cache. Against reading the cache back and flash attention over it, whole calls (us) of 16 tokens at head_dim 128, over 131072
+# and 16384 rows: 64 vectors of 8 KV heads 158 and 364, 40 and 57; 128 of 8 305 and 436, 72 and 65; 192 of 4 250 and 270, 54
+# and 49; 256 of 4 333 and 318, 70 and 54. (Over 4096 rows the packed rows win at each of them, 24 and 33 at 256; past 128 only the
+# read back's memory, 6.4 times the cache, would speak for them.)
 _HANDLE_VECTORS = 128
 _HEAD_DIMS = (32, 64, 128, 256)
 _HALVES = (16, 32, 64, 128)  # their packed rows' bytes
@@ -264,7 +266,8 @@ def decode_int4(q, k4, kp, v4, vp, n, scale, causal=False):
 
     Every token attends all n rows (as RDAttention's cached steps do), or with `causal` token t the first n - T + 1 + t.
     `n`: int, or an int64 GPU tensor of one element that the kernels read (clamped to 0 .. capacity), so that a captured
-    graph stays valid while the cache grows; a token that attends no row gives zeros. Returns q's shape and dtype."""
+    graph stays valid while the cache grows. A token that attends no row gives zeros; a query that is not finite gives NaN.
+    Returns q's shape and dtype."""
     return _decode(q, k4, kp, v4, vp, None, None, n, scale, causal)
 
 

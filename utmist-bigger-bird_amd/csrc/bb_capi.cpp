@@ -961,8 +961,8 @@ int bb_int4_dequantize(const uint8_t* kq, const void* kp, const uint8_t* vq, con
 
 // Short caches go to one split per KV head: one launch, no merge. Up to 3 chunks of 64 keys (128 at head_dim 64) for each of a
 // workgroup's 4 waves, 2 for the wide kernel (GPU time of one split against splits of 256 keys: 8 KV heads x 4 heads of 128,
-// 512 keys 7.0 and 8.3 us, 768 8.4 and 8.5, 1024 9.8 and 8.5; head_dim 64, 1536 keys 8.6 and 8.5, 2048 10.1 and 8.5; 16
-// vectors, 512 keys 8.7 and 9.6, 768 10.7 and 9.9). The host's 3.4 us for the second launch come on top.
+// 512 keys 6.9 and 8.1 us, 768 8.3 and 8.5, 1024 9.6 and 8.5; head_dim 64, 1536 keys 8.6 and 8.5, 2048 10.0 and 8.4; 16
+// vectors, 512 keys 8.7 and 9.4, 768 10.6 and 9.7). The host's 3.4 us for the second launch come on top.
 int64_t bb_int4_decode_one_split(int vectors, int D) { return (vectors <= 4 ? 768 : 512) * (D == 64 ? 2 : 1); }
 
 // Splits of the 4-bit decode: two workgroups per CU over all KV heads, of kInt4MinSplit keys at least (the kernels cut

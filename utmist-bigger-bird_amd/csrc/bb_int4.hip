@@ -566,11 +566,14 @@ BB_DEV u32x2_t two_terms(float q0, float q1) {
 //           leave lane (k, a) with the whole score of query a alone, so that no lane's exponential is idle.
 //   values  The probabilities times the scales of column group t go to column 4 t + h of the operand, so one product serves
 //           all groups (the columns of a product whose rows are another group are not used).
-// What bounds it, measured: 131072 rows x 8 KV heads x 4 heads of 128 (168 MB) take 31.8 us, 5.3 TB/s, and the merge 4; with the
-// arithmetic taken out the loads alone and the merge take 30.3 together. The rest is the first chunks' way from memory and the
-// last chunks' arithmetic, which nothing overlaps: with two stages a wave 160 KB a CU are in flight from the start, and a split
-// is 8 chunks a wave here. 64 splits a head, two workgroups per CU, 34.9 us with the merge; 48 splits 39.4, 96 splits 37.2;
-// plain instead of non-temporal loads 39.1 against 37.3 when that was tried.
+// What bounds it, measured: 131072 rows x 8 KV heads x 4 heads of 128 (168 MB) take 34.2 us a call with the merge, 4.9 TB/s, in
+// a queue of calls (traced one by one, which adds each kernel's start and end, 31.0 and 4.0); with the arithmetic taken out the
+// loads alone and the merge take 30.3 together. The rest is the first chunks' way from memory (a wave's first chunk is there
+// after 3.8 us) and the last chunks' arithmetic, which nothing overlaps: with two stages a wave 160 KB a CU are in flight from
+// the start, and a split is 8 chunks a wave here. 64 splits a head, two workgroups per CU: 35.3 us with the merge where 32 splits
+// took 34.0 to 36.0, 48 splits 38.5, 96 splits 38.6; plain instead of non-temporal loads 39.1 against 37.3 when that was tried.
+// head_dim 64 is further from memory's rate: 100000 rows (64 MB) 20.4 us, 3.1 TB/s, with 710 VALU instructions for a chunk of the
+// same 10 KB against 660, twice the exponentials and half the groups that a chunk's params and probabilities spread over.
 template <int D, bool F16>
 __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodeParams p) {
   __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][kStage];
@@ -823,10 +826,14 @@ __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodePara
 //   values  The lane's probabilities are the operand of the values' products as they are: with keys in the order of key_of_lane
 //           and key_of_step, a lane's 16 keys of 64 are those whose V codes the transposing read hands to its quarter. So no
 //           probability passes through LDS, and the maxima, sums and minima's parts stay with one vector per lane.
-// The VALU bounds it: about 650 instructions a chunk (codes to floats 230, probabilities times scales into two terms 190), 3000
-// cycles on a SIMD. 16 vectors x 8 KV heads x 128 over 32768 rows (42 MB) take 16.6 us, 4 until the first chunks are there and
-// two chunks a wave behind that; over 131072 rows, with the merge, 46 us (3.7 TB/s). With 4 vectors it is slower than the
-// kernel above (131072 rows 44 us against 37 with the merge, 512 rows 8.2 against 7.0; head_dim 64, 100000 rows 25 against 21).
+// The VALU bounds it: about 680 instructions a chunk (codes to operands 225, probabilities times scales into two terms 190), 3000
+// cycles on a SIMD. 16 vectors x 8 KV heads x 128 over 32768 rows (42 MB) take 16.6 us traced; a wave's median, in us at 2.4 GHz:
+// 2.5 until its first 20 loads are issued (the other waves of the CU issue theirs as well), 4.0 until the first chunk is
+// there, 3.9 for that chunk (the loop's code comes in with it, and the SIMD's other wave works on its own), 2.6 for the second,
+// 1.4 for the states and the partials; the slowest wave ends 1 later, and the launch is the rest. Over 131072 rows 42.3 us with
+// the merge (4.0 TB/s). Each pass of 16 vectors reads and unpacks the cache again: 64 vectors over 131072 rows 154 us. With 4
+// vectors this kernel is slower than the one above (131072 rows 40.2 us against 36.1 with the merge, 512 rows 8.1 against 6.9;
+// head_dim 64, 100000 rows 24.7 against 20.2).
 template <int D, bool F16>
 __global__ __launch_bounds__(kThreads, 2) void int4_decode_wide_kernel(Int4DecodeParams p) {
   __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][kStage];
