@@ -572,8 +572,8 @@ BB_DEV u32x2_t two_terms(float q0, float q1) {
 // after 3.8 us) and the last chunks' arithmetic, which nothing overlaps: with two stages a wave 160 KB a CU are in flight from
 // the start, and a split is 8 chunks a wave here. 64 splits a head, two workgroups per CU: 35.3 us with the merge where 32 splits
 // took 34.0 to 36.0, 48 splits 38.5, 96 splits 38.6; plain instead of non-temporal loads 39.1 against 37.3 when that was tried.
-// head_dim 64 is further from memory's rate: 100000 rows (64 MB) 20.4 us, 3.1 TB/s, with 710 VALU instructions for a chunk of the
-// same 10 KB against 660, twice the exponentials and half the groups that a chunk's params and probabilities spread over.
+// The same 10 us past a streaming read's time weigh more where there is less to read: head_dim 64, 100000 rows x 8 heads (64 MB)
+// 20.4 us, 11 past it, a split's 12.25 chunks being four rounds for one of its waves and three for the others.
 template <int D, bool F16>
 __global__ __launch_bounds__(kThreads, 2) void int4_decode_kernel(Int4DecodeParams p) {
   __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][kStage];
