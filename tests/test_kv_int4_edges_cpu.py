@@ -129,3 +129,12 @@ def test_reset_zeroes_the_rows_in_place(monkeypatch):
     for store in (layer.store_k, layer.store_v):
         assert not store.q[:, :7].any() and not store.p[:, :7].any()
     kv_int4.Int4KVLayer().reset()  # a layer that holds nothing
+
+
+def test_reset_of_a_layer_with_one_store():
+    """Between the assignments of keys and values (kv_evict's) a layer can hold one of the two."""
+    layer = _layer()
+    layer.store_v = None
+    layer.store_k.q.fill_(0x5A)
+    layer.reset()
+    assert layer.n == 5 and not layer.store_k.q[:, :5].any()
