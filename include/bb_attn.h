@@ -35,8 +35,8 @@ extern "C" {
  *        x_is_f32, and bb_int8_dequantize an output kind where it took out_is_f32 (the old values keep their
  *        meaning)
  *   203  bb_add_rms_norm, bb_silu_mul, bb_gemv and bb_gemv_norm added; later, with no parameter list changed and so
- *        under the same number, bb_gemv_norm_rope, bb_argmax_step and the bb_int4_* functions (a library built before
- *        them lacks the symbols) */
+ *        under the same number, bb_gemv_norm_rope, bb_argmax_step, the bb_int4_* and the bb_paged_* functions (a library built
+ *        before them lacks the symbols) */
 #define BB_ABI_VERSION 203
 int bb_version(void);
 
@@ -396,6 +396,52 @@ size_t bb_int4_decode_workspace(int64_t n, int T, int H, int Hkv, int D);
 /* The longest cache (n, or with n_dev the capacity) that a call with this many query vectors per KV head (T H / Hkv) attends
  * in one split: one launch, and a workspace of 0 bytes (NULL). */
 int64_t bb_int4_decode_one_split(int vectors, int D);
+
+/*
+ * Paged KV cache (no reference counterpart): K and V rows of several sequences in pages, bf16 or fp16 (is_f16).
+ *
+ * k_pages, v_pages [pages, Hkv, page, D] (strides sk[3], sv[3]: page, head, row; rows 16-byte aligned; page a power of two
+ * >= 16; D = 64 or 128). table [B, W] int32 (row stride st): entry w of a sequence is the page of its rows w page ..
+ * (w + 1) page - 1; an entry outside 0 .. pages - 1 names no page, and its rows are neither written nor attended. lens [B]
+ * int32: the rows of each sequence, this call's new ones among them (more than W page rows are W page). fresh [B] int32 or
+ * NULL (all T): how many of the T token columns are real, clamped to 0 .. T. Token j of sequence b is row lens[b] - fresh[b]
+ * + j. The lengths are read on the device, and every launch shape depends on the host arguments alone, so a captured graph
+ * stays valid while the cache grows. W page <= 2^30. A page that two rows' writes reach (one page in two sequences' tables
+ * where both write) holds either.
+ *
+ * bb_paged_append writes the real tokens' rows: k, v [B, Hkv, T, D] (strides skn[3], svn[3]: sequence, head, token), k
+ * rotated by cos, sin [B, T, D] (strides sc[2]: sequence, token; fp32 with rope_f32, else the rows' type; NULL: k as it
+ * is): x cos + (-x[D/2:], x[:D/2]) sin in fp32, rounded once. With H > 0 it also writes q_out [B, H, T, D] (strides
+ * sqo[3]), q rotated alike (every column, padding too; cos required); H = 0: no q. Rows that lie outside the table are not
+ * written.
+ */
+int bb_paged_append(const void* k, const int64_t* skn, const void* v, const int64_t* svn, const void* q, const int64_t* sq,
+                    void* q_out, const int64_t* sqo, const void* cos, const void* sin, const int64_t* sc, int rope_f32,
+                    void* k_pages, const int64_t* sk, void* v_pages, const int64_t* sv, const int32_t* table, int64_t st,
+                    const int32_t* lens, const int32_t* fresh, int B, int T, int H, int Hkv, int D, int pages, int page, int W,
+                    int is_f16, void* stream);
+
+/*
+ * Exact causal attention over the pages: out [B, H, T, D] (strides so[3]) from q [B, H, T, D] (strides sq[3]); token j
+ * attends the rows up to its own, lens - fresh + j, of the pages that its table names; scores and softmax in fp32. Zeros
+ * where it attends none, and for padding; NaN where its scores have no softmax (a query that is not finite). A row of V
+ * that is not finite reaches only the tokens that attend it. H / Hkv query heads per KV head, any number.
+ * Workspace: bb_paged_attention_workspace (0: none).
+ */
+int bb_paged_attention(const void* q, const int64_t* sq, const void* k_pages, const int64_t* sk, const void* v_pages,
+                       const int64_t* sv, const int32_t* table, int64_t st, const int32_t* lens, const int32_t* fresh, int B,
+                       int T, int H, int Hkv, int D, int pages, int page, int W, int is_f16, float scale, void* out,
+                       const int64_t* so, void* ws, size_t ws_bytes, void* stream);
+size_t bb_paged_attention_workspace(int B, int T, int H, int Hkv, int D, int page, int W);
+
+/* One step: bb_paged_append of k and v, then bb_paged_attention of the rotated q (not rotated where cos is NULL). Workspace:
+ * bb_paged_step_workspace. */
+int bb_paged_step(const void* q, const int64_t* sq, const void* k, const int64_t* skn, const void* v, const int64_t* svn,
+                  const void* cos, const void* sin, const int64_t* sc, int rope_f32, void* k_pages, const int64_t* sk,
+                  void* v_pages, const int64_t* sv, const int32_t* table, int64_t st, const int32_t* lens,
+                  const int32_t* fresh, int B, int T, int H, int Hkv, int D, int pages, int page, int W, int is_f16,
+                  float scale, void* out, const int64_t* so, void* ws, size_t ws_bytes, void* stream);
+size_t bb_paged_step_workspace(int B, int T, int H, int Hkv, int D, int page, int W);
 
 /*
  * Measurement helper (no reference counterpart): reads `bytes` (a multiple of 16, 16-byte aligned) of device memory

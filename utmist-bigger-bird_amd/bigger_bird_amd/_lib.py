@@ -74,6 +74,16 @@ SIGNATURES = {
                                      _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, c_i64p, _vp, _sz, _vp]),
     "bb_int4_decode_workspace": (_sz, [_i64, _i32, _i32, _i32, _i32]),
     "bb_int4_decode_one_split": (_i64, [_i32, _i32]),
+    "bb_paged_append": (_i32, [_vp, c_i64p, _vp, c_i64p, _vp, c_i64p, _vp, c_i64p, _vp, _vp, c_i64p, _i32,
+                               _vp, c_i64p, _vp, c_i64p, _vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                               _i32, _i32, _vp]),
+    "bb_paged_attention": (_i32, [_vp, c_i64p, _vp, c_i64p, _vp, c_i64p, _vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
+                                  _i32, _i32, _i32, _i32, _f32, _vp, c_i64p, _vp, _sz, _vp]),
+    "bb_paged_attention_workspace": (_sz, [_i32] * 7),
+    "bb_paged_step": (_i32, [_vp, c_i64p, _vp, c_i64p, _vp, c_i64p, _vp, _vp, c_i64p, _i32, _vp, c_i64p, _vp, c_i64p, _vp,
+                             _i64, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, c_i64p, _vp,
+                             _sz, _vp]),
+    "bb_paged_step_workspace": (_sz, [_i32] * 7),
 }
 
 

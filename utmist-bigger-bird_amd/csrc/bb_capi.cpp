@@ -1057,6 +1057,222 @@ int bb_int4_decode_append(const void* q, const int64_t* sq, uint8_t* kq, void* k
                           scale, causal, out, so, ws, ws_bytes, stream);
 }
 
+// ---- paged KV cache ----
+// How a call of the attention is cut (the kernels cut the lengths that they find by it).
+struct PagedSchedule {
+  int VT, tiles, unit, min_share, target, grid, merge_vecs;
+  size_t slots;
+};
+constexpr int kPagedStreamVectors = 32;  // query vectors of a KV head up to which the streaming kernel takes a call
+constexpr int kPagedStepVectors = 128;   // and up to which it takes a step, storing its new rows
+static const char* paged_schedule(int B, int T, int H, int Hkv, int D, int W, int page, bool with_new, PagedSchedule& s) {
+  const int64_t R = (int64_t)T * (H / Hkv), cap = (int64_t)W * page;
+  if (R <= kPagedStreamVectors || (with_new && R <= kPagedStepVectors)) {
+    s.VT = R <= 16 ? 16 : 32;
+    s.unit = 4 * 4096 / D;
+    s.min_share = 2;
+    s.target = 2 * kCUs;
+  } else {
+    s.VT = 256;
+    s.unit = 64;
+    s.min_share = 16;
+    s.target = kCUs;
+  }
+  const int64_t tiles = cdiv(R, s.VT), pairs = tiles * B, units = cdiv(cap, s.unit);
+  if (cap > 1ll << 30 || pairs * Hkv * units >= 1ll << 31 || R >= 1ll << 31) return "lengths out of range";
+  s.tiles = (int)tiles;
+  const int64_t most = cdiv(units, s.min_share);  // splits of a pair
+  s.grid = (int)std::min<int64_t>(pairs * Hkv * most, s.target + pairs * Hkv);
+  // a pair of more than one split has at most twice its units over the share of them
+  s.slots = most > 1 ? (size_t)std::min<int64_t>(s.grid, 2 * s.target) : 0;
+  s.merge_vecs = B * R * Hkv <= 16384 ? 1 : 16;
+  return nullptr;
+}
+
+static bool paged_strides(const int64_t* s) {
+  return s[0] >= 0 && s[1] >= 0 && s[2] >= 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
+}
+
+// The cache of a call, checked.
+static int paged_cache(const char* what, void* k, const int64_t* sk, void* v, const int64_t* sv, const int32_t* table,
+                       int64_t st, const int32_t* lens, const int32_t* fresh, int B, int T, int H, int Hkv, int D, int pages,
+                       int page, int W, bb::PagedCache& c) {
+  if (!k || !sk || !v || !sv || !table || !lens) return fail("%s: null argument", what);
+  if (B < 1 || T < 1 || Hkv < 1 || H < 0 || H % Hkv || B > 65535 || Hkv > 65535)
+    return fail("%s: q [B,H,T,D] and the pages' Hkv heads must match", what);
+  if (D != 64 && D != 128) return fail("%s: head_dim %d unsupported (64 or 128)", what, D);
+  if (page < 16 || page & (page - 1)) return fail("%s: pages of %d rows unsupported (a power of two, at least 16)", what, page);
+  if (pages < 0 || W < 1 || st < 0) return fail("%s: empty table", what);
+  if ((int64_t)W * page > 1ll << 30) return fail("%s: tables of %lld rows out of range", what, (long long)W * page);
+  if (!aligned(k, 16) || !aligned(v, 16) || !paged_strides(sk) || !paged_strides(sv) || sk[2] >= 1 << 26 || sv[2] >= 1 << 26)
+    return fail("%s: pages need a contiguous head_dim and 16-byte aligned rows", what);
+  if (!aligned(table, 4) || !aligned(lens, 4) || !aligned(fresh, 4)) return fail("%s: misaligned lengths", what);
+  c.k = static_cast<uint16_t*>(k);
+  c.v = static_cast<uint16_t*>(v);
+  c.table = table; c.lens = lens; c.fresh = fresh;
+  c.skp = sk[0]; c.skh = sk[1]; c.skr = sk[2];
+  c.svp = sv[0]; c.svh = sv[1]; c.svr = sv[2];
+  c.st = st;
+  c.pages = pages; c.W = W;
+  c.page_log2 = __builtin_ctz((unsigned)page);
+  return BB_OK;
+}
+
+static int paged_rope(const char* what, const void* cos, const void* sin, const int64_t* sc, int f32, bb::PagedRope& r) {
+  memset(&r, 0, sizeof(r));
+  if (!cos && !sin) return BB_OK;
+  if (!cos || !sin || !sc) return fail("%s: null argument", what);
+  const int whole = f32 ? 4 : 8;
+  if (!aligned(cos, 16) || !aligned(sin, 16) || sc[0] < 0 || sc[1] < 0 || sc[0] % whole || sc[1] % whole)
+    return fail("%s: cos and sin rows must be 16-byte aligned", what);
+  r.cos = cos; r.sin = sin;
+  r.s0 = sc[0]; r.s1 = sc[1];
+  r.f32 = f32 ? 1 : 0;
+  return BB_OK;
+}
+
+static int paged_rows(const char* what, const void* x, const int64_t* s) {
+  if (!x || !s) return fail("%s: null argument", what);
+  if (!aligned(x, 16) || !paged_strides(s)) return fail("%s: rows need a contiguous head_dim and 16-byte alignment", what);
+  return BB_OK;
+}
+
+int bb_paged_append(const void* k, const int64_t* skn, const void* v, const int64_t* svn, const void* q, const int64_t* sq,
+                    void* q_out, const int64_t* sqo, const void* cos, const void* sin, const int64_t* sc, int rope_f32,
+                    void* k_pages, const int64_t* sk, void* v_pages, const int64_t* sv, const int32_t* table, int64_t st,
+                    const int32_t* lens, const int32_t* fresh, int B, int T, int H, int Hkv, int D, int pages, int page, int W,
+                    int is_f16, void* stream) {
+  g_err[0] = 0;
+  const char* what = "paged_append";
+  bb::PagedAppendParams p;
+  memset(&p, 0, sizeof(p));
+  int rc = paged_cache(what, k_pages, sk, v_pages, sv, table, st, lens, fresh, B, T, H, Hkv, D, pages, page, W, p.c);
+  if (rc == BB_OK) rc = paged_rope(what, cos, sin, sc, rope_f32, p.r);
+  if (rc == BB_OK) rc = paged_rows(what, k, skn);
+  if (rc == BB_OK) rc = paged_rows(what, v, svn);
+  if (rc == BB_OK && H) rc = paged_rows(what, q, sq);
+  if (rc == BB_OK && H) rc = paged_rows(what, q_out, sqo);
+  if (rc != BB_OK) return rc;
+  if (H && !cos) return fail("%s: q is rotated: cos and sin required", what);
+  if ((int64_t)B * T * (H + 2 * Hkv) >= 1ll << 34) return fail("%s: too many rows", what);  // 2^29 workgroups
+  p.k = static_cast<const uint16_t*>(k);
+  p.v = static_cast<const uint16_t*>(v);
+  p.sk0 = skn[0]; p.sk1 = skn[1]; p.sk2 = skn[2];
+  p.sv0 = svn[0]; p.sv1 = svn[1]; p.sv2 = svn[2];
+  if (H) {
+    p.q = static_cast<const uint16_t*>(q);
+    p.qout = static_cast<uint16_t*>(q_out);
+    p.sq0 = sq[0]; p.sq1 = sq[1]; p.sq2 = sq[2];
+    p.so0 = sqo[0]; p.so1 = sqo[1]; p.so2 = sqo[2];
+  }
+  p.B = B; p.T = T; p.H = H; p.Hkv = Hkv; p.D = D;
+  p.f16 = is_f16 ? 1 : 0;
+  return hip_status(bb::launch_paged_append(p, static_cast<hipStream_t>(stream)), "bb_paged_append");
+}
+
+static size_t paged_partials(int B, int T, int H, int Hkv, int D, int page, int W, bool with_new) {
+  PagedSchedule s;
+  if (B < 1 || T < 1 || H < 1 || Hkv < 1 || H % Hkv || page < 16 || W < 1 || (D != 64 && D != 128)) return 0;
+  if (paged_schedule(B, T, H, Hkv, D, W, page, with_new, s)) return 0;
+  return s.slots * s.VT * (D + 4) * 4;
+}
+
+size_t bb_paged_attention_workspace(int B, int T, int H, int Hkv, int D, int page, int W) {
+  return paged_partials(B, T, H, Hkv, D, page, W, false);
+}
+
+size_t bb_paged_step_workspace(int B, int T, int H, int Hkv, int D, int page, int W) {
+  if (B < 1 || T < 1 || H < 1 || Hkv < 1) return 0;
+  const bool one = (int64_t)T * (H / Hkv) <= kPagedStepVectors;
+  const size_t part = paged_partials(B, T, H, Hkv, D, page, W, one);
+  return one ? part : align256(part) + (size_t)B * T * H * D * 2;  // rotated q
+}
+
+static int paged_attention_impl(const char* what, const void* q, const int64_t* sq, const void* knew, const int64_t* skn,
+                                const void* vnew, const int64_t* svn, const bb::PagedCache& c, const bb::PagedRope& r, int B,
+                                int T, int H, int Hkv, int D, int page, int is_f16, float scale, void* out,
+                                const int64_t* so, void* ws, size_t ws_bytes, void* stream) {
+  int rc = paged_rows(what, q, sq);
+  if (rc == BB_OK) rc = paged_rows(what, out, so);
+  if (rc != BB_OK) return rc;
+  if (H < 1) return fail("%s: q [B,H,T,D] and the pages' Hkv heads must match", what);
+  if (!(scale > 0.0f)) return fail("scale must be positive");
+  PagedSchedule s;
+  if (const char* e = paged_schedule(B, T, H, Hkv, D, c.W, page, knew != nullptr, s)) return fail("%s: %s", what, e);
+  const size_t need = s.slots * s.VT * (D + 4) * 4;
+  if (need && (!ws || ws_bytes < need || !aligned(ws, 16))) return fail("workspace of %zu bytes required", need);
+  bb::PagedAttnParams p;
+  memset(&p, 0, sizeof(p));
+  p.c = c;
+  p.r = r;
+  p.q = static_cast<const uint16_t*>(q);
+  p.sq0 = sq[0]; p.sq1 = sq[1]; p.sq2 = sq[2];
+  if (knew) {
+    p.knew = static_cast<const uint16_t*>(knew);
+    p.vnew = static_cast<const uint16_t*>(vnew);
+    p.skn0 = skn[0]; p.skn1 = skn[1]; p.skn2 = skn[2];
+    p.svn0 = svn[0]; p.svn1 = svn[1]; p.svn2 = svn[2];
+  }
+  p.out = static_cast<uint16_t*>(out);
+  p.so0 = so[0]; p.so1 = so[1]; p.so2 = so[2];
+  p.part = need ? static_cast<float*>(ws) : nullptr;
+  p.B = B; p.T = T; p.H = H; p.Hkv = Hkv; p.G = H / Hkv; p.D = D;
+  p.f16 = is_f16 ? 1 : 0;
+  p.VT = s.VT; p.tiles = s.tiles; p.pairs = s.tiles * B;
+  p.unit = s.unit; p.min_share = s.min_share; p.target = s.target;
+  p.grid = s.grid; p.merge_vecs = s.merge_vecs;
+  p.scale = (float)((double)scale * 1.4426950408889634);
+  return hip_status(bb::launch_paged_attention(p, static_cast<hipStream_t>(stream)), what);
+}
+
+int bb_paged_attention(const void* q, const int64_t* sq, const void* k_pages, const int64_t* sk, const void* v_pages,
+                       const int64_t* sv, const int32_t* table, int64_t st, const int32_t* lens, const int32_t* fresh, int B,
+                       int T, int H, int Hkv, int D, int pages, int page, int W, int is_f16, float scale, void* out,
+                       const int64_t* so, void* ws, size_t ws_bytes, void* stream) {
+  g_err[0] = 0;
+  bb::PagedCache c;
+  bb::PagedRope r;
+  memset(&r, 0, sizeof(r));
+  const int rc = paged_cache("paged_attention", const_cast<void*>(k_pages), sk, const_cast<void*>(v_pages), sv, table, st,
+                             lens, fresh, B, T, H, Hkv, D, pages, page, W, c);
+  if (rc != BB_OK) return rc;
+  return paged_attention_impl("paged_attention", q, sq, nullptr, nullptr, nullptr, nullptr, c, r, B, T, H, Hkv, D, page,
+                              is_f16, scale, out, so, ws, ws_bytes, stream);
+}
+
+int bb_paged_step(const void* q, const int64_t* sq, const void* k, const int64_t* skn, const void* v, const int64_t* svn,
+                  const void* cos, const void* sin, const int64_t* sc, int rope_f32, void* k_pages, const int64_t* sk,
+                  void* v_pages, const int64_t* sv, const int32_t* table, int64_t st, const int32_t* lens,
+                  const int32_t* fresh, int B, int T, int H, int Hkv, int D, int pages, int page, int W, int is_f16,
+                  float scale, void* out, const int64_t* so, void* ws, size_t ws_bytes, void* stream) {
+  g_err[0] = 0;
+  const char* what = "paged_step";
+  bb::PagedCache c;
+  bb::PagedRope r;
+  int rc = paged_cache(what, k_pages, sk, v_pages, sv, table, st, lens, fresh, B, T, H, Hkv, D, pages, page, W, c);
+  if (rc == BB_OK) rc = paged_rope(what, cos, sin, sc, rope_f32, r);
+  if (rc == BB_OK) rc = paged_rows(what, k, skn);
+  if (rc == BB_OK) rc = paged_rows(what, v, svn);
+  if (rc == BB_OK) rc = paged_rows(what, q, sq);
+  if (rc != BB_OK) return rc;
+  if (H < 1) return fail("%s: q [B,H,T,D] and the pages' Hkv heads must match", what);
+  if ((int64_t)T * (H / Hkv) <= kPagedStepVectors)  // the attention kernel rotates and stores the new rows itself
+    return paged_attention_impl(what, q, sq, k, skn, v, svn, c, r, B, T, H, Hkv, D, page, is_f16, scale, out, so, ws,
+                                ws_bytes, stream);
+  const size_t part = align256(bb_paged_attention_workspace(B, T, H, Hkv, D, page, W));
+  const size_t need = bb_paged_step_workspace(B, T, H, Hkv, D, page, W);
+  if (!ws || ws_bytes < need || !aligned(ws, 16)) return fail("workspace of %zu bytes required", need);
+  void* turned = static_cast<char*>(ws) + part;
+  const int64_t sqo[3] = {(int64_t)T * H * D, D, (int64_t)H * D};
+  if (!(scale > 0.0f)) return fail("scale must be positive");  // before the rows are written
+  rc = bb_paged_append(k, skn, v, svn, cos ? q : nullptr, sq, turned, sqo, cos, sin, sc, rope_f32, k_pages, sk, v_pages, sv,
+                       table, st, lens, fresh, B, T, cos ? H : 0, Hkv, D, pages, page, W, is_f16, stream);
+  if (rc != BB_OK) return rc;
+  memset(&r, 0, sizeof(r));
+  return paged_attention_impl(what, cos ? turned : q, cos ? sqo : sq, nullptr, nullptr, nullptr, nullptr, c, r, B, T, H, Hkv,
+                              D, page, is_f16, scale, out, so, ws, part, stream);
+}
+
 int bb_stream_read(const void* buf, size_t bytes, uint32_t* sink, int workgroups, void* stream) {
   g_err[0] = 0;
   if (!buf || !sink) return fail("stream_read: null argument");

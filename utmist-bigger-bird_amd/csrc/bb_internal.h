@@ -139,6 +139,44 @@ constexpr int64_t kInt4MinSplit = 256;  // keys of a split, at least (splits are
 constexpr int int4_part_row(int D) { return D + 4; }  // whole 16-byte pieces
 hipError_t launch_int4_decode(const Int4DecodeParams& p, hipStream_t stream);
 
+// Paged KV cache (bb_paged.hip).
+struct PagedCache {
+  uint16_t *k, *v;        // [pages, Hkv, page, D] (strides skp / svp page, skh / svh head, skr / svr row)
+  const int32_t* table;   // [B, W] (row stride st)
+  const int32_t* lens;    // [B]
+  const int32_t* fresh;   // [B], or null: all T
+  int64_t skp, skh, skr, svp, svh, svr, st;
+  int pages, W, page_log2;
+};
+struct PagedRope {
+  const void *cos, *sin;  // [B, T, D] (strides s0, s1), fp32 or the rows' type; or null
+  int64_t s0, s1;
+  int f32;
+};
+struct PagedAppendParams {
+  PagedCache c;
+  PagedRope r;
+  const uint16_t *k, *v, *q;  // [B, heads, T, D] (strides 0: sequence, 1: head, 2: token)
+  uint16_t* qout;
+  int64_t sk0, sk1, sk2, sv0, sv1, sv2, sq0, sq1, sq2, so0, so1, so2;
+  int B, T, H, Hkv, D, f16;   // H = 0: no q
+};
+hipError_t launch_paged_append(const PagedAppendParams& p, hipStream_t stream);
+struct PagedAttnParams {
+  PagedCache c;
+  PagedRope r;                 // with new rows
+  const uint16_t *q, *knew, *vnew;
+  uint16_t* out;
+  float* part;                 // slots of VT rows of D + 4 floats (output, maximum, sum), or null: no pair is split
+  int64_t sq0, sq1, sq2, skn0, skn1, skn2, svn0, svn1, svn2, so0, so1, so2;
+  int B, T, H, Hkv, G, D, f16;
+  int VT, tiles, pairs;        // query vectors of a tile, tiles, B * tiles
+  int unit, min_share, target; // keys of a unit; units of a split, at least; workgroups aimed at
+  int grid, merge_vecs;
+  float scale;                 // times log2(e)
+};
+hipError_t launch_paged_attention(const PagedAttnParams& p, hipStream_t stream);
+
 // A decode step's new K / V row folded into the first kernel that reads the cache: the row at position n - 1 (n the
 // current length, which already counts it) is read from knew / vnew instead of the cache, and the lanes that read it
 // also write it to the cache rows (k, v), so that later kernels find it there. Only when 1 <= n <= cap; knew = null

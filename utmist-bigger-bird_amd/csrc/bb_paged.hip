@@ -1,0 +1,1153 @@
+// Paged 16-bit KV cache: appending rows (with RoPE on the way) and exact causal attention over the pages, for several
+// sequences of unlike lengths in one call.
+//
+// k, v [pages, Hkv, page, D] (page a power of two >= 16); table [B, W] names the page of rows [w page, (w + 1) page) of a
+// sequence, an entry outside 0 .. pages - 1 names none (its rows are neither written nor attended); lens [B] counts a
+// sequence's rows with the call's new ones, fresh [B] how many of the T token columns are real. Token j of a sequence is row
+// lens - fresh + j and attends the rows up to its own.
+#include "bb_common.h"
+#include "bb_internal.h"
+
+namespace bb {
+namespace {
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(4))) int32_t* const_i32;  // read by scalar loads
+typedef __attribute__((__vector_size__(4 * sizeof(__bf16)))) __bf16 bf16x4_t;
+typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4_t;
+
+template <bool V>
+struct Constant {
+  static constexpr bool value = V;
+};
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr float kInf = __builtin_huge_valf();
+
+template <bool F16>
+BB_DEV float lo16(uint32_t w) {
+  if constexpr (F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(w & 0xffffu));
+  else return __uint_as_float(w << 16);
+}
+template <bool F16>
+BB_DEV float hi16(uint32_t w) {
+  if constexpr (F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16));
+  else return __uint_as_float(w & 0xffff0000u);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// The call's lengths. Everything a kernel indexes with goes through these: lens and fresh come from the caller's device
+// memory and may hold anything.
+BB_DEV int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+struct Sequence {
+  int cap;    // rows that the table has entries for
+  int n;      // rows, clamped to 0 .. cap
+  int fresh;  // real token columns, 0 .. T
+  int first;  // row of token 0 (may lie outside 0 .. cap - 1)
+  // Rows that token j attends: the first seen(j) of them.
+  BB_DEV int seen(int j) const { return j < fresh ? clampi(first + j + 1, 0, n) : 0; }
+};
+BB_DEV Sequence sequence(const PagedCache& c, int T, int b) {
+  Sequence s;
+  const int raw = c.lens[b];
+  s.cap = c.W << c.page_log2;
+  s.n = clampi(raw, 0, s.cap);
+  s.fresh = c.fresh ? clampi(c.fresh[b], 0, T) : T;
+  s.first = raw < -T ? -T : raw - s.fresh;
+  return s;
+}
+// The page of row r (0 <= r < cap) of sequence b, or -1.
+BB_DEV int page_of(const PagedCache& c, int b, int r) {
+  const int e = c.table[b * c.st + (r >> c.page_log2)];
+  return (uint32_t)e < (uint32_t)c.pages ? e : -1;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// RoPE of 8 elements x at dims d .. d + 7 and y at d + D / 2 .., in fp32, rounded once (HF's operator rounds each product
+// and the sum to the element type).
+struct Turn {
+  float cx[8], sx[8], cy[8], sy[8];
+};
+template <bool F16>
+BB_DEV void widen(const u32x4_t w, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = lo16<F16>(w[i]);
+    f[2 * i + 1] = hi16<F16>(w[i]);
+  }
+}
+template <bool F16>
+BB_DEV void load_turn(const PagedRope& r, int64_t at, int D, Turn& t) {
+  if (r.f32) {
+    const float* c = static_cast<const float*>(r.cos) + at;
+    const float* s = static_cast<const float*>(r.sin) + at;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(c + i), b = *reinterpret_cast<const f32x4_t*>(s + i);
+      const f32x4_t e = *reinterpret_cast<const f32x4_t*>(c + D / 2 + i), f = *reinterpret_cast<const f32x4_t*>(s + D / 2 + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        t.cx[i + j] = a[j];
+        t.sx[i + j] = b[j];
+        t.cy[i + j] = e[j];
+        t.sy[i + j] = f[j];
+      }
+    }
+  } else {
+    const uint16_t* c = static_cast<const uint16_t*>(r.cos) + at;
+    const uint16_t* s = static_cast<const uint16_t*>(r.sin) + at;
+    widen<F16>(ld16(c), t.cx);
+    widen<F16>(ld16(s), t.sx);
+    widen<F16>(ld16(c + D / 2), t.cy);
+    widen<F16>(ld16(s + D / 2), t.sy);
+  }
+}
+template <bool F16>
+BB_DEV void rotate(const u32x4_t x, const u32x4_t y, const Turn& t, float (&p)[8], float (&q)[8]) {
+  float a[8], b[8];
+  widen<F16>(x, a);
+  widen<F16>(y, b);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    p[i] = fmaf(a[i], t.cx[i], -(b[i] * t.sx[i]));
+    q[i] = fmaf(b[i], t.cy[i], a[i] * t.sy[i]);
+    // (the asm keeps fp16 results single-rounded: the compiler would otherwise round the sum to fp16 by an fp16 fma)
+    asm("" : "+v"(p[i]), "+v"(q[i]));
+  }
+}
+template <bool F16>
+BB_DEV void rotate(u32x4_t& x, u32x4_t& y, const Turn& t) {
+  float p[8], q[8];
+  rotate<F16>(x, y, t, p, q);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = pack2<F16>(p[2 * i], p[2 * i + 1]);
+    y[i] = pack2<F16>(q[2 * i], q[2 * i + 1]);
+  }
+}
+// Two numbers as two 16-bit terms each.
+template <bool F16>
+BB_DEV u32x2_t two_terms(float a, float b) {
+  uint32_t hi = pack2<F16>(a, b);
+  asm("" : "+v"(hi));
+  return u32x2_t{hi, pack2<F16>(a - lo16<F16>(hi), b - hi16<F16>(hi))};
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Append. A lane takes 8 elements of a row's lower half and the 8 that RoPE pairs with them; a row is D / 16 lanes, rows go
+// head by head (Q, then K, then V) through one token's, so that a wave's loads are contiguous in projections' outputs.
+template <int D, bool F16>
+__global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedAppendParams p) {
+  constexpr int LPR = D / 16;
+  const int heads = p.H + 2 * p.Hkv;
+  const int64_t unit = (int64_t)blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
+  const int d = 8 * (threadIdx.x % LPR);
+  if (unit >= (int64_t)p.B * p.T * heads) return;
+  const int64_t token = unit / heads;
+  const int head = (int)(unit - token * heads), b = (int)(token / p.T), j = (int)(token - (int64_t)b * p.T);
+  const bool is_q = head < p.H, is_k = !is_q && head < p.H + p.Hkv;
+  const uint16_t* src;
+  uint16_t* dst;
+  if (is_q) {
+    src = p.q + b * p.sq0 + head * p.sq1 + j * p.sq2;
+    dst = p.qout + b * p.so0 + head * p.so1 + j * p.so2;
+  } else {
+    const Sequence s = sequence(p.c, p.T, b);
+    const int row = s.first + j;
+    if (j >= s.fresh || row < 0 || row >= s.cap) return;
+    const int page = page_of(p.c, b, row);
+    if (page < 0) return;
+    const int in = row & ((1 << p.c.page_log2) - 1);
+    if (is_k) {
+      const int g = head - p.H;
+      src = p.k + b * p.sk0 + g * p.sk1 + j * p.sk2;
+      dst = p.c.k + page * p.c.skp + g * p.c.skh + in * p.c.skr;
+    } else {
+      const int g = head - p.H - p.Hkv;
+      src = p.v + b * p.sv0 + g * p.sv1 + j * p.sv2;
+      dst = p.c.v + page * p.c.svp + g * p.c.svh + in * p.c.svr;
+    }
+  }
+  u32x4_t x = ld16(src + d), y = ld16(src + d + D / 2);
+  if ((is_q || is_k) && p.r.cos) {
+    Turn t;
+    load_turn<F16>(p.r, b * p.r.s0 + j * p.r.s1 + d, D, t);
+    rotate<F16>(x, y, t);
+  }
+  st16(dst + d, x);
+  st16(dst + d + D / 2, y);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// How a call's work is cut. A pair is (sequence, tile of VT query vectors of a KV head; vector v = token v / G, head v % G);
+// its keys, the rows that its last real token attends, are cut into equal splits of whole units so that all splits of the
+// call are about as long: `share` units, the call's total over p.target workgroups, at least p.min_share. Each workgroup
+// finds its (pair, KV head, split) by a scan over the pairs, so lengths may stay on the device and the grid goes by the
+// capacity alone. Pairs with one split write the output, the others a partial for the merge.
+BB_DEV int wave_scan(int v) {  // inclusive sum over the lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+BB_DEV int lane_int(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+BB_DEV int udiv_up(int a, int b) { return (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b); }
+
+struct Item {
+  bool live;
+  int b, tile, g, split, splits, slot, units;
+};
+BB_DEV int pair_tile(const PagedAttnParams& p, int pair) { return p.tiles - 1 - pair % p.tiles; }  // the longest first
+// Rows that the pair's last real token attends (0: none of its tokens is real, or has rows).
+BB_DEV int pair_keys(const PagedAttnParams& p, const Sequence& s, int tile) {
+  const int j0 = tile * p.VT / p.G;
+  int j1 = (tile * p.VT + p.VT - 1) / p.G;
+  if (j1 >= s.fresh) j1 = s.fresh - 1;
+  return j1 < j0 ? 0 : s.seen(j1);
+}
+BB_DEV int pair_units(const PagedAttnParams& p, int pair) {
+  if (pair >= p.pairs) return 0;
+  const int k = pair_keys(p, sequence(p.c, p.T, pair / p.tiles), pair_tile(p, pair));
+  return k > 0 ? udiv_up(k, p.unit) : 1;
+}
+BB_DEV int share_of(const PagedAttnParams& p, int total) {
+  const int s = udiv_up(total * p.Hkv, p.target);
+  return s > p.min_share ? s : p.min_share;
+}
+// Walks the pairs (by a whole wave) to the first whose items reach past `item`, or with `item` < 0 to pair `pair`.
+struct PairPlan {
+  int pair, units, splits, slot, before;  // pair -1: no such item; slot: of KV head 0's first split; before: items of earlier pairs
+};
+BB_DEV PairPlan walk_pairs(const PagedAttnParams& p, int item, int pair, int lane) {
+  int first = 0, total = 0;
+  for (int at = 0; at < p.pairs; at += 64) {
+    const int u = pair_units(p, at + lane);
+    if (at == 0) first = u;
+    total += lane_int(wave_scan(u), 63);
+  }
+  const int share = share_of(p, total);
+  int items = 0, slots = 0;
+  for (int at = 0; at < p.pairs; at += 64) {
+    const int u = at == 0 ? first : pair_units(p, at + lane);
+    const int sp = udiv_up(u, share), mine = sp * p.Hkv, split = sp > 1 ? mine : 0;
+    const int upto = items + wave_scan(mine), slot_upto = slots + wave_scan(split);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(item < 0 ? at + lane == pair : item < upto);
+    if (in) {
+      const int l = __builtin_ctzll(in);
+      return PairPlan{at + l, lane_int(u, l), lane_int(sp, l), lane_int(slot_upto - split, l), lane_int(upto - mine, l)};
+    }
+    items = lane_int(upto, 63);
+    slots = lane_int(slot_upto, 63);
+  }
+  return PairPlan{-1, 0, 0, 0, 0};
+}
+BB_DEV PairPlan find_pair(const PagedAttnParams& p, int pair, int lane) { return walk_pairs(p, -1, pair, lane); }
+// The item with index `item`; not live where the call has fewer.
+BB_DEV Item find_item(const PagedAttnParams& p, int item, int lane) {
+  const PairPlan pl = walk_pairs(p, item, 0, lane);
+  const int rest = item - pl.before, g = rest % p.Hkv, split = rest / p.Hkv;
+  return Item{pl.pair >= 0, pl.pair / p.tiles, pair_tile(p, pl.pair), g, split, pl.splits, pl.slot + g * pl.splits + split, pl.units};
+}
+// First unit of split s of u units in n splits: equal parts.
+BB_DEV int split_begin(int u, int n, int s) { return (int)((int64_t)u * s / n); }
+
+// ---------------------------------------------------------------------------------------------------------------
+// Attention of up to 16 NR query vectors of a KV head over a split of a sequence's rows.
+template <bool F16>
+BB_DEV f32x4_t mma16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+// A value over the four lanes x, x + 16, x + 32, x + 48 of a query vector.
+BB_DEV float quarters_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return xhalf_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+BB_DEV float quarters_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return xhalf_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+BB_DEV void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+// Eight bytes of LDS per lane: of 16 lanes, lanes 4 r .. 4 r + 3 point at 16 elements of row r, and lane l gets column l,
+// row r in place r.
+BB_DEV u32x2_t read_tr16(const uint8_t* __restrict__ at) {
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)at));
+}
+
+// A chunk's rows in LDS, 16 by 16, 2 D bytes each: 16-byte piece c of row r is at place c ^ k_swz(r) of its row, so that a
+// fragment read (16 rows, one piece each of two neighbouring pieces) meets every bank once; V's swizzle keeps 32-byte
+// blocks whole and spreads the eight rows that half a wave's transposed read touches.
+template <int D>
+BB_DEV int k_swz(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
+template <int D>
+BB_DEV int v_swz(int r) { return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
+
+// One wave's stream of chunks of KC rows, 8 KB of K and of V.
+template <int D>
+struct PageStream {
+  static constexpr int KC = 4096 / D, GROUPS = KC / 16, LOADS = 8 / GROUPS;  // groups of 16 rows lie in one page
+  static constexpr int RPL = 512 / D;                                        // rows of a load
+  const PagedCache& c;
+  const_i32 table;
+  const uint16_t *kh, *vh;
+  uint32_t row, kpiece, vpiece;
+  int end;  // rows from here on are not read
+  BB_DEV PageStream(const PagedCache& c_, int b, int g, int end_, int lane) : c(c_), end(end_) {
+    table = (const_i32)(uintptr_t)(c.table + b * c.st);
+    kh = c.k + g * c.skh;
+    vh = c.v + g * c.svh;
+    row = lane / (D / 8);
+    kpiece = 16u * ((lane % (D / 8)) ^ k_swz<D>(row));
+    vpiece = 16u * ((lane % (D / 8)) ^ v_swz<D>(row));
+  }
+  // The table's entries for the chunk at row k0 (not looked at yet: they are on their way) and the page of group j of it (-1:
+  // none, or past the end).
+  BB_DEV void entries(int k0, int (&e)[GROUPS]) const {
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) {
+      const int w = (k0 + 16 * j) >> c.page_log2;
+      e[j] = table[w < c.W ? w : c.W - 1];
+    }
+  }
+  BB_DEV void settle(int k0, int (&e)[GROUPS]) const {
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) e[j] = k0 + 16 * j < end && (uint32_t)e[j] < (uint32_t)c.pages ? e[j] : -1;
+  }
+  // Always eight loads, so that the counts the waits go by are exact; rows past the end and of no page land zeros.
+  BB_DEV void fetch(bool is_v, uint8_t* to, int k0, const int (&e)[GROUPS]) const {
+    const int64_t sp = is_v ? c.svp : c.skp, sr = is_v ? c.svr : c.skr;
+    const uint32_t rb = (uint32_t)sr * 2;
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) {
+      const int r = k0 + 16 * j, left = end - r, live = e[j] < 0 ? 0 : left < 16 ? left : 16;
+      const int page = e[j] < 0 ? 0 : e[j];
+      const uint16_t* base = (is_v ? vh : kh) + page * sp + (r & ((1 << c.page_log2) - 1)) * sr;
+      const uint32_t bytes = live > 0 ? (live - 1) * rb + 2 * D : 0;
+      const __amdgpu_buffer_rsrc_t rs =
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)bytes, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const uint32_t piece = is_v ? vpiece ^ 16u * v_swz<D>(RPL * i) : kpiece ^ 16u * k_swz<D>(RPL * i);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs, reinterpret_cast<lds_void*>(reinterpret_cast<uintptr_t>(to + 1024 * (LOADS * j + i))), 16,
+            (row + RPL * i) * rb + piece, 0, 0, 2 /* non-temporal */);
+      }
+    }
+  }
+};
+
+// A step's new rows among the rows [k0, k0 + KC) of a wave's landed chunk: rotated, into the pages and into LDS over what the
+// pages held there. No other wave of the call reads these rows.
+template <int D, bool F16>
+BB_DEV void patch_new_rows(const PagedAttnParams& p, const Sequence& s, int b, int g, int k0, int lane, uint8_t* ks, uint8_t* vs) {
+  constexpr int KC = PageStream<D>::KC, LPR = D / 16;
+  const int d = 8 * (lane % LPR), c = lane % LPR;
+  for (int i = lane / LPR; i < 2 * s.fresh; i += 64 / LPR) {
+    const int j = i >> 1, row = s.first + j;
+    const bool is_v = i & 1;
+    if (row < k0 || row >= k0 + KC || row >= s.n) continue;
+    const int page = page_of(p.c, b, row);
+    if (page < 0) continue;
+    const int64_t in = row & ((1 << p.c.page_log2) - 1);
+    const uint16_t* src = is_v ? p.vnew + b * p.svn0 + g * p.svn1 + j * p.svn2 : p.knew + b * p.skn0 + g * p.skn1 + j * p.skn2;
+    uint16_t* dst = is_v ? p.c.v + page * p.c.svp + g * p.c.svh + in * p.c.svr : p.c.k + page * p.c.skp + g * p.c.skh + in * p.c.skr;
+    u32x4_t x = ld16(src + d), y = ld16(src + d + D / 2);
+    if (!is_v && p.r.cos) {
+      Turn t;
+      load_turn<F16>(p.r, b * p.r.s0 + j * p.r.s1 + d, D, t);
+      rotate<F16>(x, y, t);
+    }
+    st16(dst + d, x);
+    st16(dst + d + D / 2, y);
+    const int r = row - k0, z = is_v ? v_swz<D>(r & 15) : k_swz<D>(r & 15);
+    uint8_t* to = (is_v ? vs : ks) + r * 2 * D;
+    st16(to + 16 * (c ^ z), x);
+    st16(to + 16 * ((c + LPR) ^ z), y);
+  }
+}
+
+// A state's maximum is -inf where no row was attended, and kLowest where all scores were -inf or NaN: zeros are for the
+// former only, the latter's sums of 0 or NaN make the quotient NaN, as its softmax is.
+constexpr float kLowest = -3.4028234663852886e38f;
+template <bool F16>
+BB_DEV void store_output(const PagedAttnParams& p, int b, int g, int v, int d, f32x4_t O, float M, float L) {
+  const int j = v / p.G, h = g * p.G + v - j * p.G;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) O[k] = M == -kInf ? 0.0f : O[k] / L;
+  *reinterpret_cast<u32x2_t*>(p.out + b * p.so0 + h * p.so1 + j * p.so2 + d) =
+      u32x2_t{pack2<F16>(O[0], O[1]), pack2<F16>(O[2], O[3])};
+}
+
+// Values of V that are not finite, in a chunk that some vectors attend in part: a probability of 0 times an infinity would be
+// NaN. They are taken out of the operand, and a vector that attends one is NaN in that column.
+template <bool F16>
+BB_DEV uint32_t not_finite(uint32_t w) {  // 0xffff in the halves that are not
+  constexpr uint32_t e = F16 ? 0x7c00u : 0x7f80u;
+  return ((w & e) == e ? 0xffffu : 0u) | ((w >> 16 & e) == e ? 0xffff0000u : 0u);
+}
+
+template <int D, bool F16, int NR, bool NEW>
+__global__ __launch_bounds__(kThreads, NR > 1 && NEW ? 1 : 2) void paged_attn_kernel(PagedAttnParams p) {
+  using Stream = PageStream<D>;
+  constexpr int KC = Stream::KC, GROUPS = Stream::GROUPS, NDS = D / 32, NDB = D / 16;
+  constexpr int ROW = D + 4;  // floats of a state's row: whole 16-byte pieces, rows on other banks
+  __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][8192];
+  const int tid = threadIdx.x, lane = tid & 63, x = lane & 15, a = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Item it = find_item(p, blockIdx.x, lane);
+  if (!it.live) return;
+  const Sequence s = sequence(p.c, p.T, it.b);
+  const int keys = __builtin_amdgcn_readfirstlane(pair_keys(p, s, it.tile));
+  const int u0 = split_begin(it.units, it.splits, it.split), u1 = split_begin(it.units, it.splits, it.split + 1);
+  int begin = u0 * p.unit, end = u1 * p.unit < keys ? u1 * p.unit : keys;
+  begin = __builtin_amdgcn_readfirstlane(begin);
+  end = __builtin_amdgcn_readfirstlane(end);
+  const int v0 = it.tile * p.VT;
+  const int R = p.T * p.G - v0 < p.VT ? p.T * p.G - v0 : p.VT;
+
+  const Stream in(p.c, it.b, it.g, end, lane);
+  uint8_t *ks = sm[wave][0], *vs = sm[wave][1];
+  int k0 = begin + wave * KC;
+  int e[GROUPS], ne[GROUPS];
+  in.entries(k0, e);
+  // Q fragments: B operand of S^T = K Q^T, lane (x, a): dims 32 ds + 8 a .. of vector 16 r + x. Their loads go out before the
+  // first chunk's, which they then need not wait for.
+  u32x4_t qw[NR][NDS];
+  int lim[NR], tok[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int v = 16 * r + x < R ? v0 + 16 * r + x : v0, j = v / p.G, h = it.g * p.G + v - j * p.G;
+    tok[r] = j;
+    lim[r] = 16 * r + x < R ? s.seen(j) : 0;
+    const uint16_t* qr = p.q + it.b * p.sq0 + h * p.sq1 + j * p.sq2 + 8 * a;
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) qw[r][ds] = ld16(qr + 32 * ds);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  in.settle(k0, e);
+  in.fetch(false, ks, k0, e);
+  in.fetch(true, vs, k0, e);
+#pragma unroll
+  for (int r = 0; r < NR; ++r)
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) asm volatile("" : "+v"(qw[r][ds]));  // awaited here, not with the chunk before the loop
+  // with new rows the rotated query is kept in two terms, as exact as fp32 products of it need
+  constexpr int QT = NEW ? 2 : 1;
+  bf16x8_t qf[NR][NDS][QT];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) {
+      qf[r][ds][0] = as_bf16x8(qw[r][ds]);
+      if constexpr (NEW) qf[r][ds][1] = as_bf16x8(u32x4_t{0, 0, 0, 0});
+    }
+    if constexpr (NEW) {
+      if (p.r.cos) {
+#pragma unroll
+        for (int ds = 0; ds < NDS / 2; ++ds) {
+          Turn t;
+          float x0[8], x1[8];
+          u32x4_t w[4];
+          load_turn<F16>(p.r, it.b * p.r.s0 + tok[r] * p.r.s1 + 32 * ds + 8 * a, D, t);
+          rotate<F16>(qw[r][ds], qw[r][ds + NDS / 2], t, x0, x1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const u32x2_t lo = two_terms<F16>(x0[2 * i], x0[2 * i + 1]), hi = two_terms<F16>(x1[2 * i], x1[2 * i + 1]);
+            w[0][i] = lo[0];
+            w[1][i] = lo[1];
+            w[2][i] = hi[0];
+            w[3][i] = hi[1];
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            qf[r][ds][i] = as_bf16x8(w[i]);
+            qf[r][ds + NDS / 2][i] = as_bf16x8(w[2 + i]);
+          }
+        }
+      }
+    }
+  }
+  // the fewest rows that a token of the tile attends: chunks below need no mask (what padding gets there is not stored)
+  const int fewest = __builtin_amdgcn_readfirstlane(s.seen(v0 / p.G));
+
+  float m[NR], l[NR];
+  bool seen[NR];
+  f32x4_t o[NR][NDB];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    m[r] = -kInf;
+    l[r] = 0.0f;
+    seen[r] = false;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) o[r][db] = f32x4_t{0, 0, 0, 0};
+  }
+  uint32_t kread[NDS], vread[2];  // fragment reads: key block kb is 32 D kb bytes on (both swizzles repeat every 16 rows)
+#pragma unroll
+  for (int ds = 0; ds < NDS; ++ds) kread[ds] = 2 * D * x + 16 * ((4 * ds + a) ^ k_swz<D>(x));
+  const int vrow = 4 * a + (x >> 2);  // of 16: the lane's row and 8-byte piece x & 3 of a 32-byte block
+
+  for (; k0 < end; k0 += kWaves * KC) {
+    in.entries(k0 + kWaves * KC, ne);
+    __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8): this chunk's K has landed, its V may be in flight
+    wave_fence();
+    if (NEW && k0 + KC > s.first && k0 < s.n) {
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // V too
+      wave_fence();
+      patch_new_rows<D, F16>(p, s, it.b, it.g, k0, lane, ks, vs);
+      __builtin_amdgcn_s_waitcnt(0x0070);  // all done: the counts below hold
+      wave_fence();
+    }
+    f32x4_t y[NR][KC / 16];
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int kb = 0; kb < KC / 16; ++kb) y[r][kb] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds)
+#pragma unroll
+      for (int kb = 0; kb < KC / 16; ++kb) {
+        const bf16x8_t kf = as_bf16x8(*reinterpret_cast<const u32x4_t*>(ks + kread[ds] + 32 * D * kb));
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int t = 0; t < QT; ++t) y[r][kb] = mma16<F16>(kf, qf[r][ds][t], y[r][kb]);
+      }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): K is read, its space is free
+    wave_fence();
+    __builtin_amdgcn_sched_barrier(0);  // (the table's entries are wanted from here on, not before the products)
+    in.settle(k0 + kWaves * KC, ne);
+    in.fetch(false, ks, k0 + kWaves * KC, ne);
+
+    bool whole = k0 + KC <= fewest;
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) whole = whole && e[j] >= 0;
+    bf16x8_t pf[NR][KC / 32][2];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+#pragma unroll
+      for (int kb = 0; kb < KC / 16; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[r][kb][i] *= p.scale;
+      if (whole) {
+        seen[r] = true;
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < KC / 16; ++kb) {
+          seen[r] = seen[r] || (e[kb] >= 0 && k0 + 16 * kb < lim[r]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (e[kb] < 0 || k0 + 16 * kb + 4 * a + i >= lim[r]) y[r][kb][i] = -kInf;
+        }
+      }
+      float mx = y[r][0][0];
+#pragma unroll
+      for (int kb = 0; kb < KC / 16; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, y[r][kb][i]);
+      const float mn = fmaxf(m[r], quarters_max(mx));
+      if (__builtin_amdgcn_ballot_w64(mn > m[r])) {
+        const float alpha = mn > m[r] ? fast_exp2(m[r] - mn) : 1.0f;
+        m[r] = mn;
+        l[r] *= alpha;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[r][db][i] *= alpha;
+      }
+      const float off = m[r] == -kInf ? 0.0f : m[r];
+#pragma unroll
+      for (int st = 0; st < KC / 32; ++st) {
+        float pr[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          pr[i] = fast_exp2(y[r][2 * st + i / 4][i % 4] - off);
+          l[r] += pr[i];
+        }
+        // in two terms: with one, the probabilities' rounding would be as large as the output's own, which is all the error that
+        // there is otherwise (and the matrix cores idle here)
+        u32x4_t hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const u32x2_t t = two_terms<F16>(pr[2 * i], pr[2 * i + 1]);
+          hi[i] = t[0];
+          lo[i] = t[1];
+        }
+        pf[r][st][0] = as_bf16x8(hi);
+        pf[r][st][1] = as_bf16x8(lo);
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8): this chunk's V has landed, the next K may be in flight
+    wave_fence();
+    const auto values = [&](auto part) {
+#pragma unroll
+      for (int st = 0; st < KC / 32; ++st)
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const uint32_t at = 2 * D * vrow + 16 * ((2 * db + ((x >> 1) & 1)) ^ v_swz<D>(vrow)) + 8 * (x & 1);
+          const u32x2_t w0 = read_tr16(vs + 64 * D * st + at), w1 = read_tr16(vs + 64 * D * st + 32 * D + at);
+          u32x4_t vw = {w0[0], w0[1], w1[0], w1[1]};
+          if constexpr (decltype(part)::value) {
+            u32x4_t bad;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              bad[i] = not_finite<F16>(vw[i]);
+              vw[i] &= ~bad[i];
+            }
+            if (__builtin_amdgcn_ballot_w64((bad[0] | bad[1] | bad[2] | bad[3]) != 0)) {
+              constexpr uint32_t one = F16 ? 0x3c003c00u : 0x3f803f80u;
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                u32x4_t att;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int kb = 2 * st + i / 2, key = k0 + 16 * kb + 4 * a + 2 * (i % 2);
+                  att[i] = e[kb] < 0 ? 0u : (key < lim[r] ? one & 0xffffu : 0u) | (key + 1 < lim[r] ? one & 0xffff0000u : 0u);
+                }
+                const f32x4_t hits = mma16<F16>(as_bf16x8(u32x4_t{bad[0] & one, bad[1] & one, bad[2] & one, bad[3] & one}),
+                                                as_bf16x8(att), f32x4_t{0, 0, 0, 0});
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (hits[i] > 0.0f) o[r][db][i] = __builtin_nanf("");
+              }
+            }
+          }
+          const bf16x8_t vf = as_bf16x8(vw);
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) o[r][db] = mma16<F16>(vf, pf[r][st][t], o[r][db]);
+        }
+    };
+    if (whole) values(Constant<false>{});
+    else values(Constant<true>{});
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    wave_fence();
+    in.fetch(true, vs, k0 + kWaves * KC, ne);
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) e[j] = ne[j];
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // nothing lands in LDS any more
+
+  // The four waves' states under one maximum.
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    __syncthreads();
+    float* f = reinterpret_cast<float*>(&sm[0][0][0]) + (wave * 16 + x) * ROW;
+    const float ls = quarters_sum(l[r]);
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) *reinterpret_cast<f32x4_t*>(f + 16 * db + 4 * a) = o[r][db];
+    if (a == 0) {
+      f[D] = !seen[r] || lim[r] <= 0 ? -kInf : m[r] == -kInf ? kLowest : m[r];
+      f[D + 1] = ls;
+    }
+    __syncthreads();
+    for (int i = tid; i < 16 * (D / 4); i += kThreads) {
+      const int vv = 16 * r + i / (D / 4), d = 4 * (i % (D / 4));
+      if (vv >= R) continue;
+      const float* g = reinterpret_cast<const float*>(&sm[0][0][0]) + (i / (D / 4)) * ROW;
+      float M = -kInf, L = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) M = fmaxf(M, g[w * 16 * ROW + D]);
+      const float off = M == -kInf ? 0.0f : M;
+      f32x4_t O = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float* f = g + w * 16 * ROW;
+        const float wt = fast_exp2(f[D] - off);
+        const f32x4_t t = *reinterpret_cast<const f32x4_t*>(f + d);
+        L = fmaf(wt, f[D + 1], L);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) O[k] = fmaf(wt, t[k], O[k]);
+      }
+      if (it.splits == 1) {
+        store_output<F16>(p, it.b, it.g, v0 + vv, d, O, M, L);
+      } else {
+        float* dst = p.part + ((int64_t)it.slot * p.VT + vv) * ROW;
+        *reinterpret_cast<f32x4_t*>(dst + d) = O;
+        if (d == 0) {
+          dst[D] = M;
+          dst[D + 1] = L;
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Attention of many query vectors (prompts and their chunks): bound by the matrix cores, so a workgroup's 8 waves share every
+// K and V tile of 64 rows, 32 vectors each (two blocks of 16, so that every fragment read from LDS feeds two products).
+//   * Waves w and w + 4 share a SIMD and run half a tile apart: while one does products (O^T += V^T P^T of the tile before,
+//     then S^T = K Q^T), the other does its softmax, with workgroup barriers in between.
+//   * Tiles stream through a ring of four stages by 16-byte loads into LDS, issued two tiles ahead; each load's rows lie in one
+//     page, whose table entry came by a scalar load a tile earlier.
+//   * S^T leaves keys 16 kb + 4 a + i of vector x in lane (x, a), which is the order in which two transposed reads bring V's
+//     rows, so the probabilities are operands where they are.
+//   * The exponent's offset moves only when a probability would pass 2^8. Tiles that some vector attends in part, and every tile
+//     of a split whose table names no page somewhere, run after the others in a loop of their own with the mask.
+constexpr int kTileWaves = 8, kTileStages = 4, kTileVecs = 32 * kTileWaves, kTileRows = 64;
+constexpr float kOver = 256.0f;  // 2^8
+
+template <int D>
+struct TileLds {
+  static constexpr int BYTES = kTileRows * D * 2;         // of a K or V tile
+  static constexpr int LOADS = BYTES / 1024 / kTileWaves;  // of a wave: 2 or 1
+  static constexpr int RPL = 512 / D;                      // rows of a load
+};
+
+template <int D>
+struct TileLoader {
+  using L = TileLds<D>;
+  const PagedCache& c;
+  const_i32 table;
+  const uint16_t *kh, *vh;
+  uint32_t koff[L::LOADS], voff[L::LOADS];
+  int row0, end;  // first row of the wave's first load in a tile; rows from `end` on are not read
+  BB_DEV TileLoader(const PagedCache& c_, int b, int g, int end_, int wave, int lane) : c(c_), end(end_) {
+    table = (const_i32)(uintptr_t)(c.table + b * c.st);
+    kh = c.k + g * c.skh;
+    vh = c.v + g * c.svh;
+    row0 = L::RPL * wave;
+    const int row = lane / (D / 8), piece = lane % (D / 8);
+#pragma unroll
+    for (int i = 0; i < L::LOADS; ++i) {
+      const int r = row0 + row + L::RPL * kTileWaves * i;
+      koff[i] = row * (uint32_t)c.skr * 2 + 16 * (piece ^ k_swz<D>(r & 15));
+      voff[i] = row * (uint32_t)c.svr * 2 + 16 * (piece ^ v_swz<D>(r & 15));
+    }
+  }
+  BB_DEV int entry(int r) const {  // of row r's page
+    const int w = r >> c.page_log2;
+    return table[w < c.W ? w : c.W - 1];
+  }
+  struct Entries {
+    int e[L::LOADS];
+  };
+  BB_DEV Entries entries(int k0) const {
+    Entries x;
+#pragma unroll
+    for (int i = 0; i < L::LOADS; ++i) x.e[i] = entry(k0 + row0 + L::RPL * kTileWaves * i);
+    return x;
+  }
+  BB_DEV void load(uint8_t* kt, int wave, int k0, const Entries& x) const {
+    uint8_t* vt = kt + L::BYTES;
+#pragma unroll
+    for (int i = 0; i < L::LOADS; ++i) {
+      const int r = k0 + row0 + L::RPL * kTileWaves * i, left = end - r;
+      const bool mapped = (uint32_t)x.e[i] < (uint32_t)c.pages;
+      const int page = mapped ? x.e[i] : 0, in = r & ((1 << c.page_log2) - 1);
+      const int live = !mapped || left < 0 ? 0 : left < L::RPL ? left : L::RPL;
+      rows(kh + page * c.skp + in * c.skr, live, (uint32_t)c.skr * 2, kt + 1024 * (wave + kTileWaves * i), koff[i]);
+      rows(vh + page * c.svp + in * c.svr, live, (uint32_t)c.svr * 2, vt + 1024 * (wave + kTileWaves * i), voff[i]);
+    }
+  }
+  BB_DEV static void rows(const uint16_t* base, int live, uint32_t row_bytes, uint8_t* to, uint32_t off) {
+    const uint32_t bytes = live > 0 ? (live - 1) * row_bytes + 2 * D : 0;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)bytes, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, reinterpret_cast<lds_void*>(reinterpret_cast<uintptr_t>(to)), 16, off, 0, 0, 0);
+  }
+};
+
+// Workgroup barrier that does not drain the loads in flight (the ring publishes them by explicit vmcnt waits); nothing moves
+// across it.
+BB_DEV void ring_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+BB_DEV uint32_t lds_addr(const void* p) {
+  return (uint32_t)reinterpret_cast<uintptr_t>(
+      reinterpret_cast<__attribute__((address_space(3))) const void*>(reinterpret_cast<uintptr_t>(p)));
+}
+BB_DEV u32x4_t lds16(uint32_t at) { return *(const __attribute__((address_space(3))) u32x4_t*)(uintptr_t)at; }
+BB_DEV u32x2_t lds_tr16(uint32_t at) {
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(uintptr_t)at));
+}
+
+template <int D>
+struct TileState {
+  bf16x8_t qf[2][D / 32];  // Q^T: vector block rb, 32 dims
+  f32x4_t o[D / 16][2];    // O^T: dims 16 db + 4 a + i of vector 16 rb + x
+  f32x4_t s[4][2];         // S^T of the current tile: keys 16 kb + 4 a + i
+  bf16x8_t pk[2][2];       // P^T of the tile before: its 32-key halves
+  float m[2], l[2];        // exponent's offset; this lane's share of the sum
+};
+
+// Fragment i of a phase: i < D / 8 V's of (half st, block db), then K's of (32 dims ds, key block kb).
+template <int D>
+struct TileReads {
+  uint32_t k[D / 32], v[D / 16];
+};
+template <int D>
+BB_DEV u32x4_t tile_fragment(const TileReads<D>& rd, uint32_t kt, uint32_t vt, int i) {
+  if (i < D / 8) {
+    const int st = i / (D / 16), db = i % (D / 16);
+    const uint32_t at = vt + rd.v[db] + 64 * D * st;
+    const u32x2_t a = lds_tr16(at), b = lds_tr16(at + 32 * D);
+    return u32x4_t{a[0], a[1], b[0], b[1]};
+  }
+  const int j = i - D / 8, kb = j % 4, ds = j / 4;
+  return lds16(kt + rd.k[ds] + 32 * D * kb);
+}
+template <bool F16, int D>
+BB_DEV void tile_product(TileState<D>& t, int i, bf16x8_t f) {
+  if (i < D / 8) {
+    const int st = i / (D / 16), db = i % (D / 16);
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) t.o[db][rb] = mma16<F16>(f, t.pk[st][rb], t.o[db][rb]);
+  } else {
+    const int j = i - D / 8, kb = j % 4, ds = j / 4;
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) t.s[kb][rb] = mma16<F16>(f, t.qf[rb][ds], ds ? t.s[kb][rb] : f32x4_t{0, 0, 0, 0});
+  }
+}
+// Products of fragments FROM .. TO - 1, their reads kRing ahead.
+template <bool F16, int D, int FROM, int TO>
+BB_DEV void tile_products(TileState<D>& t, const TileReads<D>& rd, uint32_t kt, uint32_t vt) {
+  constexpr int kRing = 6;
+  u32x4_t ring[kRing];
+#pragma unroll
+  for (int i = 0; i < kRing; ++i) ring[i] = tile_fragment<D>(rd, kt, vt, FROM + i);
+#pragma unroll
+  for (int i = FROM; i < TO; ++i) {
+    tile_product<F16, D>(t, i, as_bf16x8(ring[(i - FROM) % kRing]));
+    if (i + kRing < TO) ring[(i - FROM) % kRing] = tile_fragment<D>(rd, kt, vt, i + kRing);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// P = 2^(S c - m) in 16 bits; sum: this lane's part of the row sums. (One term: its rounding is as large as the output's own;
+// a second would cost half of the products again.)
+template <bool F16, int D>
+BB_DEV void tile_exp(TileState<D>& t, float c, float (&sum)[2]) {
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb) {
+    const float nm = -t.m[rb];
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = fast_exp2(fmaf(t.s[2 * st + e / 4][rb][e % 4], c, nm));
+        sum[rb] = st == 0 && e == 0 ? p[e] : sum[rb] + p[e];
+      }
+      t.pk[st][rb] = as_bf16x8(u32x4_t{pack2<F16>(p[0], p[1]), pack2<F16>(p[2], p[3]), pack2<F16>(p[4], p[5]), pack2<F16>(p[6], p[7])});
+    }
+  }
+}
+template <int D>
+BB_DEV float tile_max(const TileState<D>& t, int rb, float c) {
+  float mx = t.s[0][rb][0];
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, t.s[kb][rb][i]);
+  return quarters_max(mx) * c;
+}
+template <int D>
+BB_DEV void tile_rescale(TileState<D>& t, int rb, float mt) {
+  const float mn = fmaxf(t.m[rb], mt), alpha = fast_exp2(t.m[rb] - mn);
+  t.m[rb] = mn;
+  t.l[rb] *= alpha;
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.o[db][rb][i] *= alpha;
+}
+// Softmax of a tile: exponentiated against the offset as it is, and again where that was too low.
+template <bool F16, int D>
+BB_DEV void tile_softmax(TileState<D>& t, float c) {
+  float sum[2];
+  tile_exp<F16, D>(t, c, sum);
+  const bool over0 = !(sum[0] <= kOver), over1 = !(sum[1] <= kOver);
+  if (__builtin_amdgcn_ballot_w64(over0 || over1)) {
+    tile_rescale<D>(t, 0, tile_max<D>(t, 0, c));
+    tile_rescale<D>(t, 1, tile_max<D>(t, 1, c));
+    tile_exp<F16, D>(t, c, sum);
+  }
+  t.l[0] += sum[0];
+  t.l[1] += sum[1];
+}
+
+template <int D, bool F16>
+__global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAttnParams p) {
+  using L = TileLds<D>;
+  constexpr int STAGE = 2 * L::BYTES, NV = D / 8, NF = D / 4, ROW = D + 4;
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[kTileStages * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, x = lane & 15, a = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), late = wave >> 2;  // waves w and w + 4 share a SIMD
+  const Item it = find_item(p, blockIdx.x, lane);
+  if (!it.live) return;
+  const Sequence s = sequence(p.c, p.T, it.b);
+  const int keys = __builtin_amdgcn_readfirstlane(pair_keys(p, s, it.tile));
+  const int u0 = __builtin_amdgcn_readfirstlane(split_begin(it.units, it.splits, it.split));
+  const int u1 = __builtin_amdgcn_readfirstlane(split_begin(it.units, it.splits, it.split + 1));
+  const int begin = u0 * kTileRows, end = u1 * kTileRows < keys ? u1 * kTileRows : keys;
+  const int v0 = it.tile * kTileVecs;
+  const int R = p.T * p.G - v0 < kTileVecs ? p.T * p.G - v0 : kTileVecs;
+
+  TileState<D> t;
+  int lim[2];
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb) {
+    const int i = 32 * wave + 16 * rb + x, v = i < R ? v0 + i : v0, j = v / p.G, h = it.g * p.G + v - j * p.G;
+    lim[rb] = i < R ? s.seen(j) : 0;
+    const uint16_t* qr = p.q + it.b * p.sq0 + h * p.sq1 + j * p.sq2 + 8 * a;
+#pragma unroll
+    for (int ds = 0; ds < D / 32; ++ds) t.qf[rb][ds] = as_bf16x8(ld16(qr + 32 * ds));
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) t.o[db][rb] = f32x4_t{0, 0, 0, 0};
+    t.m[rb] = kLowest;
+    t.l[rb] = 0.0f;
+  }
+  const TileLoader<D> in(p.c, it.b, it.g, end, wave, lane);
+  // Tiles without a mask: below the rows that the tile's first token attends, if the table names a page for all of the split.
+  // (What padding gets there is not stored.)
+  const int n_tiles = end > begin ? (end - begin + kTileRows - 1) / kTileRows : 0;
+  int open = __builtin_amdgcn_readfirstlane(s.seen(v0 / p.G)) - begin;
+  open = open < 0 ? 0 : open / kTileRows < n_tiles ? open / kTileRows : n_tiles;
+  bool hole = false;
+  for (int w = (begin >> p.c.page_log2) + lane; begin < end && w <= (end - 1) >> p.c.page_log2; w += 64)
+    hole = hole || (uint32_t)p.c.table[it.b * p.c.st + w] >= (uint32_t)p.c.pages;
+  if (__builtin_amdgcn_ballot_w64(hole)) open = 0;
+
+  TileReads<D> rd;
+  const int vrow = 4 * a + (x >> 2);
+#pragma unroll
+  for (int ds = 0; ds < D / 32; ++ds) rd.k[ds] = 2 * D * x + 16 * ((4 * ds + a) ^ k_swz<D>(x));
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db) rd.v[db] = 2 * D * vrow + 16 * ((2 * db + ((x >> 1) & 1)) ^ v_swz<D>(vrow)) + 8 * (x & 1);
+
+  auto stage = [&](int i) { return ring + (i & (kTileStages - 1)) * STAGE; };
+  auto fetch = [&](int i, const typename TileLoader<D>::Entries& e) { in.load(stage(i), wave, begin + kTileRows * i, e); };
+  auto entries = [&](int i) { return in.entries(begin + kTileRows * i); };
+  auto wait_tile = [&](bool one_in_flight) {  // all but the youngest tile's loads (all, without one in flight)
+    if (one_in_flight) __builtin_amdgcn_s_waitcnt(0x0F70 | 2 * L::LOADS);
+    else __builtin_amdgcn_s_waitcnt(0x0F70);
+  };
+  bool seen[2] = {open > 0, open > 0};
+  // The mask of tile i, and its softmax.
+  auto masked = [&](int i) {
+    const int k0 = begin + kTileRows * i;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      const bool mapped = k0 + 16 * kb < end && (uint32_t)in.entry(k0 + 16 * kb) < (uint32_t)p.c.pages;
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        seen[rb] = seen[rb] || (mapped && k0 + 16 * kb < lim[rb]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!mapped || k0 + 16 * kb + 4 * a + e >= lim[rb]) t.s[kb][rb][e] = -kInf;
+      }
+    }
+    tile_softmax<F16, D>(t, p.scale);
+  };
+  // Products of V's tile i that vectors attend in part: values that are not finite apart, as in the kernel above.
+  auto masked_values = [&](int i) {
+    const int k0 = begin + kTileRows * i;
+    const uint32_t vt = lds_addr(stage(i) + L::BYTES);
+#pragma unroll
+    for (int f = 0; f < NV; ++f) {
+      u32x4_t w = tile_fragment<D>(rd, 0, vt, f);
+      u32x4_t bad;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        bad[e] = not_finite<F16>(w[e]);
+        w[e] &= ~bad[e];
+      }
+      if (__builtin_amdgcn_ballot_w64((bad[0] | bad[1] | bad[2] | bad[3]) != 0)) {
+        constexpr uint32_t one = F16 ? 0x3c003c00u : 0x3f803f80u;
+        const int st = f / (D / 16), db = f % (D / 16);
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+          u32x4_t att;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = k0 + 32 * st + 16 * (e / 2) + 4 * a + 2 * (e % 2);
+            att[e] = (key < lim[rb] ? one & 0xffffu : 0u) | (key + 1 < lim[rb] ? one & 0xffff0000u : 0u);
+          }
+          const f32x4_t hits = mma16<F16>(as_bf16x8(u32x4_t{bad[0] & one, bad[1] & one, bad[2] & one, bad[3] & one}),
+                                          as_bf16x8(att), f32x4_t{0, 0, 0, 0});
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (hits[e] > 0.0f) t.o[db][rb][e] = __builtin_nanf("");
+        }
+      }
+      tile_product<F16, D>(t, f, as_bf16x8(w));
+    }
+  };
+
+  if (n_tiles > 0) {
+    typename TileLoader<D>::Entries e = entries(0);
+    fetch(0, e);
+    e = entries(1);
+    if (n_tiles > 1) fetch(1, e);
+    e = entries(2);
+    wait_tile(n_tiles > 1);
+    ring_barrier();
+    if (late) ring_barrier();  // the second group runs one phase behind
+    if (n_tiles > 2) fetch(2, e);
+    e = entries(3);
+    tile_products<F16, D, NV, NF>(t, rd, lds_addr(stage(0)), 0);
+    wait_tile(n_tiles > 2);
+    ring_barrier();
+    if (open > 0) tile_softmax<F16, D>(t, p.scale);
+    else masked(0);
+    ring_barrier();
+    for (int i = 1; i < open; ++i) {
+      __builtin_amdgcn_s_setprio(1);
+      tile_products<F16, D, 0, NF>(t, rd, lds_addr(stage(i)), lds_addr(stage(i - 1) + L::BYTES));
+      __builtin_amdgcn_s_setprio(0);
+      wait_tile(false);  // tile i + 1 has landed
+      ring_barrier();
+      tile_softmax<F16, D>(t, p.scale);
+      // into the stage of tile i - 2, which every wave has read
+      if (i + 2 < n_tiles) fetch(i + 2, e);
+      e = entries(i + 3);
+      ring_barrier();
+    }
+#pragma unroll 1
+    for (int i = open > 1 ? open : 1; i < n_tiles; ++i) {
+      masked_values(i - 1);
+      tile_products<F16, D, NV, NF>(t, rd, lds_addr(stage(i)), 0);
+      wait_tile(false);
+      ring_barrier();
+      masked(i);
+      if (i + 2 < n_tiles) fetch(i + 2, e);
+      e = entries(i + 3);
+      ring_barrier();
+    }
+    masked_values(n_tiles - 1);
+    if (!late) ring_barrier();  // the groups meet again
+  }
+
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb) {
+    const int i = 32 * wave + 16 * rb + x;
+    const float l = quarters_sum(t.l[rb]);
+    if (i >= R) continue;
+    if (it.splits == 1) {
+      const int v = v0 + i, j = v / p.G, h = it.g * p.G + v - j * p.G;
+      uint16_t* to = p.out + it.b * p.so0 + h * p.so1 + j * p.so2 + 4 * a;
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) {
+        f32x4_t o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = lim[rb] > 0 && seen[rb] ? t.o[db][rb][e] / l : 0.0f;
+        *reinterpret_cast<u32x2_t*>(to + 16 * db) = u32x2_t{pack2<F16>(o[0], o[1]), pack2<F16>(o[2], o[3])};
+      }
+    } else {
+      float* to = p.part + ((int64_t)it.slot * kTileVecs + i) * ROW;
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f32x4_t*>(to + 16 * db + 4 * a) = t.o[db][rb];
+      if (a == 0) {
+        to[D] = lim[rb] > 0 && seen[rb] ? t.m[rb] : -kInf;
+        to[D + 1] = l;
+      }
+    }
+  }
+}
+
+// The splits' states of a vector under one maximum. A workgroup merges p.merge_vecs vectors of a pair, its quarter or eighth
+// waves one split each in turn.
+template <int D, bool F16>
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttnParams p) {
+  constexpr int LPV = D / 4, NG = kThreads / LPV, ROW = D + 4;
+  __shared__ float st[NG][ROW];
+  const int tid = threadIdx.x, lane = tid & 63, grp = tid / LPV, d = 4 * (tid % LPV);
+  const int per_tile = p.VT / p.merge_vecs, b = blockIdx.z, g = blockIdx.y, tile = blockIdx.x / per_tile;
+  const int first = tile * p.VT + (blockIdx.x % per_tile) * p.merge_vecs;
+  if (first >= p.T * p.G) return;
+  const PairPlan pl = find_pair(p, b * p.tiles + p.tiles - 1 - tile, lane);
+  if (pl.splits < 2) return;
+  for (int v = first; v < first + p.merge_vecs && v < p.T * p.G; ++v) {
+    const float* src = p.part + ((int64_t)(pl.slot + g * pl.splits) * p.VT + v - tile * p.VT) * ROW;
+    float M = -kInf, L = 0.0f;
+    f32x4_t O = {0, 0, 0, 0};
+    for (int i = grp; i < pl.splits; i += NG) {
+      const float* f = src + (int64_t)i * p.VT * ROW;
+      const float m = f[D], mn = fmaxf(M, m), off = mn == -kInf ? 0.0f : mn;
+      const float was = fast_exp2(M - off), wt = fast_exp2(m - off);
+      const f32x4_t t = *reinterpret_cast<const f32x4_t*>(f + d);
+      M = mn;
+      L = fmaf(wt, f[D + 1], L * was);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) O[k] = fmaf(wt, t[k], O[k] * was);
+    }
+    __syncthreads();
+    *reinterpret_cast<f32x4_t*>(&st[grp][d]) = O;
+    if (d == 0) {
+      st[grp][D] = M;
+      st[grp][D + 1] = L;
+    }
+    __syncthreads();
+    if (grp == 0) {
+      M = -kInf;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) M = fmaxf(M, st[i][D]);
+      const float off = M == -kInf ? 0.0f : M;
+      L = 0.0f;
+      O = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const float wt = fast_exp2(st[i][D] - off);
+        L = fmaf(wt, st[i][D + 1], L);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) O[k] = fmaf(wt, st[i][d + k], O[k]);
+      }
+      store_output<F16>(p, b, g, v, d, O, M, L);
+    }
+  }
+}
+
+}  // namespace
+
+hipError_t launch_paged_append(const PagedAppendParams& p, hipStream_t stream) {
+  const int64_t units = (int64_t)p.B * p.T * (p.H + 2 * p.Hkv), per = kThreads / (p.D / 16);
+  const dim3 grid((unsigned)((units + per - 1) / per));
+  if (p.D == 128) {
+    if (p.f16) paged_append_kernel<128, true><<<grid, kThreads, 0, stream>>>(p);
+    else paged_append_kernel<128, false><<<grid, kThreads, 0, stream>>>(p);
+  } else {
+    if (p.f16) paged_append_kernel<64, true><<<grid, kThreads, 0, stream>>>(p);
+    else paged_append_kernel<64, false><<<grid, kThreads, 0, stream>>>(p);
+  }
+  return hipGetLastError();
+}
+
+namespace {
+template <int D, bool F16, int NR>
+hipError_t attend(const PagedAttnParams& p, hipStream_t stream) {
+  if constexpr (NR == 0) paged_tile_kernel<D, F16><<<p.grid, 64 * kTileWaves, 0, stream>>>(p);
+  else if (p.knew) paged_attn_kernel<D, F16, NR, true><<<p.grid, kThreads, 0, stream>>>(p);
+  else paged_attn_kernel<D, F16, NR, false><<<p.grid, kThreads, 0, stream>>>(p);
+  if (p.part) {
+    const dim3 grid(p.tiles * (p.VT / p.merge_vecs), p.Hkv, p.B);
+    paged_merge_kernel<D, F16><<<grid, kThreads, 0, stream>>>(p);
+  }
+  return hipGetLastError();
+}
+template <int D, bool F16>
+hipError_t attend(const PagedAttnParams& p, hipStream_t stream) {
+  if (p.VT == 16) return attend<D, F16, 1>(p, stream);
+  if (p.VT == 32) return attend<D, F16, 2>(p, stream);
+  return attend<D, F16, 0>(p, stream);
+}
+}  // namespace
+
+hipError_t launch_paged_attention(const PagedAttnParams& p, hipStream_t stream) {
+  if (p.D == 128) return p.f16 ? attend<128, true>(p, stream) : attend<128, false>(p, stream);
+  return p.f16 ? attend<64, true>(p, stream) : attend<64, false>(p, stream);
+}
+
+}  // namespace bb
