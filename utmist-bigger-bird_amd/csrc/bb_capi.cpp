@@ -1060,8 +1060,8 @@ int bb_int4_decode_append(const void* q, const int64_t* sq, uint8_t* kq, void* k
 // ---- paged KV cache ----
 // How a call of the attention is cut (the kernels cut the lengths that they find by it).
 struct PagedSchedule {
-  int VT, tiles, unit, min_share, target, grid, merge_vecs;
-  size_t slots;
+  int VT, tiles, unit, min_share, target, fit, grid, merge_vecs;
+  size_t slots, bytes;  // of partials; of the workspace: the partials, then (splits, first slot) of each pair
 };
 constexpr int kPagedStreamVectors = 32;  // query vectors of a KV head up to which the streaming kernel takes a call
 constexpr int kPagedStepVectors = 128;   // and up to which it takes a step, storing its new rows
@@ -1085,7 +1085,9 @@ static const char* paged_schedule(int B, int T, int H, int Hkv, int D, int W, in
   s.grid = (int)std::min<int64_t>(pairs * Hkv * most, s.target + pairs * Hkv);
   // a pair of more than one split has at most twice its units over the share of them
   s.slots = most > 1 ? (size_t)std::min<int64_t>(s.grid, 2 * s.target) : 0;
+  s.fit = pairs <= 64 && pairs * Hkv <= s.target;
   s.merge_vecs = B * R * Hkv <= 16384 ? 1 : 16;
+  s.bytes = s.slots ? s.slots * s.VT * (D + 4) * 4 + (size_t)pairs * 8 : 0;
   return nullptr;
 }
 
@@ -1174,7 +1176,7 @@ static size_t paged_partials(int B, int T, int H, int Hkv, int D, int page, int 
   PagedSchedule s;
   if (B < 1 || T < 1 || H < 1 || Hkv < 1 || H % Hkv || page < 16 || W < 1 || (D != 64 && D != 128)) return 0;
   if (paged_schedule(B, T, H, Hkv, D, W, page, with_new, s)) return 0;
-  return s.slots * s.VT * (D + 4) * 4;
+  return s.bytes;
 }
 
 size_t bb_paged_attention_workspace(int B, int T, int H, int Hkv, int D, int page, int W) {
@@ -1199,7 +1201,7 @@ static int paged_attention_impl(const char* what, const void* q, const int64_t* 
   if (!(scale > 0.0f)) return fail("scale must be positive");
   PagedSchedule s;
   if (const char* e = paged_schedule(B, T, H, Hkv, D, c.W, page, knew != nullptr, s)) return fail("%s: %s", what, e);
-  const size_t need = s.slots * s.VT * (D + 4) * 4;
+  const size_t need = s.bytes;
   if (need && (!ws || ws_bytes < need || !aligned(ws, 16))) return fail("workspace of %zu bytes required", need);
   bb::PagedAttnParams p;
   memset(&p, 0, sizeof(p));
@@ -1216,10 +1218,11 @@ static int paged_attention_impl(const char* what, const void* q, const int64_t* 
   p.out = static_cast<uint16_t*>(out);
   p.so0 = so[0]; p.so1 = so[1]; p.so2 = so[2];
   p.part = need ? static_cast<float*>(ws) : nullptr;
+  p.plan = need ? reinterpret_cast<int2*>(p.part + s.slots * s.VT * (D + 4)) : nullptr;
   p.B = B; p.T = T; p.H = H; p.Hkv = Hkv; p.G = H / Hkv; p.D = D;
   p.f16 = is_f16 ? 1 : 0;
   p.VT = s.VT; p.tiles = s.tiles; p.pairs = s.tiles * B;
-  p.unit = s.unit; p.min_share = s.min_share; p.target = s.target;
+  p.unit = s.unit; p.min_share = s.min_share; p.target = s.target; p.fit = s.fit;
   p.grid = s.grid; p.merge_vecs = s.merge_vecs;
   p.scale = (float)((double)scale * 1.4426950408889634);
   return hip_status(bb::launch_paged_attention(p, static_cast<hipStream_t>(stream)), what);

@@ -171,7 +171,8 @@ struct PagedAttnParams {
   int64_t sq0, sq1, sq2, skn0, skn1, skn2, svn0, svn1, svn2, so0, so1, so2;
   int B, T, H, Hkv, G, D, f16;
   int VT, tiles, pairs;        // query vectors of a tile, tiles, B * tiles
-  int unit, min_share, target; // keys of a unit; units of a split, at least; workgroups aimed at
+  int2* plan;                  // [pairs] (splits, first slot), written for the merge with part
+  int unit, min_share, target, fit; // rows of a unit; units of a split, at least; workgroups aimed at, and whether at most
   int grid, merge_vecs;
   float scale;                 // times log2(e)
 };

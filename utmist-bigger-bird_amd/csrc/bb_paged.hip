@@ -213,28 +213,36 @@ BB_DEV int pair_units(const PagedAttnParams& p, int pair) {
   const int k = pair_keys(p, sequence(p.c, p.T, pair / p.tiles), pair_tile(p, pair));
   return k > 0 ? udiv_up(k, p.unit) : 1;
 }
-BB_DEV int share_of(const PagedAttnParams& p, int total) {
-  const int s = udiv_up(total * p.Hkv, p.target);
-  return s > p.min_share ? s : p.min_share;
+// The share. With p.fit (the pairs fit a wave and the workgroups that run at once) the least, up to an eighth, for which the
+// call's splits are no more than run at once. It is never below the total over p.target workgroups, which the partials' space
+// and the grid go by: at most 2 p.target of the splits are of a pair that has several (such a pair has less than twice its
+// units over the share of them), and all splits are at most p.target + pairs * Hkv.
+BB_DEV int sum_over_lanes(int v) { return lane_int(wave_scan(v), 63); }
+BB_DEV int share_of(const PagedAttnParams& p, int first, int total) {
+  const int least = udiv_up(total * p.Hkv, p.target);
+  int share = least > p.min_share ? least : p.min_share;
+  if (p.fit)
+    while (sum_over_lanes(udiv_up(first, share)) * p.Hkv > p.target) share += share < 8 ? 1 : share / 8;
+  return share;
 }
-// Walks the pairs (by a whole wave) to the first whose items reach past `item`, or with `item` < 0 to pair `pair`.
+// Walks the pairs (by a whole wave) to the one that item `item` is of.
 struct PairPlan {
   int pair, units, splits, slot, before;  // pair -1: no such item; slot: of KV head 0's first split; before: items of earlier pairs
 };
-BB_DEV PairPlan walk_pairs(const PagedAttnParams& p, int item, int pair, int lane) {
+BB_DEV PairPlan walk_pairs(const PagedAttnParams& p, int item, int lane) {
   int first = 0, total = 0;
   for (int at = 0; at < p.pairs; at += 64) {
     const int u = pair_units(p, at + lane);
     if (at == 0) first = u;
     total += lane_int(wave_scan(u), 63);
   }
-  const int share = share_of(p, total);
+  const int share = share_of(p, first, total);
   int items = 0, slots = 0;
   for (int at = 0; at < p.pairs; at += 64) {
     const int u = at == 0 ? first : pair_units(p, at + lane);
     const int sp = udiv_up(u, share), mine = sp * p.Hkv, split = sp > 1 ? mine : 0;
     const int upto = items + wave_scan(mine), slot_upto = slots + wave_scan(split);
-    const uint64_t in = __builtin_amdgcn_ballot_w64(item < 0 ? at + lane == pair : item < upto);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(item < upto);
     if (in) {
       const int l = __builtin_ctzll(in);
       return PairPlan{at + l, lane_int(u, l), lane_int(sp, l), lane_int(slot_upto - split, l), lane_int(upto - mine, l)};
@@ -244,10 +252,11 @@ BB_DEV PairPlan walk_pairs(const PagedAttnParams& p, int item, int pair, int lan
   }
   return PairPlan{-1, 0, 0, 0, 0};
 }
-BB_DEV PairPlan find_pair(const PagedAttnParams& p, int pair, int lane) { return walk_pairs(p, -1, pair, lane); }
 // The item with index `item`; not live where the call has fewer.
 BB_DEV Item find_item(const PagedAttnParams& p, int item, int lane) {
-  const PairPlan pl = walk_pairs(p, item, 0, lane);
+  const PairPlan pl = walk_pairs(p, item, lane);
+  // the merge finds a pair's splits here
+  if (p.part && pl.pair >= 0 && item == pl.before && threadIdx.x == 0) p.plan[pl.pair] = make_int2(pl.splits, pl.slot);
   const int rest = item - pl.before, g = rest % p.Hkv, split = rest / p.Hkv;
   return Item{pl.pair >= 0, pl.pair / p.tiles, pair_tile(p, pl.pair), g, split, pl.splits, pl.slot + g * pl.splits + split, pl.units};
 }
@@ -910,6 +919,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
     t.m[rb] = kLowest;
     t.l[rb] = 0.0f;
   }
+  const bool live = 32 * wave < R;  // a wave without vectors only loads
   const TileLoader<D> in(p.c, it.b, it.g, end, wave, lane);
   // Tiles without a mask: below the rows that the tile's first token attends, if the table names a page for all of the split.
   // (What padding gets there is not stored.)
@@ -998,19 +1008,19 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
     if (late) ring_barrier();  // the second group runs one phase behind
     if (n_tiles > 2) fetch(2, e);
     e = entries(3);
-    tile_products<F16, D, NV, NF>(t, rd, lds_addr(stage(0)), 0);
+    if (live) tile_products<F16, D, NV, NF>(t, rd, lds_addr(stage(0)), 0);
     wait_tile(n_tiles > 2);
     ring_barrier();
-    if (open > 0) tile_softmax<F16, D>(t, p.scale);
-    else masked(0);
+    if (live && open > 0) tile_softmax<F16, D>(t, p.scale);
+    else if (live) masked(0);
     ring_barrier();
     for (int i = 1; i < open; ++i) {
       __builtin_amdgcn_s_setprio(1);
-      tile_products<F16, D, 0, NF>(t, rd, lds_addr(stage(i)), lds_addr(stage(i - 1) + L::BYTES));
+      if (live) tile_products<F16, D, 0, NF>(t, rd, lds_addr(stage(i)), lds_addr(stage(i - 1) + L::BYTES));
       __builtin_amdgcn_s_setprio(0);
       wait_tile(false);  // tile i + 1 has landed
       ring_barrier();
-      tile_softmax<F16, D>(t, p.scale);
+      if (live) tile_softmax<F16, D>(t, p.scale);
       // into the stage of tile i - 2, which every wave has read
       if (i + 2 < n_tiles) fetch(i + 2, e);
       e = entries(i + 3);
@@ -1018,16 +1028,18 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
     }
 #pragma unroll 1
     for (int i = open > 1 ? open : 1; i < n_tiles; ++i) {
-      masked_values(i - 1);
-      tile_products<F16, D, NV, NF>(t, rd, lds_addr(stage(i)), 0);
+      if (live) {
+        masked_values(i - 1);
+        tile_products<F16, D, NV, NF>(t, rd, lds_addr(stage(i)), 0);
+      }
       wait_tile(false);
       ring_barrier();
-      masked(i);
+      if (live) masked(i);
       if (i + 2 < n_tiles) fetch(i + 2, e);
       e = entries(i + 3);
       ring_barrier();
     }
-    masked_values(n_tiles - 1);
+    if (live) masked_values(n_tiles - 1);
     if (!late) ring_barrier();  // the groups meet again
   }
 
@@ -1064,25 +1076,48 @@ template <int D, bool F16>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttnParams p) {
   constexpr int LPV = D / 4, NG = kThreads / LPV, ROW = D + 4;
   __shared__ float st[NG][ROW];
-  const int tid = threadIdx.x, lane = tid & 63, grp = tid / LPV, d = 4 * (tid % LPV);
+  const int tid = threadIdx.x, grp = tid / LPV, d = 4 * (tid % LPV);
   const int per_tile = p.VT / p.merge_vecs, b = blockIdx.z, g = blockIdx.y, tile = blockIdx.x / per_tile;
   const int first = tile * p.VT + (blockIdx.x % per_tile) * p.merge_vecs;
   if (first >= p.T * p.G) return;
-  const PairPlan pl = find_pair(p, b * p.tiles + p.tiles - 1 - tile, lane);
-  if (pl.splits < 2) return;
+  const int2 pl = p.plan[b * p.tiles + p.tiles - 1 - tile];
+  const int splits = pl.x;
+  if (splits < 2) return;
   for (int v = first; v < first + p.merge_vecs && v < p.T * p.G; ++v) {
-    const float* src = p.part + ((int64_t)(pl.slot + g * pl.splits) * p.VT + v - tile * p.VT) * ROW;
+    const float* src = p.part + ((int64_t)(pl.y + g * splits) * p.VT + v - tile * p.VT) * ROW;
     float M = -kInf, L = 0.0f;
     f32x4_t O = {0, 0, 0, 0};
-    for (int i = grp; i < pl.splits; i += NG) {
-      const float* f = src + (int64_t)i * p.VT * ROW;
-      const float m = f[D], mn = fmaxf(M, m), off = mn == -kInf ? 0.0f : mn;
-      const float was = fast_exp2(M - off), wt = fast_exp2(m - off);
-      const f32x4_t t = *reinterpret_cast<const f32x4_t*>(f + d);
-      M = mn;
-      L = fmaf(wt, f[D + 1], L * was);
+    constexpr int U = 4;  // splits whose loads are in flight together
+    for (int i = grp; i < splits; i += U * NG) {
+      float m[U], l[U], mn = M;
+      f32x4_t t[U];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) O[k] = fmaf(wt, t[k], O[k] * was);
+      for (int k = 0; k < U; ++k) {
+        const int at = i + k * NG < splits ? i + k * NG : i;
+        const float* f = src + (int64_t)at * p.VT * ROW;
+        const u32x2_t ml = *reinterpret_cast<const u32x2_t*>(f + D);
+        m[k] = __uint_as_float(ml[0]);
+        l[k] = __uint_as_float(ml[1]);
+        t[k] = *reinterpret_cast<const f32x4_t*>(f + d);
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (i + k * NG >= splits) m[k] = -kInf;
+        mn = fmaxf(mn, m[k]);
+      }
+      const float off = mn == -kInf ? 0.0f : mn, was = fast_exp2(M - off);
+      M = mn;
+      L *= was;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) O[j] *= was;
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (i + k * NG >= splits) continue;
+        const float wt = fast_exp2(m[k] - off);
+        L = fmaf(wt, l[k], L);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) O[j] = fmaf(wt, t[k][j], O[j]);
+      }
     }
     __syncthreads();
     *reinterpret_cast<f32x4_t*>(&st[grp][d]) = O;
