@@ -56,7 +56,9 @@ CACHE = [
     (dict(W=1 << 25), "out of range"),
     (dict(sk=_s(65536, 8192, 100)), "16-byte aligned rows"),
     (dict(sv=_s(-65536, 8192, 128)), "16-byte aligned rows"),
-    (dict(sv=_s(65536, 8192, 1 << 27)), "16-byte aligned rows"),
+    (dict(sv=_s(65536, 8192, 1 << 27)), "out of range"),
+    (dict(sk=_s(1 << 31, 8192, 128)), "out of range"),
+    (dict(page=1 << 20, W=1, sk=_s(1 << 27, 1 << 27, 1024)), "out of range"),
     (dict(fresh=ctypes.c_void_p(18)), "misaligned lengths"),
 ]
 

@@ -1060,8 +1060,8 @@ int bb_int4_decode_append(const void* q, const int64_t* sq, uint8_t* kq, void* k
 // ---- paged KV cache ----
 // How a call of the attention is cut (the kernels cut the lengths that they find by it).
 struct PagedSchedule {
-  int VT, tiles, unit, min_share, target, fit, grid, merge_vecs;
-  size_t slots, bytes;  // of partials; of the workspace: the partials, then (splits, first slot) of each pair
+  int VT, tiles, unit, min_share, target, fit_quarters, grid;
+  size_t slots, bytes;  // of partials; of the workspace: the partials, then what each slot holds and how many are used
 };
 constexpr int kPagedStreamVectors = 32;  // query vectors of a KV head up to which the streaming kernel takes a call
 constexpr int kPagedStepVectors = 128;   // and up to which it takes a step, storing its new rows
@@ -1071,23 +1071,25 @@ static const char* paged_schedule(int B, int T, int H, int Hkv, int D, int W, in
     s.VT = R <= 16 ? 16 : 32;
     s.unit = 4 * 4096 / D;
     s.min_share = 2;
+    s.fit_quarters = 1 << 20;
     s.target = 2 * kCUs;
   } else {
     s.VT = 256;
     s.unit = 64;
-    s.min_share = 16;
+    s.min_share = 8;
+    s.fit_quarters = 5;
     s.target = kCUs;
   }
   const int64_t tiles = cdiv(R, s.VT), pairs = tiles * B, units = cdiv(cap, s.unit);
-  if (cap > 1ll << 30 || pairs * Hkv * units >= 1ll << 31 || R >= 1ll << 31) return "lengths out of range";
+  if (cap > 1ll << 28 || pairs * Hkv * units >= 1ll << 30 || R >= 1ll << 22 || pairs * Hkv >= 1ll << 22)
+    return "lengths out of range";  // the kernels divide numbers of 23 bits
   s.tiles = (int)tiles;
   const int64_t most = cdiv(units, s.min_share);  // splits of a pair
   s.grid = (int)std::min<int64_t>(pairs * Hkv * most, s.target + pairs * Hkv);
   // a pair of more than one split has at most twice its units over the share of them
   s.slots = most > 1 ? (size_t)std::min<int64_t>(s.grid, 2 * s.target) : 0;
-  s.fit = pairs <= 64 && pairs * Hkv <= s.target;
-  s.merge_vecs = B * R * Hkv <= 16384 ? 1 : 16;
-  s.bytes = s.slots ? s.slots * s.VT * (D + 4) * 4 + (size_t)pairs * 8 : 0;
+  if (pairs > 64 || pairs * Hkv > s.target) s.fit_quarters = 0;
+  s.bytes = s.slots ? s.slots * s.VT * (D + 4) * 4 + (s.slots + 1) * 16 : 0;
   return nullptr;
 }
 
@@ -1105,9 +1107,12 @@ static int paged_cache(const char* what, void* k, const int64_t* sk, void* v, co
   if (D != 64 && D != 128) return fail("%s: head_dim %d unsupported (64 or 128)", what, D);
   if (page < 16 || page & (page - 1)) return fail("%s: pages of %d rows unsupported (a power of two, at least 16)", what, page);
   if (pages < 0 || W < 1 || st < 0) return fail("%s: empty table", what);
-  if ((int64_t)W * page > 1ll << 30) return fail("%s: tables of %lld rows out of range", what, (long long)W * page);
-  if (!aligned(k, 16) || !aligned(v, 16) || !paged_strides(sk) || !paged_strides(sv) || sk[2] >= 1 << 26 || sv[2] >= 1 << 26)
+  if ((int64_t)W * page > 1ll << 28) return fail("%s: tables of %lld rows out of range", what, (long long)W * page);
+  if (!aligned(k, 16) || !aligned(v, 16) || !paged_strides(sk) || !paged_strides(sv))
     return fail("%s: pages need a contiguous head_dim and 16-byte aligned rows", what);
+  for (const int64_t* s : {sk, sv})  // a page's rows and the stride of pages are 32-bit offsets
+    if (s[0] >= 1ll << 31 || s[2] >= 1 << 26 || s[2] * page >= 1ll << 30)
+      return fail("%s: pages of this size are out of range", what);
   if (!aligned(table, 4) || !aligned(lens, 4) || !aligned(fresh, 4)) return fail("%s: misaligned lengths", what);
   c.k = static_cast<uint16_t*>(k);
   c.v = static_cast<uint16_t*>(v);
@@ -1218,12 +1223,14 @@ static int paged_attention_impl(const char* what, const void* q, const int64_t* 
   p.out = static_cast<uint16_t*>(out);
   p.so0 = so[0]; p.so1 = so[1]; p.so2 = so[2];
   p.part = need ? static_cast<float*>(ws) : nullptr;
-  p.plan = need ? reinterpret_cast<int2*>(p.part + s.slots * s.VT * (D + 4)) : nullptr;
+  p.plan = need ? reinterpret_cast<int4*>(p.part + s.slots * s.VT * (D + 4)) : nullptr;
   p.B = B; p.T = T; p.H = H; p.Hkv = Hkv; p.G = H / Hkv; p.D = D;
   p.f16 = is_f16 ? 1 : 0;
   p.VT = s.VT; p.tiles = s.tiles; p.pairs = s.tiles * B;
-  p.unit = s.unit; p.min_share = s.min_share; p.target = s.target; p.fit = s.fit;
-  p.grid = s.grid; p.merge_vecs = s.merge_vecs;
+  p.unit_log2 = __builtin_ctz(s.unit); p.min_share = s.min_share; p.target_log2 = __builtin_ctz(s.target);
+  p.inv_G = 1.0f / (float)p.G; p.inv_B = 1.0f / (float)B; p.inv_Hkv = 1.0f / (float)Hkv;
+  p.fit_quarters = s.fit_quarters;
+  p.grid = s.grid; p.slots = (int)s.slots;
   p.scale = (float)((double)scale * 1.4426950408889634);
   return hip_status(bb::launch_paged_attention(p, static_cast<hipStream_t>(stream)), what);
 }

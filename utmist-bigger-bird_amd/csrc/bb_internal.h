@@ -171,9 +171,11 @@ struct PagedAttnParams {
   int64_t sq0, sq1, sq2, skn0, skn1, skn2, svn0, svn1, svn2, so0, so1, so2;
   int B, T, H, Hkv, G, D, f16;
   int VT, tiles, pairs;        // query vectors of a tile, tiles, B * tiles
-  int2* plan;                  // [pairs] (splits, first slot), written for the merge with part
-  int unit, min_share, target, fit; // rows of a unit; units of a split, at least; workgroups aimed at, and whether at most
-  int grid, merge_vecs;
+  int4* plan;                  // of each slot (sequence, tile, KV head, split | splits << 16), then (slots used, -, -, -)
+  int unit_log2, min_share, target_log2;  // rows of a unit; units of a split, at least; workgroups aimed at
+  int fit_quarters;                       // see share_of
+  float inv_G, inv_B, inv_Hkv;
+  int grid, slots;
   float scale;                 // times log2(e)
 };
 hipError_t launch_paged_attention(const PagedAttnParams& p, hipStream_t stream);

@@ -194,74 +194,127 @@ BB_DEV int wave_scan(int v) {  // inclusive sum over the lanes
   return v;
 }
 BB_DEV int lane_int(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
-BB_DEV int udiv_up(int a, int b) { return (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b); }
-
-struct Item {
-  bool live;
-  int b, tile, g, split, splits, slot, units;
-};
-BB_DEV int pair_tile(const PagedAttnParams& p, int pair) { return p.tiles - 1 - pair % p.tiles; }  // the longest first
+// v / d for 0 <= v < 2^23, 0 < d, from a float reciprocal of d (a division of integers is some 40 instructions, and the code
+// before the loops is run once, as its lines come in).
+BB_DEV int quotient(int v, float inv, int d) {
+  int q = (int)((float)v * inv);
+  const int r = v - q * d;
+  q = r < 0 ? q - 1 : r >= d ? q + 1 : q;
+  return q;
+}
+BB_DEV int token_of(const PagedAttnParams& p, int v) { return quotient(v, p.inv_G, p.G); }
+// Pair `pair` is tile pair_tile of sequence pair % B: the sequences' last tiles, which are the longest, come first.
+BB_DEV int pair_tile(const PagedAttnParams& p, int pair) { return p.tiles == 1 ? 0 : p.tiles - 1 - quotient(pair, p.inv_B, p.B); }
+BB_DEV int pair_sequence(const PagedAttnParams& p, int pair, int tile) { return pair - (p.tiles - 1 - tile) * p.B; }
+BB_DEV int pair_index(const PagedAttnParams& p, int b, int tile) { return (p.tiles - 1 - tile) * p.B + b; }
 // Rows that the pair's last real token attends (0: none of its tokens is real, or has rows).
 BB_DEV int pair_keys(const PagedAttnParams& p, const Sequence& s, int tile) {
-  const int j0 = tile * p.VT / p.G;
-  int j1 = (tile * p.VT + p.VT - 1) / p.G;
+  const int j0 = token_of(p, tile * p.VT);
+  int j1 = p.tiles == 1 ? p.T - 1 : token_of(p, tile * p.VT + p.VT - 1);
   if (j1 >= s.fresh) j1 = s.fresh - 1;
   return j1 < j0 ? 0 : s.seen(j1);
 }
 BB_DEV int pair_units(const PagedAttnParams& p, int pair) {
   if (pair >= p.pairs) return 0;
-  const int k = pair_keys(p, sequence(p.c, p.T, pair / p.tiles), pair_tile(p, pair));
-  return k > 0 ? udiv_up(k, p.unit) : 1;
+  const int tile = pair_tile(p, pair), k = pair_keys(p, sequence(p.c, p.T, pair_sequence(p, pair, tile)), tile);
+  return (k + (1 << p.unit_log2) - 1) >> p.unit_log2;
 }
-// The share. With p.fit (the pairs fit a wave and the workgroups that run at once) the least, up to an eighth, for which the
-// call's splits are no more than run at once. It is never below the total over p.target workgroups, which the partials' space
-// and the grid go by: at most 2 p.target of the splits are of a pair that has several (such a pair has less than twice its
-// units over the share of them), and all splits are at most p.target + pairs * Hkv.
+// The share of a split, and the splits of a pair. Where the pairs fit a wave and the workgroups that run at once (p.fit_quarters
+// > 0) and it wastes little (F / least <= p.fit_quarters / 4), the share is the F for which the call's splits are just no more
+// than run at once, and the rest of a pair is a split too; otherwise a pair's units over the least share are rounded, so that
+// pairs a little over it stay whole. The share is never below the total over the workgroups aimed at, which the partials' space
+// and the grid go by: a pair of several splits has at most twice its units over the share of them, so these are at most twice
+// the workgroups aimed at, and all splits at most those and pairs * Hkv.
 BB_DEV int sum_over_lanes(int v) { return lane_int(wave_scan(v), 63); }
-BB_DEV int share_of(const PagedAttnParams& p, int first, int total) {
-  const int least = udiv_up(total * p.Hkv, p.target);
-  int share = least > p.min_share ? least : p.min_share;
-  if (p.fit)
-    while (sum_over_lanes(udiv_up(first, share)) * p.Hkv > p.target) share += share < 8 ? 1 : share / 8;
-  return share;
-}
-// Walks the pairs (by a whole wave) to the one that item `item` is of.
-struct PairPlan {
-  int pair, units, splits, slot, before;  // pair -1: no such item; slot: of KV head 0's first split; before: items of earlier pairs
+struct Share {
+  int units;
+  bool fit;
+  BB_DEV int splits(int u) const {
+    const int n = quotient(fit ? u + units - 1 : u + units / 2, 1.0f / (float)units, units);
+    return n > 0 || u == 0 ? n : 1;
+  }
 };
-BB_DEV PairPlan walk_pairs(const PagedAttnParams& p, int item, int lane) {
+BB_DEV Share share_of(const PagedAttnParams& p, int first, int total) {
+  const int least = (total * p.Hkv + (1 << p.target_log2) - 1) >> p.target_log2;
+  Share s{least > p.min_share ? least : p.min_share, false};
+  if (p.fit_quarters > 0) {
+    Share f{s.units, true};
+    while (sum_over_lanes(f.splits(first)) * p.Hkv > 1 << p.target_log2) f.units += f.units < 8 ? 1 : f.units / 8;
+    if (4 * (int64_t)f.units <= (int64_t)p.fit_quarters * s.units) s = f;
+  }
+  return s;
+}
+// What a workgroup does: split `split` of a pair, or (zero) the output of a pair without rows to attend, or nothing.
+struct Item {
+  bool live, zero;
+  int b, tile, g, split, splits, slot, units;
+};
+// The item with index `item`, by a whole wave: the splits of all pairs in order, then the pairs without any, KV heads fastest.
+// (Pairs without rows among the others would hold up the dispatch of long ones behind them.)
+BB_DEV Item find_item(const PagedAttnParams& p, int item, int lane) {
   int first = 0, total = 0;
   for (int at = 0; at < p.pairs; at += 64) {
     const int u = pair_units(p, at + lane);
     if (at == 0) first = u;
-    total += lane_int(wave_scan(u), 63);
+    total += sum_over_lanes(u);
   }
-  const int share = share_of(p, first, total);
-  int items = 0, slots = 0;
-  for (int at = 0; at < p.pairs; at += 64) {
+  const Share share = share_of(p, first, total);
+  int pair = -1, units = 0, splits = 0, slot = 0, before = 0, items = 0, slots = 0;
+  for (int at = 0; at < p.pairs && (pair < 0 || item == 0); at += 64) {  // (item 0 counts all slots)
     const int u = at == 0 ? first : pair_units(p, at + lane);
-    const int sp = udiv_up(u, share), mine = sp * p.Hkv, split = sp > 1 ? mine : 0;
+    const int sp = share.splits(u), mine = sp * p.Hkv, split = sp > 1 ? mine : 0;
     const int upto = items + wave_scan(mine), slot_upto = slots + wave_scan(split);
     const uint64_t in = __builtin_amdgcn_ballot_w64(item < upto);
-    if (in) {
+    if (in && pair < 0) {
       const int l = __builtin_ctzll(in);
-      return PairPlan{at + l, lane_int(u, l), lane_int(sp, l), lane_int(slot_upto - split, l), lane_int(upto - mine, l)};
+      pair = at + l;
+      units = lane_int(u, l);
+      splits = lane_int(sp, l);
+      slot = lane_int(slot_upto - split, l);
+      before = lane_int(upto - mine, l);
     }
     items = lane_int(upto, 63);
     slots = lane_int(slot_upto, 63);
   }
-  return PairPlan{-1, 0, 0, 0, 0};
+  Item it;
+  it.live = pair >= 0;
+  if (!it.live) {
+    int nth = quotient(item - items, p.inv_Hkv, p.Hkv);
+    before = items + nth * p.Hkv;
+    for (int at = 0; at < p.pairs && pair < 0; at += 64) {
+      const uint64_t none = __builtin_amdgcn_ballot_w64(at + lane < p.pairs && (at == 0 ? first : pair_units(p, at + lane)) == 0);
+      const int here = __builtin_popcountll(none);
+      if (nth < here) {
+        const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(none >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)none, 0));
+        pair = at + __builtin_ctzll(__builtin_amdgcn_ballot_w64((none >> lane & 1) && rank == nth));
+      }
+      nth -= here;
+    }
+  }
+  it.zero = !it.live && pair >= 0;
+  const int rest = item - before;
+  it.split = it.live ? quotient(rest, p.inv_Hkv, p.Hkv) : 0;
+  it.g = rest - it.split * p.Hkv;
+  it.tile = pair_tile(p, pair < 0 ? 0 : pair);
+  it.b = pair_sequence(p, pair < 0 ? 0 : pair, it.tile);
+  it.splits = splits;
+  it.slot = slot + it.g * splits + it.split;
+  it.units = units;
+  if (p.part && threadIdx.x == 0) {  // for the merge
+    if (splits > 1) p.plan[it.slot] = make_int4(it.b, it.tile, it.g, it.split | splits << 16);
+    if (item == 0) p.plan[p.slots].x = slots;
+  }
+  return it;
 }
-// The item with index `item`; not live where the call has fewer.
-BB_DEV Item find_item(const PagedAttnParams& p, int item, int lane) {
-  const PairPlan pl = walk_pairs(p, item, lane);
-  // the merge finds a pair's splits here
-  if (p.part && pl.pair >= 0 && item == pl.before && threadIdx.x == 0) p.plan[pl.pair] = make_int2(pl.splits, pl.slot);
-  const int rest = item - pl.before, g = rest % p.Hkv, split = rest / p.Hkv;
-  return Item{pl.pair >= 0, pl.pair / p.tiles, pair_tile(p, pl.pair), g, split, pl.splits, pl.slot + g * pl.splits + split, pl.units};
+// Zeros for a pair's tokens.
+BB_DEV void store_zeros(const PagedAttnParams& p, const Item& it, int D, int tid, int threads) {
+  for (int i = tid; i < p.VT * (D / 8); i += threads) {
+    const int v = it.tile * p.VT + i / (D / 8), j = token_of(p, v), h = it.g * p.G + v - j * p.G;
+    if (v < p.T * p.G) st16(p.out + it.b * p.so0 + h * p.so1 + j * p.so2 + 8 * (i % (D / 8)), u32x4_t{0, 0, 0, 0});
+  }
 }
 // First unit of split s of u units in n splits: equal parts.
-BB_DEV int split_begin(int u, int n, int s) { return (int)((int64_t)u * s / n); }
+BB_DEV int split_begin(int u, int n, int s) { return n == 1 ? s * u : (int)((int64_t)u * s / n); }
 
 // ---------------------------------------------------------------------------------------------------------------
 // Attention of up to 16 NR query vectors of a KV head over a split of a sequence's rows.
@@ -300,6 +353,30 @@ BB_DEV int k_swz(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
 template <int D>
 BB_DEV int v_swz(int r) { return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
 
+// `rows` rows of a head's pages from row r on (all in one page) as a buffer of that size; empty for page < 0. (Everything here is
+// one value a wave; the range by a minimum and selects alone: a clamp goes to the vector unit, and then each load is a loop over
+// the values that its descriptor might have.)
+struct PageRows {
+  const char* at;
+  uint32_t bytes;
+};
+BB_DEV PageRows page_rows(const PagedCache& c, bool is_v, const uint16_t* head, int page, int r, int rows, int row_bytes) {
+  const uint32_t stride = (uint32_t)(is_v ? c.svr : c.skr) * 2, sp = (uint32_t)(is_v ? c.svp : c.skp);
+  const uint32_t at = page < 0 ? 0u : (uint32_t)page;
+  const uint32_t in = (uint32_t)(r & ((1 << c.page_log2) - 1)) * stride;
+  uint32_t bytes = (uint32_t)(rows - 1) * stride + (uint32_t)row_bytes;
+  bytes = page < 0 || rows <= 0 ? 0u : bytes;
+  return PageRows{reinterpret_cast<const char*>(head) + (uint64_t)at * sp * 2 + in, bytes};
+}
+
+// 16 bytes a lane of those rows into LDS at `to` (one value a wave) + 16 lane.
+template <int AUX>
+BB_DEV void load_rows(const PageRows& at, uint8_t* to, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at.at), 0, (int)at.bytes, 0x00020000),
+      reinterpret_cast<lds_void*>(reinterpret_cast<uintptr_t>(to)), 16, off, 0, 0, AUX);
+}
+
 // One wave's stream of chunks of KC rows, 8 KB of K and of V.
 template <int D>
 struct PageStream {
@@ -333,22 +410,15 @@ struct PageStream {
   }
   // Always eight loads, so that the counts the waits go by are exact; rows past the end and of no page land zeros.
   BB_DEV void fetch(bool is_v, uint8_t* to, int k0, const int (&e)[GROUPS]) const {
-    const int64_t sp = is_v ? c.svp : c.skp, sr = is_v ? c.svr : c.skr;
-    const uint32_t rb = (uint32_t)sr * 2;
+    const uint32_t rb = (uint32_t)(is_v ? c.svr : c.skr) * 2;
 #pragma unroll
     for (int j = 0; j < GROUPS; ++j) {
-      const int r = k0 + 16 * j, left = end - r, live = e[j] < 0 ? 0 : left < 16 ? left : 16;
-      const int page = e[j] < 0 ? 0 : e[j];
-      const uint16_t* base = (is_v ? vh : kh) + page * sp + (r & ((1 << c.page_log2) - 1)) * sr;
-      const uint32_t bytes = live > 0 ? (live - 1) * rb + 2 * D : 0;
-      const __amdgpu_buffer_rsrc_t rs =
-          __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)bytes, 0x00020000);
+      const int r = k0 + 16 * j;
+      const PageRows at = page_rows(c, is_v, is_v ? vh : kh, e[j], r, end - r < 16 ? end - r : 16, 2 * D);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const uint32_t piece = is_v ? vpiece ^ 16u * v_swz<D>(RPL * i) : kpiece ^ 16u * k_swz<D>(RPL * i);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rs, reinterpret_cast<lds_void*>(reinterpret_cast<uintptr_t>(to + 1024 * (LOADS * j + i))), 16,
-            (row + RPL * i) * rb + piece, 0, 0, 2 /* non-temporal */);
+        load_rows<2 /* non-temporal */>(at, to + 1024 * (LOADS * j + i), (row + RPL * i) * rb + piece);
       }
     }
   }
@@ -389,7 +459,7 @@ BB_DEV void patch_new_rows(const PagedAttnParams& p, const Sequence& s, int b, i
 constexpr float kLowest = -3.4028234663852886e38f;
 template <bool F16>
 BB_DEV void store_output(const PagedAttnParams& p, int b, int g, int v, int d, f32x4_t O, float M, float L) {
-  const int j = v / p.G, h = g * p.G + v - j * p.G;
+  const int j = token_of(p, v), h = g * p.G + v - j * p.G;
 #pragma unroll
   for (int k = 0; k < 4; ++k) O[k] = M == -kInf ? 0.0f : O[k] / L;
   *reinterpret_cast<u32x2_t*>(p.out + b * p.so0 + h * p.so1 + j * p.so2 + d) =
@@ -413,11 +483,12 @@ __global__ __launch_bounds__(kThreads, NR > 1 && NEW ? 1 : 2) void paged_attn_ke
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 15, a = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Item it = find_item(p, blockIdx.x, lane);
+  if (it.zero) store_zeros(p, it, D, tid, kThreads);
   if (!it.live) return;
   const Sequence s = sequence(p.c, p.T, it.b);
   const int keys = __builtin_amdgcn_readfirstlane(pair_keys(p, s, it.tile));
   const int u0 = split_begin(it.units, it.splits, it.split), u1 = split_begin(it.units, it.splits, it.split + 1);
-  int begin = u0 * p.unit, end = u1 * p.unit < keys ? u1 * p.unit : keys;
+  int begin = u0 << p.unit_log2, end = u1 << p.unit_log2 < keys ? u1 << p.unit_log2 : keys;
   begin = __builtin_amdgcn_readfirstlane(begin);
   end = __builtin_amdgcn_readfirstlane(end);
   const int v0 = it.tile * p.VT;
@@ -434,7 +505,7 @@ __global__ __launch_bounds__(kThreads, NR > 1 && NEW ? 1 : 2) void paged_attn_ke
   int lim[NR], tok[NR];
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
-    const int v = 16 * r + x < R ? v0 + 16 * r + x : v0, j = v / p.G, h = it.g * p.G + v - j * p.G;
+    const int v = 16 * r + x < R ? v0 + 16 * r + x : v0, j = token_of(p, v), h = it.g * p.G + v - j * p.G;
     tok[r] = j;
     lim[r] = 16 * r + x < R ? s.seen(j) : 0;
     const uint16_t* qr = p.q + it.b * p.sq0 + h * p.sq1 + j * p.sq2 + 8 * a;
@@ -486,7 +557,7 @@ __global__ __launch_bounds__(kThreads, NR > 1 && NEW ? 1 : 2) void paged_attn_ke
     }
   }
   // the fewest rows that a token of the tile attends: chunks below need no mask (what padding gets there is not stored)
-  const int fewest = __builtin_amdgcn_readfirstlane(s.seen(v0 / p.G));
+  const int fewest = __builtin_amdgcn_readfirstlane(s.seen(token_of(p, v0)));
 
   float m[NR], l[NR];
   bool seen[NR];
@@ -551,10 +622,10 @@ __global__ __launch_bounds__(kThreads, NR > 1 && NEW ? 1 : 2) void paged_attn_ke
       } else {
 #pragma unroll
         for (int kb = 0; kb < KC / 16; ++kb) {
-          seen[r] = seen[r] || (e[kb] >= 0 && k0 + 16 * kb < lim[r]);
+          const int stop = e[kb] < 0 ? 0 : lim[r], row = k0 + 16 * kb;
+          seen[r] |= row < stop;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (e[kb] < 0 || k0 + 16 * kb + 4 * a + i >= lim[r]) y[r][kb][i] = -kInf;
+          for (int i = 0; i < 4; ++i) y[r][kb][i] = row + 4 * a + i < stop ? y[r][kb][i] : -kInf;
         }
       }
       float mx = y[r][0][0];
@@ -636,7 +707,8 @@ __global__ __launch_bounds__(kThreads, NR > 1 && NEW ? 1 : 2) void paged_attn_ke
             for (int t = 0; t < 2; ++t) o[r][db] = mma16<F16>(vf, pf[r][st][t], o[r][db]);
         }
     };
-    if (whole) values(Constant<false>{});
+    // (one token attends all rows that were read)
+    if (whole || p.T == 1) values(Constant<false>{});
     else values(Constant<true>{});
     __builtin_amdgcn_s_waitcnt(0xC07F);
     wave_fence();
@@ -696,12 +768,12 @@ __global__ __launch_bounds__(kThreads, NR > 1 && NEW ? 1 : 2) void paged_attn_ke
 // K and V tile of 64 rows, 32 vectors each (two blocks of 16, so that every fragment read from LDS feeds two products).
 //   * Waves w and w + 4 share a SIMD and run half a tile apart: while one does products (O^T += V^T P^T of the tile before,
 //     then S^T = K Q^T), the other does its softmax, with workgroup barriers in between.
-//   * Tiles stream through a ring of four stages by 16-byte loads into LDS, issued two tiles ahead; each load's rows lie in one
+//   * Tiles stream through rings of four stages by 16-byte loads into LDS, two tiles before they are wanted; each load's rows lie in one
 //     page, whose table entry came by a scalar load a tile earlier.
 //   * S^T leaves keys 16 kb + 4 a + i of vector x in lane (x, a), which is the order in which two transposed reads bring V's
 //     rows, so the probabilities are operands where they are.
 //   * The exponent's offset moves only when a probability would pass 2^8. Tiles that some vector attends in part, and every tile
-//     of a split whose table names no page somewhere, run after the others in a loop of their own with the mask.
+//     of a split whose table names no page somewhere, take a mask; they come last.
 constexpr int kTileWaves = 8, kTileStages = 4, kTileVecs = 32 * kTileWaves, kTileRows = 64;
 constexpr float kOver = 256.0f;  // 2^8
 
@@ -746,22 +818,14 @@ struct TileLoader {
     for (int i = 0; i < L::LOADS; ++i) x.e[i] = entry(k0 + row0 + L::RPL * kTileWaves * i);
     return x;
   }
-  BB_DEV void load(uint8_t* kt, int wave, int k0, const Entries& x) const {
-    uint8_t* vt = kt + L::BYTES;
+  // This wave's part of the K or V tile of rows k0 .., into `to`: always LOADS loads; rows past the end and of no page land zeros.
+  BB_DEV void load(bool is_v, uint8_t* to, int wave, int k0, const Entries& x) const {
 #pragma unroll
     for (int i = 0; i < L::LOADS; ++i) {
-      const int r = k0 + row0 + L::RPL * kTileWaves * i, left = end - r;
-      const bool mapped = (uint32_t)x.e[i] < (uint32_t)c.pages;
-      const int page = mapped ? x.e[i] : 0, in = r & ((1 << c.page_log2) - 1);
-      const int live = !mapped || left < 0 ? 0 : left < L::RPL ? left : L::RPL;
-      rows(kh + page * c.skp + in * c.skr, live, (uint32_t)c.skr * 2, kt + 1024 * (wave + kTileWaves * i), koff[i]);
-      rows(vh + page * c.svp + in * c.svr, live, (uint32_t)c.svr * 2, vt + 1024 * (wave + kTileWaves * i), voff[i]);
+      const int r = k0 + row0 + L::RPL * kTileWaves * i, page = (uint32_t)x.e[i] < (uint32_t)c.pages ? x.e[i] : -1;
+      const PageRows at = page_rows(c, is_v, is_v ? vh : kh, page, r, end - r < L::RPL ? end - r : L::RPL, 2 * D);
+      load_rows<0>(at, to + 1024 * (wave + kTileWaves * i), is_v ? voff[i] : koff[i]);
     }
-  }
-  BB_DEV static void rows(const uint16_t* base, int live, uint32_t row_bytes, uint8_t* to, uint32_t off) {
-    const uint32_t bytes = live > 0 ? (live - 1) * row_bytes + 2 * D : 0;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)bytes, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, reinterpret_cast<lds_void*>(reinterpret_cast<uintptr_t>(to)), 16, off, 0, 0, 0);
   }
 };
 
@@ -893,43 +957,68 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
   using L = TileLds<D>;
   constexpr int STAGE = 2 * L::BYTES, NV = D / 8, NF = D / 4, ROW = D + 4;
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kTileStages * STAGE];
+  __shared__ int odd[kTileStages];  // whether V's tile there may hold values that are not finite (never taken back)
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 15, a = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), late = wave >> 2;  // waves w and w + 4 share a SIMD
+  if (tid < kTileStages) odd[tid] = 0;  // (the barrier before the first products comes before any use)
   const Item it = find_item(p, blockIdx.x, lane);
+  if (it.zero) store_zeros(p, it, D, tid, 64 * kTileWaves);
   if (!it.live) return;
   const Sequence s = sequence(p.c, p.T, it.b);
   const int keys = __builtin_amdgcn_readfirstlane(pair_keys(p, s, it.tile));
   const int u0 = __builtin_amdgcn_readfirstlane(split_begin(it.units, it.splits, it.split));
   const int u1 = __builtin_amdgcn_readfirstlane(split_begin(it.units, it.splits, it.split + 1));
   const int begin = u0 * kTileRows, end = u1 * kTileRows < keys ? u1 * kTileRows : keys;
+  const int n_tiles = (end - begin + kTileRows - 1) / kTileRows;  // 1 at least
   const int v0 = it.tile * kTileVecs;
   const int R = p.T * p.G - v0 < kTileVecs ? p.T * p.G - v0 : kTileVecs;
+  const bool live = 32 * wave < R;  // a wave without vectors only loads
 
+  // Tile i's K and V are in stage i % 4 of their halves of the ring.
+  const TileLoader<D> in(p.c, it.b, it.g, end, wave, lane);
+  auto k_at = [&](int i) { return ring + (i & (kTileStages - 1)) * L::BYTES; };
+  auto v_at = [&](int i) { return ring + (kTileStages + (i & (kTileStages - 1))) * L::BYTES; };
+  auto entries = [&](int i) { return in.entries(begin + kTileRows * i); };
+  auto fetch_k = [&](int i, const typename TileLoader<D>::Entries& e) { in.load(false, k_at(i), wave, begin + kTileRows * i, e); };
+  auto fetch_v = [&](int i, const typename TileLoader<D>::Entries& e) { in.load(true, v_at(i), wave, begin + kTileRows * i, e); };
+  typename TileLoader<D>::Entries e0 = entries(0), e1 = entries(1), e2 = entries(2);
+
+  // The queries' and the table's loads go out before the first tiles', which they then need not wait for.
   TileState<D> t;
   int lim[2];
 #pragma unroll
   for (int rb = 0; rb < 2; ++rb) {
-    const int i = 32 * wave + 16 * rb + x, v = i < R ? v0 + i : v0, j = v / p.G, h = it.g * p.G + v - j * p.G;
+    const int i = 32 * wave + 16 * rb + x, v = i < R ? v0 + i : v0, j = token_of(p, v), h = it.g * p.G + v - j * p.G;
     lim[rb] = i < R ? s.seen(j) : 0;
     const uint16_t* qr = p.q + it.b * p.sq0 + h * p.sq1 + j * p.sq2 + 8 * a;
 #pragma unroll
     for (int ds = 0; ds < D / 32; ++ds) t.qf[rb][ds] = as_bf16x8(ld16(qr + 32 * ds));
-#pragma unroll
-    for (int db = 0; db < D / 16; ++db) t.o[db][rb] = f32x4_t{0, 0, 0, 0};
-    t.m[rb] = kLowest;
-    t.l[rb] = 0.0f;
   }
-  const bool live = 32 * wave < R;  // a wave without vectors only loads
-  const TileLoader<D> in(p.c, it.b, it.g, end, wave, lane);
+  uint32_t most = 0;  // of the entries of the split's rows
+  for (int w = (begin >> p.c.page_log2) + lane; w <= (end - 1) >> p.c.page_log2; w += 64) {
+    const uint32_t e = (uint32_t)p.c.table[it.b * p.c.st + w];
+    most = e > most ? e : most;
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  // Round j of loads, in the softmax of tile j, is K of tile j + 3 (over tile j - 1's, whose products the other group too is
+  // past) and V of tile j + 2 (over tile j - 2's): K j + 1 and V j, wanted next, are two rounds old.
+  constexpr int kRound = 2 * L::LOADS;
+  fetch_k(0, e0);
+  fetch_k(1, e1);
+  fetch_v(0, e0);
+  fetch_k(2, e2);
+  fetch_v(1, e1);
+  e0 = entries(3);  // of the next round's K; e2: of its V
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+    for (int ds = 0; ds < D / 32; ++ds) asm volatile("" : "+v"(t.qf[rb][ds]));  // awaited here
+
   // Tiles without a mask: below the rows that the tile's first token attends, if the table names a page for all of the split.
   // (What padding gets there is not stored.)
-  const int n_tiles = end > begin ? (end - begin + kTileRows - 1) / kTileRows : 0;
-  int open = __builtin_amdgcn_readfirstlane(s.seen(v0 / p.G)) - begin;
-  open = open < 0 ? 0 : open / kTileRows < n_tiles ? open / kTileRows : n_tiles;
-  bool hole = false;
-  for (int w = (begin >> p.c.page_log2) + lane; begin < end && w <= (end - 1) >> p.c.page_log2; w += 64)
-    hole = hole || (uint32_t)p.c.table[it.b * p.c.st + w] >= (uint32_t)p.c.pages;
-  if (__builtin_amdgcn_ballot_w64(hole)) open = 0;
+  const bool holes = __builtin_amdgcn_ballot_w64(most >= (uint32_t)p.c.pages) != 0;
+  int open = __builtin_amdgcn_readfirstlane(s.seen(token_of(p, v0))) - begin;
+  open = open < 0 || holes ? 0 : open / kTileRows < n_tiles ? open / kTileRows : n_tiles;
 
   TileReads<D> rd;
   const int vrow = 4 * a + (x >> 2);
@@ -938,124 +1027,144 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
 #pragma unroll
   for (int db = 0; db < D / 16; ++db) rd.v[db] = 2 * D * vrow + 16 * ((2 * db + ((x >> 1) & 1)) ^ v_swz<D>(vrow)) + 8 * (x & 1);
 
-  auto stage = [&](int i) { return ring + (i & (kTileStages - 1)) * STAGE; };
-  auto fetch = [&](int i, const typename TileLoader<D>::Entries& e) { in.load(stage(i), wave, begin + kTileRows * i, e); };
-  auto entries = [&](int i) { return in.entries(begin + kTileRows * i); };
-  auto wait_tile = [&](bool one_in_flight) {  // all but the youngest tile's loads (all, without one in flight)
-    if (one_in_flight) __builtin_amdgcn_s_waitcnt(0x0F70 | 2 * L::LOADS);
-    else __builtin_amdgcn_s_waitcnt(0x0F70);
-  };
-  bool seen[2] = {open > 0, open > 0};
-  // The mask of tile i, and its softmax.
-  auto masked = [&](int i) {
+  int top[2] = {-1, -1};  // a row before `lim` on a page of the table's, where tiles with a mask have one
+  // The mask of tile i.
+  auto mask = [&](int i) {
     const int k0 = begin + kTileRows * i;
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
-      const bool mapped = k0 + 16 * kb < end && (uint32_t)in.entry(k0 + 16 * kb) < (uint32_t)p.c.pages;
+      int to = end;  // the block's rows from here on are not attended
+      if (holes && (uint32_t)in.entry(k0 + 16 * kb) >= (uint32_t)p.c.pages) to = 0;
 #pragma unroll
       for (int rb = 0; rb < 2; ++rb) {
-        seen[rb] = seen[rb] || (mapped && k0 + 16 * kb < lim[rb]);
+        const int stop = to < lim[rb] ? to : lim[rb], first = k0 + 16 * kb;
+        top[rb] = first < stop ? first : top[rb];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!mapped || k0 + 16 * kb + 4 * a + e >= lim[rb]) t.s[kb][rb][e] = -kInf;
+        for (int e = 0; e < 4; ++e) t.s[kb][rb][e] = first + 4 * a + e < stop ? t.s[kb][rb][e] : -kInf;
       }
     }
-    tile_softmax<F16, D>(t, p.scale);
   };
-  // Products of V's tile i that vectors attend in part: values that are not finite apart, as in the kernel above.
+  // A probability of 0 times a value that is not finite would be NaN. So each wave looks at the V rows that it loaded of a tile
+  // that vectors attend in part, before the barrier that lets the others at them, and where one is not finite the products take
+  // such values out of the operand, and vectors that attend one are NaN in that column.
+  auto look_at_values = [&](int i) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int j = 0; j < L::LOADS; ++j) {
+      const u32x4_t w = lds16(lds_addr(v_at(i)) + 1024 * (wave + kTileWaves * j) + 16 * lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) any |= not_finite<F16>(w[e]);
+    }
+    if (__builtin_amdgcn_ballot_w64(any != 0)) odd[i & (kTileStages - 1)] = 1;
+  };
+  auto odd_values = [&](int i) { return __builtin_amdgcn_readfirstlane(odd[i & (kTileStages - 1)]) != 0; };
   auto masked_values = [&](int i) {
-    const int k0 = begin + kTileRows * i;
-    const uint32_t vt = lds_addr(stage(i) + L::BYTES);
+    const uint32_t vt = lds_addr(v_at(i));
+    constexpr uint32_t one = F16 ? 0x3c003c00u : 0x3f803f80u;
 #pragma unroll
     for (int f = 0; f < NV; ++f) {
-      u32x4_t w = tile_fragment<D>(rd, 0, vt, f);
-      u32x4_t bad;
+      const int st = f / (D / 16), db = f % (D / 16);
+      int key0 = begin + kTileRows * i + 32 * st + 4 * a;
+      asm volatile("" : "+v"(key0));  // (nothing of this is held across the loop around)
+      u32x4_t v = tile_fragment<D>(rd, 0, vt, f), bad;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        bad[e] = not_finite<F16>(w[e]);
-        w[e] &= ~bad[e];
+        bad[e] = not_finite<F16>(v[e]);
+        v[e] &= ~bad[e];
+        bad[e] &= one;
       }
-      if (__builtin_amdgcn_ballot_w64((bad[0] | bad[1] | bad[2] | bad[3]) != 0)) {
-        constexpr uint32_t one = F16 ? 0x3c003c00u : 0x3f803f80u;
-        const int st = f / (D / 16), db = f % (D / 16);
+      tile_product<F16, D>(t, f, as_bf16x8(v));
 #pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-          u32x4_t att;
+      for (int rb = 0; rb < 2; ++rb) {
+        u32x4_t att;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = k0 + 32 * st + 16 * (e / 2) + 4 * a + 2 * (e % 2);
-            att[e] = (key < lim[rb] ? one & 0xffffu : 0u) | (key + 1 < lim[rb] ? one & 0xffff0000u : 0u);
-          }
-          const f32x4_t hits = mma16<F16>(as_bf16x8(u32x4_t{bad[0] & one, bad[1] & one, bad[2] & one, bad[3] & one}),
-                                          as_bf16x8(att), f32x4_t{0, 0, 0, 0});
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (hits[e] > 0.0f) t.o[db][rb][e] = __builtin_nanf("");
+        for (int e = 0; e < 4; ++e) {
+          const int key = key0 + 16 * (e / 2) + 2 * (e % 2);
+          att[e] = (key < lim[rb] ? one & 0xffffu : 0u) | (key + 1 < lim[rb] ? one & 0xffff0000u : 0u);
         }
+        const f32x4_t hits = mma16<F16>(as_bf16x8(bad), as_bf16x8(att), f32x4_t{0, 0, 0, 0});
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (hits[e] > 0.0f) t.o[db][rb][e] = __builtin_nanf("");
       }
-      tile_product<F16, D>(t, f, as_bf16x8(w));
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  if (n_tiles > 0) {
-    typename TileLoader<D>::Entries e = entries(0);
-    fetch(0, e);
-    e = entries(1);
-    if (n_tiles > 1) fetch(1, e);
-    e = entries(2);
-    wait_tile(n_tiles > 1);
-    ring_barrier();
-    if (late) ring_barrier();  // the second group runs one phase behind
-    if (n_tiles > 2) fetch(2, e);
-    e = entries(3);
-    if (live) tile_products<F16, D, NV, NF>(t, rd, lds_addr(stage(0)), 0);
-    wait_tile(n_tiles > 2);
-    ring_barrier();
-    if (live && open > 0) tile_softmax<F16, D>(t, p.scale);
-    else if (live) masked(0);
-    ring_barrier();
-    for (int i = 1; i < open; ++i) {
-      __builtin_amdgcn_s_setprio(1);
-      if (live) tile_products<F16, D, 0, NF>(t, rd, lds_addr(stage(i)), lds_addr(stage(i - 1) + L::BYTES));
-      __builtin_amdgcn_s_setprio(0);
-      wait_tile(false);  // tile i + 1 has landed
-      ring_barrier();
-      if (live) tile_softmax<F16, D>(t, p.scale);
-      // into the stage of tile i - 2, which every wave has read
-      if (i + 2 < n_tiles) fetch(i + 2, e);
-      e = entries(i + 3);
-      ring_barrier();
-    }
-#pragma unroll 1
-    for (int i = open > 1 ? open : 1; i < n_tiles; ++i) {
-      if (live) {
-        masked_values(i - 1);
-        tile_products<F16, D, NV, NF>(t, rd, lds_addr(stage(i)), 0);
-      }
-      wait_tile(false);
-      ring_barrier();
-      if (live) masked(i);
-      if (i + 2 < n_tiles) fetch(i + 2, e);
-      e = entries(i + 3);
-      ring_barrier();
-    }
-    if (live) masked_values(n_tiles - 1);
-    if (!late) ring_barrier();  // the groups meet again
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb) {
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) t.o[db][rb] = f32x4_t{0, 0, 0, 0};
+    t.m[rb] = kLowest;
+    t.l[rb] = 0.0f;
   }
-
+  __builtin_amdgcn_s_waitcnt(0x0F70 | 2 * kRound);  // K of tile 0 has landed
+  ring_barrier();
+  if (late) ring_barrier();  // the second group runs one phase behind
+  if (live) tile_products<F16, D, NV, NF>(t, rd, lds_addr(k_at(0)), 0);
+  __builtin_amdgcn_s_waitcnt(0x0F70 | kRound);
+  if (open == 0) look_at_values(0);
+  ring_barrier();
+  if (live) {
+    if (open == 0) mask(0);
+    tile_softmax<F16, D>(t, p.scale);
+  }
+  auto round = [&](int j) {
+    fetch_k(j + 3, e0);
+    fetch_v(j + 2, e2);
+    e2 = e0;
+    e0 = entries(j + 4);
+  };
+  round(0);
+  ring_barrier();
+  for (int i = 1; i < open; ++i) {
+    __builtin_amdgcn_s_setprio(1);
+    if (live) tile_products<F16, D, 0, NF>(t, rd, lds_addr(k_at(i)), lds_addr(v_at(i - 1)));
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_s_waitcnt(0x0F70 | kRound);
+    ring_barrier();
+    if (live) tile_softmax<F16, D>(t, p.scale);
+    round(i);
+    ring_barrier();
+  }
+  auto values = [&](int i) {
+    if (i >= open && odd_values(i)) masked_values(i);
+    else tile_products<F16, D, 0, NV>(t, rd, 0, lds_addr(v_at(i)));
+  };
+#pragma unroll 1
+  for (int i = open > 1 ? open : 1; i < n_tiles; ++i) {
+    if (live) {
+      values(i - 1);
+      tile_products<F16, D, NV, NF>(t, rd, lds_addr(k_at(i)), 0);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70 | kRound);
+    look_at_values(i);
+    ring_barrier();
+    if (live) {
+      mask(i);
+      tile_softmax<F16, D>(t, p.scale);
+    }
+    round(i);
+    ring_barrier();
+  }
+  if (live) values(n_tiles - 1);
+  if (!late) ring_barrier();  // the groups meet again
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // nothing lands in LDS any more
 #pragma unroll
   for (int rb = 0; rb < 2; ++rb) {
     const int i = 32 * wave + 16 * rb + x;
     const float l = quarters_sum(t.l[rb]);
+    const bool seen = lim[rb] > 0 && (open > 0 || top[rb] >= 0);
+    const float inv = 1.0f / l;  // (another rounding of 2^-24, instead of 64 divisions a lane)
     if (i >= R) continue;
     if (it.splits == 1) {
-      const int v = v0 + i, j = v / p.G, h = it.g * p.G + v - j * p.G;
+      const int v = v0 + i, j = token_of(p, v), h = it.g * p.G + v - j * p.G;
       uint16_t* to = p.out + it.b * p.so0 + h * p.so1 + j * p.so2 + 4 * a;
 #pragma unroll
       for (int db = 0; db < D / 16; ++db) {
         f32x4_t o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = lim[rb] > 0 && seen[rb] ? t.o[db][rb][e] / l : 0.0f;
+        for (int e = 0; e < 4; ++e) o[e] = seen ? t.o[db][rb][e] * inv : 0.0f;
         *reinterpret_cast<u32x2_t*>(to + 16 * db) = u32x2_t{pack2<F16>(o[0], o[1]), pack2<F16>(o[2], o[3])};
       }
     } else {
@@ -1063,37 +1172,41 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
 #pragma unroll
       for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f32x4_t*>(to + 16 * db + 4 * a) = t.o[db][rb];
       if (a == 0) {
-        to[D] = lim[rb] > 0 && seen[rb] ? t.m[rb] : -kInf;
+        to[D] = seen ? t.m[rb] : -kInf;
         to[D + 1] = l;
       }
     }
   }
 }
 
-// The splits' states of a vector under one maximum. A workgroup merges p.merge_vecs vectors of a pair, its quarter or eighth
-// waves one split each in turn.
+// The splits' states of each vector under one maximum. Split s of n of a pair merges, in gridDim.y workgroups, the s-th part of
+// its vectors: a group of D / 4 lanes a vector, or all groups of the workgroup one vector where that is its part.
 template <int D, bool F16>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttnParams p) {
   constexpr int LPV = D / 4, NG = kThreads / LPV, ROW = D + 4;
   __shared__ float st[NG][ROW];
   const int tid = threadIdx.x, grp = tid / LPV, d = 4 * (tid % LPV);
-  const int per_tile = p.VT / p.merge_vecs, b = blockIdx.z, g = blockIdx.y, tile = blockIdx.x / per_tile;
-  const int first = tile * p.VT + (blockIdx.x % per_tile) * p.merge_vecs;
-  if (first >= p.T * p.G) return;
-  const int2 pl = p.plan[b * p.tiles + p.tiles - 1 - tile];
-  const int splits = pl.x;
-  if (splits < 2) return;
-  for (int v = first; v < first + p.merge_vecs && v < p.T * p.G; ++v) {
-    const float* src = p.part + ((int64_t)(pl.y + g * splits) * p.VT + v - tile * p.VT) * ROW;
-    float M = -kInf, L = 0.0f;
-    f32x4_t O = {0, 0, 0, 0};
-    constexpr int U = 4;  // splits whose loads are in flight together
-    for (int i = grp; i < splits; i += U * NG) {
+  const int4 rec = p.plan[blockIdx.x];
+  if ((int)blockIdx.x >= p.plan[p.slots].x) return;
+  const int b = rec.x, tile = rec.y, g = rec.z, split = rec.w & 0xffff, splits = rec.w >> 16;
+  const int R = p.T * p.G - tile * p.VT < p.VT ? p.T * p.G - tile * p.VT : p.VT;
+  const int parts = splits * gridDim.y, part = split * gridDim.y + blockIdx.y;
+  const int from = R * part / parts, to = R * (part + 1) / parts;
+  const float* slots = p.part + (int64_t)(blockIdx.x - split) * p.VT * ROW;
+  float M, L;
+  f32x4_t O;
+  auto merge = [&](int v, int first, int step) {  // splits first, first + step, ..
+    const float* src = slots + (int64_t)v * ROW;
+    constexpr int U = 4;  // whose loads are in flight together
+    M = -kInf;
+    L = 0.0f;
+    O = f32x4_t{0, 0, 0, 0};
+    for (int i = first; i < splits; i += U * step) {
       float m[U], l[U], mn = M;
       f32x4_t t[U];
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const int at = i + k * NG < splits ? i + k * NG : i;
+        const int at = i + k * step < splits ? i + k * step : i;
         const float* f = src + (int64_t)at * p.VT * ROW;
         const u32x2_t ml = *reinterpret_cast<const u32x2_t*>(f + D);
         m[k] = __uint_as_float(ml[0]);
@@ -1102,7 +1215,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttnParams p
       }
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        if (i + k * NG >= splits) m[k] = -kInf;
+        if (i + k * step >= splits) m[k] = -kInf;
         mn = fmaxf(mn, m[k]);
       }
       const float off = mn == -kInf ? 0.0f : mn, was = fast_exp2(M - off);
@@ -1112,37 +1225,44 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttnParams p
       for (int j = 0; j < 4; ++j) O[j] *= was;
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        if (i + k * NG >= splits) continue;
+        if (i + k * step >= splits) continue;
         const float wt = fast_exp2(m[k] - off);
         L = fmaf(wt, l[k], L);
 #pragma unroll
         for (int j = 0; j < 4; ++j) O[j] = fmaf(wt, t[k][j], O[j]);
       }
     }
-    __syncthreads();
-    *reinterpret_cast<f32x4_t*>(&st[grp][d]) = O;
-    if (d == 0) {
-      st[grp][D] = M;
-      st[grp][D + 1] = L;
+  };
+  if (to - from > 1) {
+    for (int v = from + grp; v < to; v += NG) {
+      merge(v, 0, 1);
+      store_output<F16>(p, b, g, tile * p.VT + v, d, O, M, L);
     }
-    __syncthreads();
-    if (grp == 0) {
-      M = -kInf;
-#pragma unroll
-      for (int i = 0; i < NG; ++i) M = fmaxf(M, st[i][D]);
-      const float off = M == -kInf ? 0.0f : M;
-      L = 0.0f;
-      O = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        const float wt = fast_exp2(st[i][D] - off);
-        L = fmaf(wt, st[i][D + 1], L);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) O[k] = fmaf(wt, st[i][d + k], O[k]);
-      }
-      store_output<F16>(p, b, g, v, d, O, M, L);
-    }
+    return;
   }
+  if (to == from) return;
+  merge(from, grp, NG);
+  *reinterpret_cast<f32x4_t*>(&st[grp][d]) = O;
+  if (d == 0) {
+    st[grp][D] = M;
+    st[grp][D + 1] = L;
+  }
+  __syncthreads();
+  if (grp != 0) return;
+  M = -kInf;
+#pragma unroll
+  for (int i = 0; i < NG; ++i) M = fmaxf(M, st[i][D]);
+  const float off = M == -kInf ? 0.0f : M;
+  L = 0.0f;
+  O = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < NG; ++i) {
+    const float wt = fast_exp2(st[i][D] - off);
+    L = fmaf(wt, st[i][D + 1], L);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) O[k] = fmaf(wt, st[i][d + k], O[k]);
+  }
+  store_output<F16>(p, b, g, tile * p.VT + from, d, O, M, L);
 }
 
 }  // namespace
@@ -1167,7 +1287,7 @@ hipError_t attend(const PagedAttnParams& p, hipStream_t stream) {
   else if (p.knew) paged_attn_kernel<D, F16, NR, true><<<p.grid, kThreads, 0, stream>>>(p);
   else paged_attn_kernel<D, F16, NR, false><<<p.grid, kThreads, 0, stream>>>(p);
   if (p.part) {
-    const dim3 grid(p.tiles * (p.VT / p.merge_vecs), p.Hkv, p.B);
+    const dim3 grid(p.slots, p.VT > 32 ? 4 : 1);  // a tile's parts are many vectors
     paged_merge_kernel<D, F16><<<grid, kThreads, 0, stream>>>(p);
   }
   return hipGetLastError();
