@@ -1001,8 +1001,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
   }
   __builtin_amdgcn_sched_barrier(0);
   // Round j of loads, in the softmax of tile j, is K of tile j + 3 (over tile j - 1's, whose products the other group too is
-  // past) and V of tile j + 2 (over tile j - 2's): K j + 1 and V j, wanted next, are two rounds old.
-  constexpr int kRound = 2 * L::LOADS;
+  // past) and V of tile j + 2 (over tile j - 2's): K j + 1 and V j, wanted next, are two rounds old. At head_dim 64, where the
+  // softmax is the longer phase, the round comes behind the products instead (the same tiles are free by then).
+  constexpr int kRound = 2 * L::LOADS, kFlight = D == 64 ? 2 * kRound : kRound;
   fetch_k(0, e0);
   fetch_k(1, e1);
   fetch_v(0, e0);
@@ -1101,30 +1102,32 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
   __builtin_amdgcn_s_waitcnt(0x0F70 | 2 * kRound);  // K of tile 0 has landed
   ring_barrier();
   if (late) ring_barrier();  // the second group runs one phase behind
-  if (live) tile_products<F16, D, NV, NF>(t, rd, lds_addr(k_at(0)), 0);
-  __builtin_amdgcn_s_waitcnt(0x0F70 | kRound);
-  if (open == 0) look_at_values(0);
-  ring_barrier();
-  if (live) {
-    if (open == 0) mask(0);
-    tile_softmax<F16, D>(t, p.scale);
-  }
   auto round = [&](int j) {
     fetch_k(j + 3, e0);
     fetch_v(j + 2, e2);
     e2 = e0;
     e0 = entries(j + 4);
   };
-  round(0);
+  if (live) tile_products<F16, D, NV, NF>(t, rd, lds_addr(k_at(0)), 0);
+  if (D == 64) round(0);
+  __builtin_amdgcn_s_waitcnt(0x0F70 | kFlight);
+  if (open == 0) look_at_values(0);
+  ring_barrier();
+  if (live) {
+    if (open == 0) mask(0);
+    tile_softmax<F16, D>(t, p.scale);
+  }
+  if (D != 64) round(0);
   ring_barrier();
   for (int i = 1; i < open; ++i) {
     __builtin_amdgcn_s_setprio(1);
     if (live) tile_products<F16, D, 0, NF>(t, rd, lds_addr(k_at(i)), lds_addr(v_at(i - 1)));
+    if (D == 64) round(i);
     __builtin_amdgcn_s_setprio(0);
-    __builtin_amdgcn_s_waitcnt(0x0F70 | kRound);
+    __builtin_amdgcn_s_waitcnt(0x0F70 | kFlight);
     ring_barrier();
     if (live) tile_softmax<F16, D>(t, p.scale);
-    round(i);
+    if (D != 64) round(i);
     ring_barrier();
   }
   auto values = [&](int i) {
@@ -1137,14 +1140,15 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
       values(i - 1);
       tile_products<F16, D, NV, NF>(t, rd, lds_addr(k_at(i)), 0);
     }
-    __builtin_amdgcn_s_waitcnt(0x0F70 | kRound);
+    if (D == 64) round(i);
+    __builtin_amdgcn_s_waitcnt(0x0F70 | kFlight);
     look_at_values(i);
     ring_barrier();
     if (live) {
       mask(i);
       tile_softmax<F16, D>(t, p.scale);
     }
-    round(i);
+    if (D != 64) round(i);
     ring_barrier();
   }
   if (live) values(n_tiles - 1);
