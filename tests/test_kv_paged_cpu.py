@@ -148,3 +148,129 @@ def test_plain_form_is_attention_over_contiguous_rows():
     out, _ = plain.attend(q, kp, vp, table, [n], 0.125, None, 0.0)
     x[:, :, 16:32] = -torch.inf
     assert torch.allclose(out[0], torch.softmax(x, -1) @ v, atol=1e-12)
+
+
+# ---------------------------------------------------------------- the cache's lengths and pages
+def _cache(batch=3, pages=10, page=16, rows=None, layers=2):
+    from transformers import LlamaConfig
+
+    from bigger_bird_amd import make_paged_cache
+
+    cfg = LlamaConfig(vocab_size=32, hidden_size=256, intermediate_size=64, num_hidden_layers=layers, num_attention_heads=4,
+                      num_key_value_heads=2)
+    return make_paged_cache(cfg, batch, pages, page, rows, device="cpu")
+
+
+def _run(cache, t, padded=False, positions=1):
+    """A forward pass's part in the bookkeeping: every layer begins the step of t columns."""
+    for layer in cache.layers:
+        layer.begin(t, padded, positions)
+
+
+def _consistent(cache):
+    held = [p for seq in cache._pages for p in seq]
+    assert sorted(held + cache._free) == list(range(cache.arena.shape[2]))  # every page once
+    for b, pages in enumerate(cache._pages):
+        assert len(pages) == -(-cache.lengths[b] // cache.page)
+        assert cache.table[b].tolist() == pages + [-1] * (cache.width - len(pages))
+    assert cache.lens.tolist() == cache.lengths
+
+
+def test_cache_steps():
+    c = _cache()
+    assert c.get_seq_length() == 0 and c.arena.shape == (2, 2, 10, 2, 16, 64) and len(c.layers) == 2
+    _run(c, 20)
+    _consistent(c)
+    assert c.lengths == [20] * 3 and len(c._free) == 4 and c.get_seq_length() == 20 and c._new_of(20) is None
+    _run(c, 1)
+    assert c.lengths == [21] * 3
+    c.extend([0, 12, 1])
+    assert c.get_seq_length() == 21 and c.positions().tolist() == [list(range(21, 33))] * 3
+    with pytest.raises(ValueError, match="has not run"):
+        c.extend([1, 1, 1])
+    with pytest.raises(ValueError, match="12 new tokens, the input 5 columns"):
+        c.layers[0].begin(5, False, 3)
+    _run(c, 13, padded=True)
+    assert c.lengths == [21, 33, 22] and c._new_of(13).tolist() == [0, 12, 1] and c.get_seq_length() == 33
+    _consistent(c)
+    with pytest.raises(ValueError, match="need position_ids"):
+        _run(c, 1)
+    assert c.lengths == [21, 33, 22]  # refused before anything changed
+    _run(c, 1, positions=3)
+    assert c.positions(2).tolist() == [[22, 23], [34, 35], [23, 24]]
+    _consistent(c)
+
+
+def test_cache_refusals_change_nothing():
+    c = _cache(batch=2, pages=3, page=16, rows=32)
+    with pytest.raises(ValueError, match="by a mask"):
+        _run(c, 5, padded=True)
+    with pytest.raises(ValueError, match="past the rows"):
+        c.extend([33, 0])
+    with pytest.raises(ValueError, match="no free pages"):
+        c.extend([17, 17])
+    for bad in ([1], [1, -1]):
+        with pytest.raises(ValueError, match="one count"):
+            c.extend(bad)
+    assert c.lengths == [0, 0] and len(c._free) == 3 and not c._left
+    _consistent(c)
+    c.extend([17, 16])
+    _run(c, 17, positions=2)
+    with pytest.raises(ValueError, match="no free pages"):
+        _run(c, 1, positions=2)
+    assert c.lengths == [17, 16]
+    _consistent(c)
+    for kw in (dict(page=8), dict(page=48), dict(pages=0), dict(batch=0)):
+        with pytest.raises(ValueError, match="PagedCache"):
+            _cache(**kw)
+    with pytest.raises(ValueError, match="RDAttention only"):
+        c.update(torch.zeros(2, 2, 1, 64), torch.zeros(2, 2, 1, 64), 0)
+
+
+def test_cache_truncate_and_release():
+    c = _cache(batch=3, pages=9, page=16)
+    c.extend([40, 33, 16])
+    _run(c, 40, positions=3)
+    c.truncate([32, 33, 0])
+    assert c.lengths == [32, 33, 0] and len(c._free) == 4
+    _consistent(c)
+    for bad in ([33, 33, 0], [32, 33, -1], [32]):
+        with pytest.raises(ValueError, match="one length"):
+            c.truncate(bad)
+    c.release(1)
+    assert c.lengths == [32, 0, 0] and len(c._free) == 7
+    _consistent(c)
+    c.extend([0, 90, 5])  # a step that does not run is taken back
+    c.truncate([32, 0, 0])
+    _consistent(c)
+    c.crop(-3)
+    assert c.lengths == [29, 0, 0]
+    with pytest.raises(NotImplementedError):
+        c.crop(3)
+    c.release([0, 2])
+    assert c.nbytes() == 0 and len(c._free) == 9
+    c.reset()
+    _consistent(c)
+
+
+def test_rdattention_refuses_what_a_paged_cache_cannot_do():
+    from types import SimpleNamespace
+
+    from bigger_bird_amd import RDAttention
+
+    c = _cache(batch=2)
+    lin = torch.nn.Linear(256, 256, bias=False)
+    kv = torch.nn.Linear(256, 128, bias=False)
+    base = SimpleNamespace(config=SimpleNamespace(num_attention_heads=4, num_key_value_heads=2), layer_idx=0, head_dim=64,
+                           scaling=0.125, q_proj=lin, k_proj=kv, v_proj=kv, o_proj=lin)
+    pe = torch.ones(1, 3, 64), torch.zeros(1, 3, 64)
+    with pytest.raises(ValueError, match="holds no gradients"):
+        RDAttention(base)(torch.zeros(2, 3, 256), pe, None, c)
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="kv_evict"):
+            RDAttention(base, kv_evict=True)(torch.zeros(2, 3, 256), pe, None, c)
+        with pytest.raises(ValueError, match="2 sequences, the input has 3"):
+            RDAttention(base)(torch.zeros(3, 3, 256), pe, None, c)
+        with pytest.raises(ValueError, match="by a mask"):
+            RDAttention(base)(torch.zeros(2, 3, 256), pe, torch.zeros(2, 1, 3, 3), c)
+    assert c.lengths == [0, 0]

@@ -492,3 +492,144 @@ def test_refusals(dev):
         with pytest.raises(ValueError, match=msg):
             fn()
         assert torch.equal(before.view(torch.int16), kp.view(torch.int16))
+
+
+# ---------------------------------------------------------------- under a model
+def _model(dev, arm, dtype=BF16, kv_heads=2, **kw):
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    from bigger_bird_amd import install
+
+    cfg = LlamaConfig(vocab_size=512, hidden_size=1024, intermediate_size=1024, num_hidden_layers=2, num_attention_heads=8,
+                      num_key_value_heads=kv_heads, max_position_embeddings=4096, rope_theta=500000.0, attn_implementation="sdpa")
+    torch.manual_seed(0)
+    m = LlamaForCausalLM(cfg).eval().to(dev, dtype)
+    return install(m, arm, **kw)
+
+
+class _Outputs:
+    """Every layer's attention output (the input of o_proj) of each call."""
+
+    def __init__(self, model):
+        self.calls = []
+        for layer in model.model.layers:
+            layer.self_attn.o_proj.register_forward_pre_hook(lambda m, a: self.calls.append(a[0].detach().clone()))
+
+    def take(self):
+        out, self.calls = self.calls, []
+        return out
+
+
+def _alike(got, want, what):
+    """Two runs of one model in 16 bits, the attention of one by other kernels: the bar of the module's other tests."""
+    err = (got.float() - want.float()).abs()
+    assert err.max().item() <= 2e-2 and err.mean().item() <= 2e-3, f"{what}: max {err.max().item():.3e} mean {err.mean().item():.3e}"
+
+
+@pytest.mark.parametrize("arm,dtype", [("dense_rd", BF16), ("rd", BF16), ("rd", FP16)])
+def test_model_batch_against_single_sequences(arm, dtype, dev):
+    """Prompts of unlike lengths in one padded batch, then steps of one token and of several, against each sequence alone on the
+    16-bit cache: every layer's attention output. (A step of several tokens behind cached ones goes token by token there.)"""
+    _say("model", arm, dtype)
+    from transformers import DynamicCache
+
+    from bigger_bird_amd import make_paged_cache
+
+    model = _model(dev, arm, dtype, **({} if arm == "dense_rd" else dict(sink=64, window=512, vertical=128, exact_tail=64)))
+    taken = _Outputs(model)
+    lens = [1000, 300, 17]
+    g = torch.Generator().manual_seed(1)
+    ids = torch.randint(0, 512, (3, 1000), generator=g).to(dev)
+    later = torch.randint(0, 512, (3, 5), generator=g).to(dev)
+    with torch.no_grad():
+        alone = []
+        for b, n in enumerate(lens):
+            cache = DynamicCache(config=model.config)
+            model(input_ids=ids[b:b + 1, :n], past_key_values=cache, use_cache=True)
+            steps = [taken.take()]
+            for i in range(5):
+                model(input_ids=later[b:b + 1, i:i + 1], past_key_values=cache, use_cache=True)
+                steps.append(taken.take())
+            alone.append(steps)
+        cache = make_paged_cache(model.config, 3, 120, page=16, dtype=dtype, device=dev)
+        for part in cache.arena.flatten(0, 1):
+            part.fill_(float("nan"))  # what memory held before
+        cache.extend(lens)
+        model(input_ids=ids, position_ids=cache.positions(1000), past_key_values=cache, use_cache=True)
+        got = taken.take()
+        for b, n in enumerate(lens):
+            for i in range(2):
+                _alike(got[i][b, :n], alone[b][0][i][0], f"prompt {b} layer {i}")
+                assert (got[i][b, n:] == 0).all()
+        assert cache.lengths == lens
+        for i in range(2):  # one token each
+            model(input_ids=later[:, i:i + 1], position_ids=cache.positions(1), past_key_values=cache, use_cache=True)
+            got = taken.take()
+            for b in range(3):
+                for j in range(2):
+                    _alike(got[j][b], alone[b][1 + i][j][0], f"step {i} of {b} layer {j}")
+        cache.extend([3, 0, 2])  # several tokens of some sequences
+        model(input_ids=later[:, 2:5], position_ids=cache.positions(3), past_key_values=cache, use_cache=True)
+        got = taken.take()
+        for b, m in ((0, 3), (2, 2)):
+            for i in range(m):
+                for j in range(2):
+                    _alike(got[j][b, i], alone[b][3 + i][j][0, 0], f"token {i} of {b} layer {j}")
+        assert cache.lengths == [1005, 302, 21]
+        # the drafted tokens of the first are taken back, the third makes room: its pages go to the second
+        cache.truncate([1002, 302, 21])
+        cache.release(2)
+        cache.extend([1, 3, 0])
+        ids2 = torch.stack([later[0, 2:5], later[1, 2:5], later[2, 2:5]])
+        model(input_ids=ids2, position_ids=cache.positions(3), past_key_values=cache, use_cache=True)
+        got = taken.take()
+        for j in range(2):
+            _alike(got[j][0, 0], alone[0][3][j][0, 0], "after truncate")
+            for i in range(3):
+                _alike(got[j][1, i], alone[1][3 + i][j][0, 0], "after release")
+            assert (got[j][0, 1:] == 0).all() and (got[j][2] == 0).all()
+
+
+def test_model_generate(dev):
+    """Hugging Face's generate over a paged cache: prompts of one length, greedy, the tokens of each alone on the 16-bit cache as
+    far as the logits' order is clear of 16-bit differences."""
+    _say("generate")
+    from transformers import DynamicCache
+
+    from bigger_bird_amd import make_paged_cache
+
+    model = _model(dev, "dense_rd")
+    ids = torch.randint(0, 512, (2, 40), generator=torch.Generator().manual_seed(2)).to(dev)
+    with torch.no_grad():
+        cache = make_paged_cache(model.config, 2, 20, page=16, device=dev)
+        got = model.generate(ids, past_key_values=cache, do_sample=False, max_new_tokens=12, pad_token_id=0)
+        assert got.shape == (2, 52) and cache.lengths == [51, 51]
+        for b in range(2):
+            one = DynamicCache(config=model.config)
+            out = model(input_ids=ids[b:b + 1], past_key_values=one, use_cache=True)
+            for i in range(12):
+                logits = out.logits[0, -1].float()
+                token = got[b, 40 + i]
+                assert logits[token] >= logits.max() - 0.05
+                out = model(input_ids=token.view(1, 1), past_key_values=one, use_cache=True)
+
+
+def test_model_refusals_on_a_paged_cache(dev):
+    _say("model refusals")
+    from bigger_bird_amd import make_paged_cache
+
+    model = _model(dev, "dense_rd")
+    ids = torch.zeros(2, 8, dtype=torch.long, device=dev)
+    cache = make_paged_cache(model.config, 2, 20, page=16, device=dev)
+    mask = torch.ones(2, 8, dtype=torch.long, device=dev)
+    mask[1, :3] = 0
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="not by a mask"):
+            model(input_ids=ids, attention_mask=mask, past_key_values=cache, use_cache=True)
+        assert cache.lengths == [0, 0]
+        cache.extend([8, 5])
+        model(input_ids=ids, position_ids=cache.positions(8), past_key_values=cache, use_cache=True)
+        with pytest.raises(ValueError, match="need position_ids"):
+            model(input_ids=ids[:, :1], past_key_values=cache, use_cache=True)
+    with pytest.raises(ValueError, match="holds no gradients"):
+        model(input_ids=ids, past_key_values=cache, use_cache=True)

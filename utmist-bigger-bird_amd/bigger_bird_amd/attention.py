@@ -155,6 +155,9 @@ class RDAttention(nn.Module):
         q = self.q_proj(hidden_states).view(b, t, self.num_heads, self.head_dim).transpose(1, 2)
         k = self.k_proj(hidden_states).view(b, t, self.num_kv_heads, self.head_dim).transpose(1, 2)
         v = self.v_proj(hidden_states).view(b, t, self.num_kv_heads, self.head_dim).transpose(1, 2)
+        paged = self._paged_layer(past_key_values)
+        if paged is not None:
+            return self._forward_paged(paged, q, k, v, position_embeddings, attention_mask)
         if torch.is_grad_enabled() and q.requires_grad:
             return self._forward_autograd(q, k, v, position_embeddings, past_key_values)
         q, k = rope_inplace(q, *position_embeddings), rope_inplace(k, *position_embeddings)
@@ -172,6 +175,51 @@ class RDAttention(nn.Module):
                 self.evict(past_key_values, q, k, v)
         out = out.transpose(1, 2).reshape(b, t, -1)
         return self.o_proj(out), None
+
+    def _paged_layer(self, past_key_values):
+        """This layer's pages where the cache is a PagedCache, else None."""
+        from .kv_paged import PagedKVLayer
+
+        layers = getattr(past_key_values, "layers", None)
+        layer = layers[self.layer_idx] if layers and self.layer_idx < len(layers) else None
+        return layer if isinstance(layer, PagedKVLayer) else None
+
+    def _forward_paged(self, layer, q, k, v, position_embeddings, attention_mask):
+        """forward over a PagedCache: a batch of sequences, whose new tokens are written to the pages and attend every row up to
+        their own (paged_step). A step of prompts that start empty runs the sparse prefill, a sequence at a time, on the
+        prompts longer than sink + window of a layer that is not dense."""
+        if torch.is_grad_enabled() and q.requires_grad:
+            raise ValueError("a paged cache holds no gradients: run under torch.no_grad()")
+        if self.kv_evict:
+            raise ValueError("kv_evict does not compact a paged cache")
+        b, h, t, _ = q.shape
+        cos, sin = position_embeddings
+        if b != len(layer.cache.lengths):
+            raise ValueError(f"the paged cache holds {len(layer.cache.lengths)} sequences, the input has {b}")
+        new = layer.begin(t, attention_mask is not None, cos.shape[0] if cos.ndim == 3 else 1)
+        lengths = layer.cache.lengths
+        prompts = all(n == s for n, s in zip(lengths, new) if s)  # every sequence with new tokens starts here
+        if self.dense or not prompts or max(new) <= self.sink + self.window:
+            out = layer.attend(q, k, v, self.scaling, cos, sin)
+            return self.o_proj(out.transpose(1, 2).reshape(b, t, -1)), None
+        q, k = rope_inplace(q, cos, sin), rope_inplace(k, cos, sin)
+        layer.append(k, v)
+        if b == 1 and new[0] == t:
+            out = self.sparse_prefill(q, k, v)
+            return self.o_proj(out.transpose(1, 2).reshape(b, t, -1)), None
+        out = q.new_zeros(b, t, h, self.head_dim).transpose(1, 2)
+        routes = []
+        for i, n in enumerate(new):
+            qi, ki, vi = q[i:i + 1, :, :n], k[i:i + 1, :, :n], v[i:i + 1, :, :n]
+            if n > self.sink + self.window:
+                out[i:i + 1, :, :n] = self.sparse_prefill(qi, ki, vi)
+                routes.append(self.last_routes)
+            else:
+                if n:
+                    out[i:i + 1, :, :n] = self.exact_attention(qi, ki, vi, n, n)
+                routes.append(None)
+        self.last_routes = routes[0] if b == 1 else routes
+        return self.o_proj(out.transpose(1, 2).reshape(b, t, -1)), None
 
     def _forward_autograd(self, q, k, v, position_embeddings, past_key_values):
         """forward with autograd on, as the reference takes it (modal_rd/attention.py:118-119, 127-129, 140-141): RoPE

@@ -9,10 +9,14 @@ sequence; an entry outside 0 .. pages - 1 names no page, and its rows are neithe
 of each sequence, the call's new ones among them), new [B] int32 (how many of the T token columns are real; None: all). Token j
 of sequence b is row lens[b] - new[b] + j and attends the rows up to its own. All three are read by the kernels, so a captured
 graph follows them.
+
+`make_paged_cache` puts them under a model whose attention RDAttention is: batches of sequences, where the other caches hold one.
 """
 import functools
 
 import torch
+from transformers import DynamicCache
+from transformers.cache_utils import DynamicLayer
 
 from . import _lib
 from .kv_int4 import _copy, _launch_on
@@ -229,3 +233,170 @@ def paged_step(q, k, v, k_pages, v_pages, table, lens, scale, cos=None, sin=None
                lens.data_ptr(), _lib.ptr(new), *sizes, float(scale), out.data_ptr(), so, _lib.ptr(ws), ws_bytes,
                _lib.stream_of(q))
     return out
+
+
+class PagedKVLayer(DynamicLayer):
+    """One layer's pages of a PagedCache. RDAttention attends them (`attend`, `append`); other consumers are refused, as there are
+    no contiguous keys and values to hand out."""
+
+    def __init__(self, cache, index, k_pages, v_pages):
+        super().__init__()
+        self.cache, self.index, self.k_pages, self.v_pages = cache, index, k_pages, v_pages
+        self.dtype, self.device = k_pages.dtype, k_pages.device
+        self.is_initialized = True
+
+    def begin(self, t, padded, positions):
+        """The current step's new tokens per sequence, for this layer: `t` columns (begun here, with every column real, unless
+        PagedCache.extend did). `padded`: whether the model was given a mask; `positions`: how many sequences' angles it was
+        given."""
+        return self.cache._begin(self.index, t, padded, positions)
+
+    def append(self, k, v):
+        """The step's rows k, v [B, Hkv, T, d], rotated already, into the pages."""
+        c = self.cache
+        paged_append(k, v, self.k_pages, self.v_pages, c.table, c.lens, new=c._new_of(k.shape[2]))
+
+    def attend(self, q, k, v, scale, cos, sin):
+        """The step's rows into the pages, k rotated by cos, sin [B or 1, T, d], and the attention of the rotated q."""
+        c = self.cache
+        b, _, t, _ = q.shape
+        cos, sin = (x.expand(b, t, x.shape[-1]) for x in (cos, sin))
+        return paged_step(q, k, v, self.k_pages, self.v_pages, c.table, c.lens, scale, cos=cos, sin=sin, new=c._new_of(t))
+
+    def lazy_initialization(self, key_states, value_states, *args, **kwargs):
+        pass
+
+    def update(self, key_states, value_states, *args, **kwargs):
+        raise ValueError("a paged cache is attended by RDAttention only (install the model's attention)")
+
+    def get_seq_length(self, *args, **kwargs):
+        """Rows of the longest sequence before the current step."""
+        return max(self.cache._before())
+
+    def get_mask_sizes(self, query_length, *args, **kwargs):
+        return query_length, 0  # no mask is read: a step's tokens alone, which a model without padding needs none for
+
+    def crop(self, tokens_to_remove):
+        raise NotImplementedError("crop the whole PagedCache")
+
+    reset = reorder_cache = batch_repeat_interleave = batch_select_indices = crop
+
+
+class PagedCache(DynamicCache):
+    """A model's KV cache in pages: `batch` sequences of unlike lengths share `pages` pages of `page` rows a layer.
+
+    A forward pass is a step: its first layer takes pages for the new tokens of every sequence (as many as the input has columns,
+    or what `extend` said just before, with the padding on the right), and every layer then writes and attends them.
+    `positions(t)` are the step's position ids, needed once sequences differ in length. `truncate` takes rows back (drafted
+    tokens that were not accepted), `release` empties sequences, whose pages others then take."""
+
+    def __init__(self, config, batch, pages, page=64, rows=None, dtype=torch.bfloat16, device="cuda"):
+        super().__init__(config=config)
+        cfg = config.get_text_config(decoder=True)
+        d = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+        if page < 16 or page & (page - 1):
+            raise ValueError("PagedCache: pages of a power of two of rows, at least 16")
+        if batch < 1 or pages < 1 or d not in (64, 128) or dtype not in _ROWS:
+            raise ValueError("PagedCache: bf16 or fp16 rows of head_dim 64 or 128, one sequence and page at least")
+        self.page, self.width = page, -(-(rows or pages * page) // page)
+        shape = (cfg.num_hidden_layers, 2, pages, cfg.num_key_value_heads, page, d)
+        with torch.inference_mode(False):  # updated in place in either mode
+            self.arena = torch.empty(shape, dtype=dtype, device=device)
+            self.table = torch.full((batch, self.width), -1, dtype=torch.int32, device=device)
+            self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+            self.new = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.lengths = [0] * batch          # rows of each sequence, the current step's among them
+        self._pages = [[] for _ in range(batch)]
+        self._free = list(range(pages))[::-1]
+        self._step, self._left = [0] * batch, set()  # new tokens of the current step, layers that have not run it
+        self._declared = False
+        self.layers = [PagedKVLayer(self, i, a[0], a[1]) for i, a in enumerate(self.arena)]
+
+    def _before(self):
+        return [n - s for n, s in zip(self.lengths, self._step)] if self._left else self.lengths
+
+    def extend(self, new):
+        """Begin a step of new[b] tokens of sequence b (0: none): pages are taken for them. The next forward pass runs it; its
+        input has max(new) columns or more, each sequence's tokens first."""
+        new = [int(x) for x in new]
+        if self._left:
+            raise ValueError("PagedCache: the step before has not run through every layer (truncate takes it back)")
+        if len(new) != len(self.lengths) or min(new) < 0:
+            raise ValueError("PagedCache: one count of new tokens per sequence")
+        after = [n + s for n, s in zip(self.lengths, new)]
+        need = [-(-n // self.page) - len(p) for n, p in zip(after, self._pages)]
+        if max(after) > self.width * self.page:
+            raise ValueError("PagedCache: a sequence is past the rows that the cache was made for")
+        if sum(x for x in need if x > 0) > len(self._free):
+            raise ValueError("PagedCache: no free pages left")
+        for b, x in enumerate(need):
+            if x > 0:
+                at = len(self._pages[b])
+                self._pages[b] += [self._free.pop() for _ in range(x)]
+                self.table[b, at:at + x].copy_(torch.tensor(self._pages[b][at:], dtype=torch.int32))
+        self.lengths, self._step, self._left = after, new, set(range(len(self.layers)))
+        self.lens.copy_(torch.tensor(after, dtype=torch.int32))
+        self.new.copy_(torch.tensor(new, dtype=torch.int32))
+        self._declared = True
+
+    def _begin(self, layer, t, padded, positions):
+        begun = layer in self._left
+        step, before = (self._step, self._before()) if begun else ([t] * len(self.lengths), self.lengths)
+        if max(step) > t:
+            raise ValueError(f"PagedCache: the step has {max(step)} new tokens, the input {t} columns")
+        if len(step) > 1 and padded and not (begun and self._declared):
+            raise ValueError("PagedCache: padding goes by extend(new tokens of each sequence) and to the right, not by a mask")
+        if positions == 1 and any(s and n != max(before) for n, s in zip(before, step)):
+            raise ValueError("PagedCache: sequences of unlike lengths need position_ids (positions)")
+        if not begun:
+            self.extend(step)
+            self._declared = False
+        self._left.discard(layer)
+        return self._step
+
+    def _new_of(self, t):
+        return None if all(s == t for s in self._step) else self.new
+
+    def positions(self, t=None):
+        """Position ids [B, t] of a step's columns (t: as many as its longest has), of the step that extend began or the next."""
+        before = torch.tensor(self._before(), device=self.lens.device)
+        return before[:, None] + torch.arange(max(self._step) if t is None else t, device=self.lens.device)
+
+    def truncate(self, lengths):
+        """Keep the first lengths[b] rows of each sequence; whole pages behind them become free. A step that did not run is taken
+        back with it."""
+        lengths = [int(x) for x in lengths]
+        if len(lengths) != len(self.lengths) or any(not 0 <= x <= n for x, n in zip(lengths, self.lengths)):
+            raise ValueError("PagedCache: one length per sequence, of rows that it has")
+        for b, n in enumerate(lengths):
+            keep = -(-n // self.page)
+            if keep < len(self._pages[b]):
+                self.table[b, keep:len(self._pages[b])].fill_(-1)
+                self._free += self._pages[b][keep:][::-1]
+                del self._pages[b][keep:]
+        self.lengths, self._step, self._left = lengths, [0] * len(lengths), set()
+        self.lens.copy_(torch.tensor(lengths, dtype=torch.int32))
+        self.new.zero_()
+
+    def release(self, sequences):
+        """Empty these sequences (an index or several)."""
+        gone = {sequences} if isinstance(sequences, int) else set(sequences)
+        self.truncate([0 if b in gone else n for b, n in enumerate(self.lengths)])
+
+    def crop(self, tokens_to_remove):
+        if tokens_to_remove > 0:
+            raise NotImplementedError("PagedCache.crop supports negative token counts only")
+        self.truncate([max(0, n + tokens_to_remove) for n in self.lengths])
+
+    def reset(self):
+        self.truncate([0] * len(self.lengths))
+
+    def nbytes(self):
+        """Bytes of the pages that sequences hold, over all layers."""
+        return sum(len(p) for p in self._pages) * self.arena[:, :, 0].numel() * self.arena.element_size()
+
+
+def make_paged_cache(config, batch, pages, page=64, rows=None, dtype=torch.bfloat16, device="cuda"):
+    """A PagedCache for `batch` sequences over `pages` pages of `page` rows in each layer (rows: the longest that a sequence may
+    become; None: all pages')."""
+    return PagedCache(config, batch, pages, page, rows, dtype, device)
