@@ -340,7 +340,7 @@ BB_DEV void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 // Eight bytes of LDS per lane: of 16 lanes, lanes 4 r .. 4 r + 3 point at 16 elements of row r, and lane l gets column l,
-// row r in place r.
+// row r in place r. (`restrict`: no load into LDS in flight writes what is read here; the compiler would wait for all of them.)
 BB_DEV u32x2_t read_tr16(const uint8_t* __restrict__ at) {
   return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)at));
 }
@@ -784,9 +784,13 @@ struct TileLds {
   static constexpr int RPL = 512 / D;                      // rows of a load
 };
 
-template <int D>
+// The loads of a wave's part of a tile. ONE: pages of 64 rows and more, so a tile lies in one page and a descriptor serves all of a
+// wave's loads of it (with smaller pages each load has its own: some 130 scalar instructions a tile instead of 40, in the phase
+// that the matrix cores wait for).
+template <int D, bool ONE>
 struct TileLoader {
   using L = TileLds<D>;
+  static constexpr int PAGES = ONE ? 1 : L::LOADS;
   const PagedCache& c;
   const_i32 table;
   const uint16_t *kh, *vh;
@@ -800,9 +804,9 @@ struct TileLoader {
     const int row = lane / (D / 8), piece = lane % (D / 8);
 #pragma unroll
     for (int i = 0; i < L::LOADS; ++i) {
-      const int r = row0 + row + L::RPL * kTileWaves * i;
-      koff[i] = row * (uint32_t)c.skr * 2 + 16 * (piece ^ k_swz<D>(r & 15));
-      voff[i] = row * (uint32_t)c.svr * 2 + 16 * (piece ^ v_swz<D>(r & 15));
+      const int r = row0 + row + L::RPL * kTileWaves * i, at = ONE ? r : row;
+      koff[i] = at * (uint32_t)c.skr * 2 + 16 * (piece ^ k_swz<D>(r & 15));
+      voff[i] = at * (uint32_t)c.svr * 2 + 16 * (piece ^ v_swz<D>(r & 15));
     }
   }
   BB_DEV int entry(int r) const {  // of row r's page
@@ -810,20 +814,25 @@ struct TileLoader {
     return table[w < c.W ? w : c.W - 1];
   }
   struct Entries {
-    int e[L::LOADS];
+    int e[PAGES];
   };
   BB_DEV Entries entries(int k0) const {
     Entries x;
 #pragma unroll
-    for (int i = 0; i < L::LOADS; ++i) x.e[i] = entry(k0 + row0 + L::RPL * kTileWaves * i);
+    for (int i = 0; i < PAGES; ++i) x.e[i] = entry(k0 + (ONE ? 0 : row0 + L::RPL * kTileWaves * i));
     return x;
   }
   // This wave's part of the K or V tile of rows k0 .., into `to`: always LOADS loads; rows past the end and of no page land zeros.
   BB_DEV void load(bool is_v, uint8_t* to, int wave, int k0, const Entries& x) const {
+    constexpr int ROWS = ONE ? kTileRows : L::RPL;
+    PageRows at;
 #pragma unroll
     for (int i = 0; i < L::LOADS; ++i) {
-      const int r = k0 + row0 + L::RPL * kTileWaves * i, page = (uint32_t)x.e[i] < (uint32_t)c.pages ? x.e[i] : -1;
-      const PageRows at = page_rows(c, is_v, is_v ? vh : kh, page, r, end - r < L::RPL ? end - r : L::RPL, 2 * D);
+      if (i < PAGES) {
+        const int r = ONE ? k0 : k0 + row0 + L::RPL * kTileWaves * i;
+        const int page = (uint32_t)x.e[i] < (uint32_t)c.pages ? x.e[i] : -1;
+        at = page_rows(c, is_v, is_v ? vh : kh, page, r, end - r < ROWS ? end - r : ROWS, 2 * D);
+      }
       load_rows<0>(at, to + 1024 * (wave + kTileWaves * i), is_v ? voff[i] : koff[i]);
     }
   }
@@ -844,7 +853,7 @@ BB_DEV uint32_t lds_addr(const void* p) {
 }
 BB_DEV u32x4_t lds16(uint32_t at) { return *(const __attribute__((address_space(3))) u32x4_t*)(uintptr_t)at; }
 BB_DEV u32x2_t lds_tr16(uint32_t at) {
-  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(uintptr_t)at));
+  return read_tr16((const uint8_t*)(const __attribute__((address_space(3))) uint8_t*)(uintptr_t)at);
 }
 
 template <int D>
@@ -952,7 +961,7 @@ BB_DEV void tile_softmax(TileState<D>& t, float c) {
   t.l[1] += sum[1];
 }
 
-template <int D, bool F16>
+template <int D, bool F16, bool ONE>
 __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAttnParams p) {
   using L = TileLds<D>;
   constexpr int STAGE = 2 * L::BYTES, NV = D / 8, NF = D / 4, ROW = D + 4;
@@ -975,13 +984,13 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
   const bool live = 32 * wave < R;  // a wave without vectors only loads
 
   // Tile i's K and V are in stage i % 4 of their halves of the ring.
-  const TileLoader<D> in(p.c, it.b, it.g, end, wave, lane);
+  const TileLoader<D, ONE> in(p.c, it.b, it.g, end, wave, lane);
   auto k_at = [&](int i) { return ring + (i & (kTileStages - 1)) * L::BYTES; };
   auto v_at = [&](int i) { return ring + (kTileStages + (i & (kTileStages - 1))) * L::BYTES; };
   auto entries = [&](int i) { return in.entries(begin + kTileRows * i); };
-  auto fetch_k = [&](int i, const typename TileLoader<D>::Entries& e) { in.load(false, k_at(i), wave, begin + kTileRows * i, e); };
-  auto fetch_v = [&](int i, const typename TileLoader<D>::Entries& e) { in.load(true, v_at(i), wave, begin + kTileRows * i, e); };
-  typename TileLoader<D>::Entries e0 = entries(0), e1 = entries(1), e2 = entries(2);
+  auto fetch_k = [&](int i, const typename TileLoader<D, ONE>::Entries& e) { in.load(false, k_at(i), wave, begin + kTileRows * i, e); };
+  auto fetch_v = [&](int i, const typename TileLoader<D, ONE>::Entries& e) { in.load(true, v_at(i), wave, begin + kTileRows * i, e); };
+  typename TileLoader<D, ONE>::Entries e0 = entries(0), e1 = entries(1), e2 = entries(2);
 
   // The queries' and the table's loads go out before the first tiles', which they then need not wait for.
   TileState<D> t;
@@ -1287,7 +1296,10 @@ hipError_t launch_paged_append(const PagedAppendParams& p, hipStream_t stream) {
 namespace {
 template <int D, bool F16, int NR>
 hipError_t attend(const PagedAttnParams& p, hipStream_t stream) {
-  if constexpr (NR == 0) paged_tile_kernel<D, F16><<<p.grid, 64 * kTileWaves, 0, stream>>>(p);
+  if constexpr (NR == 0) {
+    if (1 << p.c.page_log2 >= kTileRows) paged_tile_kernel<D, F16, true><<<p.grid, 64 * kTileWaves, 0, stream>>>(p);
+    else paged_tile_kernel<D, F16, false><<<p.grid, 64 * kTileWaves, 0, stream>>>(p);
+  }
   else if (p.knew) paged_attn_kernel<D, F16, NR, true><<<p.grid, kThreads, 0, stream>>>(p);
   else paged_attn_kernel<D, F16, NR, false><<<p.grid, kThreads, 0, stream>>>(p);
   if (p.part) {
