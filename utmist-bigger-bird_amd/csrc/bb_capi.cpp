@@ -1063,8 +1063,16 @@ struct PagedSchedule {
   int VT, tiles, unit, min_share, target, fit_quarters, grid;
   size_t slots, bytes;  // of partials; of the workspace: the partials, then what each slot holds and how many are used
 };
-constexpr int kPagedStreamVectors = 32;  // query vectors of a KV head up to which the streaming kernel takes a call
-constexpr int kPagedStepVectors = 128;   // and up to which it takes a step, storing its new rows
+// Query vectors of a KV head up to which the streaming kernel takes a call. (us streaming and in tiles of 64 rows, 8 KV heads,
+// head_dim 128: 16 vectors 12.3 and 18.3 at 4096 rows, 35 and 42 at 8 x 8192, 30 and 30 at 32768; 32: 15.4 and 19, 39 and 43, 33 and
+// 31; 64, which read the cache twice where they stream: 17 and 20, 53 and 44, 50 and 33.)
+constexpr int kPagedStreamVectors = 32;
+// And up to which it takes a step by itself, rotating q and storing the new rows; more go through the append, and their rotated q
+// is rounded. (By itself and in two, the same sizes: 16 vectors 16.5 and 19.3, 38 and 39, 33 and 34 us; 32: 22 and 20, 45 and 44, 39
+// and 37; 64: 24 and 24, 61 and 49, 58 and 37; 128: 33 and 27, 85 and 54, 78 and 42. The outputs' error against 64 bits is 0.0017 of
+// them by itself, which is their own rounding, and 0.0029 to 0.0032 in two. Of up to 128 vectors, where single tokens and drafts
+// of a few end, the error decides.)
+constexpr int kPagedStepVectors = 128;
 static const char* paged_schedule(int B, int T, int H, int Hkv, int D, int W, int page, bool with_new, PagedSchedule& s) {
   const int64_t R = (int64_t)T * (H / Hkv), cap = (int64_t)W * page;
   if (R <= kPagedStreamVectors || (with_new && R <= kPagedStepVectors)) {

@@ -475,7 +475,7 @@ BB_DEV uint32_t not_finite(uint32_t w) {  // 0xffff in the halves that are not
 }
 
 template <int D, bool F16, int NR, bool NEW>
-__global__ __launch_bounds__(kThreads, NR > 1 && NEW ? 1 : 2) void paged_attn_kernel(PagedAttnParams p) {
+__global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnParams p) {
   using Stream = PageStream<D>;
   constexpr int KC = Stream::KC, GROUPS = Stream::GROUPS, NDS = D / 32, NDB = D / 16;
   constexpr int ROW = D + 4;  // floats of a state's row: whole 16-byte pieces, rows on other banks
@@ -520,15 +520,23 @@ __global__ __launch_bounds__(kThreads, NR > 1 && NEW ? 1 : 2) void paged_attn_ke
   for (int r = 0; r < NR; ++r)
 #pragma unroll
     for (int ds = 0; ds < NDS; ++ds) asm volatile("" : "+v"(qw[r][ds]));  // awaited here, not with the chunk before the loop
-  // with new rows the rotated query is kept in two terms, as exact as fp32 products of it need
+  // With new rows the rotated query is kept in two terms, as exact as fp32 products of it need; of 32 vectors in LDS, as two
+  // workgroups a CU have no registers for it (one alone: 46 us where these take 39, 32 vectors over 32768 rows of 8 heads). All
+  // waves write the same there, and each reads what it wrote or the same.
   constexpr int QT = NEW ? 2 : 1;
-  bf16x8_t qf[NR][NDS][QT];
+  constexpr bool AWAY = NEW && NR > 1;
+  __shared__ __attribute__((aligned(16))) uint8_t qs[AWAY ? NR * NDS * QT * 1024 : 16];
+  bf16x8_t qf[NR][AWAY ? 1 : NDS][QT];
+  auto put_q = [&](int r, int ds, int i, u32x4_t w) {
+    if constexpr (AWAY) st16(qs + 1024 * (QT * (NDS * r + ds) + i) + 16 * lane, w);
+    else qf[r][ds][i] = as_bf16x8(w);
+  };
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
 #pragma unroll
     for (int ds = 0; ds < NDS; ++ds) {
-      qf[r][ds][0] = as_bf16x8(qw[r][ds]);
-      if constexpr (NEW) qf[r][ds][1] = as_bf16x8(u32x4_t{0, 0, 0, 0});
+      put_q(r, ds, 0, qw[r][ds]);
+      if constexpr (NEW) put_q(r, ds, 1, u32x4_t{0, 0, 0, 0});
     }
     if constexpr (NEW) {
       if (p.r.cos) {
@@ -549,8 +557,8 @@ __global__ __launch_bounds__(kThreads, NR > 1 && NEW ? 1 : 2) void paged_attn_ke
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            qf[r][ds][i] = as_bf16x8(w[i]);
-            qf[r][ds + NDS / 2][i] = as_bf16x8(w[2 + i]);
+            put_q(r, ds, i, w[i]);
+            put_q(r, ds + NDS / 2, i, w[2 + i]);
           }
         }
       }
@@ -592,15 +600,22 @@ __global__ __launch_bounds__(kThreads, NR > 1 && NEW ? 1 : 2) void paged_attn_ke
 #pragma unroll
       for (int kb = 0; kb < KC / 16; ++kb) y[r][kb] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-    for (int ds = 0; ds < NDS; ++ds)
+    for (int ds = 0; ds < NDS; ++ds) {
+      if constexpr (AWAY)
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+            qf[r][0][t] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(qs + 1024 * (QT * (NDS * r + ds) + t) + 16 * lane));
 #pragma unroll
       for (int kb = 0; kb < KC / 16; ++kb) {
         const bf16x8_t kf = as_bf16x8(*reinterpret_cast<const u32x4_t*>(ks + kread[ds] + 32 * D * kb));
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int t = 0; t < QT; ++t) y[r][kb] = mma16<F16>(kf, qf[r][ds][t], y[r][kb]);
+          for (int t = 0; t < QT; ++t) y[r][kb] = mma16<F16>(kf, qf[r][AWAY ? 0 : ds][t], y[r][kb]);
       }
+    }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): K is read, its space is free
     wave_fence();
     __builtin_amdgcn_sched_barrier(0);  // (the table's entries are wanted from here on, not before the products)
