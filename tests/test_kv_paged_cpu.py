@@ -87,6 +87,7 @@ def test_attention_refusals(over, msg):
     (dict(sc=_s(2, 128), f32=1), "cos and sin rows must be 16-byte aligned"),
     (dict(skn=_s(1024, 4, 1024)), "16-byte alignment"),
     (dict(T=1 << 30), "too many rows"),
+    (dict(T=(1 << 22) + 1, B=1, H=112), "too many rows"),  # 2^29 rows of 8 lanes and more: more threads than a launch has
 ])
 def test_append_refusals(over, msg):
     rc, err = _append(**over)
@@ -237,6 +238,10 @@ def test_cache_truncate_and_release():
     for bad in ([33, 33, 0], [32, 33, -1], [32]):
         with pytest.raises(ValueError, match="one length"):
             c.truncate(bad)
+    for bad in (3, -1, [0, 3]):
+        with pytest.raises(ValueError, match="no such sequence"):
+            c.release(bad)
+    assert c.lengths == [32, 33, 0]
     c.release(1)
     assert c.lengths == [32, 0, 0] and len(c._free) == 7
     _consistent(c)

@@ -135,7 +135,7 @@ def paged_append(k, v, k_pages, v_pages, table, lens, cos=None, sin=None, q=None
     """The new K / V rows k, v [B, Hkv, T, d] into the pages; with cos, sin ([B, T, d] or [T, d], fp32 or the rows' dtype) k is
     rotated on the way: x cos + (-x[d/2:], x[:d/2]) sin in fp32, rounded once. With q [B, H, T, d] (cos, sin required) returns q
     rotated alike, in [B, T, H, d] memory (padding columns too); else None. Rows that lie outside the table or on no page are
-    not written. Two tokens of a call must not share a row."""
+    not written. Two tokens of a call must not share a row of a page."""
     what = "paged_append"
     device = _device_of(what, k, v, k_pages, v_pages, table, lens, cos, sin, q, new)
     (copy, sk, sv, sq, so, sc, f32, skp, svp, st, sizes) = _append_plan(
@@ -212,7 +212,8 @@ def _step_plan(q, k, v, kp, vp, table, lens, cos, sin, new):
 def paged_step(q, k, v, k_pages, v_pages, table, lens, scale, cos=None, sin=None, new=None):
     """One step: paged_append(k, v, ..., cos, sin, q) and paged_attention of the rotated q, in one call (q and k as they are
     where cos is None). Up to 128 query vectors of a KV head (T * H / Hkv) one kernel does both, and its rotated queries are not
-    rounded. Returns [B, H, T, d] in [B, T, H, d] memory."""
+    rounded. A row that the call writes must not be attended in it by another sequence, nor at another place of its own table.
+    Returns [B, H, T, d] in [B, T, H, d] memory."""
     what = "paged_step"
     device = _device_of(what, q, k, v, k_pages, v_pages, table, lens, cos, sin, new)
     copy, sq, sk, sv, sc, f32, skp, svp, st, sizes, so, ws_bytes = _step_plan(
@@ -381,6 +382,8 @@ class PagedCache(DynamicCache):
     def release(self, sequences):
         """Empty these sequences (an index or several)."""
         gone = {sequences} if isinstance(sequences, int) else set(sequences)
+        if not gone <= set(range(len(self.lengths))):
+            raise ValueError("PagedCache: no such sequence")
         self.truncate([0 if b in gone else n for b, n in enumerate(self.lengths)])
 
     def crop(self, tokens_to_remove):
