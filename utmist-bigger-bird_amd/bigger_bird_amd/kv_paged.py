@@ -12,6 +12,7 @@ graph follows them.
 
 `make_paged_cache` puts them under a model whose attention RDAttention is: batches of sequences, where the other caches hold one.
 """
+import ctypes
 import functools
 
 import torch
@@ -25,10 +26,29 @@ _ROWS = (torch.bfloat16, torch.float16)
 _FAR = (1 << 31) - 1
 
 
-# A step of a few tokens is one or two kernels of microseconds, so what depends on shapes, strides and dtypes alone is checked and
-# laid out for the library once per such layout; addresses are looked at in every call.
-def _layout(x):
-    return None if x is None else (x.shape, x.stride(), x.dtype)
+# A step of a few tokens is one or two kernels of microseconds, so what depends on shapes, strides, dtypes and devices alone is
+# checked and laid out for the library once per such layout (the library's arguments as the ctypes objects that they become);
+# addresses are looked at in every call.
+def _layouts(*tensors):
+    return [x if x is None else (x.shape, x.stride(), x.dtype, x.get_device()) for x in tensors]
+
+
+def _device_of(what, *layouts):
+    """The index of the one ROCm device that holds every tensor (the kernels run on the current stream there)."""
+    devices = {x[3] for x in layouts if x is not None}
+    if -1 in devices:
+        raise ValueError(f"{what} runs on the ROCm device only (got a tensor that is not on it)")
+    if len(devices) != 1:
+        raise ValueError(f"{what}: tensors on different devices")
+    return devices.pop()
+
+
+def _i64s(*vals):
+    return ctypes.cast(_lib.i64s(*vals), _lib.c_i64p)
+
+
+def _i32s(*vals):
+    return tuple(map(ctypes.c_int, vals))
 
 
 def _aligned(layout, rows=8):
@@ -39,12 +59,12 @@ def _aligned(layout, rows=8):
 
 def _strides3(layout):
     s = layout[1]
-    return _lib.i64s(s[0], s[1], s[2])
+    return _i64s(s[0], s[1], s[2])
 
 
 def _check_cache(what, rows, kp, vp, table, lens, new):
     """(heads, pages, page, W) of a call's cache, checked against tokens [B, heads, T, d]; arguments are layouts."""
-    (shape, _, dtype), (ps, pst, pd), (vs, vst, vd) = rows, kp, vp
+    (shape, _, dtype, _), (ps, _, pd, _), (vs, _, vd, _) = rows, kp, vp
     if len(shape) != 4:
         raise ValueError(f"{what}: rows must be [B, heads, T, d]")
     b, d = shape[0], shape[3]
@@ -75,7 +95,7 @@ def _check_rope(what, cos, sin, b, t, d, dtype):
     if cos[2] != sin[2] or not (f32 or cos[2] == dtype):
         raise ValueError(f"{what}: cos and sin must be fp32 or of the rows' dtype")
     strides = []
-    for shape, s, _ in (cos, sin):
+    for shape, s, _, _ in (cos, sin):
         if len(shape) == 2:
             shape, s = (1, *shape), (0, *s)
         if len(shape) != 3 or shape[2] != d or any(n != 1 and n != m for n, m in zip(shape, (b, t))):
@@ -83,7 +103,7 @@ def _check_rope(what, cos, sin, b, t, d, dtype):
         strides.append((0 if shape[0] == 1 else s[0], 0 if shape[1] == 1 else s[1], s[2]))
     whole = 4 if f32 else 8
     ok = strides[0] == strides[1] and strides[0][2] == 1 and not any(i % whole for i in strides[0][:2])
-    return not ok, _lib.i64s(*strides[0][:2]), int(f32)
+    return not ok, _i64s(*strides[0][:2]), int(f32)
 
 
 def _whole_rope(cos, sin, b, t, d):
@@ -91,20 +111,10 @@ def _whole_rope(cos, sin, b, t, d):
     return tuple(_copy(x.expand(b, t, d)) for x in (cos, sin))
 
 
-def _heads_last(shape, like):
-    """A fresh tensor [B, h, T, d] in [B, T, h, d] memory (an output projection's order)."""
+def _heads_last(shape):
+    """The strides of a tensor [B, h, T, d] in [B, T, h, d] memory (an output projection's order)."""
     b, h, t, d = shape
-    return torch.empty_strided((b, h, t, d), (t * h * d, d, h * d, 1), dtype=like.dtype, device=like.device)
-
-
-def _device_of(what, first, *tensors):
-    """The index of the one ROCm device that holds every tensor (the kernels run on the current stream there)."""
-    device = first.get_device()
-    for x in tensors:
-        if x is not None and x.get_device() != device or device < 0:
-            _lib.require_gpu(first, *tensors, what=what)
-            raise ValueError(f"{what}: tensors on different devices")
-    return device
+    return t * h * d, d, h * d, 1
 
 
 def _check_addresses(what, k_pages, v_pages):
@@ -115,6 +125,7 @@ def _check_addresses(what, k_pages, v_pages):
 @functools.lru_cache(maxsize=512)
 def _append_plan(k, v, kp, vp, table, lens, cos, sin, q, new):
     what = "paged_append"
+    device = _device_of(what, k, v, kp, vp, table, lens, cos, sin, q, new)
     if v[0] != k[0] or v[2] != k[2]:
         raise ValueError(f"{what}: k and v must share a shape and dtype")
     hk, pages, page, w = _check_cache(what, k, kp, vp, table, lens, new)
@@ -126,9 +137,10 @@ def _append_plan(k, v, kp, vp, table, lens, cos, sin, q, new):
     copy_rope, sc, f32 = _check_rope(what, cos, sin, b, t, d, k[2])
     heads = 0 if q is None else q[0][1]
     copy = not (_aligned(k) and _aligned(v) and (q is None or _aligned(q))) or copy_rope
-    sq = (_strides3(q), _lib.i64s(t * heads * d, d, heads * d)) if heads else (None, None)
-    return (copy, _strides3(k), _strides3(v), *sq, sc, f32, _strides3(kp), _strides3(vp), table[1][0],
-            (b, t, heads, hk, d, pages, page, w, int(k[2] is torch.float16)))
+    so = _heads_last(q[0]) if q is not None else None
+    sq = (_strides3(q), _i64s(*so[:3])) if heads else (None, None)
+    return (device, copy, so, _strides3(k), _strides3(v), *sq, sc, f32, _strides3(kp), _strides3(vp), table[1][0],
+            _i32s(b, t, heads, hk, d, pages, page, w, k[2] is torch.float16))
 
 
 def paged_append(k, v, k_pages, v_pages, table, lens, cos=None, sin=None, q=None, new=None):
@@ -137,20 +149,18 @@ def paged_append(k, v, k_pages, v_pages, table, lens, cos=None, sin=None, q=None
     rotated alike, in [B, T, H, d] memory (padding columns too); else None. Rows that lie outside the table or on no page are
     not written. Two tokens of a call must not share a row of a page."""
     what = "paged_append"
-    device = _device_of(what, k, v, k_pages, v_pages, table, lens, cos, sin, q, new)
-    (copy, sk, sv, sq, so, sc, f32, skp, svp, st, sizes) = _append_plan(
-        _layout(k), _layout(v), _layout(k_pages), _layout(v_pages), _layout(table), _layout(lens), _layout(cos), _layout(sin),
-        _layout(q), _layout(new))
+    device, copy, out_strides, sk, sv, sq, so, sc, f32, skp, svp, st, sizes = _append_plan(
+        *_layouts(k, v, k_pages, v_pages, table, lens, cos, sin, q, new))
     pk, pv, kp, vp = k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
     pq, pc, ps = _lib.ptr(q) or 0, _lib.ptr(cos) or 0, _lib.ptr(sin) or 0
     _check_addresses(what, kp, vp)
     if k.numel() == 0:
-        return None if q is None else _heads_last(q.shape, q)
+        return None if q is None else q.new_empty_strided(q.shape, out_strides)
     if copy or (pk | pv | pq | pc | ps) & 15:
         if cos is not None:
             cos, sin = _whole_rope(cos, sin, k.shape[0], k.shape[2], k.shape[3])
         return paged_append(_copy(k), _copy(v), k_pages, v_pages, table, lens, cos, sin, None if q is None else _copy(q), new)
-    out = None if q is None else _heads_last(q.shape, q)
+    out = None if q is None else q.new_empty_strided(q.shape, out_strides)
     _launch_on(device, _lib.lib().bb_paged_append, pk, sk, pv, sv, pq, sq, _lib.ptr(out), so, pc, ps, sc, f32, kp, skp, vp, svp,
                table.data_ptr(), st, lens.data_ptr(), _lib.ptr(new), *sizes, _lib.stream_of(k))
     return out
@@ -166,11 +176,13 @@ def _check_queries(what, q, hk):
 @functools.lru_cache(maxsize=512)
 def _attention_plan(q, kp, vp, table, lens, new):
     what = "paged_attention"
+    device = _device_of(what, q, kp, vp, table, lens, new)
     hk, pages, page, w = _check_cache(what, q, kp, vp, table, lens, new)
     b, h, t, d = _check_queries(what, q, hk)
     ws = _lib.lib().bb_paged_attention_workspace(b, t, h, hk, d, page, w)
-    return (not _aligned(q), _strides3(q), _strides3(kp), _strides3(vp), table[1][0],
-            (b, t, h, hk, d, pages, page, w, int(q[2] is torch.float16)), _lib.i64s(t * h * d, d, h * d), ws)
+    so = _heads_last(q[0])
+    return (device, not _aligned(q), so, _strides3(q), _strides3(kp), _strides3(vp), table[1][0],
+            _i32s(b, t, h, hk, d, pages, page, w, q[2] is torch.float16), _i64s(*so[:3]), ws)
 
 
 def paged_attention(q, k_pages, v_pages, table, lens, scale, new=None):
@@ -179,16 +191,15 @@ def paged_attention(q, k_pages, v_pages, table, lens, scale, new=None):
     [B, H, T, d] in [B, T, H, d] memory; zeros for padding and where a token attends no row, NaN for a query that is not
     finite."""
     what = "paged_attention"
-    device = _device_of(what, q, k_pages, v_pages, table, lens, new)
-    copy, sq, skp, svp, st, sizes, so, ws_bytes = _attention_plan(
-        _layout(q), _layout(k_pages), _layout(v_pages), _layout(table), _layout(lens), _layout(new))
+    device, copy, out_strides, sq, skp, svp, st, sizes, so, ws_bytes = _attention_plan(
+        *_layouts(q, k_pages, v_pages, table, lens, new))
     pq, kp, vp = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
     _check_addresses(what, kp, vp)
     if q.numel() == 0:
-        return _heads_last(q.shape, q)
+        return q.new_empty_strided(q.shape, out_strides)
     if copy or pq & 15:
         return paged_attention(_copy(q), k_pages, v_pages, table, lens, scale, new)
-    out = _heads_last(q.shape, q)
+    out = q.new_empty_strided(q.shape, out_strides)
     ws = _lib.workspace(ws_bytes, q.device) if ws_bytes else None
     _launch_on(device, _lib.lib().bb_paged_attention, pq, sq, kp, skp, vp, svp, table.data_ptr(), st, lens.data_ptr(),
                _lib.ptr(new), *sizes, float(scale), out.data_ptr(), so, _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
@@ -198,15 +209,17 @@ def paged_attention(q, k_pages, v_pages, table, lens, scale, new=None):
 @functools.lru_cache(maxsize=512)
 def _step_plan(q, k, v, kp, vp, table, lens, cos, sin, new):
     what = "paged_step"
+    device = _device_of(what, q, k, v, kp, vp, table, lens, cos, sin, new)
     hk, pages, page, w = _check_cache(what, q, kp, vp, table, lens, new)
     b, h, t, d = _check_queries(what, q, hk)
     if k[0] != (b, hk, t, d) or v[0] != k[0] or k[2] != q[2] or v[2] != q[2]:
         raise ValueError(f"{what}: k and v [B, Hkv, T, d] and q [B, H, T, d] must match the pages")
     copy_rope, sc, f32 = _check_rope(what, cos, sin, b, t, d, q[2])
     ws = _lib.lib().bb_paged_step_workspace(b, t, h, hk, d, page, w)
-    return (copy_rope or not (_aligned(q) and _aligned(k) and _aligned(v)), _strides3(q), _strides3(k), _strides3(v), sc, f32,
-            _strides3(kp), _strides3(vp), table[1][0], (b, t, h, hk, d, pages, page, w, int(q[2] is torch.float16)),
-            _lib.i64s(t * h * d, d, h * d), ws)
+    so = _heads_last(q[0])
+    return (device, copy_rope or not (_aligned(q) and _aligned(k) and _aligned(v)), so, _strides3(q), _strides3(k), _strides3(v),
+            sc, f32, _strides3(kp), _strides3(vp), table[1][0], _i32s(b, t, h, hk, d, pages, page, w, q[2] is torch.float16),
+            _i64s(*so[:3]), ws)
 
 
 def paged_step(q, k, v, k_pages, v_pages, table, lens, scale, cos=None, sin=None, new=None):
@@ -215,20 +228,18 @@ def paged_step(q, k, v, k_pages, v_pages, table, lens, scale, cos=None, sin=None
     rounded. A row that the call writes must not be attended in it by another sequence, nor at another place of its own table.
     Returns [B, H, T, d] in [B, T, H, d] memory."""
     what = "paged_step"
-    device = _device_of(what, q, k, v, k_pages, v_pages, table, lens, cos, sin, new)
-    copy, sq, sk, sv, sc, f32, skp, svp, st, sizes, so, ws_bytes = _step_plan(
-        _layout(q), _layout(k), _layout(v), _layout(k_pages), _layout(v_pages), _layout(table), _layout(lens), _layout(cos),
-        _layout(sin), _layout(new))
+    device, copy, out_strides, sq, sk, sv, sc, f32, skp, svp, st, sizes, so, ws_bytes = _step_plan(
+        *_layouts(q, k, v, k_pages, v_pages, table, lens, cos, sin, new))
     pq, pk, pv, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
     pc, ps = _lib.ptr(cos) or 0, _lib.ptr(sin) or 0
     _check_addresses(what, kp, vp)
     if q.numel() == 0:
-        return _heads_last(q.shape, q)
+        return q.new_empty_strided(q.shape, out_strides)
     if copy or (pq | pk | pv | pc | ps) & 15:
         if cos is not None:
             cos, sin = _whole_rope(cos, sin, q.shape[0], q.shape[2], q.shape[3])
         return paged_step(_copy(q), _copy(k), _copy(v), k_pages, v_pages, table, lens, scale, cos, sin, new)
-    out = _heads_last(q.shape, q)
+    out = q.new_empty_strided(q.shape, out_strides)
     ws = _lib.workspace(ws_bytes, q.device) if ws_bytes else None
     _launch_on(device, _lib.lib().bb_paged_step, pq, sq, pk, sk, pv, sv, pc, ps, sc, f32, kp, skp, vp, svp, table.data_ptr(), st,
                lens.data_ptr(), _lib.ptr(new), *sizes, float(scale), out.data_ptr(), so, _lib.ptr(ws), ws_bytes,
