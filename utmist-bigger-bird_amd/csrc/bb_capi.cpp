@@ -1076,15 +1076,20 @@ constexpr int kPagedStepVectors = 128;
 static const char* paged_schedule(int B, int T, int H, int Hkv, int D, int W, int page, bool with_new, PagedSchedule& s) {
   const int64_t R = (int64_t)T * (H / Hkv), cap = (int64_t)W * page;
   if (R <= kPagedStreamVectors || (with_new && R <= kPagedStepVectors)) {
+    // Two workgroups run on a CU (aiming at half as many, 32 x 8192 rows 114 us instead of 106; at twice, 131072 rows 91 for 87).
+    // A split of one chunk a wave is no faster than of two (4099 rows 15.4 and 15.5 us, four 18.2).
     s.VT = R <= 16 ? 16 : 32;
     s.unit = 4 * 4096 / D;
     s.min_share = 2;
     s.fit_quarters = 1 << 20;
     s.target = 2 * kCUs;
   } else {
+    // One workgroup runs on a CU (aiming at two a CU, 4096 tokens 147 us instead of 130). Short splits pay until their start is as
+    // long as they are (64 tokens over 4096 rows, splits of 16, 8, 4 and 2 tiles at least: 37.5, 28.7, 27.1 and 26.3 us). Fitted
+    // shares where they waste at most a quarter: 129 tokens over 32768 rows 94 us, 135 with rounded ones.
     s.VT = 256;
     s.unit = 64;
-    s.min_share = 8;
+    s.min_share = 4;
     s.fit_quarters = 5;
     s.target = kCUs;
   }

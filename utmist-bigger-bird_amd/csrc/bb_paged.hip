@@ -134,8 +134,10 @@ BB_DEV u32x2_t two_terms(float a, float b) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Append. A lane takes 8 elements of a row's lower half and the 8 that RoPE pairs with them; a row is D / 16 lanes, rows go
-// head by head (Q, then K, then V) through one token's, so that a wave's loads are contiguous in projections' outputs.
+// Append: K' = x cos + (-x[D/2:], x[:D/2]) sin of each new row into its page, V as it is, Q' beside. Bound by memory, each element
+// read and written once. A lane takes 8 elements of a row's lower half and the 8 that RoPE pairs with them; a row is D / 16 lanes,
+// rows go head by head (Q, then K, then V) through one token's, so that a wave's loads are contiguous in projections' outputs.
+// 8111 tokens of 32 + 8 + 8 heads of 128, bf16: 204 MB in 33 us, 6.1 TB/s (a large copy: 5.1); one token of 64 sequences: 3.6 us.
 template <int D, bool F16>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedAppendParams p) {
   constexpr int LPR = D / 16;
@@ -239,8 +241,10 @@ BB_DEV Share share_of(const PagedAttnParams& p, int first, int total) {
   Share s{least > p.min_share ? least : p.min_share, false};
   if (p.fit_quarters > 0) {
     Share f{s.units, true};
-    while (sum_over_lanes(f.splits(first)) * p.Hkv > 1 << p.target_log2) f.units += f.units < 8 ? 1 : f.units / 8;
-    if (4 * (int64_t)f.units <= (int64_t)p.fit_quarters * s.units) s = f;
+    const int64_t bound = (int64_t)p.fit_quarters * s.units;  // looked at in between: each try is a scan, some 0.3 us
+    while (4 * (int64_t)f.units <= bound && sum_over_lanes(f.splits(first)) * p.Hkv > 1 << p.target_log2)
+      f.units += f.units < 8 ? 1 : f.units / 8;
+    if (4 * (int64_t)f.units <= bound) s = f;
   }
   return s;
 }
@@ -317,7 +321,18 @@ BB_DEV void store_zeros(const PagedAttnParams& p, const Item& it, int D, int tid
 BB_DEV int split_begin(int u, int n, int s) { return n == 1 ? s * u : (int)((int64_t)u * s / n); }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Attention of up to 16 NR query vectors of a KV head over a split of a sequence's rows.
+// Attention of up to 16 NR query vectors of a KV head over a split of a sequence's rows: o = sum_i 2^(c q.k_i - m) v_i / sum_i
+// 2^(c q.k_i - m), m the running maximum. Bound by memory, so the loads never wait for the arithmetic:
+//   * Four waves, each with a stream of its own: chunks of 8 KB of K and 8 KB of V go straight into the wave's LDS by 16-byte
+//     loads, non-temporal, through a buffer as long as the rows that there are (the rest lands as zeros). The next chunk's K goes
+//     out when this one's is read, its V when this one's is, and exact vmcnt waits tell them apart. No barrier until the waves'
+//     states meet. Two workgroups a CU have 128 KB in flight there.
+//   * S^T = K Q^T leaves keys 16 kb + 4 a + i of vector x in lane (x, a), the order in which two transposed reads bring V's rows,
+//     so the probabilities are operands of O^T = V^T P^T where they are.
+//   * Splits go by the units of 4 chunks that there are, KV heads fastest, so that a head's pages stay with one XCD's L2.
+// One token (4 query heads a KV head of 128, 8 KV heads, bf16) of 32 sequences of up to 8192 rows: 639 MB in 104 us and 2 of the
+// merge behind it, 6.0 TB/s (a streaming read: 6.9); of one of 131072: 537 MB in 84 and 2. What is left is the start (launch,
+// plan, table, first chunk: 9 us in which little is loaded) and XCDs that end up to 8 % apart.
 template <bool F16>
 BB_DEV f32x4_t mma16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
   if constexpr (F16)
@@ -779,16 +794,23 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnParams
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Attention of many query vectors (prompts and their chunks): bound by the matrix cores, so a workgroup's 8 waves share every
-// K and V tile of 64 rows, 32 vectors each (two blocks of 16, so that every fragment read from LDS feeds two products).
+// Attention of many query vectors (prompts and their chunks): bound by the matrix cores and what feeds them, so a workgroup's 8
+// waves share every K and V tile of 64 rows, 32 vectors each (two blocks of 16, so that every fragment read from LDS feeds two
+// products).
 //   * Waves w and w + 4 share a SIMD and run half a tile apart: while one does products (O^T += V^T P^T of the tile before,
 //     then S^T = K Q^T), the other does its softmax, with workgroup barriers in between.
-//   * Tiles stream through rings of four stages by 16-byte loads into LDS, two tiles before they are wanted; each load's rows lie in one
-//     page, whose table entry came by a scalar load a tile earlier.
+//   * Tiles stream through rings of four stages by 16-byte loads into LDS, two tiles before they are wanted; each load's rows lie in
+//     one page, whose table entry came by a scalar load a tile earlier.
 //   * S^T leaves keys 16 kb + 4 a + i of vector x in lane (x, a), which is the order in which two transposed reads bring V's
 //     rows, so the probabilities are operands where they are.
 //   * The exponent's offset moves only when a probability would pass 2^8. Tiles that some vector attends in part, and every tile
 //     of a split whose table names no page somewhere, take a mask; they come last.
+// 4096 tokens of 32 heads of 128 (8 KV heads) over 32768 rows, bf16: 1604 us, 1285 TFLOP/s (a large product: 1256), 1.7 us a tile
+// and workgroup at a clock that the power holds at 1.9 to 2.0 GHz; the matrix cores are busy 60 % of it, the LDS reads of 256 KB a
+// tile (8 waves x 32 KB) take about as long as the products. head_dim 64, fp16: 1070 us, 963 TFLOP/s, 1.26 us a tile: as many
+// exponentials for half the products. Shapes tried there: four waves of 32 vectors, three workgroups a CU and one barrier a tile,
+// 1150 us (four prompts of 2048 tokens 63 against 64); eight waves with one barrier a tile 1210; the row sums by products with ones
+// 1090; two workgroups of eight waves a CU (128 registers) spill.
 constexpr int kTileWaves = 8, kTileStages = 4, kTileVecs = 32 * kTileWaves, kTileRows = 64;
 constexpr float kOver = 256.0f;  // 2^8
 
@@ -1208,7 +1230,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
 }
 
 // The splits' states of each vector under one maximum. Split s of n of a pair merges, in gridDim.y workgroups, the s-th part of
-// its vectors: a group of D / 4 lanes a vector, or all groups of the workgroup one vector where that is its part.
+// its vectors: a group of D / 4 lanes a vector, or all groups of the workgroup one vector where that is its part. 4 us traced, of
+// which 2 lie beside the attention's end, whatever it merges; a quarter or half of the workgroups in a loop over the slots are no
+// faster.
 template <int D, bool F16>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttnParams p) {
   constexpr int LPV = D / 4, NG = kThreads / LPV, ROW = D + 4;
