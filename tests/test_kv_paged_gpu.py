@@ -381,6 +381,43 @@ def test_many_sequences(dev):
         _check(got, want, tol, BF16)
 
 
+@pytest.mark.parametrize("b,long,T,H,hk", [(70, 9000, 1, 4, 2), (70, 5000, 3, 8, 2), (66, 4000, 40, 2, 2), (1100, 3000, 1, 2, 1)])
+def test_many_sequences_of_unlike_lengths(b, long, T, H, hk, dev):
+    """One long sequence, which is split, among many short or empty ones; the call, its step and replays of both in a graph."""
+    _say("many sequences of unlike lengths", b, T)
+    gen = torch.Generator(device=dev).manual_seed(6)
+    lens = [(7 * i) % 40 if i % 3 else 0 for i in range(b)]
+    lens[b // 2] = long
+    new = [min(T, n) for n in lens]
+    q, kp, vp, table, ln, _ = _attend_case(lens, None, T, H, hk, 64, 16, BF16, dev)
+    k, v = (_heads(gen, b, hk, T, 64, BF16, dev) for _ in "kv")
+    nw = _int(new, dev)
+    streams = T * H // hk <= STREAM_VECTORS
+    want, tol = plain.attend(q, kp, vp, table, lens, 0.125, new, _p_step(BF16, streams))
+    _check(paged_attention(q, kp, vp, table, ln, 0.125, new=nw), want, tol, BF16)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        paged_attention(q, kp, vp, table, ln, 0.125, new=nw)
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        out = paged_attention(q, kp, vp, table, ln, 0.125, new=nw)
+        stepped = paged_step(q, k, v, kp, vp, table, ln, 0.125, new=nw)
+    for turn in range(3):  # the long sequence moves
+        lens[b // 2 - turn], lens[b // 2 - turn - 1] = lens[b // 2 - turn - 1], lens[b // 2 - turn]
+        table[[b // 2 - turn, b // 2 - turn - 1]] = table[[b // 2 - turn - 1, b // 2 - turn]]
+        new = [min(T, n) for n in lens]
+        ln.copy_(_int(lens, dev))
+        nw.copy_(_int(new, dev))
+        before = paged_attention(q, kp, vp, table, ln, 0.125, new=nw)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, before)
+        if streams:  # (of 40 vectors the step is the streaming kernel's, the attention the tiles')
+            assert torch.equal(stepped, paged_attention(q, kp, vp, table, ln, 0.125, new=nw))
+        want, tol = plain.attend(q, kp, vp, table, lens, 0.125, new, _p_step(BF16, T * H // hk <= STEP_VECTORS))
+        _check(stepped, want, tol, BF16)
+
+
 @pytest.mark.parametrize("T", [1, 50])
 def test_captured_steps_follow_the_cache(T, dev):
     """Two captured graphs over one cache, replayed in turn while the lengths and the table grow, with eager work between: every

@@ -1061,7 +1061,8 @@ int bb_int4_decode_append(const void* q, const int64_t* sq, uint8_t* kq, void* k
 // How a call of the attention is cut (the kernels cut the lengths that they find by it).
 struct PagedSchedule {
   int VT, tiles, unit, min_share, target, fit_quarters, grid;
-  size_t slots, bytes;  // of partials; of the workspace: the partials, then what each slot holds and how many are used
+  size_t slots, items;  // of partials; of workgroups that are laid out by a kernel before (more than a wave's pairs)
+  size_t part, bytes;   // of the partials with what each slot holds and how many are used; of the workspace: these, then the items
 };
 // Query vectors of a KV head up to which the streaming kernel takes a call. (us streaming and in tiles of 64 rows, 8 KV heads,
 // head_dim 128: 16 vectors 12.3 and 18.3 at 4096 rows, 35 and 42 at 8 x 8192, 30 and 30 at 32768; 32: 15.4 and 19, 39 and 43, 33 and
@@ -1102,7 +1103,9 @@ static const char* paged_schedule(int B, int T, int H, int Hkv, int D, int W, in
   // a pair of more than one split has at most twice its units over the share of them
   s.slots = most > 1 ? (size_t)std::min<int64_t>(s.grid, 2 * s.target) : 0;
   if (pairs > 64 || pairs * Hkv > s.target) s.fit_quarters = 0;
-  s.bytes = s.slots ? s.slots * s.VT * (D + 4) * 4 + (s.slots + 1) * 16 : 0;
+  s.part = s.slots ? s.slots * s.VT * (D + 4) * 4 + (s.slots + 1) * 16 : 0;
+  s.items = pairs > 64 ? (size_t)s.grid : 0;
+  s.bytes = s.part + s.items * 16;
   return nullptr;
 }
 
@@ -1235,8 +1238,9 @@ static int paged_attention_impl(const char* what, const void* q, const int64_t* 
   }
   p.out = static_cast<uint16_t*>(out);
   p.so0 = so[0]; p.so1 = so[1]; p.so2 = so[2];
-  p.part = need ? static_cast<float*>(ws) : nullptr;
-  p.plan = need ? reinterpret_cast<int4*>(p.part + s.slots * s.VT * (D + 4)) : nullptr;
+  p.part = s.slots ? static_cast<float*>(ws) : nullptr;
+  p.plan = s.slots ? reinterpret_cast<int4*>(p.part + s.slots * s.VT * (D + 4)) : nullptr;
+  p.items = s.items ? reinterpret_cast<int4*>(static_cast<char*>(ws) + s.part) : nullptr;
   p.B = B; p.T = T; p.H = H; p.Hkv = Hkv; p.G = H / Hkv; p.D = D;
   p.f16 = is_f16 ? 1 : 0;
   p.VT = s.VT; p.tiles = s.tiles; p.pairs = s.tiles * B;

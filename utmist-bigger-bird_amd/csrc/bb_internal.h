@@ -172,6 +172,7 @@ struct PagedAttnParams {
   int B, T, H, Hkv, G, D, f16;
   int VT, tiles, pairs;        // query vectors of a tile, tiles, B * tiles
   int4* plan;                  // of each slot (sequence, tile, KV head, split | splits << 16), then (slots used, -, -, -)
+  int4* items;                 // of each workgroup (paged_plan_kernel), or null: up to 64 pairs, each workgroup finds its own
   int unit_log2, min_share, target_log2;  // rows of a unit; units of a split, at least; workgroups aimed at
   int fit_quarters;                       // see share_of
   float inv_G, inv_B, inv_Hkv;

@@ -184,8 +184,8 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedAppendParam
 // How a call's work is cut. A pair is (sequence, tile of VT query vectors of a KV head; vector v = token v / G, head v % G);
 // its keys, the rows that its last real token attends, are cut into equal splits of whole units so that all splits of the
 // call are about as long: `share` units, the call's total over p.target workgroups, at least p.min_share. Each workgroup
-// finds its (pair, KV head, split) by a scan over the pairs, so lengths may stay on the device and the grid goes by the
-// capacity alone. Pairs with one split write the output, the others a partial for the merge.
+// finds its (pair, KV head, split) by the lengths on the device, and the grid goes by the capacity alone. Pairs with one split
+// write the output, the others a partial for the merge.
 BB_DEV int wave_scan(int v) {  // inclusive sum over the lanes
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
   v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
@@ -251,64 +251,124 @@ BB_DEV Share share_of(const PagedAttnParams& p, int first, int total) {
 // What a workgroup does: split `split` of a pair, or (zero) the output of a pair without rows to attend, or nothing.
 struct Item {
   bool live, zero;
-  int b, tile, g, split, splits, slot, units;
+  int b, tile, g, split, splits, slot;
 };
 // The item with index `item`, by a whole wave: the splits of all pairs in order, then the pairs without any, KV heads fastest.
-// (Pairs without rows among the others would hold up the dispatch of long ones behind them.)
+// (Pairs without rows among the others would hold up the dispatch of long ones behind them.) Up to a wave's pairs it is found by a
+// scan in each workgroup, 1.5 to 2 us at its start; more are laid out by a kernel before. (With scans of 64 at a time and with that
+// kernel: 4 prompts of up to 2048 tokens, 128 pairs, 67 and 65 us; one token of 512 sequences of up to 512 rows 128 and 107, of
+// 4096 of them 2429 and 824; 512 prompts of up to 128 tokens 732 and 349.)
 BB_DEV Item find_item(const PagedAttnParams& p, int item, int lane) {
-  int first = 0, total = 0;
-  for (int at = 0; at < p.pairs; at += 64) {
-    const int u = pair_units(p, at + lane);
-    if (at == 0) first = u;
-    total += sum_over_lanes(u);
-  }
-  const Share share = share_of(p, first, total);
-  int pair = -1, units = 0, splits = 0, slot = 0, before = 0, items = 0, slots = 0;
-  for (int at = 0; at < p.pairs && (pair < 0 || item == 0); at += 64) {  // (item 0 counts all slots)
-    const int u = at == 0 ? first : pair_units(p, at + lane);
-    const int sp = share.splits(u), mine = sp * p.Hkv, split = sp > 1 ? mine : 0;
-    const int upto = items + wave_scan(mine), slot_upto = slots + wave_scan(split);
-    const uint64_t in = __builtin_amdgcn_ballot_w64(item < upto);
-    if (in && pair < 0) {
-      const int l = __builtin_ctzll(in);
-      pair = at + l;
-      units = lane_int(u, l);
-      splits = lane_int(sp, l);
-      slot = lane_int(slot_upto - split, l);
-      before = lane_int(upto - mine, l);
-    }
-    items = lane_int(upto, 63);
-    slots = lane_int(slot_upto, 63);
-  }
   Item it;
-  it.live = pair >= 0;
-  if (!it.live) {
-    int nth = quotient(item - items, p.inv_Hkv, p.Hkv);
-    before = items + nth * p.Hkv;
-    for (int at = 0; at < p.pairs && pair < 0; at += 64) {
-      const uint64_t none = __builtin_amdgcn_ballot_w64(at + lane < p.pairs && (at == 0 ? first : pair_units(p, at + lane)) == 0);
-      const int here = __builtin_popcountll(none);
-      if (nth < here) {
-        const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(none >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)none, 0));
-        pair = at + __builtin_ctzll(__builtin_amdgcn_ballot_w64((none >> lane & 1) && rank == nth));
-      }
-      nth -= here;
+  if (p.items) {
+    const int4 r = p.items[item];
+    it.live = r.z > 0;
+    it.zero = r.z == 0;
+    it.b = __builtin_amdgcn_readfirstlane((uint32_t)r.x >> 16);
+    it.g = __builtin_amdgcn_readfirstlane(r.x & 0xffff);
+    it.tile = __builtin_amdgcn_readfirstlane(r.y);
+    it.split = __builtin_amdgcn_readfirstlane(r.z & 0xffff);
+    it.splits = __builtin_amdgcn_readfirstlane(r.z >> 16);
+    it.slot = __builtin_amdgcn_readfirstlane(r.w);
+  } else {
+    const int u = pair_units(p, lane), total = sum_over_lanes(u);
+    const int sp = share_of(p, u, total).splits(u), mine = sp * p.Hkv, split = sp > 1 ? mine : 0;
+    const int upto = wave_scan(mine), slot_upto = wave_scan(split), items = lane_int(upto, 63);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(item < upto);
+    it.live = in != 0;
+    int pair = -1, splits = 0, slot = 0, before;
+    if (it.live) {
+      pair = __builtin_ctzll(in);
+      splits = lane_int(sp, pair);
+      slot = lane_int(slot_upto - split, pair);
+      before = lane_int(upto - mine, pair);
+    } else {
+      const int nth = quotient(item - items, p.inv_Hkv, p.Hkv);
+      before = items + nth * p.Hkv;
+      const uint64_t none = __builtin_amdgcn_ballot_w64(lane < p.pairs && u == 0);
+      const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(none >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)none, 0));
+      if (nth < __builtin_popcountll(none)) pair = __builtin_ctzll(__builtin_amdgcn_ballot_w64((none >> lane & 1) && rank == nth));
     }
+    it.zero = !it.live && pair >= 0;
+    const int rest = item - before;
+    it.split = it.live ? quotient(rest, p.inv_Hkv, p.Hkv) : 0;
+    it.g = rest - it.split * p.Hkv;
+    it.tile = pair_tile(p, pair < 0 ? 0 : pair);
+    it.b = pair_sequence(p, pair < 0 ? 0 : pair, it.tile);
+    it.splits = splits;
+    it.slot = slot + it.g * splits + it.split;
+    if (p.part && item == 0 && threadIdx.x == 0) p.plan[p.slots].x = lane_int(slot_upto, 63);
   }
-  it.zero = !it.live && pair >= 0;
-  const int rest = item - before;
-  it.split = it.live ? quotient(rest, p.inv_Hkv, p.Hkv) : 0;
-  it.g = rest - it.split * p.Hkv;
-  it.tile = pair_tile(p, pair < 0 ? 0 : pair);
-  it.b = pair_sequence(p, pair < 0 ? 0 : pair, it.tile);
-  it.splits = splits;
-  it.slot = slot + it.g * splits + it.split;
-  it.units = units;
-  if (p.part && threadIdx.x == 0) {  // for the merge
-    if (splits > 1) p.plan[it.slot] = make_int4(it.b, it.tile, it.g, it.split | splits << 16);
-    if (item == 0) p.plan[p.slots].x = slots;
-  }
+  if (p.part && threadIdx.x == 0 && it.splits > 1)  // for the merge
+    p.plan[it.slot] = make_int4(it.b, it.tile, it.g, it.split | it.splits << 16);
   return it;
+}
+// The same for more than a wave's pairs, in one workgroup: items[i] is (sequence << 16 | KV head, tile, split | splits << 16, slot),
+// 0 splits for a pair without rows, -1 for nothing.
+constexpr int kPlanThreads = 1024;
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedAttnParams p) {
+  constexpr int WAVES = kPlanThreads / 64;
+  __shared__ int sums[2][3][WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int turn = 0;
+  // v[i]'s inclusive sums over the workgroup's threads up to this one, and over all of them.
+  auto scan = [&](int (&v)[3], int (&all)[3]) {
+    turn ^= 1;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      v[i] = wave_scan(v[i]);
+      if (lane == 63) sums[turn][i][wave] = v[i];
+    }
+    __syncthreads();  // (the space of the scan before is not written again until all have read it: that is this barrier too)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      all[i] = 0;
+      for (int w = 0; w < WAVES; ++w) {
+        const int x = sums[turn][i][w];
+        all[i] += x;
+        v[i] += w < wave ? x : 0;
+      }
+    }
+  };
+  int v[3] = {0, 0, 0}, all[3];
+  for (int pair = tid; pair < p.pairs; pair += kPlanThreads) v[0] += pair_units(p, pair);
+  scan(v, all);
+  const Share share = share_of(p, 0, all[0]);
+  int items = 0, slots = 0, zeros = 0;
+  for (int at = 0; at < p.pairs; at += kPlanThreads) {
+    const int pair = at + tid, u = pair_units(p, pair), sp = share.splits(u), mine = sp * p.Hkv;
+    v[0] = mine;
+    v[1] = sp > 1 ? mine : 0;
+    v[2] = 0;
+    const int split = v[1];
+    scan(v, all);
+    if (sp > 0) {
+      const int tile = pair_tile(p, pair), b = pair_sequence(p, pair, tile);
+      const int first = items + v[0] - mine, slot = slots + v[1] - split;
+      for (int s = 0; s < sp; ++s)
+        for (int g = 0; g < p.Hkv; ++g) {
+          const int i = first + s * p.Hkv + g;
+          if (i < p.grid) p.items[i] = make_int4((int)((uint32_t)b << 16 | g), tile, s | sp << 16, slot + g * sp + s);
+        }
+    }
+    items += all[0];
+    slots += all[1];
+  }
+  for (int at = 0; at < p.pairs; at += kPlanThreads) {
+    const int pair = at + tid;
+    const bool none = pair < p.pairs && pair_units(p, pair) == 0;
+    v[0] = none ? p.Hkv : 0;
+    v[1] = v[2] = 0;
+    scan(v, all);
+    if (none) {
+      const int tile = pair_tile(p, pair), b = pair_sequence(p, pair, tile), first = items + zeros + v[0] - p.Hkv;
+      for (int g = 0; g < p.Hkv; ++g)
+        if (first + g < p.grid) p.items[first + g] = make_int4((int)((uint32_t)b << 16 | g), tile, 0, 0);
+    }
+    zeros += all[0];
+  }
+  for (int i = items + zeros + tid; i < p.grid; i += kPlanThreads) p.items[i] = make_int4(0, 0, -1, 0);
+  if (tid == 0 && p.part) p.plan[p.slots].x = slots;
 }
 // Zeros for a pair's tokens.
 BB_DEV void store_zeros(const PagedAttnParams& p, const Item& it, int D, int tid, int threads) {
@@ -502,7 +562,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnParams
   if (!it.live) return;
   const Sequence s = sequence(p.c, p.T, it.b);
   const int keys = __builtin_amdgcn_readfirstlane(pair_keys(p, s, it.tile));
-  const int u0 = split_begin(it.units, it.splits, it.split), u1 = split_begin(it.units, it.splits, it.split + 1);
+  const int units = (keys + (1 << p.unit_log2) - 1) >> p.unit_log2;
+  const int u0 = split_begin(units, it.splits, it.split), u1 = split_begin(units, it.splits, it.split + 1);
   int begin = u0 << p.unit_log2, end = u1 << p.unit_log2 < keys ? u1 << p.unit_log2 : keys;
   begin = __builtin_amdgcn_readfirstlane(begin);
   end = __builtin_amdgcn_readfirstlane(end);
@@ -1012,8 +1073,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
   if (!it.live) return;
   const Sequence s = sequence(p.c, p.T, it.b);
   const int keys = __builtin_amdgcn_readfirstlane(pair_keys(p, s, it.tile));
-  const int u0 = __builtin_amdgcn_readfirstlane(split_begin(it.units, it.splits, it.split));
-  const int u1 = __builtin_amdgcn_readfirstlane(split_begin(it.units, it.splits, it.split + 1));
+  const int units = (keys + kTileRows - 1) / kTileRows;
+  const int u0 = __builtin_amdgcn_readfirstlane(split_begin(units, it.splits, it.split));
+  const int u1 = __builtin_amdgcn_readfirstlane(split_begin(units, it.splits, it.split + 1));
   const int begin = u0 * kTileRows, end = u1 * kTileRows < keys ? u1 * kTileRows : keys;
   const int n_tiles = (end - begin + kTileRows - 1) / kTileRows;  // 1 at least
   const int v0 = it.tile * kTileVecs;
@@ -1356,6 +1418,7 @@ hipError_t attend(const PagedAttnParams& p, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_paged_attention(const PagedAttnParams& p, hipStream_t stream) {
+  if (p.items) paged_plan_kernel<<<1, kPlanThreads, 0, stream>>>(p);
   if (p.D == 128) return p.f16 ? attend<128, true>(p, stream) : attend<128, false>(p, stream);
   return p.f16 ? attend<64, true>(p, stream) : attend<64, false>(p, stream);
 }
