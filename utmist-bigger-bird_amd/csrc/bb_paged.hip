@@ -500,7 +500,8 @@ struct PageStream {
 };
 
 // A step's new rows among the rows [k0, k0 + KC) of a wave's landed chunk: rotated, into the pages and into LDS over what the
-// pages held there. No other wave of the call reads these rows.
+// pages held there. No other wave of the head's tile has these rows; where a head has several tiles, each does this for itself, and
+// the pages get the same values from each.
 template <int D, bool F16>
 BB_DEV void patch_new_rows(const PagedAttnParams& p, const Sequence& s, int b, int g, int k0, int lane, uint8_t* ks, uint8_t* vs) {
   constexpr int KC = PageStream<D>::KC, LPR = D / 16;
