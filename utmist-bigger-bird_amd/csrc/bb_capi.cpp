@@ -1069,8 +1069,8 @@ struct PagedSchedule {
 // 31; 64, which read the cache twice where they stream: 17 and 20, 53 and 44, 50 and 33.)
 constexpr int kPagedStreamVectors = 32;
 // And up to which it takes a step by itself, rotating q and storing the new rows; more go through the append, and their rotated q
-// is rounded. (By itself and in two, the same sizes: 16 vectors 16.5 and 19.3, 38 and 39, 33 and 34 us; 32: 22 and 20, 45 and 44, 39
-// and 37; 64: 24 and 24, 61 and 49, 58 and 37; 128: 33 and 27, 85 and 54, 78 and 42. The outputs' error against 64 bits is 0.0017 of
+// is rounded. (By itself and in two, the same sizes: 16 vectors 16.5 and 18.7, 38 and 40, 33 and 33 us; 32: 21 and 20, 45 and 44, 39
+// and 36; 64: 24 and 22, 53 and 48, 53 and 37; 128: 32 and 26, 69 and 54, 60 and 42. The outputs' error against 64 bits is 0.0017 of
 // them by itself, which is their own rounding, and 0.0029 to 0.0032 in two. Of up to 128 vectors, where single tokens and drafts
 // of a few end, the error decides.)
 constexpr int kPagedStepVectors = 128;

@@ -452,8 +452,10 @@ BB_DEV void load_rows(const PageRows& at, uint8_t* to, uint32_t off) {
       reinterpret_cast<lds_void*>(reinterpret_cast<uintptr_t>(to)), 16, off, 0, 0, AUX);
 }
 
-// One wave's stream of chunks of KC rows, 8 KB of K and of V.
-template <int D>
+// One wave's stream of chunks of KC rows, 8 KB of K and of V. AUX: of its loads, 2 (non-temporal) where a row is read once (32
+// sequences of 8192 rows 107 us, 122 without), 0 where a head has several tiles and reads it again (a step of 64 vectors over 32768
+// rows 53 us, 57 with; of 128 63 and 77).
+template <int D, int AUX>
 struct PageStream {
   static constexpr int KC = 4096 / D, GROUPS = KC / 16, LOADS = 8 / GROUPS;  // groups of 16 rows lie in one page
   static constexpr int RPL = 512 / D;                                        // rows of a load
@@ -493,7 +495,7 @@ struct PageStream {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const uint32_t piece = is_v ? vpiece ^ 16u * v_swz<D>(RPL * i) : kpiece ^ 16u * k_swz<D>(RPL * i);
-        load_rows<2 /* non-temporal */>(at, to + 1024 * (LOADS * j + i), (row + RPL * i) * rb + piece);
+        load_rows<AUX>(at, to + 1024 * (LOADS * j + i), (row + RPL * i) * rb + piece);
       }
     }
   }
@@ -504,7 +506,7 @@ struct PageStream {
 // the pages get the same values from each.
 template <int D, bool F16>
 BB_DEV void patch_new_rows(const PagedAttnParams& p, const Sequence& s, int b, int g, int k0, int lane, uint8_t* ks, uint8_t* vs) {
-  constexpr int KC = PageStream<D>::KC, LPR = D / 16;
+  constexpr int KC = PageStream<D, 0>::KC, LPR = D / 16;
   const int d = 8 * (lane % LPR), c = lane % LPR;
   for (int i = lane / LPR; i < 2 * s.fresh; i += 64 / LPR) {
     const int j = i >> 1, row = s.first + j;
@@ -550,9 +552,9 @@ BB_DEV uint32_t not_finite(uint32_t w) {  // 0xffff in the halves that are not
   return ((w & e) == e ? 0xffffu : 0u) | ((w >> 16 & e) == e ? 0xffff0000u : 0u);
 }
 
-template <int D, bool F16, int NR, bool NEW>
+template <int D, bool F16, int NR, bool NEW, int AUX>
 __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnParams p) {
-  using Stream = PageStream<D>;
+  using Stream = PageStream<D, AUX>;
   constexpr int KC = Stream::KC, GROUPS = Stream::GROUPS, NDS = D / 32, NDB = D / 16;
   constexpr int ROW = D + 4;  // floats of a state's row: whole 16-byte pieces, rows on other banks
   __shared__ __attribute__((aligned(16))) uint8_t sm[kWaves][2][8192];
@@ -1402,8 +1404,9 @@ hipError_t attend(const PagedAttnParams& p, hipStream_t stream) {
     if (1 << p.c.page_log2 >= kTileRows) paged_tile_kernel<D, F16, true><<<p.grid, 64 * kTileWaves, 0, stream>>>(p);
     else paged_tile_kernel<D, F16, false><<<p.grid, 64 * kTileWaves, 0, stream>>>(p);
   }
-  else if (p.knew) paged_attn_kernel<D, F16, NR, true><<<p.grid, kThreads, 0, stream>>>(p);
-  else paged_attn_kernel<D, F16, NR, false><<<p.grid, kThreads, 0, stream>>>(p);
+  else if (NR == 2 && p.tiles > 1) paged_attn_kernel<D, F16, 2, true, 0><<<p.grid, kThreads, 0, stream>>>(p);  // (a step)
+  else if (p.knew) paged_attn_kernel<D, F16, NR, true, 2><<<p.grid, kThreads, 0, stream>>>(p);
+  else paged_attn_kernel<D, F16, NR, false, 2><<<p.grid, kThreads, 0, stream>>>(p);
   if (p.part) {
     const dim3 grid(p.slots, p.VT > 32 ? 4 : 1);  // a tile's parts are many vectors
     paged_merge_kernel<D, F16><<<grid, kThreads, 0, stream>>>(p);
