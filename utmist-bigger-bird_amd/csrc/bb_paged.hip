@@ -948,6 +948,9 @@ BB_DEV void ring_barrier() {
   __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
+// The waves of a workgroup see what this one stored in LDS behind the next ring_barrier, which waits for no store by itself.
+// (A release fence waits for the loads in flight too.)
+BB_DEV void publish() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 BB_DEV uint32_t lds_addr(const void* p) {
   return (uint32_t)reinterpret_cast<uintptr_t>(
       reinterpret_cast<__attribute__((address_space(3))) const void*>(reinterpret_cast<uintptr_t>(p)));
@@ -1070,7 +1073,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
   __shared__ int odd[kTileStages];  // whether V's tile there may hold values that are not finite (never taken back)
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 15, a = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), late = wave >> 2;  // waves w and w + 4 share a SIMD
-  if (tid < kTileStages) odd[tid] = 0;  // (the barrier before the first products comes before any use)
+  if (tid < kTileStages) {  // (the barrier before the first products comes before any use)
+    odd[tid] = 0;
+    publish();
+  }
   const Item it = find_item(p, blockIdx.x, lane);
   if (it.zero) store_zeros(p, it, D, tid, 64 * kTileWaves);
   if (!it.live) return;
@@ -1167,7 +1173,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
 #pragma unroll
       for (int e = 0; e < 4; ++e) any |= not_finite<F16>(w[e]);
     }
-    if (__builtin_amdgcn_ballot_w64(any != 0)) odd[i & (kTileStages - 1)] = 1;
+    if (__builtin_amdgcn_ballot_w64(any != 0)) {
+      odd[i & (kTileStages - 1)] = 1;
+      publish();
+    }
   };
   auto odd_values = [&](int i) { return __builtin_amdgcn_readfirstlane(odd[i & (kTileStages - 1)]) != 0; };
   auto masked_values = [&](int i) {
