@@ -375,10 +375,10 @@ class PagedCache(DynamicCache):
         return before[:, None] + torch.arange(max(self._step) if t is None else t, device=self.lens.device)
 
     def truncate(self, lengths):
-        """Keep the first lengths[b] rows of each sequence; whole pages behind them become free. A step that did not run is taken
-        back with it."""
+        """Keep the first lengths[b] rows of each sequence; whole pages behind them become free. A step that did not run through
+        every layer is taken back with it: its rows are none that a sequence has."""
         lengths = [int(x) for x in lengths]
-        if len(lengths) != len(self.lengths) or any(not 0 <= x <= n for x, n in zip(lengths, self.lengths)):
+        if len(lengths) != len(self.lengths) or any(not 0 <= x <= n for x, n in zip(lengths, self._before())):
             raise ValueError("PagedCache: one length per sequence, of rows that it has")
         for b, n in enumerate(lengths):
             keep = -(-n // self.page)
@@ -391,16 +391,16 @@ class PagedCache(DynamicCache):
         self.new.zero_()
 
     def release(self, sequences):
-        """Empty these sequences (an index or several)."""
+        """Empty these sequences (an index or several); a step that did not run is taken back."""
         gone = {sequences} if isinstance(sequences, int) else set(sequences)
         if not gone <= set(range(len(self.lengths))):
             raise ValueError("PagedCache: no such sequence")
-        self.truncate([0 if b in gone else n for b, n in enumerate(self.lengths)])
+        self.truncate([0 if b in gone else n for b, n in enumerate(self._before())])
 
     def crop(self, tokens_to_remove):
         if tokens_to_remove > 0:
             raise NotImplementedError("PagedCache.crop supports negative token counts only")
-        self.truncate([max(0, n + tokens_to_remove) for n in self.lengths])
+        self.truncate([max(0, n + tokens_to_remove) for n in self._before()])
 
     def reset(self):
         self.truncate([0] * len(self.lengths))
