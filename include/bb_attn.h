@@ -429,7 +429,7 @@ int bb_paged_append(const void* k, const int64_t* skn, const void* v, const int6
  * attends the rows up to its own, lens - fresh + j, of the pages that its table names; scores and softmax in fp32. Zeros
  * where it attends none, and for padding; NaN where its scores have no softmax (a query that is not finite). A row of V
  * that is not finite reaches only the tokens that attend it. H / Hkv query heads per KV head, any number.
- * Workspace: bb_paged_attention_workspace (0: none).
+ * Workspace: bb_paged_attention_workspace (0: none, or a call that is refused).
  */
 int bb_paged_attention(const void* q, const int64_t* sq, const void* k_pages, const int64_t* sk, const void* v_pages,
                        const int64_t* sv, const int32_t* table, int64_t st, const int32_t* lens, const int32_t* fresh, int B,
@@ -437,8 +437,8 @@ int bb_paged_attention(const void* q, const int64_t* sq, const void* k_pages, co
                        const int64_t* so, void* ws, size_t ws_bytes, void* stream);
 size_t bb_paged_attention_workspace(int B, int T, int H, int Hkv, int D, int page, int W);
 
-/* One step: bb_paged_append of k and v, then bb_paged_attention of the rotated q (not rotated where cos is NULL). Workspace:
- * bb_paged_step_workspace. */
+/* One step: bb_paged_append of k and v, then bb_paged_attention of the rotated q (not rotated where cos is NULL). A call that is
+ * refused writes nothing. Workspace: bb_paged_step_workspace (0: none, or a call that is refused). */
 int bb_paged_step(const void* q, const int64_t* sq, const void* k, const int64_t* skn, const void* v, const int64_t* svn,
                   const void* cos, const void* sin, const int64_t* sc, int rope_f32, void* k_pages, const int64_t* sk,
                   void* v_pages, const int64_t* sv, const int32_t* table, int64_t st, const int32_t* lens,

@@ -1,8 +1,13 @@
 """Paged KV cache without a GPU, at its edges: steps that are taken back, masks, and calls that are refused before a launch."""
+import ctypes
+
 import pytest
 import torch
 
-from test_kv_paged_cpu import _cache, _consistent, _run
+from bigger_bird_amd import _lib
+from test_kv_paged_cpu import P16, _cache, _consistent, _run, _s, _step
+
+P16_ODD = ctypes.c_void_p(24)
 
 
 def _two(lengths=(20, 10)):
@@ -44,3 +49,24 @@ def test_truncate_refuses_rows_that_were_not_written():
     c.truncate([21, 34])
     assert c.lengths == [21, 34]
     _consistent(c)
+
+
+# ---------------------------------------------------------------- the C ABI's checks
+@pytest.mark.parametrize("over,msg", [
+    (dict(out=P16_ODD), "16-byte alignment"),
+    (dict(so=_s(4096, 130, 4096)), "16-byte alignment"),
+    (dict(scale=0.0), "scale must be positive"),
+    (dict(B=1, T=128, H=1 << 15, Hkv=1), "lengths out of range"),
+])
+def test_a_step_of_many_vectors_is_refused_before_it_writes(over, msg):
+    """64 tokens of four heads a KV head are two launches, the append and the attention: what the second refuses is refused before
+    the first (which there is no GPU for here, so that its error would be another)."""
+    rc, err = _step(**{**dict(T=64, ws=P16, ws_bytes=1 << 40), **over})
+    assert rc == -1 and msg in err, err
+
+
+def test_no_workspace_for_a_call_that_is_refused():
+    L = _lib.lib()
+    assert L.bb_paged_step_workspace(1, 64, 32, 8, 128, 64, 4) == 64 * 32 * 128 * 2
+    for bad in [(1, 128, 1 << 15, 1, 128, 64, 4), (1, 64, 32, 8, 96, 64, 4), (1, 64, 30, 8, 128, 64, 4), (1, 64, 32, 8, 128, 64, 0)]:
+        assert L.bb_paged_attention_workspace(*bad) == 0 and L.bb_paged_step_workspace(*bad) == 0

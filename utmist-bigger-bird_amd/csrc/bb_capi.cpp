@@ -1193,28 +1193,30 @@ int bb_paged_append(const void* k, const int64_t* skn, const void* v, const int6
   return hip_status(bb::launch_paged_append(p, static_cast<hipStream_t>(stream)), "bb_paged_append");
 }
 
-static size_t paged_partials(int B, int T, int H, int Hkv, int D, int page, int W, bool with_new) {
-  PagedSchedule s;
-  if (B < 1 || T < 1 || H < 1 || Hkv < 1 || H % Hkv || page < 16 || W < 1 || (D != 64 && D != 128)) return 0;
-  if (paged_schedule(B, T, H, Hkv, D, W, page, with_new, s)) return 0;
-  return s.bytes;
+// The schedule of a call of these sizes; false: there is no such call.
+static bool paged_sizes(int B, int T, int H, int Hkv, int D, int page, int W, bool with_new, PagedSchedule& s) {
+  if (B < 1 || T < 1 || H < 1 || Hkv < 1 || H % Hkv || page < 16 || W < 1 || (D != 64 && D != 128)) return false;
+  return paged_schedule(B, T, H, Hkv, D, W, page, with_new, s) == nullptr;
 }
 
 size_t bb_paged_attention_workspace(int B, int T, int H, int Hkv, int D, int page, int W) {
-  return paged_partials(B, T, H, Hkv, D, page, W, false);
+  PagedSchedule s;
+  return paged_sizes(B, T, H, Hkv, D, page, W, false, s) ? s.bytes : 0;
 }
 
 size_t bb_paged_step_workspace(int B, int T, int H, int Hkv, int D, int page, int W) {
   if (B < 1 || T < 1 || H < 1 || Hkv < 1) return 0;
   const bool one = (int64_t)T * (H / Hkv) <= kPagedStepVectors;
-  const size_t part = paged_partials(B, T, H, Hkv, D, page, W, one);
-  return one ? part : align256(part) + (size_t)B * T * H * D * 2;  // rotated q
+  PagedSchedule s;
+  if (!paged_sizes(B, T, H, Hkv, D, page, W, one, s)) return 0;
+  return one ? s.bytes : align256(s.bytes) + (size_t)B * T * H * D * 2;  // rotated q
 }
 
-static int paged_attention_impl(const char* what, const void* q, const int64_t* sq, const void* knew, const int64_t* skn,
-                                const void* vnew, const int64_t* svn, const bb::PagedCache& c, const bb::PagedRope& r, int B,
-                                int T, int H, int Hkv, int D, int page, int is_f16, float scale, void* out,
-                                const int64_t* so, void* ws, size_t ws_bytes, void* stream) {
+// A call of the attention, checked and laid out.
+static int paged_attention_params(const char* what, const void* q, const int64_t* sq, const void* knew, const int64_t* skn,
+                                  const void* vnew, const int64_t* svn, const bb::PagedCache& c, const bb::PagedRope& r, int B,
+                                  int T, int H, int Hkv, int D, int page, int is_f16, float scale, void* out,
+                                  const int64_t* so, void* ws, size_t ws_bytes, bb::PagedAttnParams& p) {
   int rc = paged_rows(what, q, sq);
   if (rc == BB_OK) rc = paged_rows(what, out, so);
   if (rc != BB_OK) return rc;
@@ -1224,7 +1226,6 @@ static int paged_attention_impl(const char* what, const void* q, const int64_t* 
   if (const char* e = paged_schedule(B, T, H, Hkv, D, c.W, page, knew != nullptr, s)) return fail("%s: %s", what, e);
   const size_t need = s.bytes;
   if (need && (!ws || ws_bytes < need || !aligned(ws, 16))) return fail("workspace of %zu bytes required", need);
-  bb::PagedAttnParams p;
   memset(&p, 0, sizeof(p));
   p.c = c;
   p.r = r;
@@ -1249,7 +1250,7 @@ static int paged_attention_impl(const char* what, const void* q, const int64_t* 
   p.fit_quarters = s.fit_quarters;
   p.grid = s.grid; p.slots = (int)s.slots;
   p.scale = (float)((double)scale * 1.4426950408889634);
-  return hip_status(bb::launch_paged_attention(p, static_cast<hipStream_t>(stream)), what);
+  return BB_OK;
 }
 
 int bb_paged_attention(const void* q, const int64_t* sq, const void* k_pages, const int64_t* sk, const void* v_pages,
@@ -1260,11 +1261,15 @@ int bb_paged_attention(const void* q, const int64_t* sq, const void* k_pages, co
   bb::PagedCache c;
   bb::PagedRope r;
   memset(&r, 0, sizeof(r));
-  const int rc = paged_cache("paged_attention", const_cast<void*>(k_pages), sk, const_cast<void*>(v_pages), sv, table, st,
-                             lens, fresh, B, T, H, Hkv, D, pages, page, W, c);
+  const char* what = "paged_attention";
+  int rc = paged_cache(what, const_cast<void*>(k_pages), sk, const_cast<void*>(v_pages), sv, table, st, lens, fresh, B, T, H,
+                       Hkv, D, pages, page, W, c);
+  bb::PagedAttnParams p;
+  if (rc == BB_OK)
+    rc = paged_attention_params(what, q, sq, nullptr, nullptr, nullptr, nullptr, c, r, B, T, H, Hkv, D, page, is_f16, scale,
+                                out, so, ws, ws_bytes, p);
   if (rc != BB_OK) return rc;
-  return paged_attention_impl("paged_attention", q, sq, nullptr, nullptr, nullptr, nullptr, c, r, B, T, H, Hkv, D, page,
-                              is_f16, scale, out, so, ws, ws_bytes, stream);
+  return hip_status(bb::launch_paged_attention(p, static_cast<hipStream_t>(stream)), what);
 }
 
 int bb_paged_step(const void* q, const int64_t* sq, const void* k, const int64_t* skn, const void* v, const int64_t* svn,
@@ -1283,21 +1288,28 @@ int bb_paged_step(const void* q, const int64_t* sq, const void* k, const int64_t
   if (rc == BB_OK) rc = paged_rows(what, q, sq);
   if (rc != BB_OK) return rc;
   if (H < 1) return fail("%s: q [B,H,T,D] and the pages' Hkv heads must match", what);
-  if ((int64_t)T * (H / Hkv) <= kPagedStepVectors)  // the attention kernel rotates and stores the new rows itself
-    return paged_attention_impl(what, q, sq, k, skn, v, svn, c, r, B, T, H, Hkv, D, page, is_f16, scale, out, so, ws,
-                                ws_bytes, stream);
-  const size_t part = align256(bb_paged_attention_workspace(B, T, H, Hkv, D, page, W));
-  const size_t need = bb_paged_step_workspace(B, T, H, Hkv, D, page, W);
+  bb::PagedAttnParams p;
+  if ((int64_t)T * (H / Hkv) <= kPagedStepVectors) {  // the attention kernel rotates and stores the new rows itself
+    rc = paged_attention_params(what, q, sq, k, skn, v, svn, c, r, B, T, H, Hkv, D, page, is_f16, scale, out, so, ws, ws_bytes, p);
+    if (rc != BB_OK) return rc;
+    return hip_status(bb::launch_paged_attention(p, static_cast<hipStream_t>(stream)), what);
+  }
+  // (all that the attention refuses is refused before the rows are written)
+  PagedSchedule sch;
+  if (const char* e = paged_schedule(B, T, H, Hkv, D, W, page, false, sch)) return fail("%s: %s", what, e);
+  const size_t part = align256(sch.bytes), need = part + (size_t)B * T * H * D * 2;
   if (!ws || ws_bytes < need || !aligned(ws, 16)) return fail("workspace of %zu bytes required", need);
   void* turned = static_cast<char*>(ws) + part;
   const int64_t sqo[3] = {(int64_t)T * H * D, D, (int64_t)H * D};
-  if (!(scale > 0.0f)) return fail("scale must be positive");  // before the rows are written
+  bb::PagedRope none;
+  memset(&none, 0, sizeof(none));
+  rc = paged_attention_params(what, cos ? turned : q, cos ? sqo : sq, nullptr, nullptr, nullptr, nullptr, c, none, B, T, H, Hkv, D,
+                              page, is_f16, scale, out, so, ws, part, p);
+  if (rc != BB_OK) return rc;
   rc = bb_paged_append(k, skn, v, svn, cos ? q : nullptr, sq, turned, sqo, cos, sin, sc, rope_f32, k_pages, sk, v_pages, sv,
                        table, st, lens, fresh, B, T, cos ? H : 0, Hkv, D, pages, page, W, is_f16, stream);
   if (rc != BB_OK) return rc;
-  memset(&r, 0, sizeof(r));
-  return paged_attention_impl(what, cos ? turned : q, cos ? sqo : sq, nullptr, nullptr, nullptr, nullptr, c, r, B, T, H, Hkv,
-                              D, page, is_f16, scale, out, so, ws, part, stream);
+  return hip_status(bb::launch_paged_attention(p, static_cast<hipStream_t>(stream)), what);
 }
 
 int bb_stream_read(const void* buf, size_t bytes, uint32_t* sink, int workgroups, void* stream) {
