@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from bigger_bird_amd import _lib
-from test_kv_paged_cpu import P16, _cache, _consistent, _run, _s, _step
+from test_kv_paged_cpu import P16, _append, _cache, _consistent, _run, _s, _step
 
 P16_ODD = ctypes.c_void_p(24)
 
@@ -70,3 +70,9 @@ def test_no_workspace_for_a_call_that_is_refused():
     assert L.bb_paged_step_workspace(1, 64, 32, 8, 128, 64, 4) == 64 * 32 * 128 * 2
     for bad in [(1, 128, 1 << 15, 1, 128, 64, 4), (1, 64, 32, 8, 96, 64, 4), (1, 64, 30, 8, 128, 64, 4), (1, 64, 32, 8, 128, 64, 0)]:
         assert L.bb_paged_attention_workspace(*bad) == 0 and L.bb_paged_step_workspace(*bad) == 0
+
+
+@pytest.mark.parametrize("sizes", [dict(B=1 << 15, T=1 << 30, H=65534, Hkv=1), dict(B=65535, T=(1 << 31) - 1, H=(1 << 31) - 1, Hkv=1)])
+def test_more_rows_than_64_bits_count(sizes):
+    rc, err = _append(**sizes)
+    assert rc == -1 and "too many rows" in err, err

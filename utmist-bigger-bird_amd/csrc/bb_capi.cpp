@@ -1177,7 +1177,7 @@ int bb_paged_append(const void* k, const int64_t* skn, const void* v, const int6
   if (rc == BB_OK && H) rc = paged_rows(what, q_out, sqo);
   if (rc != BB_OK) return rc;
   if (H && !cos) return fail("%s: q is rotated: cos and sin required", what);
-  if ((int64_t)B * T * (H + 2 * Hkv) * (D / 16) > (1ll << 32) - 256) return fail("%s: too many rows", what);  // threads of a launch
+  if ((__int128)B * T * (H + 2ll * Hkv) * (D / 16) > (1ll << 32) - 256) return fail("%s: too many rows", what);  // threads of a launch
   p.k = static_cast<const uint16_t*>(k);
   p.v = static_cast<const uint16_t*>(v);
   p.sk0 = skn[0]; p.sk1 = skn[1]; p.sk2 = skn[2];
