@@ -407,8 +407,9 @@ int64_t bb_int4_decode_one_split(int vectors, int D);
  * NULL (all T): how many of the T token columns are real, clamped to 0 .. T. Token j of sequence b is row lens[b] - fresh[b]
  * + j. The lengths are read on the device, and every launch shape depends on the host arguments alone, so a captured graph
  * stays valid while the cache grows. W page <= 2^28; strides below 2^31 elements between pages and 2^30 in one; an append's
- * B T (H + 2 Hkv) D at most 2^36. The attention takes calls of fewer than 2^22 query vectors a KV head (T H / Hkv), and of 2^22
- * tiles of 256 of them over all heads. A row of a page that two tokens of a call are written to (one page in two sequences'
+ * B T (H + 2 Hkv) D at most 2^36. The attention takes calls of fewer than 2^22 query vectors a KV head (T H / Hkv) and of
+ * fewer than 2^22 tiles of them over all sequences and KV heads (of 256 vectors; of 32 where there are no more, in a step up
+ * to 128), whatever the width of the table. A row of a page that two tokens of a call are written to (one page in two sequences'
  * tables where both write) holds either; where a step writes a row that another sequence attends in the same call, or that the
  * table names at a second place, either value is attended there.
  *

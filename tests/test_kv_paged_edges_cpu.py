@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from bigger_bird_amd import _lib
-from test_kv_paged_cpu import P16, _append, _cache, _consistent, _run, _s, _step
+from test_kv_paged_cpu import P16, _append, _attention, _cache, _consistent, _run, _s, _step
 
 P16_ODD = ctypes.c_void_p(24)
 
@@ -76,3 +76,17 @@ def test_no_workspace_for_a_call_that_is_refused():
 def test_more_rows_than_64_bits_count(sizes):
     rc, err = _append(**sizes)
     assert rc == -1 and "too many rows" in err, err
+
+
+@pytest.mark.parametrize("sizes", [dict(B=64, T=4096, W=32768), dict(B=64, T=4096, W=1 << 22), dict(B=60000, T=1, W=1 << 22)])
+def test_a_wide_table_is_no_reason_to_refuse(sizes):
+    """How many sequences a call may have does not go by the rows that its table has room for."""
+    rc, err = _attention(**sizes)
+    assert rc == -1 and "workspace of" in err, err
+    rc, err = _step(**{**sizes, "scale": 0.0, "ws": P16, "ws_bytes": 1 << 50})
+    assert rc == -1 and "scale must be positive" in err, err
+    a = dict(B=64, T=1, H=32, Hkv=8, D=128, page=64, W=4) | sizes
+    L = _lib.lib()
+    assert 0 < L.bb_paged_attention_workspace(*a.values()) <= L.bb_paged_step_workspace(*a.values())
+    rc, err = _attention(**{**sizes, "B": 65535, "T": 1 << 13})  # but by its own tiles
+    assert rc == -1 and "out of range" in err, err

@@ -5,7 +5,7 @@ import torch
 
 import paged_plain as plain
 from bigger_bird_amd import paged_attention
-from test_kv_paged_gpu import BF16, FP16, STREAM_VECTORS, _attend_case, _check, _p_step, _say
+from test_kv_paged_gpu import BF16, FP16, STREAM_VECTORS, _attend_case, _check, _heads, _int, _p_step, _pages, _say
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +29,21 @@ def test_a_value_that_is_not_finite_wherever_it_lies(n, d, dtype, dev):
         if j:
             _check(got[:, :, :j], want[:, :, :j], tol[:, :, :j], dtype)
         assert not torch.isfinite(got[:, :, j:].float()).any()
+
+
+@pytest.mark.parametrize("B", [40, 70])  # up to 64 sequences each workgroup finds its work; more are laid out before
+@pytest.mark.parametrize("T", [1, 40])
+def test_tables_of_many_rows(B, T, dev):
+    """A table of 2^28 rows, the most there may be, over sequences of a few hundred that share their pages."""
+    _say("wide tables", B, T)
+    gen = torch.Generator(device=dev).manual_seed(B + T)
+    kp, vp = _pages(gen, 12, 8, 64, 64, BF16, dev)
+    one = torch.full((1, 1 << 22), -1, dtype=torch.int32, device=dev)
+    one[0, :12] = torch.randperm(12, generator=gen, device=dev).int()
+    lens = [(97 * i) % 700 for i in range(B)]
+    new = [min(T, n) for n in lens]
+    q = _heads(gen, B, 8, T, 64, BF16, dev)
+    table = one.expand(B, -1)
+    got = paged_attention(q, kp, vp, table, _int(lens, dev), 0.125, new=_int(new, dev))
+    want, tol = plain.attend(q, kp, vp, table[:, :12], lens, 0.125, new, _p_step(BF16, T <= STREAM_VECTORS))
+    _check(got, want, tol, BF16)

@@ -1094,9 +1094,10 @@ static const char* paged_schedule(int B, int T, int H, int Hkv, int D, int W, in
     s.fit_quarters = 5;
     s.target = kCUs;
   }
+  // The kernels divide numbers of 23 bits: query vectors, tiles and pairs, units of a table's rows (2^28 at most).
+  if (cap > 1ll << 28 || R >= 1ll << 22) return "lengths out of range";
   const int64_t tiles = cdiv(R, s.VT), pairs = tiles * B, units = cdiv(cap, s.unit);
-  if (cap > 1ll << 28 || pairs * Hkv * units >= 1ll << 30 || R >= 1ll << 22 || pairs * Hkv >= 1ll << 22)
-    return "lengths out of range";  // the kernels divide numbers of 23 bits
+  if (pairs * Hkv >= 1ll << 22) return "lengths out of range";
   s.tiles = (int)tiles;
   const int64_t most = cdiv(units, s.min_share);  // splits of a pair
   s.grid = (int)std::min<int64_t>(pairs * Hkv * most, s.target + pairs * Hkv);

@@ -236,8 +236,10 @@ struct Share {
     return n > 0 || u == 0 ? n : 1;
   }
 };
-BB_DEV Share share_of(const PagedAttnParams& p, int first, int total) {
-  const int least = (total * p.Hkv + (1 << p.target_log2) - 1) >> p.target_log2;
+constexpr int kMostUnits = 1 << 22;  // of a pair, and so of a share: 2^28 rows of 64
+BB_DEV Share share_of(const PagedAttnParams& p, int first, int64_t total) {
+  const int64_t even = (total * p.Hkv + (1 << p.target_log2) - 1) >> p.target_log2;
+  const int least = even < kMostUnits ? (int)even : kMostUnits;
   Share s{least > p.min_share ? least : p.min_share, false};
   if (p.fit_quarters > 0) {
     Share f{s.units, true};
@@ -330,10 +332,12 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedAttnParam
       }
     }
   };
-  int v[3] = {0, 0, 0}, all[3];
-  for (int pair = tid; pair < p.pairs; pair += kPlanThreads) v[0] += pair_units(p, pair);
+  // A thread's units are a number of 34 bits (2^12 pairs of 2^22), summed in two parts.
+  int64_t units = 0;
+  for (int pair = tid; pair < p.pairs; pair += kPlanThreads) units += pair_units(p, pair);
+  int v[3] = {(int)(units & 0xfffff), (int)(units >> 20), 0}, all[3];
   scan(v, all);
-  const Share share = share_of(p, 0, all[0]);
+  const Share share = share_of(p, 0, ((int64_t)all[1] << 20) + all[0]);
   int items = 0, slots = 0, zeros = 0;
   for (int at = 0; at < p.pairs; at += kPlanThreads) {
     const int pair = at + tid, u = pair_units(p, pair), sp = share.splits(u), mine = sp * p.Hkv;
