@@ -4,8 +4,9 @@ import pytest
 import torch
 
 import paged_plain as plain
-from bigger_bird_amd import paged_attention
-from test_kv_paged_gpu import BF16, FP16, STREAM_VECTORS, _attend_case, _check, _heads, _int, _p_step, _pages, _say
+from bigger_bird_amd import paged_attention, paged_step
+from paged_plain import HALF_STEP
+from test_kv_paged_gpu import BF16, FP16, FP32, STREAM_VECTORS, _attend_case, _check, _heads, _int, _p_step, _pages, _say, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,32 @@ def test_tables_of_many_rows(B, T, dev):
     got = paged_attention(q, kp, vp, table, _int(lens, dev), 0.125, new=_int(new, dev))
     want, tol = plain.attend(q, kp, vp, table[:, :12], lens, 0.125, new, _p_step(BF16, T <= STREAM_VECTORS))
     _check(got, want, tol, BF16)
+
+
+@pytest.mark.parametrize("T,H,hk", [(1, 8, 2), (8, 8, 2), (20, 8, 2)])  # one block of 16 vectors, 32 of them, three tiles of 32
+@pytest.mark.parametrize("d", [128, 64])
+@pytest.mark.parametrize("rot", [FP16, FP32])
+def test_rotated_queries_past_what_fp16_holds(T, H, hk, d, rot, dev):
+    """Pairs of 50000 turned by 45 degrees are 70711, and angles with a factor (as scaled RoPE has them) make them larger; a query
+    that is not finite is NaN still, beside them."""
+    _say("large queries", T, H, d, rot)
+    gen = torch.Generator(device=dev).manual_seed(T)
+    lens = [700, 65]
+    table, p = _table(gen, lens, 16, dev)
+    kp, vp = _pages(gen, p, hk, 16, d, FP16, dev)
+    q, k, v = (_heads(gen, 2, h, T, d, FP16, dev) for h in (H, hk, hk))
+    q[0, ::2] = q[0, ::2].sign() * 50000  # one sequence's every second head; the others are as they were
+    cos = torch.full((2, T, d), 0.70710678, device=dev).to(rot)
+    sin = cos.clone()
+    if rot == FP32:
+        cos[0], sin[0] = cos[0] * 300, sin[0] * 300
+        k[0] /= 300
+    q[1, 1, T - 1, 3] = float("nan")
+    got = paged_step(q, k, v, kp, vp, table, _int(lens, dev), 2.0 ** -24, cos=cos, sin=sin)
+    assert torch.isnan(got[1, 1, T - 1]).all()
+    got[1, 1, T - 1], q[1, 1, T - 1] = 0, 0
+    qr = plain.rotate(q, cos[:, None], sin[:, None])
+    assert (qr.abs().amax(-1)[0, ::2] > 65519).any()
+    want, tol = plain.attend(qr, kp, vp, table, lens, 2.0 ** -24, None, _p_step(FP16, True), HALF_STEP[FP16] ** 2 + 2.0 ** -20)
+    got[1, 1, T - 1] = want[1, 1, T - 1].half()
+    _check(got, want, tol, FP16)

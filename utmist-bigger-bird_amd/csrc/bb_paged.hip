@@ -614,36 +614,51 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnParams
     if constexpr (AWAY) st16(qs + 1024 * (QT * (NDS * r + ds) + i) + 16 * lane, w);
     else qf[r][ds][i] = as_bf16x8(w);
   };
+  float scale[NR];  // of the scores
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
+    scale[r] = p.scale;
+    if (NEW && p.r.cos) {
+      float t[NDS][8];
 #pragma unroll
-    for (int ds = 0; ds < NDS; ++ds) {
-      put_q(r, ds, 0, qw[r][ds]);
-      if constexpr (NEW) put_q(r, ds, 1, u32x4_t{0, 0, 0, 0});
-    }
-    if constexpr (NEW) {
-      if (p.r.cos) {
+      for (int ds = 0; ds < NDS / 2; ++ds) {
+        Turn turn;
+        load_turn<F16>(p.r, it.b * p.r.s0 + tok[r] * p.r.s1 + 32 * ds + 8 * a, D, turn);
+        rotate<F16>(qw[r][ds], qw[r][ds + NDS / 2], turn, t[ds], t[ds + NDS / 2]);
+      }
+      if constexpr (F16) {  // a rotated query may lie past what fp16 holds: a power of two goes over to its scores' scale
+        float top = 0.0f;
 #pragma unroll
-        for (int ds = 0; ds < NDS / 2; ++ds) {
-          Turn t;
-          float x0[8], x1[8];
-          u32x4_t w[4];
-          load_turn<F16>(p.r, it.b * p.r.s0 + tok[r] * p.r.s1 + 32 * ds + 8 * a, D, t);
-          rotate<F16>(qw[r][ds], qw[r][ds + NDS / 2], t, x0, x1);
+        for (int ds = 0; ds < NDS; ++ds)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const u32x2_t lo = two_terms<F16>(x0[2 * i], x0[2 * i + 1]), hi = two_terms<F16>(x1[2 * i], x1[2 * i + 1]);
-            w[0][i] = lo[0];
-            w[1][i] = lo[1];
-            w[2][i] = hi[0];
-            w[3][i] = hi[1];
-          }
+          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(t[ds][i]));
+        if (__builtin_amdgcn_ballot_w64(top > 65504.0f)) {
+          top = quarters_max(top);
+          const int e = top > 65504.0f && top < kInf ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
+          scale[r] = ldexpf(p.scale, e);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            put_q(r, ds, i, w[i]);
-            put_q(r, ds + NDS / 2, i, w[2 + i]);
-          }
+          for (int ds = 0; ds < NDS; ++ds)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[ds][i] = ldexpf(t[ds][i], -e);
         }
+      }
+#pragma unroll
+      for (int ds = 0; ds < NDS; ++ds) {
+        u32x4_t w[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const u32x2_t two = two_terms<F16>(t[ds][2 * i], t[ds][2 * i + 1]);
+          w[0][i] = two[0];
+          w[1][i] = two[1];
+        }
+        put_q(r, ds, 0, w[0]);
+        put_q(r, ds, 1, w[1]);
+      }
+    } else {
+#pragma unroll
+      for (int ds = 0; ds < NDS; ++ds) {
+        put_q(r, ds, 0, qw[r][ds]);
+        if constexpr (NEW) put_q(r, ds, 1, u32x4_t{0, 0, 0, 0});
       }
     }
   }
@@ -714,7 +729,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnParams
 #pragma unroll
       for (int kb = 0; kb < KC / 16; ++kb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[r][kb][i] *= p.scale;
+        for (int i = 0; i < 4; ++i) y[r][kb][i] *= F16 && NEW ? scale[r] : p.scale;
       if (whole) {
         seen[r] = true;
       } else {
