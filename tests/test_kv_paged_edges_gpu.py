@@ -77,3 +77,32 @@ def test_rotated_queries_past_what_fp16_holds(T, H, hk, d, rot, dev):
     want, tol = plain.attend(qr, kp, vp, table, lens, 2.0 ** -24, None, _p_step(FP16, True), HALF_STEP[FP16] ** 2 + 2.0 ** -20)
     got[1, 1, T - 1] = want[1, 1, T - 1].half()
     _check(got, want, tol, FP16)
+
+
+@pytest.mark.parametrize("T", [1, 40, 300])
+@pytest.mark.parametrize("size", [1.109375, 1.3359375])
+@pytest.mark.parametrize("dtype,exponents", [(BF16, (0, 20, 26, 28, 33, 60, 100)), (FP16, (0, 14, 22, 24, 26, 28))])
+def test_large_scores_of_any_mantissa(T, size, dtype, exponents, dev):
+    """Scores of 64 * size * 2^e and their negatives, whose product with scale log2(e) is not exact: all the same, so that the output
+    is the mean of the values, and falling by 64 * 2^(e - 5) a row, where the first row takes all for scores of 2^20 and more.
+
+    Tolerance: a probability is 2^x for all rows alike, its rounding as an operand of HALF_STEP in the numerator only; sums of 400
+    terms in fp32; the output's rounding."""
+    _say("large scores", T, size, dtype)
+    q, kp, vp, table, lens, _ = _attend_case([400], None, T, 4, 2, 64, 16, dtype, dev)
+    row = torch.arange(16, device=dev)
+    for e in exponents:
+        a, b = (2.0 ** (e // 2), 2.0 ** (e - e // 2)) if dtype == FP16 else (1.0, 2.0 ** e)
+        for sign in (1.0, -1.0):
+            qq = torch.full_like(q, sign * a)
+            kp[:] = size * b
+            want, _ = plain.attend(qq, kp, vp, table, [400], 1.0, None, 0.0)
+            mean, _ = plain.attend(qq, kp, vp.abs(), table, [400], 1.0, None, 0.0)
+            _check(paged_attention(qq, kp, vp, table, lens, 1.0), want, (HALF_STEP[dtype] + 400 * 2.0 ** -23) * mean, dtype)
+        if e < 20:
+            continue
+        # the first page's rows size, size - 1/32, .., the rest lower than all of them
+        kp[:] = b / 2
+        kp[table[0, 0].item()] = ((size - row / 32) * b).to(dtype)[:, None]
+        first = vp[table[0, 0].item(), :, 0].double()[None, :, None].repeat_interleave(2, 1).expand(1, 4, T, 64)
+        _check(paged_attention(torch.full_like(q, a), kp, vp, table, lens, 1.0), first, HALF_STEP[dtype] * first.abs(), dtype)

@@ -208,7 +208,6 @@ BB_DEV int token_of(const PagedAttnParams& p, int v) { return quotient(v, p.inv_
 // Pair `pair` is tile pair_tile of sequence pair % B: the sequences' last tiles, which are the longest, come first.
 BB_DEV int pair_tile(const PagedAttnParams& p, int pair) { return p.tiles == 1 ? 0 : p.tiles - 1 - quotient(pair, p.inv_B, p.B); }
 BB_DEV int pair_sequence(const PagedAttnParams& p, int pair, int tile) { return pair - (p.tiles - 1 - tile) * p.B; }
-BB_DEV int pair_index(const PagedAttnParams& p, int b, int tile) { return (p.tiles - 1 - tile) * p.B + b; }
 // Rows that the pair's last real token attends (0: none of its tokens is real, or has rows).
 BB_DEV int pair_keys(const PagedAttnParams& p, const Sequence& s, int tile) {
   const int j0 = token_of(p, tile * p.VT);
@@ -986,6 +985,7 @@ struct TileState {
   f32x4_t s[4][2];         // S^T of the current tile: keys 16 kb + 4 a + i
   bf16x8_t pk[2][2];       // P^T of the tile before: its 32-key halves
   float m[2], l[2];        // exponent's offset; this lane's share of the sum
+  float at[2];             // the offset that a tile is tried with: m, or -inf (see tile_softmax)
 };
 
 // Fragment i of a phase: i < D / 8 V's of (half st, block db), then K's of (32 dims ds, key block kb).
@@ -1032,18 +1032,26 @@ BB_DEV void tile_products(TileState<D>& t, const TileReads<D>& rd, uint32_t kt, 
 }
 
 // P = 2^(S c - m) in 16 bits; sum: this lane's part of the row sums. (One term: its rounding is as large as the output's own;
-// a second would cost half of the products again.)
-template <bool F16, int D>
-BB_DEV void tile_exp(TileState<D>& t, float c, float (&sum)[2]) {
+// a second would cost half of the products again.) ROUNDED: S c is rounded before m is taken off; the asm keeps the compiler from
+// fusing the two.
+template <bool F16, int D, bool ROUNDED>
+BB_DEV void tile_exp(TileState<D>& t, float c, const float (&m)[2], float (&sum)[2]) {
 #pragma unroll
   for (int rb = 0; rb < 2; ++rb) {
-    const float nm = -t.m[rb];
+    const float nm = -m[rb];
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = fast_exp2(fmaf(t.s[2 * st + e / 4][rb][e % 4], c, nm));
+        const float s = t.s[2 * st + e / 4][rb][e % 4];
+        if constexpr (ROUNDED) {
+          float x = s * c;
+          asm("" : "+v"(x));
+          p[e] = fast_exp2(x + nm);
+        } else {
+          p[e] = fast_exp2(fmaf(s, c, nm));
+        }
         sum[rb] = st == 0 && e == 0 ? p[e] : sum[rb] + p[e];
       }
       t.pk[st][rb] = as_bf16x8(u32x4_t{pack2<F16>(p[0], p[1]), pack2<F16>(p[2], p[3]), pack2<F16>(p[4], p[5]), pack2<F16>(p[6], p[7])});
@@ -1060,25 +1068,40 @@ BB_DEV float tile_max(const TileState<D>& t, int rb, float c) {
   return quarters_max(mx) * c;
 }
 template <int D>
-BB_DEV void tile_rescale(TileState<D>& t, int rb, float mt) {
-  const float mn = fmaxf(t.m[rb], mt), alpha = fast_exp2(t.m[rb] - mn);
-  t.m[rb] = mn;
+BB_DEV void tile_rescale(TileState<D>& t, int rb, float m) {
+  const float alpha = fast_exp2(t.m[rb] - m);
   t.l[rb] *= alpha;
 #pragma unroll
   for (int db = 0; db < D / 16; ++db)
 #pragma unroll
     for (int i = 0; i < 4; ++i) t.o[db][rb][i] *= alpha;
 }
-// Softmax of a tile: exponentiated against the offset as it is, and again where that was too low.
+// Softmax of a tile: exponentiated against the offset as it is, and again where that was too low. The exponent is the exact S c less
+// m, the largest S c rounded; from 2^24 on the two lie further apart than 2, and past 2^29 no probability is left between 0 and
+// infinity. So such a wave's S c are rounded too; and its tiles are tried with an offset of -inf, which is too low for all, so that
+// the others pay nothing for it (a branch on a flag in each tile cost 1 to 3 %).
 template <bool F16, int D>
 BB_DEV void tile_softmax(TileState<D>& t, float c) {
   float sum[2];
-  tile_exp<F16, D>(t, c, sum);
+  tile_exp<F16, D, false>(t, c, t.at, sum);
   const bool over0 = !(sum[0] <= kOver), over1 = !(sum[1] <= kOver);
-  if (__builtin_amdgcn_ballot_w64(over0 || over1)) {
-    tile_rescale<D>(t, 0, tile_max<D>(t, 0, c));
-    tile_rescale<D>(t, 1, tile_max<D>(t, 1, c));
-    tile_exp<F16, D>(t, c, sum);
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(over0 || over1) != 0, 0)) {
+    float m[2];
+    bool large = false;
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+      m[rb] = fmaxf(t.m[rb], tile_max<D>(t, rb, c));
+      tile_rescale<D>(t, rb, m[rb]);
+      large |= m[rb] > kLowest && fabsf(m[rb]) >= 16777216.0f;
+    }
+    large = __builtin_amdgcn_ballot_w64(large) != 0;
+    if (__builtin_expect(large, 0)) tile_exp<F16, D, true>(t, c, m, sum);
+    else tile_exp<F16, D, false>(t, c, m, sum);
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {  // (in place, so that nothing is copied where this branch is not taken)
+      asm("v_mov_b32 %0, %1" : "+v"(t.m[rb]) : "v"(m[rb]));
+      asm("v_mov_b32 %0, %1" : "+v"(t.at[rb]) : "v"(large ? -kInf : m[rb]));
+    }
   }
   t.l[0] += sum[0];
   t.l[1] += sum[1];
@@ -1235,7 +1258,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
   for (int rb = 0; rb < 2; ++rb) {
 #pragma unroll
     for (int db = 0; db < D / 16; ++db) t.o[db][rb] = f32x4_t{0, 0, 0, 0};
-    t.m[rb] = kLowest;
+    t.m[rb] = t.at[rb] = kLowest;
     t.l[rb] = 0.0f;
   }
   __builtin_amdgcn_s_waitcnt(0x0F70 | 2 * kRound);  // K of tile 0 has landed
