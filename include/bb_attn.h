@@ -429,7 +429,8 @@ int bb_paged_append(const void* k, const int64_t* skn, const void* v, const int6
  * Exact causal attention over the pages: out [B, H, T, D] (strides so[3]) from q [B, H, T, D] (strides sq[3]); token j
  * attends the rows up to its own, lens - fresh + j, of the pages that its table names; scores and softmax in fp32. Zeros
  * where it attends none, and for padding; NaN where its scores have no softmax (a query that is not finite). A row of V
- * that is not finite reaches only the tokens that attend it. H / Hkv query heads per KV head, any number.
+ * that is not finite reaches only the tokens that attend it: their column is +inf or -inf, or NaN where they attend both or a
+ * NaN. H / Hkv query heads per KV head, any number.
  * Workspace: bb_paged_attention_workspace (0: none, or a call that is refused).
  */
 int bb_paged_attention(const void* q, const int64_t* sq, const void* k_pages, const int64_t* sk, const void* v_pages,

@@ -6,7 +6,7 @@ import torch
 import paged_plain as plain
 from bigger_bird_amd import paged_attention, paged_step
 from paged_plain import HALF_STEP
-from test_kv_paged_gpu import BF16, FP16, FP32, STREAM_VECTORS, _attend_case, _check, _heads, _int, _p_step, _pages, _say, _table
+from test_kv_paged_gpu import BF16, FP16, FP32, STEP_VECTORS, STREAM_VECTORS, _attend_case, _check, _heads, _int, _p_step, _pages, _say, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +106,78 @@ def test_large_scores_of_any_mantissa(T, size, dtype, exponents, dev):
         kp[table[0, 0].item()] = ((size - row / 32) * b).to(dtype)[:, None]
         first = vp[table[0, 0].item(), :, 0].double()[None, :, None].repeat_interleave(2, 1).expand(1, 4, T, 64)
         _check(paged_attention(torch.full_like(q, a), kp, vp, table, lens, 1.0), first, HALF_STEP[dtype] * first.abs(), dtype)
+
+
+def _infinite_values(q, kp, vp, table, lens, T, page, dtype, gen):
+    """Infinities and NaN into some columns of V, at rows that tokens attend: +inf, -inf and NaN alone, +inf and -inf together and
+    two of a sign; a row early in the sequence, in the middle, among the last T, and one whose scores are far below the others'."""
+    inf, nan = float("inf"), float("nan")
+    at = lambda b, r: (table[b, r // page].item(), slice(None), r % page)
+    for b, n in enumerate(lens):
+        if not n:
+            continue
+        rows = [0, n // 3, n // 2, max(0, n - 2), n - 1]
+        kp[at(b, rows[1])] = -3 * q[b, ::q.shape[1] // kp.shape[1], 0]  # for the first head's first token: scores far below
+        for c, marks in enumerate(([(0, inf)], [(1, -inf)], [(2, nan)], [(3, inf), (0, -inf)], [(4, inf), (2, inf)], [(4, -inf)],
+                                   [(1, inf), (4, nan)], [(0, -inf), (3, -inf)])):
+            for r, x in marks:
+                page_, _, row = at(b, rows[r])
+                vp[page_, :, row, 7 * c + 1] = x
+
+
+def _attend_infinities(q, kp, vp, table, lens, scale, new, p_step):
+    """plain.attend of the finite values, and over it what attended infinities and NaN come to: a softmax's probabilities are all
+    positive, so +inf, -inf, or NaN where there are both or a NaN. (Looked up in V itself: torch's softmax in 64 bits on the GPU
+    gives 0 for e^-95, and 0 times an infinity is not what the formula says.)"""
+    finite = torch.where(torch.isfinite(vp), vp, 0)
+    want, tol = plain.attend(q, kp, finite, table, lens, scale, new, p_step)
+    B, H, T, d = q.shape
+    hk, page = vp.shape[1], vp.shape[2]
+    up, down = (torch.zeros(B, hk, T, d, dtype=torch.bool, device=q.device) for _ in "+-")
+    for b in range(B):
+        v, _ = plain.rows_of(vp, table, b, lens[b])
+        is_up, is_down = (torch.isnan(v) | (v == x) for x in (float("inf"), -float("inf")))
+        for j in range(T):
+            n = plain.seen(lens, new, T, table.shape[1] * page, b, j)
+            up[b, :, j], down[b, :, j] = is_up[:, :n].any(1), is_down[:, :n].any(1)
+    up, down = (x.repeat_interleave(H // hk, 1) for x in (up, down))
+    want[up], want[down], want[up & down] = float("inf"), -float("inf"), float("nan")
+    return want, tol
+
+
+def _check_with_infinities(got, want, tol, dtype):
+    assert torch.isinf(want).any() and torch.isnan(want).any()
+    whole = torch.isfinite(want)
+    for f in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert (f(got) == f(want)).all(), (f.__name__, (f(got) != f(want)).nonzero()[:5].tolist())
+    zero = torch.zeros_like(want)
+    _check(torch.where(whole, got, 0), torch.where(whole, want, zero), tol, dtype)
+
+
+@pytest.mark.parametrize("lens,T,H,hk", [([300, 47, 0], 1, 8, 2), ([300, 47, 9], 4, 8, 2), ([9001, 70], 1, 4, 1), ([700, 45], 8, 12, 3),
+                                         ([300, 90], 40, 8, 2), ([700], 300, 4, 4), ([5000], 70, 8, 2)])
+@pytest.mark.parametrize("d,dtype", [(128, BF16), (64, FP16), (64, BF16), (128, FP16)])
+def test_infinite_values_that_are_attended(lens, T, H, hk, d, dtype, dev):
+    """A column that attends +inf is +inf, with -inf too or NaN it is NaN, in every kernel and however small the probability; the
+    other columns are not touched. In the step the last rows come in as new ones."""
+    _say("infinite values", lens, T, H, hk, d, dtype)
+    gen = torch.Generator(device=dev).manual_seed(T)
+    new = [min(T, n) for n in lens]
+    q, kp, vp, table, ln, nw = _attend_case(lens, new, T, H, hk, d, 16, dtype, dev)
+    _infinite_values(q, kp, vp, table, lens, T, 16, dtype, gen)
+    scale = 2 * d ** -0.5
+    for step in (False, True):
+        streams = T * H // hk <= (STEP_VECTORS if step else STREAM_VECTORS)
+        want, tol = _attend_infinities(q, kp, vp, table, lens, scale, new, _p_step(dtype, streams))
+        if step:
+            k, v = (torch.zeros(len(lens), hk, T, d, dtype=dtype, device=dev) for _ in "kv")
+            for b, n in enumerate(lens):
+                for j in range(new[b]):
+                    r = n - new[b] + j
+                    page, row = table[b, r // 16].item(), r % 16
+                    k[b, :, j], v[b, :, j] = kp[page, :, row], vp[page, :, row]
+                    kp[page, :, row], vp[page, :, row] = 0, float("nan")
+            got = paged_step(q, k, v, kp, vp, table, ln, scale, new=nw)
+        else:
+            got = paged_attention(q, kp, vp, table, ln, scale, new=nw)
+        _check_with_infinities(got, want, tol, dtype)

@@ -189,7 +189,8 @@ def paged_attention(q, k_pages, v_pages, table, lens, scale, new=None):
     """Exact causal attention of q [B, H, T, d] over the pages: token j of a sequence attends the rows up to its own,
     lens - new + j. One token a sequence, a few drafted ones or a chunk of a prompt; sequences of unlike lengths. Returns
     [B, H, T, d] in [B, T, H, d] memory; zeros for padding and where a token attends no row, NaN for a query that is not
-    finite."""
+    finite. A value of V that is not finite reaches the tokens that attend it alone: +inf, -inf, or NaN where both or a NaN are
+    attended."""
     what = "paged_attention"
     device, copy, out_strides, sq, skp, svp, st, sizes, so, ws_bytes = _attention_plan(
         *_layouts(q, k_pages, v_pages, table, lens, new))

@@ -554,7 +554,43 @@ BB_DEV uint32_t not_finite(uint32_t w) {  // 0xffff in the halves that are not
   constexpr uint32_t e = F16 ? 0x7c00u : 0x7f80u;
   return ((w & e) == e ? 0xffffu : 0u) | ((w >> 16 & e) == e ? 0xffff0000u : 0u);
 }
-
+// What a column comes to whose values are not all finite goes by the values alone: +inf, -inf, or NaN where both or NaN are
+// attended, however small their probabilities (which may be 0 as operands, and then make NaN of an infinity). So a sum that is not
+// finite is looked up at its end: `pos` and `neg` are the first of the rows [begin, end) on a page whose value at d + k is +inf or
+// NaN, -inf or NaN. (begin: a multiple of 4.)
+constexpr int kNoRow = 0x7fffffff;
+template <bool F16, int N>
+BB_DEV void first_not_finite(const PagedCache& c, int b, const uint16_t* vh, int begin, int end, int d, int (&pos)[N], int (&neg)[N]) {
+  constexpr uint32_t inf = F16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+  for (int k = 0; k < N; ++k) pos[k] = neg[k] = kNoRow;
+#pragma unroll 1
+  for (int r = begin; r < end; r += 4) {
+    const int page = page_of(c, b, r);
+    if (page < 0) continue;
+    const uint16_t* v = vh + page * c.svp + (r & ((1 << c.page_log2) - 1)) * c.svr + d;
+    uint16_t h[4][N];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k) h[i][k] = v[(r + i < end ? i : 0) * c.svr + k];
+#pragma unroll
+    for (int i = 3; i >= 0; --i)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const uint32_t size = h[i][k] & 0x7fffu;
+        const int row = size < inf ? kNoRow : r + i < end ? r + i : r;
+        pos[k] = row < pos[k] && h[i][k] != (inf | 0x8000u) ? row : pos[k];
+        neg[k] = row < neg[k] && h[i][k] != inf ? row : neg[k];
+      }
+  }
+}
+// `o` where the first `seen` rows are attended.
+BB_DEV float with_infinities(float o, int pos, int neg, int seen) {
+  if (pos < seen) o = neg < seen ? __builtin_nanf("") : kInf;
+  else if (neg < seen) o = -kInf;
+  return o;
+}
 template <int D, bool F16, int NR, bool NEW, int AUX>
 __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnParams p) {
   using Stream = PageStream<D, AUX>;
@@ -861,6 +897,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnParams
 #pragma unroll
         for (int k = 0; k < 4; ++k) O[k] = fmaf(wt, t[k], O[k]);
       }
+      if (!(fabsf(O[0]) + fabsf(O[1]) + fabsf(O[2]) + fabsf(O[3]) < kInf) && L > 0.0f && L < kInf) {
+        int pos[4], neg[4];
+        first_not_finite<F16>(p.c, it.b, p.c.v + it.g * p.c.svh, begin, end, d, pos, neg);
+        const int attended = s.seen(token_of(p, v0 + vv));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) O[k] = with_infinities(O[k], pos[k], neg[k], attended);
+      }
       if (it.splits == 1) {
         store_output<F16>(p, it.b, it.g, v0 + vv, d, O, M, L);
       } else {
@@ -1112,6 +1155,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
   using L = TileLds<D>;
   constexpr int STAGE = 2 * L::BYTES, NV = D / 8, NF = D / 4, ROW = D + 4;
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kTileStages * STAGE];
+  __shared__ int first[2][D];       // see first_not_finite
   __shared__ int odd[kTileStages];  // whether V's tile there may hold values that are not finite (never taken back)
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 15, a = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), late = wave >> 2;  // waves w and w + 4 share a SIMD
@@ -1316,10 +1360,40 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedAtt
   if (live) values(n_tiles - 1);
   if (!late) ring_barrier();  // the groups meet again
   __builtin_amdgcn_s_waitcnt(0x0F70);  // nothing lands in LDS any more
+  bool bad[2];  // sums that are not finite
+#pragma unroll
+  for (int rb = 0; rb < 2; ++rb) {
+    t.l[rb] = quarters_sum(t.l[rb]);
+    f32x4_t size = {0, 0, 0, 0};
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) size[e] += fabsf(t.o[db][rb][e]);
+    bad[rb] = lim[rb] > 0 && t.l[rb] > 0.0f && t.l[rb] < kInf && !(size[0] + size[1] + size[2] + size[3] < kInf);
+  }
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad[0] || bad[1]) != 0, 0)) {
+    constexpr int N = D / 64;
+    int pos[N], neg[N];
+    first_not_finite<F16>(p.c, it.b, in.vh, begin, end, N * lane, pos, neg);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {  // (the same from every wave that comes here)
+      first[0][N * lane + k] = pos[k];
+      first[1][N * lane + k] = neg[k];
+    }
+    publish();
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb)
+      if (bad[rb])
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            t.o[db][rb][e] = with_infinities(t.o[db][rb][e], first[0][16 * db + 4 * a + e], first[1][16 * db + 4 * a + e], lim[rb]);
+  }
 #pragma unroll
   for (int rb = 0; rb < 2; ++rb) {
     const int i = 32 * wave + 16 * rb + x;
-    const float l = quarters_sum(t.l[rb]);
+    const float l = t.l[rb];
     const bool seen = lim[rb] > 0 && (open > 0 || top[rb] >= 0);
     const float inv = 1.0f / l;  // (another rounding of 2^-24, instead of 64 divisions a lane)
     if (i >= R) continue;
@@ -1401,9 +1475,22 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttnParams p
       }
     }
   };
+  // Infinities are attended values (see first_not_finite), which a weight of 0 does not make NaN.
+  auto look_up = [&](int v) {
+    if (fabsf(O[0]) + fabsf(O[1]) + fabsf(O[2]) + fabsf(O[3]) < kInf || !(L > 0.0f && L < kInf)) return;
+    f32x4_t sum = {0, 0, 0, 0};
+    for (int i = 0; i < splits; ++i) {
+      const f32x4_t o = *reinterpret_cast<const f32x4_t*>(slots + ((int64_t)i * p.VT + v) * ROW + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] += fabsf(o[j]) < kInf ? 0.0f : o[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) O[j] = sum[j] == 0.0f ? O[j] : sum[j];
+  };
   if (to - from > 1) {
     for (int v = from + grp; v < to; v += NG) {
       merge(v, 0, 1);
+      look_up(v);
       store_output<F16>(p, b, g, tile * p.VT + v, d, O, M, L);
     }
     return;
@@ -1430,6 +1517,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttnParams p
 #pragma unroll
     for (int k = 0; k < 4; ++k) O[k] = fmaf(wt, st[i][d + k], O[k]);
   }
+  look_up(from);
   store_output<F16>(p, b, g, tile * p.VT + from, d, O, M, L);
 }
 
