@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from bigger_bird_amd import _lib
+from bigger_bird_amd.kv_paged import _append_plan, _attention_plan, _step_plan
 from test_kv_paged_cpu import P16, _append, _attention, _cache, _consistent, _run, _s, _step
 
 P16_ODD = ctypes.c_void_p(24)
@@ -90,3 +91,23 @@ def test_a_wide_table_is_no_reason_to_refuse(sizes):
     assert 0 < L.bb_paged_attention_workspace(*a.values()) <= L.bb_paged_step_workspace(*a.values())
     rc, err = _attention(**{**sizes, "B": 65535, "T": 1 << 13})  # but by its own tiles
     assert rc == -1 and "out of range" in err, err
+
+
+# ---------------------------------------------------------------- the Python calls' checks
+def _layout(*shape, stride=None, dtype=torch.bfloat16):
+    """What the plans go by, of a tensor that could lie on the first GPU."""
+    x = torch.empty_strided(shape, stride, dtype=dtype, device="meta") if stride else torch.empty(shape, dtype=dtype, device="meta")
+    return x.shape, x.stride(), x.dtype, 0
+
+
+@pytest.mark.parametrize("d,wide", [(100, 104), (96, 96), (32, 32), (256, 256), (65, 72)])
+def test_other_head_dims_are_refused_by_the_plans(d, wide):
+    """Rows of 100 elements in pages padded to 104 cannot be copied to aligned rows: they are refused before that is tried."""
+    pages = _layout(3, 2, 16, d, stride=(2 * 16 * wide, 16 * wide, wide, 1))
+    table, lens = _layout(1, 2, dtype=torch.int32), _layout(1, dtype=torch.int32)
+    q, k = _layout(1, 4, 1, d), _layout(1, 2, 1, d)
+    for call in (lambda: _attention_plan(q, pages, pages, table, lens, None),
+                 lambda: _append_plan(k, k, pages, pages, table, lens, None, None, None, None),
+                 lambda: _step_plan(q, k, k, pages, pages, table, lens, None, None, None)):
+        with pytest.raises(ValueError, match=f"head_dim {d} unsupported"):
+            call()

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import paged_plain as plain
-from bigger_bird_amd import paged_attention, paged_step
+from bigger_bird_amd import paged_append, paged_attention, paged_step
 from paged_plain import HALF_STEP
 from test_kv_paged_gpu import BF16, FP16, FP32, STEP_VECTORS, STREAM_VECTORS, _attend_case, _check, _heads, _int, _p_step, _pages, _say, _table
 
@@ -181,3 +181,14 @@ def test_infinite_values_that_are_attended(lens, T, H, hk, d, dtype, dev):
         else:
             got = paged_attention(q, kp, vp, table, ln, scale, new=nw)
         _check_with_infinities(got, want, tol, dtype)
+
+
+def test_rows_without_an_aligned_copy_are_refused(dev):
+    _say("head_dim 100")
+    pages = torch.zeros(3, 2, 16, 104, dtype=BF16, device=dev)[..., :100]
+    table, lens = _int([[0, 1]], dev), _int([20], dev)
+    q, k = torch.zeros(1, 4, 1, 100, dtype=BF16, device=dev), torch.zeros(1, 2, 1, 100, dtype=BF16, device=dev)
+    for call in (lambda: paged_attention(q, pages, pages, table, lens, 1.0), lambda: paged_append(k, k, pages, pages, table, lens),
+                 lambda: paged_step(q, k, k, pages, pages, table, lens, 1.0)):
+        with pytest.raises(ValueError, match="head_dim 100 unsupported"):
+            call()

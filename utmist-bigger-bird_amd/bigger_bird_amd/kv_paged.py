@@ -72,6 +72,8 @@ def _check_cache(what, rows, kp, vp, table, lens, new):
         raise ValueError(f"{what}: bf16 or fp16 rows and pages of one dtype required")
     if len(ps) != 4 or ps != vs or ps[3] != d or not ps[0] or not ps[1]:
         raise ValueError(f"{what}: k_pages and v_pages must be [pages, Hkv, page, d] with the rows' d")
+    if d not in (64, 128):  # (here, as rows of others have no aligned copy that the library could refuse)
+        raise ValueError(f"{what}: head_dim {d} unsupported (64 or 128)")
     if table[2] != torch.int32 or lens[2] != torch.int32 or (new is not None and new[2] != torch.int32):
         raise ValueError(f"{what}: table, lens and new must be int32")
     if len(table[0]) != 2 or table[0][0] != b or lens[0] != (b,) or (new is not None and new[0] != (b,)):
