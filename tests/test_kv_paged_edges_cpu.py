@@ -111,3 +111,64 @@ def test_other_head_dims_are_refused_by_the_plans(d, wide):
                  lambda: _step_plan(q, k, k, pages, pages, table, lens, None, None, None)):
         with pytest.raises(ValueError, match=f"head_dim {d} unsupported"):
             call()
+
+
+# ---------------------------------------------------------------- masks
+def _masks(t):
+    causal = torch.ones(1, 1, t, t, dtype=torch.bool).tril()
+    bias = torch.where(causal, 0.0, torch.finfo(torch.float32).min)
+    left, right, packed = causal.clone(), causal.clone(), causal.clone()
+    left[..., :2] = False
+    right[..., t - 1] = False
+    packed[..., t // 2:, :t // 2] = False
+    padded = torch.ones(1, t, dtype=torch.long)
+    padded[0, 0] = 0
+    plain = [causal, bias, bias.to(torch.bfloat16), torch.ones(1, t, dtype=torch.long), torch.ones(1, t, dtype=torch.bool)]
+    hiding = [left, right, packed, torch.where(left, 0.0, -float("inf")), torch.where(right, 0.0, torch.finfo(torch.float32).min),
+              padded, padded.bool(), object()]
+    return plain, hiding
+
+
+def test_a_mask_that_hides_rows_of_one_sequence_is_refused():
+    """A mask is not read by the attention. One sequence takes the causal mask that some attention implementations always make, and
+    is refused one that hides any of its rows from its last token; a step that extend began goes by its counts."""
+    plain_masks, hiding = _masks(6)
+    for mask in plain_masks:
+        c = _cache(batch=1)
+        for layer in c.layers:
+            layer.begin(6, mask, 1)
+        assert c.lengths == [6] and not c._left
+    for mask in (*hiding, True):
+        c = _cache(batch=1)
+        with pytest.raises(ValueError, match="by a mask"):
+            c.layers[0].begin(6, mask, 1)
+        assert c.lengths == [0] and not c._left
+        c.extend([4])
+        for layer in c.layers:
+            layer.begin(6, mask, 1)
+        assert c.lengths == [4]
+    c = _cache(batch=2)  # several sequences: any mask, as before
+    for mask in (*plain_masks, *hiding):
+        with pytest.raises(ValueError, match="by a mask"):
+            c.layers[0].begin(6, mask, 1)
+
+
+def test_rdattention_hands_the_mask_on():
+    from types import SimpleNamespace
+
+    from bigger_bird_amd import RDAttention
+
+    lin, kv = torch.nn.Linear(256, 256, bias=False), torch.nn.Linear(256, 128, bias=False)
+    base = SimpleNamespace(config=SimpleNamespace(num_attention_heads=4, num_key_value_heads=2), layer_idx=0, head_dim=64,
+                           scaling=0.125, q_proj=lin, k_proj=kv, v_proj=kv, o_proj=lin)
+    pe = torch.ones(1, 6, 64), torch.zeros(1, 6, 64)
+    plain_masks, hiding = _masks(6)
+    with torch.no_grad():
+        for mask in hiding:
+            c = _cache(batch=1)
+            with pytest.raises(ValueError, match="by a mask"):
+                RDAttention(base)(torch.zeros(1, 6, 256), pe, mask, c)
+            assert c.lengths == [0]
+        for mask in plain_masks:  # taken, up to the rows' dtype (fp32 here), which the step refuses on any device
+            with pytest.raises(ValueError, match="ROCm device only"):
+                RDAttention(base)(torch.zeros(1, 6, 256), pe, mask, _cache(batch=1))

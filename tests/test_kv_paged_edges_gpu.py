@@ -6,7 +6,7 @@ import torch
 import paged_plain as plain
 from bigger_bird_amd import paged_append, paged_attention, paged_step
 from paged_plain import HALF_STEP
-from test_kv_paged_gpu import BF16, FP16, FP32, STEP_VECTORS, STREAM_VECTORS, _attend_case, _check, _heads, _int, _p_step, _pages, _say, _table
+from test_kv_paged_gpu import BF16, FP16, FP32, STEP_VECTORS, STREAM_VECTORS, _attend_case, _check, _heads, _int, _model, _p_step, _pages, _say, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -192,3 +192,32 @@ def test_rows_without_an_aligned_copy_are_refused(dev):
                  lambda: paged_step(q, k, k, pages, pages, table, lens, 1.0)):
         with pytest.raises(ValueError, match="head_dim 100 unsupported"):
             call()
+
+
+def test_model_masks_of_one_sequence(dev):
+    """With eager attention a model always makes a causal mask: one sequence runs, prompt, chunk and token, as without one; a padded
+    prompt is refused, and run by its count after extend."""
+    _say("masks of one sequence")
+    from bigger_bird_amd import make_paged_cache
+
+    model = _model(dev, "dense_rd")
+    ids = torch.randint(0, 512, (1, 60), generator=torch.Generator().manual_seed(3)).to(dev)
+    mask = torch.ones(1, 40, dtype=torch.long, device=dev)
+    outs = []
+    with torch.no_grad():
+        for kind in ("sdpa", "eager"):
+            model.config._attn_implementation = kind
+            cache = make_paged_cache(model.config, 1, 20, page=16, device=dev)
+            outs.append([model(input_ids=ids[:, a:b], past_key_values=cache, use_cache=True).logits for a, b in ((0, 40), (40, 59), (59, 60))])
+            assert cache.lengths == [60]
+            for side in (slice(0, 3), slice(37, 40)):
+                cache, padded = make_paged_cache(model.config, 1, 20, page=16, device=dev), mask.clone()
+                padded[:, side] = 0
+                with pytest.raises(ValueError, match="not by a mask"):
+                    model(input_ids=ids[:, :40], attention_mask=padded, past_key_values=cache, use_cache=True)
+                assert cache.lengths == [0]
+            cache.extend([37])
+            got = model(input_ids=ids[:, :40], attention_mask=padded, past_key_values=cache, use_cache=True).logits
+            assert cache.lengths == [37] and torch.equal(got[:, :37], outs[0][0][:, :37])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)

@@ -196,7 +196,7 @@ class RDAttention(nn.Module):
         cos, sin = position_embeddings
         if b != len(layer.cache.lengths):
             raise ValueError(f"the paged cache holds {len(layer.cache.lengths)} sequences, the input has {b}")
-        new = layer.begin(t, attention_mask is not None, cos.shape[0] if cos.ndim == 3 else 1)
+        new = layer.begin(t, attention_mask, cos.shape[0] if cos.ndim == 3 else 1)
         lengths = layer.cache.lengths
         prompts = all(n == s for n, s in zip(lengths, new) if s)  # every sequence with new tokens starts here
         if self.dense or not prompts or max(new) <= self.sink + self.window:

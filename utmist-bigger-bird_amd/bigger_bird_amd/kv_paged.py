@@ -250,6 +250,17 @@ def paged_step(q, k, v, k_pages, v_pages, table, lens, scale, cos=None, sin=None
     return out
 
 
+def _hides_rows(mask):
+    """Whether a mask (None or False: none; True: one that does) hides any row from the last token, as padding on either side and
+    packed sequences do and the causal mask does not. Looks at the mask's values: the host waits for them."""
+    if mask is None or isinstance(mask, bool):
+        return bool(mask)
+    if not torch.is_tensor(mask) or mask.ndim < 2:
+        return True
+    last = mask[..., -1, :] if mask.ndim > 2 else mask
+    return bool((last < 0).any() if last.dtype.is_floating_point else (last == 0).any())
+
+
 class PagedKVLayer(DynamicLayer):
     """One layer's pages of a PagedCache. RDAttention attends them (`attend`, `append`); other consumers are refused, as there are
     no contiguous keys and values to hand out."""
@@ -262,8 +273,8 @@ class PagedKVLayer(DynamicLayer):
 
     def begin(self, t, padded, positions):
         """The current step's new tokens per sequence, for this layer: `t` columns (begun here, with every column real, unless
-        PagedCache.extend did). `padded`: whether the model was given a mask; `positions`: how many sequences' angles it was
-        given."""
+        PagedCache.extend did). `padded`: the mask that the model was given, if any (True: one that hides rows); `positions`: how
+        many sequences' angles it was given."""
         return self.cache._begin(self.index, t, padded, positions)
 
     def append(self, k, v):
@@ -359,7 +370,7 @@ class PagedCache(DynamicCache):
         step, before = (self._step, self._before()) if begun else ([t] * len(self.lengths), self.lengths)
         if max(step) > t:
             raise ValueError(f"PagedCache: the step has {max(step)} new tokens, the input {t} columns")
-        if len(step) > 1 and padded and not (begun and self._declared):
+        if not begun and (len(step) > 1 and padded is not None and padded is not False or _hides_rows(padded)):
             raise ValueError("PagedCache: padding goes by extend(new tokens of each sequence) and to the right, not by a mask")
         if positions == 1 and any(s and n != max(before) for n, s in zip(before, step)):
             raise ValueError("PagedCache: sequences of unlike lengths need position_ids (positions)")
