@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.nn.attention.flex_attention import create_block_mask
 
 from bigger_bird_amd import _lib
 from bigger_bird_amd.kv_paged import _append_plan, _attention_plan, _step_plan
@@ -123,8 +124,10 @@ def _masks(t):
     packed[..., t // 2:, :t // 2] = False
     padded = torch.ones(1, t, dtype=torch.long)
     padded[0, 0] = 0
-    plain = [causal, bias, bias.to(torch.bfloat16), torch.ones(1, t, dtype=torch.long), torch.ones(1, t, dtype=torch.bool)]
-    hiding = [left, right, packed, torch.where(left, 0.0, -float("inf")), torch.where(right, 0.0, torch.finfo(torch.float32).min),
+    blocks = [create_block_mask(f, 1, None, t, t, device="cpu") for f in
+              (lambda b, h, i, j: j <= i, lambda b, h, i, j: (j <= i) & (padded[b, j] != 0))]
+    plain = [blocks[0], torch.ones(1, 1, 0, 0, dtype=torch.bool), causal, bias, bias.to(torch.bfloat16), torch.ones(1, t, dtype=torch.long), torch.ones(1, t, dtype=torch.bool)]
+    hiding = [blocks[1], left, right, packed, torch.where(left, 0.0, -float("inf")), torch.where(right, 0.0, torch.finfo(torch.float32).min),
               padded, padded.bool(), object()]
     return plain, hiding
 

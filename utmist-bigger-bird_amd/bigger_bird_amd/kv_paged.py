@@ -255,8 +255,14 @@ def _hides_rows(mask):
     packed sequences do and the causal mask does not. Looks at the mask's values: the host waits for them."""
     if mask is None or isinstance(mask, bool):
         return bool(mask)
+    if hasattr(mask, "mask_mod"):  # a flex attention's BlockMask: a function of (batch, head, query, key)
+        device = mask.kv_num_blocks.device
+        t, zero = mask.seq_lengths[0], torch.zeros((), dtype=torch.int64, device=device)
+        return not bool(mask.mask_mod(zero, zero, zero + t - 1, torch.arange(t, device=device)).all())
     if not torch.is_tensor(mask) or mask.ndim < 2:
         return True
+    if mask.numel() == 0:
+        return False
     last = mask[..., -1, :] if mask.ndim > 2 else mask
     return bool((last < 0).any() if last.dtype.is_floating_point else (last == 0).any())
 
