@@ -221,3 +221,29 @@ def test_model_masks_of_one_sequence(dev):
             assert cache.lengths == [37] and torch.equal(got[:, :37], outs[0][0][:, :37])
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("layout", ["heads", "rows", "pool", "padded"])
+@pytest.mark.parametrize("T,H,hk", [(1, 8, 2), (6, 8, 2), (90, 8, 2)])
+@pytest.mark.parametrize("d,dtype,page", [(128, BF16, 16), (64, FP16, 64)])
+def test_infinite_values_in_any_layout_beside_unnamed_pages(layout, T, H, hk, d, dtype, page, dev):
+    """The rows that infinities are looked up in are those of the table's pages, with the pages' strides, up to each token's own."""
+    _say("infinite values", layout, T, d, dtype, page)
+    gen = torch.Generator(device=dev).manual_seed(T + page)
+    lens, T_new = [1500, 200], [T, max(1, T // 2)]
+    q, kp, vp, table, ln, nw = _attend_case(lens, T_new, T, H, hk, d, page, dtype, dev, layout)
+    own = torch.zeros(kp.shape[0], page, dtype=torch.bool, device=dev)
+    for b, n in enumerate(lens):
+        for r in range(n):
+            own[table[b, r // page].item(), r % page] = True
+    vp.masked_fill_(~own[:, None, :, None], float("-inf"))  # what no sequence holds
+    table[0, 3], table[1, 1] = -1, 2 ** 30
+    for b, n in enumerate(lens):
+        for c, (r, x) in enumerate(((0, float("inf")), (n // 2, float("-inf")), (n - 1, float("inf")), (n - 1, float("nan")),
+                                    (3 * page + 1 if b == 0 else page + 1, float("inf")))):  # the last on a page that is not named
+            e = int(table[b, r // page])
+            if 0 <= e < vp.shape[0]:
+                vp[e, :, r % page, 9 * c + 2] = x
+    want, tol = _attend_infinities(q, kp, vp, table, lens, d ** -0.5, T_new, _p_step(dtype, T * H // hk <= STREAM_VECTORS))
+    got = paged_attention(q, kp, vp, table, ln, d ** -0.5, new=nw)
+    _check_with_infinities(got, want, tol, dtype)
