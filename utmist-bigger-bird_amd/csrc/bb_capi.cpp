@@ -1065,20 +1065,23 @@ struct PagedSchedule {
   size_t part, bytes;   // of the partials with what each slot holds and how many are used; of the workspace: these, then the items
 };
 // Query vectors of a KV head up to which the streaming kernel takes a call. (us streaming and in tiles of 64 rows, 8 KV heads,
-// head_dim 128: 16 vectors 12.3 and 18.3 at 4096 rows, 35 and 42 at 8 x 8192, 30 and 30 at 32768; 32: 15.4 and 19, 39 and 43, 33 and
-// 31; 64, which read the cache twice where they stream: 17 and 20, 53 and 44, 50 and 33.)
+// head_dim 128: 16 vectors 12.1 and 15.1 at 4096 rows, 35 and 42 at 8 sequences of up to 8192, 30 and 33 at 32768; 32: 15.1 and 15.5,
+// 39 and 43, 33 and 34; 64, which read the cache twice where they stream: 17 and 17, 53 and 45, 50 and 35.)
 constexpr int kPagedStreamVectors = 32;
 // And up to which it takes a step by itself, rotating q and storing the new rows; more go through the append, and their rotated q
-// is rounded. (By itself and in two, the same sizes: 16 vectors 16.5 and 18.7, 38 and 40, 33 and 33 us; 32: 21 and 20, 45 and 44, 39
-// and 36; 64: 24 and 22, 53 and 48, 53 and 37; 128: 32 and 26, 69 and 54, 60 and 42. The outputs' error against 64 bits is 0.0017 of
-// them by itself, which is their own rounding, and 0.0029 to 0.0032 in two. Of up to 128 vectors, where single tokens and drafts
-// of a few end, the error decides.)
+// is rounded. (By itself and in two, the same sizes: 16 vectors 15.8 and 16.6, 38 and 38.5, 33 and 33 us; 32: 21 and 18, 45 and 43,
+// 39 and 36; 64: 24 and 20, 55 and 48, 54 and 39; 128: 31 and 24, 70 and 52, 62 and 42. The outputs' error against 64 bits is 0.0017
+// of them by itself, which is their own rounding, and 0.0029 to 0.0032 in two. Of up to 128 vectors, where single tokens and drafts
+// of a few end, the error decides; the time would decide for two from 32 on.)
 constexpr int kPagedStepVectors = 128;
 static const char* paged_schedule(int B, int T, int H, int Hkv, int D, int W, int page, bool with_new, PagedSchedule& s) {
   const int64_t R = (int64_t)T * (H / Hkv), cap = (int64_t)W * page;
   if (R <= kPagedStreamVectors || (with_new && R <= kPagedStepVectors)) {
     // Two workgroups run on a CU (aiming at half as many, 32 x 8192 rows 114 us instead of 106; at twice, 131072 rows 91 for 87).
     // A split of one chunk a wave is no faster than of two (4099 rows 15.4 and 15.5 us, four 18.2).
+    // The fitted share has no bound here, which suits sequences of comparable lengths. Where they are not, and their number times the
+    // KV heads comes near the 512 workgroups, the longest is left to few: one of 131072 rows beside 63 of 512 takes 1140 us (8 KV
+    // heads; beside 64, where the share is rounded, 133, and beside 47, 111).
     s.VT = R <= 16 ? 16 : 32;
     s.unit = 4 * 4096 / D;
     s.min_share = 2;

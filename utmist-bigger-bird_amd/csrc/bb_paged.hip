@@ -221,9 +221,9 @@ BB_DEV int pair_units(const PagedAttnParams& p, int pair) {
   return (k + (1 << p.unit_log2) - 1) >> p.unit_log2;
 }
 // The share of a split, and the splits of a pair. Where the pairs fit a wave and the workgroups that run at once (p.fit_quarters
-// > 0) and it wastes little (F / least <= p.fit_quarters / 4), the share is the F for which the call's splits are just no more
-// than run at once, and the rest of a pair is a split too; otherwise a pair's units over the least share are rounded, so that
-// pairs a little over it stay whole. The share is never below the total over the workgroups aimed at, which the partials' space
+// > 0), the share is the F for which the call's splits are just no more than run at once, if F / least <= p.fit_quarters / 4 (5 / 4
+// in tiles, where it so wastes little; any in the streaming kernel), and the rest of a pair is a split too; otherwise a pair's units
+// over the least share are rounded, so that pairs a little over it stay whole. The share is never below the total over the workgroups aimed at, which the partials' space
 // and the grid go by: a pair of several splits has at most twice its units over the share of them, so these are at most twice
 // the workgroups aimed at, and all splits at most those and pairs * Hkv.
 BB_DEV int sum_over_lanes(int v) { return lane_int(wave_scan(v), 63); }
@@ -457,7 +457,7 @@ BB_DEV void load_rows(const PageRows& at, uint8_t* to, uint32_t off) {
 
 // One wave's stream of chunks of KC rows, 8 KB of K and of V. AUX: of its loads, 2 (non-temporal) where a row is read once (32
 // sequences of 8192 rows 107 us, 122 without), 0 where a head has several tiles and reads it again (a step of 64 vectors over 32768
-// rows 53 us, 57 with; of 128 63 and 77).
+// rows 54 us, 57 with; of 128 62 and 77).
 template <int D, int AUX>
 struct PageStream {
   static constexpr int KC = 4096 / D, GROUPS = KC / 16, LOADS = 8 / GROUPS;  // groups of 16 rows lie in one page
@@ -930,9 +930,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnParams
 //     rows, so the probabilities are operands where they are.
 //   * The exponent's offset moves only when a probability would pass 2^8. Tiles that some vector attends in part, and every tile
 //     of a split whose table names no page somewhere, take a mask; they come last.
-// 4096 tokens of 32 heads of 128 (8 KV heads) over 32768 rows, bf16: 1604 us, 1285 TFLOP/s (a large product: 1256), 1.7 us a tile
+// 4096 tokens of 32 heads of 128 (8 KV heads) over 32768 rows, bf16: 1605 us, 1285 TFLOP/s (a large product: 1256), 1.7 us a tile
 // and workgroup at a clock that the power holds at 1.9 to 2.0 GHz; the matrix cores are busy 60 % of it, the LDS reads of 256 KB a
-// tile (8 waves x 32 KB) take about as long as the products. head_dim 64, fp16: 1070 us, 963 TFLOP/s, 1.26 us a tile: as many
+// tile (8 waves x 32 KB) take about as long as the products. head_dim 64, fp16: 1080 us, 954 TFLOP/s, 1.26 us a tile: as many
 // exponentials for half the products. Shapes tried there: four waves of 32 vectors, three workgroups a CU and one barrier a tile,
 // 1150 us (four prompts of 2048 tokens 63 against 64); eight waves with one barrier a tile 1210; the row sums by products with ones
 // 1090; two workgroups of eight waves a CU (128 registers) spill.
