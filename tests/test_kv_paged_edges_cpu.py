@@ -126,7 +126,8 @@ def _masks(t):
     padded[0, 0] = 0
     blocks = [create_block_mask(f, 1, None, t, t, device="cpu") for f in
               (lambda b, h, i, j: j <= i, lambda b, h, i, j: (j <= i) & (padded[b, j] != 0))]
-    plain = [blocks[0], torch.ones(1, 1, 0, 0, dtype=torch.bool), causal, bias, bias.to(torch.bfloat16), torch.ones(1, t, dtype=torch.long), torch.ones(1, t, dtype=torch.bool)]
+    plain = [blocks[0], torch.ones(1, 1, 0, 0, dtype=torch.bool), causal, bias, bias.to(torch.bfloat16),
+             torch.ones(1, t, dtype=torch.long), torch.ones(1, t, dtype=torch.bool)]
     hiding = [blocks[1], left, right, packed, torch.where(left, 0.0, -float("inf")), torch.where(right, 0.0, torch.finfo(torch.float32).min),
               padded, padded.bool(), object()]
     return plain, hiding

@@ -6,7 +6,8 @@ import torch
 import paged_plain as plain
 from bigger_bird_amd import paged_append, paged_attention, paged_step
 from paged_plain import HALF_STEP
-from test_kv_paged_gpu import BF16, FP16, FP32, STEP_VECTORS, STREAM_VECTORS, _attend_case, _check, _heads, _int, _model, _p_step, _pages, _say, _table
+from test_kv_paged_gpu import (BF16, FP16, FP32, STEP_VECTORS, STREAM_VECTORS, _attend_case, _check, _heads, _int, _model, _p_step,
+                               _pages, _say, _table)
 
 pytestmark = pytest.mark.gpu
 
@@ -208,7 +209,8 @@ def test_model_masks_of_one_sequence(dev):
         for kind in ("sdpa", "eager"):
             model.config._attn_implementation = kind
             cache = make_paged_cache(model.config, 1, 20, page=16, device=dev)
-            outs.append([model(input_ids=ids[:, a:b], past_key_values=cache, use_cache=True).logits for a, b in ((0, 40), (40, 59), (59, 60))])
+            outs.append([model(input_ids=ids[:, a:b], past_key_values=cache, use_cache=True).logits
+                         for a, b in ((0, 40), (40, 59), (59, 60))])
             assert cache.lengths == [60]
             for side in (slice(0, 3), slice(37, 40)):
                 cache, padded = make_paged_cache(model.config, 1, 20, page=16, device=dev), mask.clone()

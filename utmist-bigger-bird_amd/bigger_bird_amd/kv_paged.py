@@ -147,9 +147,9 @@ def _append_plan(k, v, kp, vp, table, lens, cos, sin, q, new):
 
 def paged_append(k, v, k_pages, v_pages, table, lens, cos=None, sin=None, q=None, new=None):
     """The new K / V rows k, v [B, Hkv, T, d] into the pages; with cos, sin ([B, T, d] or [T, d], fp32 or the rows' dtype) k is
-    rotated on the way: x cos + (-x[d/2:], x[:d/2]) sin in fp32, rounded once (in fp16 to an infinity past 65519). With q [B, H, T, d] (cos, sin required) returns q
-    rotated alike, in [B, T, H, d] memory (padding columns too); else None. Rows that lie outside the table or on no page are
-    not written. Two tokens of a call must not share a row of a page."""
+    rotated on the way: x cos + (-x[d/2:], x[:d/2]) sin in fp32, rounded once (in fp16 to an infinity past 65519). With q [B, H,
+    T, d] (cos, sin required) returns q rotated alike, in [B, T, H, d] memory (padding columns too); else None. Rows that lie
+    outside the table or on no page are not written. Two tokens of a call must not share a row of a page."""
     what = "paged_append"
     device, copy, out_strides, sk, sv, sq, so, sc, f32, skp, svp, st, sizes = _append_plan(
         *_layouts(k, v, k_pages, v_pages, table, lens, cos, sin, q, new))
@@ -188,14 +188,13 @@ def _attention_plan(q, kp, vp, table, lens, new):
 
 
 def paged_attention(q, k_pages, v_pages, table, lens, scale, new=None):
-    """Exact causal attention of q [B, H, T, d] over the pages: token j of a sequence attends the rows up to its own,
-    lens - new + j. One token a sequence, a few drafted ones or a chunk of a prompt; sequences of unlike lengths. Scores, softmax
-    and sums are fp32. The probabilities meet V as two terms of the rows' dtype up to 32 query vectors of a KV head (T * H / Hkv), so
+    """Exact causal attention of q [B, H, T, d] over the pages: token j of a sequence attends the rows up to its own, lens - new
+    + j. One token a sequence, a few drafted ones or a chunk of a prompt; sequences of unlike lengths. Scores, softmax and sums
+    are fp32. The probabilities meet V as two terms of the rows' dtype up to 32 query vectors of a KV head (T * H / Hkv), so
     that the output's own rounding is all its error; of more vectors they are one, rounded to the dtype (0.0023 of the output's
-    norm in bf16, where its rounding alone is 0.0017). Returns
-    [B, H, T, d] in [B, T, H, d] memory; zeros for padding and where a token attends no row, NaN for a query that is not
-    finite. A value of V that is not finite reaches the tokens that attend it alone: +inf, -inf, or NaN where both or a NaN are
-    attended."""
+    norm in bf16, where its rounding alone is 0.0017). Returns [B, H, T, d] in [B, T, H, d] memory; zeros for padding and where
+    a token attends no row, NaN for a query that is not finite. A value of V that is not finite reaches the tokens that attend
+    it alone: +inf, -inf, or NaN where both or a NaN are attended."""
     what = "paged_attention"
     device, copy, out_strides, sq, skp, svp, st, sizes, so, ws_bytes = _attention_plan(
         *_layouts(q, k_pages, v_pages, table, lens, new))
@@ -230,10 +229,11 @@ def _step_plan(q, k, v, kp, vp, table, lens, cos, sin, new):
 
 def paged_step(q, k, v, k_pages, v_pages, table, lens, scale, cos=None, sin=None, new=None):
     """One step: paged_append(k, v, ..., cos, sin, q) and paged_attention of the rotated q, in one call (q and k as they are
-    where cos is None). Up to 128 query vectors of a KV head (T * H / Hkv) one kernel does both, and neither its rotated queries nor
-    its probabilities are rounded to the rows' dtype; above they are, as paged_append and paged_attention do (0.0029 to 0.0032 of
-    the output's norm in bf16, and a rotated fp16 query is infinite past 65519). A row that the call writes must not be attended in it by another sequence, nor at another place of its own table.
-    Returns [B, H, T, d] in [B, T, H, d] memory."""
+    where cos is None). Up to 128 query vectors of a KV head (T * H / Hkv) one kernel does both, and neither its rotated queries
+    nor its probabilities are rounded to the rows' dtype; above they are, as paged_append and paged_attention do (0.0029 to
+    0.0032 of the output's norm in bf16, and a rotated fp16 query is infinite past 65519). A row that the call writes must not
+    be attended in it by another sequence, nor at another place of its own table. Returns [B, H, T, d] in [B, T, H, d]
+    memory."""
     what = "paged_step"
     device, copy, out_strides, sq, sk, sv, sc, f32, skp, svp, st, sizes, so, ws_bytes = _step_plan(
         *_layouts(q, k, v, k_pages, v_pages, table, lens, cos, sin, new))

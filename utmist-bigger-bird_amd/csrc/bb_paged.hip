@@ -220,12 +220,12 @@ BB_DEV int pair_units(const PagedAttnParams& p, int pair) {
   const int tile = pair_tile(p, pair), k = pair_keys(p, sequence(p.c, p.T, pair_sequence(p, pair, tile)), tile);
   return (k + (1 << p.unit_log2) - 1) >> p.unit_log2;
 }
-// The share of a split, and the splits of a pair. Where the pairs fit a wave and the workgroups that run at once (p.fit_quarters
-// > 0), the share is the F for which the call's splits are just no more than run at once, if F / least <= p.fit_quarters / 4 (5 / 4
-// in tiles, where it so wastes little; any in the streaming kernel), and the rest of a pair is a split too; otherwise a pair's units
-// over the least share are rounded, so that pairs a little over it stay whole. The share is never below the total over the workgroups aimed at, which the partials' space
-// and the grid go by: a pair of several splits has at most twice its units over the share of them, so these are at most twice
-// the workgroups aimed at, and all splits at most those and pairs * Hkv.
+// The share of a split, and the splits of a pair. Where the pairs fit a wave and the workgroups that run at once (p.fit_quarters >
+// 0), the share is the F for which the call's splits are just no more than run at once, if F / least <= p.fit_quarters / 4 (5 / 4
+// in tiles, where it so wastes little; any in the streaming kernel), and the rest of a pair is a split too; otherwise a pair's
+// units over the least share are rounded, so that pairs a little over it stay whole. The share is never below the total over the
+// workgroups aimed at, which the partials' space and the grid go by: a pair of several splits has at most twice its units over the
+// share of them, so these are at most twice the workgroups aimed at, and all splits at most those and pairs * Hkv.
 BB_DEV int sum_over_lanes(int v) { return lane_int(wave_scan(v), 63); }
 struct Share {
   int units;
